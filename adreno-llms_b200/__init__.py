@@ -24,6 +24,16 @@ HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "nnopt_b200.h")
 NN_OK, NN_ERR_ARG, NN_ERR_CUDA, NN_ERR_UNSUPPORTED, NN_ERR_IO, NN_ERR_NOTFOUND, NN_ERR_COMM, NN_ERR_TIMEOUT = 0, -1, -2, -3, -4, -5, -6, -7
 
 
+NN_KV_FORMATS = {"fp16": 0, "int8": 1, "fp8": 2}
+
+
+class KVBatch(ctypes.Structure):
+    """The sequences of a call on a paged key/value cache (nn_kv_batch): host bounds, and device pointers."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("num_seqs", "num_rows", "max_new", "max_len", "table_stride")] + [
+        (n, ctypes.c_void_p) for n in ("row_start", "kv_len", "page_table")]
+
+
 class NNError(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"nnopt_b200 error {code}: {msg}")
@@ -49,7 +59,7 @@ def load():
         raise FileNotFoundError(f"{LIB_PATH} not built; run python adreno-llms_b200/build.py")
     L = ctypes.CDLL(LIB_PATH)
     vp, i, sz, cp = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_char_p
-    pvp = ctypes.POINTER(ctypes.c_void_p)
+    pvp, pkb, i64 = ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(KVBatch), ctypes.c_int64
     sig = {
         "nn_last_error": ([], cp), "nn_version": ([], cp),
         "nn_init": ([i, pvp], i), "nn_shutdown": ([vp], i), "nn_stream": ([vp], vp), "nn_sync": ([vp], i),
@@ -100,6 +110,11 @@ def load():
         "nn_comm_pick_unsent": ([vp, ctypes.c_uint, vp], i),
         "nn_linear_argmax_sharded_rows": ([vp, i, i, i, vp, vp, vp, vp], i),
         "nn_device_count": ([], i),
+        "nn_kv_cache_create": ([vp, i, i, i, i, i, vp, vp, vp, vp, pvp], i), "nn_kv_cache_free": ([vp], i),
+        "nn_kv_write": ([vp, vp, pkb, vp, i64, vp, i64], i),
+        "nn_rope_kv_write": ([vp, vp, pkb, vp, vp, i, i, i, vp, i64, vp, i64, vp, i64, vp, i64], i),
+        "nn_kv_read": ([vp, vp, pkb, vp, i64, vp, i64], i),
+        "nn_attention": ([vp, vp, pkb, i, vp, i64, vp, i64, ctypes.c_float, i, i], i),
     }
     for name, (args, res) in sig.items():
         if hasattr(L, name):
@@ -244,6 +259,23 @@ class Context:
     def rmsnorm_gate_up_silu(self, M, N, K, x, gamma, eps, Wg, Wu, out):
         _check(self.L.nn_rmsnorm_gate_up_silu(self.h, M, N, K, x, gamma, eps, Wg, Wu, out))
 
+    # -- paged key/value cache and attention --
+    def kv_cache(self, fmt, num_pages, page_size, kv_heads, head_dim, k, v, k_scale=None, v_scale=None):
+        return KVCache(self, fmt, num_pages, page_size, kv_heads, head_dim, k, v, k_scale, v_scale)
+
+    def kv_write(self, cache, batch, k, k_stride, v, v_stride):
+        _check(self.L.nn_kv_write(self.h, cache.h, batch, k, k_stride, v, v_stride))
+
+    def rope_kv_write(self, cache, batch, cos, sin, table_len, rotary_dim, q_heads, q, q_stride, q_out, q_out_stride, k, k_stride, v, v_stride):
+        _check(self.L.nn_rope_kv_write(self.h, cache.h, batch, cos, sin, table_len, rotary_dim, q_heads, q, q_stride, q_out, q_out_stride,
+                                       k, k_stride, v, v_stride))
+
+    def kv_read(self, cache, batch, k_out, k_stride, v_out, v_stride):
+        _check(self.L.nn_kv_read(self.h, cache.h, batch, k_out, k_stride, v_out, v_stride))
+
+    def attention(self, cache, batch, q_heads, q, q_stride, out, out_stride, scale, window=0, sinks=0):
+        _check(self.L.nn_attention(self.h, cache.h, batch, q_heads, q, q_stride, out, out_stride, scale, window, sinks))
+
     def l2_flush(self):
         _check(self.L.nn_l2_flush(self.h))
 
@@ -303,6 +335,21 @@ class QuantWeight:
                 self.ctx.free(self.scale)
             self.ctx.free(self.buf)
             self.buf = self.scale = None
+
+
+class KVCache:
+    """The handle of one layer's paged key/value cache (nn_kv_cache) over buffers that the caller keeps; fmt "fp16", "int8" or "fp8"."""
+
+    def __init__(self, ctx: Context, fmt: str, num_pages, page_size, kv_heads, head_dim, k, v, k_scale=None, v_scale=None):
+        self.L, self.h = ctx.L, None
+        h = ctypes.c_void_p()
+        _check(ctx.L.nn_kv_cache_create(ctx.h, NN_KV_FORMATS[fmt], num_pages, page_size, kv_heads, head_dim, k, v, k_scale, v_scale, ctypes.byref(h)))
+        self.h = h
+
+    def close(self):
+        if self.h:
+            self.L.nn_kv_cache_free(self.h)
+            self.h = None
 
 
 class Comm:

@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "../../include/nnopt_b200.h"
+#include "attention.h"
 #include "internal.h"
 #include "kernels.h"
 #include "plan.h"
@@ -58,25 +59,6 @@ std::string op_label(int M, int N, int K, int fmt, const char* form) {
     else snprintf(b, sizeof(b), "gemm_M%d_K%d_N%d_%s%s", M, K, N, fmt_name(fmt), form);
     return b;
 }
-
-struct ProfScope {  // event pair around whatever the scope enqueues
-    nn_context* c;
-    size_t slot = (size_t)-1;
-    template <class Label>   // called only when the profile is on: building a label costs more than a launch's other host work
-    ProfScope(nn_context* ctx, Label&& label) : c(ctx) {
-        if (!c || !c->profiling || c->capturing) return;
-        ProfPending p;
-        p.label = label();
-        if (cudaEventCreate(&p.start) != cudaSuccess) return;
-        if (cudaEventCreate(&p.stop) != cudaSuccess) { cudaEventDestroy(p.start); return; }
-        cudaEventRecord(p.start, c->stream);
-        c->prof_pending.push_back(p);
-        slot = c->prof_pending.size() - 1;
-    }
-    ~ProfScope() {
-        if (slot != (size_t)-1) cudaEventRecord(c->prof_pending[slot].stop, c->stream);
-    }
-};
 
 void prof_add(std::map<std::string, ProfAgg>& agg, const std::string& label, double us) {
     ProfAgg& a = agg[label];
@@ -255,6 +237,8 @@ extern "C" int nn_sync(nn_context* c) {
     if (*c->status_host != 0) {
         const int s = *c->status_host;
         *c->status_host = 0;
+        if (s == STATUS_BAD_TABLE)
+            return NN_FAIL(NN_ERR_ARG, "a page number, length or position of a key/value batch was out of range; the rows and keys it concerned were left out");
         cudaMemsetAsync(c->argmax_slot, 0, 32, c->stream);  // a cut-short launch may have left its words set
         cudaMemsetAsync(c->sk_flags, 0, SK_MAX_BLOCKS * sizeof(unsigned), c->stream);
         return NN_FAIL(NN_ERR_TIMEOUT, "a device-side bounded wait ran out (status %d); results of the last calls are invalid", s);

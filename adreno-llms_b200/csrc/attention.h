@@ -1,0 +1,69 @@
+// Launch interface of the paged key/value cache and of the attention over it.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kv_index.h"
+
+namespace nnb {
+
+struct KvView {   // one layer's cache
+    void* k;
+    void* v;
+    uint16_t* k_scale;   // fp16 per cell row; null with KV_FP16
+    uint16_t* v_scale;
+    int fmt, num_pages, page_shift, kv_heads, dim;
+};
+struct KvSeqs {   // the sequences of a call, on the device
+    const int* row_start;    // [num_seqs + 1]
+    const int* kv_len;       // [num_seqs]
+    const int* page_table;   // [num_seqs][table_stride]
+    int num_seqs, num_rows, table_stride;
+    int max_len;             // at most table_stride << page_shift
+};
+
+struct KvWriteArgs {
+    KvView c;
+    KvSeqs s;
+    const uint16_t* q;       // null: no queries to rotate
+    uint16_t* q_out;
+    const uint16_t* k;
+    const uint16_t* v;
+    const float* cos;        // [table_len][rotary / 2]
+    const float* sin;
+    int table_len, rotary;   // rotary 0: no rotation
+    int q_heads;
+    int64_t q_stride, qo_stride, k_stride, v_stride;   // values from row to row
+    int* status;
+};
+cudaError_t launch_kv_write(const KvWriteArgs& a, cudaStream_t st, bool pdl);
+
+struct KvReadArgs {
+    KvView c;
+    KvSeqs s;
+    uint16_t* k_out;
+    uint16_t* v_out;
+    int64_t k_stride, v_stride;
+    int* status;
+};
+cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t st, bool pdl);
+
+struct AttnArgs {
+    KvView c;
+    KvSeqs s;
+    const uint16_t* q;
+    uint16_t* out;
+    int q_heads, group;      // group: query heads to a kv head
+    int64_t q_stride, o_stride;
+    float scale;
+    int window, sinks;       // window 0: none
+    int* status;
+};
+cudaError_t launch_attention(const AttnArgs& a, cudaStream_t st, bool pdl);
+
+// What a kernel of these leaves in the context's status word when the tables or lengths that it was given are out of range
+// (nn_sync reports it as an argument error; other non-zero values are waits that ran out).
+constexpr int STATUS_BAD_TABLE = 1 << 20;
+
+}  // namespace nnb

@@ -64,6 +64,25 @@ struct nn_context {
     long long launches = 0, launches_at_capture = 0;
 };
 
+struct ProfScope {  // event pair around whatever the scope enqueues
+    nn_context* c;
+    size_t slot = (size_t)-1;
+    template <class Label>   // called only when the profile is on: building a label costs more than a launch's other host work
+    ProfScope(nn_context* ctx, Label&& label) : c(ctx) {
+        if (!c || !c->profiling || c->capturing) return;
+        ProfPending p;
+        p.label = label();
+        if (cudaEventCreate(&p.start) != cudaSuccess) return;
+        if (cudaEventCreate(&p.stop) != cudaSuccess) { cudaEventDestroy(p.start); return; }
+        cudaEventRecord(p.start, c->stream);
+        c->prof_pending.push_back(p);
+        slot = c->prof_pending.size() - 1;
+    }
+    ~ProfScope() {
+        if (slot != (size_t)-1) cudaEventRecord(c->prof_pending[slot].stop, c->stream);
+    }
+};
+
 namespace nnb {
 
 struct ResolvedW {

@@ -38,6 +38,7 @@ typedef struct nn_context nn_context; /* OpenCLContext + its cl_command_queue */
 typedef struct nn_weights nn_weights; /* class Weights */
 typedef struct nn_plan nn_plan;       /* a recorded decode step */
 typedef struct nn_comm nn_comm;       /* row-sharding communicator (one rank per GPU) */
+typedef struct nn_kv_cache nn_kv_cache; /* a layer's paged key/value cache */
 typedef void* nn_buf;                 /* device pointer; stands in for cl_mem */
 
 enum {
@@ -168,6 +169,63 @@ int nn_argmax(nn_context* ctx, int n, nn_buf logits_fp16, nn_buf out_index_i32);
  * Replaces the pair LmHead::forward + argmax_block/argmax_final
  * (src/models/smollm2-135m-instruct/src/layers/lm_head.cpp:36-67, kernels/argmax.cl:33,80). */
 int nn_linear_argmax(nn_context* ctx, int N, int K, nn_buf x, nn_buf W, nn_buf logits_fp16, nn_buf out_index_i32);
+
+/* ---- paged key/value cache and the attention over it: what stands between the q/k/v projections and
+ *      o_proj in a decoder layer (Attention::forward_decode_into_residual,
+ *      src/models/smollm2-135m-instruct/src/layers/attention.cpp:724-769: fused_rope_kvwrite_m1 and
+ *      fused_decode_attn_m1, one sequence, one contiguous fp16 cache).  Here the cache is in pages, in
+ *      fp16 or 8 bits, of several sequences of any length, and a call takes one or many new tokens of each.
+ *
+ *   A cache is what one layer keeps: two buffers (keys, values) of
+ *   [num_pages][kv_heads][page_size][head_dim] cells of 2 bytes (NN_KV_FP16) or 1, and with 8 bits two of fp16 scales
+ *   [num_pages][kv_heads][page_size].  A cell row stands for code * scale.  The caller allocates them (16-byte
+ *   aligned) and keeps them; the handle only describes them.  page_size 16, 32, 64, 128 or 256; head_dim 64 or 128.
+ *   Pages need no initial contents.  Codes are those that nn_kv_write leaves (no e4m3 NaNs).
+ *
+ *   A batch describes the sequences of a call in device memory that the call reads when it runs, so that a recorded
+ *   step takes new lengths at every replay:
+ *     row_start   int32 [num_seqs + 1], ascending: rows row_start[s] .. row_start[s + 1] - 1 of the call's operands are the new
+ *                 tokens of sequence s (none, one or many).  Rows behind row_start[num_seqs] are neither read nor written.
+ *     kv_len      int32 [num_seqs]: positions of the sequence, its new tokens included: the last row has position kv_len - 1.
+ *     page_table  int32 [num_seqs][table_stride]: position p lies in page page_table[s][p / page_size], slot p % page_size.
+ *                 Entries behind the last position are not read.
+ *   and bounds for the host: num_rows rows in every operand; max_new, the most new rows of a sequence (it picks the kernel: a
+ *   longer one is served all the same); max_len, beyond which no sequence is (at most table_stride * page_size).
+ *   A page number, length or position that is out of range makes the next nn_sync return NN_ERR_ARG; rows and keys that it concerns
+ *   are left out, nothing out of bounds is touched.
+ *   Operands are fp16 rows of [heads][head_dim], 16-byte aligned; strides count values from row to row (a multiple of 8;
+ *   0: dense), so that q, k and v may be columns of one buffer.
+ *
+ *   nn_kv_write       k and v rows into the cache.  8 bits: scale = the smallest fp16 with scale * Q >= the row's largest
+ *                     magnitude (per position and head; Q = 127, or 448 for e4m3; the fp16 below where that product passes
+ *                     65504; 1 for a row of zeros), code = value / scale
+ *                     rounded to nearest even.  A row with an infinity or a NaN reads back as NaN as a whole.
+ *   nn_rope_kv_write  the same with the rotation of queries and keys to their positions first, in one launch: of every head
+ *                     dims i and i + rotary_dim / 2 turn together, y_i = x_i cos - x_j sin, y_j = x_j cos + x_i sin, with cos and
+ *                     sin fp32 [table_len][rotary_dim / 2] by position; the cache takes the rotated key rounded to fp16.
+ *                     rotary_dim a multiple of 16, at most head_dim.  q_out may be q.  q_heads 0, q and q_out NULL: keys only.
+ *   nn_kv_read        the same rows read back: half(code * scale).  Its rows are the last row_start[s + 1] - row_start[s]
+ *                     positions of each sequence (all of them where that is kv_len[s]); a row whose page is out of range is zeros.
+ *   nn_attention      out[r, h] = sum_k softmax_k(scale * q[r, h] . k) v over the keys k that the row's position p sees:
+ *                     k <= p and, with window > 0, k > p - window or k < sinks (the first tokens stay visible).  Query head h reads
+ *                     head h / (q_heads / kv_heads) of the cache.  A row that sees nothing (a position below 0) gives zeros.
+ *                     What hidden cells hold, NaN and infinities included, has no influence.  out must not overlap q.
+ *                     scale finite and positive. ------------------------------------------------------------------ */
+enum { NN_KV_FP16 = 0, NN_KV_INT8 = 1, NN_KV_FP8 = 2 /* e4m3 */ };
+typedef struct nn_kv_batch {
+    int num_seqs, num_rows, max_new, max_len, table_stride;
+    nn_buf row_start, kv_len, page_table;
+} nn_kv_batch;
+int nn_kv_cache_create(nn_context* ctx, int format, int num_pages, int page_size, int kv_heads, int head_dim, nn_buf k_pages, nn_buf v_pages,
+                       nn_buf k_scale, nn_buf v_scale, nn_kv_cache** out);
+/* (a handle made without a context serves checks of arguments alone: every call refuses it in the end) */
+int nn_kv_cache_free(nn_kv_cache* cache); /* the handle; recordings that used it stay valid as long as the buffers do */
+int nn_kv_write(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, nn_buf k, int64_t k_stride, nn_buf v, int64_t v_stride);
+int nn_rope_kv_write(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, nn_buf cos_f32, nn_buf sin_f32, int table_len, int rotary_dim, int q_heads,
+                     nn_buf q, int64_t q_stride, nn_buf q_out, int64_t q_out_stride, nn_buf k, int64_t k_stride, nn_buf v, int64_t v_stride);
+int nn_kv_read(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, nn_buf k_out, int64_t k_stride, nn_buf v_out, int64_t v_stride);
+int nn_attention(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, int q_heads, nn_buf q, int64_t q_stride, nn_buf out, int64_t out_stride, float scale,
+                 int window, int sinks);
 
 /* Arg-max for callers that are not allowed to allocate device memory (a real-time thread
  * under a no-allocation rule, a host application that owns the whole device heap through its
