@@ -59,8 +59,16 @@ struct AttnArgs {
     float scale;
     int window, sinks;       // window 0: none
     int* status;
+    void* parts;             // partial results of items that blocks share: the context's, for one call at a time
+    unsigned* counters;      // blocks of such an item that have arrived (0 between launches)
 };
-cudaError_t launch_attention(const AttnArgs& a, cudaStream_t st, bool pdl);
+struct AttnMaps;
+cudaError_t attention_configure();
+cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl);
+constexpr int ATTN_MAX_BLOCKS = 256;
+constexpr size_t ATTN_DECODE_PART = 17 * 512;   // two per block
+constexpr size_t ATTN_PARTS_BYTES = 2 * ATTN_MAX_BLOCKS * ATTN_DECODE_PART;
+constexpr size_t ATTN_COUNTER_BYTES = ATTN_MAX_BLOCKS * sizeof(unsigned);
 
 // What a kernel of these leaves in the context's status word when the tables or lengths that it was given are out of range
 // (nn_sync reports it as an argument error; other non-zero values are waits that ran out).

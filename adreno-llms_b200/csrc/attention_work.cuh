@@ -1,0 +1,190 @@
+// How a call's work is dealt out to blocks.
+//
+// An item is a tile of queries (up to `tokens` new tokens of one sequence, times the `group` query heads that share a cache head) with the
+// key tiles that some of them see, at least one (an item that sees nothing still has zeros to write).  Items are numbered by
+// sequence, head and query tile, their key tiles are strung together, and block b takes units [b * chunk, (b + 1) * chunk) of that string:
+// every block has the same number, whatever the lengths are, and all lengths stay on the device, so that a recorded call takes new ones.
+// A piece of an item in one block is a segment; the blocks of an item that is cut leave partial results to be joined.
+#pragma once
+#include "kv_cells.cuh"
+
+namespace nnb {
+
+struct WorkShape {
+    int group;     // query heads of a token in an item
+    int tokens;    // tokens of an item
+    int vheads;    // items side by side: cache heads (times the parts of a head's query heads)
+    int tile;      // keys of a unit
+    int window, sinks;
+};
+
+struct SeqWork {
+    int row0, n, len, tiles_q;   // first row, new tokens, length, query tiles
+};
+
+struct Segment {
+    int seq, vhead, qt;
+    int row0, n, len;       // of the sequence
+    int first, count;       // key tiles [first, first + count) of the item
+    int total;              // key tiles of the item
+    long long unit0;        // number of the item's first unit
+    // positions of the item's first and last token
+    __device__ __forceinline__ int p0(const WorkShape& w) const { return len - n + qt * w.tokens; }
+    __device__ __forceinline__ int p1(const WorkShape& w) const { return len - n + min((qt + 1) * w.tokens, n) - 1; }
+    __device__ __forceinline__ TileRange tiles(const WorkShape& w) const { return visible_tiles(p0(w), p1(w), w.window, w.sinks, w.tile); }
+};
+
+__device__ __forceinline__ SeqWork load_seq(const KvSeqs& s, const WorkShape& w, int i, bool* bad = nullptr) {
+    const SeqExtent e = seq_extent(s.row_start[i], s.row_start[i + 1], s.kv_len[i], s.num_rows, s.max_len);
+    if (bad) *bad = e.bad;
+    SeqWork q;
+    q.row0 = e.row0;
+    q.n = e.row1 - e.row0;
+    q.len = e.len;
+    q.tiles_q = (q.n + w.tokens - 1) / w.tokens;
+    return q;
+}
+__device__ __forceinline__ int item_tiles(const SeqWork& q, const WorkShape& w, int qt) {
+    const int p0 = q.len - q.n + qt * w.tokens, p1 = q.len - q.n + min((qt + 1) * w.tokens, q.n) - 1;
+    return max(1, visible_tiles(p0, p1, w.window, w.sinks, w.tile).tiles());
+}
+// Key tiles of all query tiles of a sequence; by a whole warp.
+__device__ __forceinline__ long long seq_tiles(const SeqWork& q, const WorkShape& w) {
+    long long t = 0;
+    for (int i = threadIdx.x & 31; i < q.tiles_q; i += 32) t += item_tiles(q, w, i);
+    if (q.tiles_q > 1) {   // (uniform)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        return t;
+    }
+    return __shfl_sync(0xffffffffu, t, 0);
+}
+
+// Where a block's units are.  Copies of a walk go on independently; next() is called by whole warps.
+struct Walk {
+    long long u, end;      // the next unit, and the block's last one + 1
+    int seq, vhead, qt, first;
+    SeqWork q;
+
+    __device__ __forceinline__ bool next(const KvSeqs& s, const WorkShape& w, Segment* out) {
+        if (u >= end) return false;
+        while (qt >= q.tiles_q) {
+            qt = 0;
+            if (q.tiles_q == 0 || ++vhead >= w.vheads) {
+                vhead = 0;
+                if (++seq >= s.num_seqs) {   // (no units are left: not reached while u < end)
+                    u = end;
+                    return false;
+                }
+                q = load_seq(s, w, seq);
+            }
+        }
+        const int total = item_tiles(q, w, qt);
+        out->seq = seq;
+        out->vhead = vhead;
+        out->qt = qt;
+        out->row0 = q.row0;
+        out->n = q.n;
+        out->len = q.len;
+        out->first = first;
+        out->total = total;
+        out->unit0 = u - first;
+        out->count = (int)min((long long)(total - first), end - u);
+        u += out->count;
+        first = 0;
+        ++qt;
+        return true;
+    }
+};
+
+struct WorkShared {
+    static constexpr int SEQS = 256;
+    SeqWork q[SEQS];
+    long long units[SEQS];
+};
+
+// The walk of this block, by all its threads.  `least`: the fewest units that are worth a block.  *chunk: units of a block.
+// (Two passes over the sequences: how many units there are, then where this block's begin.  The first of up to 256 sequences keeps
+// everything in shared memory for the second.)
+__device__ __forceinline__ Walk find_work(const KvSeqs& s, const WorkShape& w, WorkShared* sh, int least, long long* chunk, int* status) {
+    const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x / 32, warp = tid / 32;
+    Walk k;
+    k.u = k.end = 0;
+    k.seq = k.vhead = k.qt = k.first = 0;
+    k.q = SeqWork{0, 0, 0, 0};
+    long long total = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        long long base = 0;
+        for (int c0 = 0; c0 < s.num_seqs; c0 += WorkShared::SEQS) {
+            const int cnt = min(WorkShared::SEQS, s.num_seqs - c0);
+            if (pass == 0 || s.num_seqs > WorkShared::SEQS) {
+                __syncthreads();
+                for (int i = tid; i < cnt; i += blockDim.x) {
+                    bool bad;
+                    sh->q[i] = load_seq(s, w, c0 + i, &bad);
+                    if (bad) *status = STATUS_BAD_TABLE;
+                }
+                __syncthreads();
+                for (int i = warp; i < cnt; i += warps) {
+                    const long long t = seq_tiles(sh->q[i], w);
+                    if (lane == 0) sh->units[i] = t * w.vheads;
+                }
+                __syncthreads();
+            }
+            for (int i0 = 0; i0 < cnt; i0 += 32) {
+                const long long mine = i0 + lane < cnt ? sh->units[i0 + lane] : 0;
+                long long upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += x;
+                }
+                if (pass == 1) {
+                    const unsigned hit = __ballot_sync(0xffffffffu, base + upto > k.u);
+                    if (hit) {   // the sequence of the block's first unit
+                        const int l = __ffs(hit) - 1;
+                        const long long before = base + __shfl_sync(0xffffffffu, upto - mine, l);
+                        const long long per_head = __shfl_sync(0xffffffffu, mine, l) / w.vheads;
+                        long long rest = k.u - before;
+                        k.seq = c0 + i0 + l;
+                        k.q = sh->q[i0 + l];
+                        k.vhead = (int)(rest / per_head);
+                        rest -= k.vhead * per_head;
+                        for (int q0 = 0;; q0 += 32) {   // and its query tile
+                            long long n = q0 + lane < k.q.tiles_q ? item_tiles(k.q, w, q0 + lane) : 0, run = n;
+#pragma unroll
+                            for (int o = 1; o < 32; o <<= 1) {
+                                const long long x = __shfl_up_sync(0xffffffffu, run, o);
+                                if (lane >= o) run += x;
+                            }
+                            const unsigned in = __ballot_sync(0xffffffffu, run > rest);
+                            if (in || q0 + 32 >= k.q.tiles_q) {
+                                const int j = in ? __ffs(in) - 1 : 0;
+                                k.qt = q0 + j;
+                                k.first = (int)(rest - __shfl_sync(0xffffffffu, run - n, j));
+                                break;
+                            }
+                            rest -= __shfl_sync(0xffffffffu, run, 31);
+                        }
+                        return k;
+                    }
+                }
+                base += __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        if (pass == 0) {
+            total = base;
+            long long c = (total + gridDim.x - 1) / gridDim.x;
+            *chunk = c < least ? least : c;
+            k.u = blockIdx.x * *chunk;
+            k.end = min(total, k.u + *chunk);
+            if (k.u >= total) {
+                k.u = k.end = 0;
+                return k;
+            }
+        }
+    }
+    return k;
+}
+
+}  // namespace nnb

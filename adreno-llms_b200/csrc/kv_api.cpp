@@ -2,10 +2,12 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <new>
 #include <string>
 
 #include "../../include/nnopt_b200.h"
 #include "attention.h"
+#include "attention_maps.h"
 #include "internal.h"
 #include "kernels.h"
 
@@ -14,12 +16,35 @@ using namespace nnb;
 struct nn_kv_cache {
     int device;
     KvView view;
+    AttnMaps maps;
 };
 
 static bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 static size_t cache_bytes(const KvView& v) {
     return ((size_t)v.num_pages * v.kv_heads << v.page_shift) * (size_t)v.dim * kv_cell_bytes(v.fmt);
+}
+
+#define CUDA_TRY(call)                                                                        \
+    do {                                                                                      \
+        cudaError_t e_ = (call);                                                              \
+        if (e_ != cudaSuccess) return NN_FAIL(NN_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_)); \
+    } while (0)
+
+// The partial results of items that several blocks share: one buffer for all calls of the context, which run one after the other.
+static int attention_workspace(nn_context* c) {
+    if (c->attn_parts) return NN_OK;
+    if (c->capturing) return NN_FAIL(NN_ERR_UNSUPPORTED, "nn_kv_cache_create: the context's first cache cannot be made while a plan is being recorded");
+    CUDA_TRY(attention_configure());
+    void* parts = nullptr;
+    CUDA_TRY(cudaMalloc(&parts, ATTN_PARTS_BYTES + ATTN_COUNTER_BYTES));
+    const cudaError_t e = cudaMemset((char*)parts + ATTN_PARTS_BYTES, 0, ATTN_COUNTER_BYTES);
+    if (e != cudaSuccess) {
+        cudaFree(parts);
+        return NN_FAIL(NN_ERR_CUDA, "nn_kv_cache_create: %s", cudaGetErrorString(e));
+    }
+    c->attn_parts = parts;
+    return NN_OK;
 }
 
 extern "C" int nn_kv_cache_create(nn_context* c, int format, int num_pages, int page_size, int kv_heads, int head_dim, nn_buf k, nn_buf v,
@@ -39,9 +64,7 @@ extern "C" int nn_kv_cache_create(nn_context* c, int format, int num_pages, int 
         return NN_FAIL(NN_ERR_ARG, "nn_kv_cache_create: %s", scaled ? "an 8-bit cache needs both scale buffers" : "an fp16 cache has no scale buffers");
     if (!aligned(k, 16) || !aligned(v, 16) || !aligned(k_scale, 16) || !aligned(v_scale, 16))
         return NN_FAIL(NN_ERR_ARG, "nn_kv_cache_create: pages and scales must be 16-byte aligned");
-    nn_kv_cache* h = new nn_kv_cache();
-    h->device = c ? c->device : -1;
-    KvView& w = h->view;
+    KvView w = {};
     w.k = k;
     w.v = v;
     w.k_scale = (uint16_t*)k_scale;
@@ -51,6 +74,15 @@ extern "C" int nn_kv_cache_create(nn_context* c, int format, int num_pages, int 
     for (w.page_shift = 0; (1 << w.page_shift) < page_size;) ++w.page_shift;
     w.kv_heads = kv_heads;
     w.dim = head_dim;
+    AttnMaps maps = {};
+    if (c) {
+        CUDA_TRY(cudaSetDevice(c->device));
+        const int rc = attention_workspace(c);
+        if (rc) return rc;
+        if (!encode_attention_maps(w, &maps)) return NN_FAIL(NN_ERR_CUDA, "nn_kv_cache_create: no tensor maps for these pages (k=%p v=%p)", k, v);
+    }
+    nn_kv_cache* h = new (std::nothrow) nn_kv_cache{c ? c->device : -1, w, maps};
+    if (!h) return NN_FAIL(NN_ERR_ARG, "nn_kv_cache_create: out of host memory");
     *out = h;
     return NN_OK;
 }
@@ -105,6 +137,7 @@ static int take_batch(nn_context* c, const nn_kv_cache* h, const nn_kv_batch* b,
         *empty = true;
         return NN_OK;
     }
+    if (b->max_len > 1 << 30) return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: max_len=%d is more than 2^30", who, b->max_len);
     if (b->max_new <= 0 || b->max_len <= 0 || b->table_stride <= 0)
         return NN_FAIL(NN_ERR_ARG, "%s: max_new=%d max_len=%d table_stride=%d", who, b->max_new, b->max_len, b->table_stride);
     if (!b->row_start || !b->kv_len || !b->page_table) return NN_FAIL(NN_ERR_ARG, "%s: null row_start, kv_len or page_table", who);
@@ -123,8 +156,12 @@ static int take_batch(nn_context* c, const nn_kv_cache* h, const nn_kv_batch* b,
 }
 
 // Last of the checks (the others need no GPU).  The calling thread may have another device current.
-static int make_current(const nn_context* c, const nn_kv_cache* h, const char* who) {
+static int make_current(nn_context* c, const nn_kv_cache* h, const char* who) {
     if (!c) return NN_FAIL(NN_ERR_ARG, "%s: null context", who);
+    if (!c->attn_parts) {   // a context that has made no cache of its own
+        const int rc = attention_workspace(c);
+        if (rc) return rc;
+    }
     if (h->device != c->device) return NN_FAIL(NN_ERR_ARG, "%s: the cache was made for device %d, the context is of device %d", who, h->device, c->device);
     int now = -1;
     if (cudaGetDevice(&now) != cudaSuccess || now != c->device) {
@@ -253,7 +290,9 @@ extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b,
     if ((rc = make_current(c, h, who))) return rc;
     a.status = c->status_dev;
     ProfScope prof(c, [&] { return std::string("attention_") + kv_name(a.c.fmt) + "_seqs" + std::to_string(b->num_seqs) + "_rows" + std::to_string(b->num_rows); });
-    const cudaError_t e = launch_attention(a, c->stream, c->use_pdl);
+    a.parts = c->attn_parts;
+    a.counters = (unsigned*)((char*)c->attn_parts + ATTN_PARTS_BYTES);
+    const cudaError_t e = launch_attention(a, h->maps, b->max_new, c->sm_count, c->stream, c->use_pdl);
     if (e != cudaSuccess) return NN_FAIL(NN_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     c->in_flight.wrote(out, rows_bytes(ro, b->num_rows));
     c->launches++;

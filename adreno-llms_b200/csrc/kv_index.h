@@ -20,13 +20,13 @@ NNB_HD constexpr float kv_max_code(int fmt) { return fmt == KV_INT8 ? 127.f : 44
 // The new rows of a sequence and its length, brought into range: 0 <= row0 <= row1 <= num_rows, 0 <= len <= max_len.
 struct SeqExtent {
     int row0, row1, len;
-    bool bad;   // the length had to be cut
+    bool bad;   // something had to be cut
 };
 NNB_HD SeqExtent seq_extent(int start, int end, int kv_len, int num_rows, int max_len) {
     SeqExtent e;
     e.row0 = start < 0 ? 0 : start > num_rows ? num_rows : start;
     e.row1 = end < e.row0 ? e.row0 : end > num_rows ? num_rows : end;
-    e.bad = kv_len < 0 || kv_len > max_len;
+    e.bad = start < 0 || end < start || end > num_rows || kv_len < 0 || kv_len > max_len;
     e.len = kv_len < 0 ? 0 : kv_len > max_len ? max_len : kv_len;
     return e;
 }

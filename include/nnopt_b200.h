@@ -190,7 +190,7 @@ int nn_linear_argmax(nn_context* ctx, int N, int K, nn_buf x, nn_buf W, nn_buf l
  *     page_table  int32 [num_seqs][table_stride]: position p lies in page page_table[s][p / page_size], slot p % page_size.
  *                 Entries behind the last position are not read.
  *   and bounds for the host: num_rows rows in every operand; max_new, the most new rows of a sequence (it picks the kernel: a
- *   longer one is served all the same); max_len, beyond which no sequence is (at most table_stride * page_size).
+ *   longer one is served all the same); max_len, beyond which no sequence is (at most table_stride * page_size, and 2^30).
  *   A page number, length or position that is out of range makes the next nn_sync return NN_ERR_ARG; rows and keys that it concerns
  *   are left out, nothing out of bounds is touched.
  *   Operands are fp16 rows of [heads][head_dim], 16-byte aligned; strides count values from row to row (a multiple of 8;

@@ -19,7 +19,7 @@ int main() {
     for (int s : odd) for (int e : odd) for (int n : odd) {
         const SeqExtent x = seq_extent(s, e, n, 40, 64);
         CHECK(0 <= x.row0 && x.row0 <= x.row1 && x.row1 <= 40 && 0 <= x.len && x.len <= 64);
-        CHECK(x.bad == (n < 0 || n > 64));
+        CHECK(x.bad == (n < 0 || n > 64 || s < 0 || e < s || e > 40));
         if (s >= 0 && s <= e && e <= 40) CHECK(x.row0 == s && x.row1 == e);
     }
     for (int p : odd) CHECK(page_ok(p, 40) == (p >= 0 && p < 40));
@@ -107,7 +107,7 @@ NO_CONTEXT = b"null context"
 @pytest.mark.parametrize("change,text", [
     ({}, NO_CONTEXT), (dict(num_seqs=0), NO_CONTEXT), (dict(num_rows=0, row_start=None), NO_CONTEXT), (dict(num_seqs=-1), b"num_seqs"), (dict(num_rows=-1), b"num_rows"),
     (dict(max_new=0), b"max_new"), (dict(max_len=0), b"max_len"), (dict(table_stride=0), b"table_stride"), (dict(max_len=129), b"page table row"),
-    (dict(max_len=128), NO_CONTEXT), (dict(table_stride=1 << 30, max_len=(1 << 31) - 1), NO_CONTEXT),
+    (dict(max_len=128), NO_CONTEXT), (dict(table_stride=1 << 30, max_len=1 << 30), NO_CONTEXT),
     (dict(row_start=None), b"null row_start"), (dict(kv_len=None), b"null row_start"), (dict(page_table=None), b"null row_start"), (dict(kv_len=4 * BUF + 2), b"4-byte"),
 ])
 def test_batch_refusals(nnb, built_lib, call, change, text):
