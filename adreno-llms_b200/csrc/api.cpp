@@ -212,7 +212,7 @@ extern "C" int nn_shutdown(nn_context* c) {
     }
     for (auto& kv : c->registry) free_scale_pad(kv.second);
     if (c->flush_buf) cudaFree(c->flush_buf);
-    if (c->attn_parts) cudaFree(c->attn_parts);
+    if (c->attn_work) cudaFree(c->attn_work);
     if (c->argmax_slot) cudaFree(c->argmax_slot);
     if (c->norm_scratch) cudaFree(c->norm_scratch);
     if (c->stage_img) cudaFree(c->stage_img);
@@ -242,7 +242,7 @@ extern "C" int nn_sync(nn_context* c) {
             return NN_FAIL(NN_ERR_ARG, "a page number, length or position of a key/value batch was out of range; the rows and keys it concerned were left out");
         cudaMemsetAsync(c->argmax_slot, 0, 32, c->stream);  // a cut-short launch may have left its words set
         cudaMemsetAsync(c->sk_flags, 0, SK_MAX_BLOCKS * sizeof(unsigned), c->stream);
-        if (c->attn_parts) cudaMemsetAsync((char*)c->attn_parts + ATTN_PARTS_BYTES, 0, ATTN_COUNTER_BYTES, c->stream);
+        if (c->attn_work) cudaMemsetAsync(c->attn_work, 0, ATTN_COUNTER_BYTES, c->stream);
         return NN_FAIL(NN_ERR_TIMEOUT, "a device-side bounded wait ran out (status %d); results of the last calls are invalid", s);
     }
     return NN_OK;

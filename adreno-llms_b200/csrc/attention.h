@@ -59,16 +59,18 @@ struct AttnArgs {
     float scale;
     int window, sinks;       // window 0: none
     int* status;
+    unsigned* counters;      // blocks of a shared item that have arrived (0 between launches)
+    int4* items;             // shared items, by the block that begins them
     void* parts;             // partial results of items that blocks share: the context's, for one call at a time
-    unsigned* counters;      // blocks of such an item that have arrived (0 between launches)
 };
 struct AttnMaps;
 cudaError_t attention_configure();
 cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl);
 constexpr int ATTN_MAX_BLOCKS = 256;
-constexpr size_t ATTN_DECODE_PART = 17 * 512;   // two per block
-constexpr size_t ATTN_PARTS_BYTES = 2 * ATTN_MAX_BLOCKS * ATTN_DECODE_PART;
-constexpr size_t ATTN_COUNTER_BYTES = ATTN_MAX_BLOCKS * sizeof(unsigned);
+constexpr size_t ATTN_DECODE_PART = 17 * 512, ATTN_CHUNK_PART = 256 * 128 * 4 + 256 * 8;   // two per block
+// The workspace: counters, items, parts.
+constexpr size_t ATTN_COUNTER_BYTES = ATTN_MAX_BLOCKS * sizeof(unsigned), ATTN_HEAD_BYTES = ATTN_COUNTER_BYTES + ATTN_MAX_BLOCKS * sizeof(int4);
+inline size_t attention_workspace_bytes(int sm_count) { return ATTN_HEAD_BYTES + 2 * (size_t)(sm_count < ATTN_MAX_BLOCKS ? sm_count : ATTN_MAX_BLOCKS) * ATTN_CHUNK_PART; }
 
 // What a kernel of these leaves in the context's status word when the tables or lengths that it was given are out of range
 // (nn_sync reports it as an argument error; other non-zero values are waits that ran out).

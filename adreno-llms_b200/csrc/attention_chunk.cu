@@ -1,0 +1,697 @@
+// Attention of many query rows to a cache head (chunks of new tokens, prompts, drafts): two products on the tensor cores per tile of keys.
+//
+//   t_k = scale log2(e) q.k,  w_k = 2^(t_k - m),  out = sum w_k v_k / sum w_k       m: a running reference at most 8 below the maximum of t
+//
+// (8-bit cells: the scales join the scores and weights as in attention_decode.cu: codes are exact in fp16, no rounding is added.)
+//
+// An item is up to 256 query rows: two tiles of 128, each new tokens times the query heads of a cache head, so that a cell is
+// fetched once for all heads that share it.  With no more than 128 rows the two tiles hold the same rows and take the key tiles in turn.
+// A block is one of each SM:
+//   * warps 0-3 and 4-7: the softmax of one query tile each, a thread per row: scores come from tensor memory, the weights go back there
+//     as fp16 in the scores' place (the A operand of the second product).  The sums of outputs stay in tensor memory and
+//     are scaled again only when a row's maximum has grown by more than 2^8.
+//   * warp 8: issues all tcgen05.mma: scores = Q K^T (both K-major), out += weights V (V as it lies in the cache, MN-major).  While one
+//     query tile is in its softmax the other one has the tensor cores.
+//   * warp 9: tensor copies (fp16: straight into the operands; 8-bit: codes into a ring of half tiles).
+//   * warps 10-13, 8-bit cells only: codes to fp16 operands, and the keys' factors.
+// The exponentials bound it next to the products: 128 x 128 scores take 1024 clocks of the SM's exponential units and D * 8 clocks of
+// its tensor cores for both products.
+#include "attention_maps.h"
+#include "attention_row.cuh"
+#include "attention_work.cuh"
+#include "tcgen05.cuh"
+
+namespace nnb {
+namespace {
+
+constexpr int BN = 128;   // keys of a tile
+
+template <int FMT, int D>
+struct Chunk {
+    static constexpr bool CODES = FMT != KV_FP16;
+    static constexpr int HALVES = D / 64;                        // 128-byte columns of an operand tile
+    static constexpr int TILE = BN * D * 2;                      // bytes of an operand tile
+    static constexpr int RING = D == 64 ? 4 : 2;                 // key tiles, and as many value tiles
+    // What the softmax needs of a key tile outlives the tile: tile t goes in when the products of tile t - RING are done, and then the softmax
+    // of tile t - RING - 2 is.  (Its copies begin up to two tiles earlier.)
+    static constexpr int META = D == 64 ? 8 : 4;
+    static constexpr int HERE = 8;                               // which keys of a tile were copied: noted when its copies begin
+    static constexpr int RAW_KEYS = 64, RAW = RAW_KEYS * D;      // half tiles of codes
+    static constexpr int RAW_STAGE = RAW + 256;                  // with the scales of keys and values
+    static constexpr int RAWS = CODES ? (D == 64 ? 6 : 3) : 0;
+    static constexpr int THREADS = CODES ? 448 : 320;
+    // shared memory
+    static constexpr int O_Q = 0, O_K = O_Q + 2 * TILE, O_V = O_K + RING * TILE, O_RAW = O_V + RING * TILE, O_META = O_RAW + RAWS * RAW_STAGE;
+    static constexpr int META_BYTES = CODES ? BN * 12 : 0;       // a: factor of the score, b: its summand, 1 / scale of the value
+    static constexpr int O_HERE = O_META + META * META_BYTES, O_SUMS = O_HERE + HERE * 4, O_BARS = O_SUMS + BN * 8;
+    static constexpr int B_KFULL = 0, B_KEMPTY = B_KFULL + RING, B_VFULL = B_KEMPTY + RING, B_VEMPTY = B_VFULL + RING, B_META = B_VEMPTY + RING,
+                         B_RFULL = B_META + META, B_REMPTY = B_RFULL + RAWS, B_Q = B_REMPTY + RAWS, B_S = B_Q + 2, B_P = B_S + 2, B_O = B_P + 2, B_FIX = B_O + 2, B_DONE = B_FIX + 1,
+                         BARS = B_DONE + 1;
+    static constexpr int O_TMEM = O_BARS + BARS * 8, O_DEAD = O_TMEM + 4, BYTES = O_DEAD + 4, SMEM = BYTES + 1024;
+    static_assert(SMEM <= 227 * 1024, "shared memory");
+    static_assert(O_BARS % 8 == 0 && O_RAW % 128 == 0 && RAW_STAGE % 16 == 0 && O_META % 16 == 0, "alignment");
+    static_assert(sizeof(WorkShared) <= 2 * TILE, "the work list lies where the queries will");
+};
+constexpr int T_S = 0, T_O = 256;   // tensor memory: two tiles of scores (and weights), two of outputs
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {
+    uint32_t u[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]),
+          "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]),
+          "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+        : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]),
+                   "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15]), "+r"(u[16]), "+r"(u[17]), "+r"(u[18]), "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]),
+                   "+r"(u[23]), "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]), "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])
+                 :: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(u[i]);
+}
+// An operand whose N dimension lies together (V: dims of a key): tiles of 64 dims x 8 keys; the leading offset is the distance of
+// two 64-dim columns, the stride that of two groups of 8 keys (1024 bytes).
+__device__ __forceinline__ uint32_t desc_lo_mn(uint32_t saddr, uint32_t column_bytes) { return ((saddr >> 4) & 0x3FFFu) | ((column_bytes >> 4) << 16); }
+constexpr uint32_t IDESC_B_MN = 1u << 16;
+
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// 16 bytes `chunk` of row `row` of an operand tile
+__device__ __forceinline__ uint32_t operand_at(uint32_t tile, int row, int chunk) {
+    return tile + (chunk >> 3) * (BN * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+
+// What an item's rows are: query tile i (0 or 1) holds tokens [first(i), last(i)] of the sequence.
+struct ItemRows {
+    int t0, t1;       // tokens of the item
+    int per;          // tokens of a query tile
+    bool turns;       // both query tiles hold the same rows
+    __device__ __forceinline__ ItemRows(const Segment& s, const WorkShape& w) {
+        t0 = s.qt * w.tokens;
+        t1 = min(t0 + w.tokens, s.n) - 1;
+        per = w.tokens / 2;
+        turns = t1 - t0 + 1 <= per;
+    }
+    __device__ __forceinline__ int first(int i) const { return turns ? t0 : t0 + i * per; }
+    __device__ __forceinline__ int last(int i) const { return turns ? t1 : min(t1, t0 + (i + 1) * per - 1); }
+};
+
+template <int FMT, int D>
+__global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_kernel(const __grid_constant__ AttnMaps maps, const AttnArgs a) {
+    using C = Chunk<FMT, D>;
+    constexpr int RAWS = C::CODES ? C::RAWS : 1;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t base = smem_u32(smem), bars = base + C::O_BARS;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+    auto bar = [&](int i) { return bars + (uint32_t)i * 8; };
+    volatile int* dead = reinterpret_cast<volatile int*>(smem + C::O_DEAD);
+    // Waits of whole warps.  When one runs out the block carries on without waiting: what it computes is void, and ends.
+    auto wait = [&](int b, uint32_t parity) {
+        uint32_t ok = mbar_try_wait(bar(b), parity);
+        if (__all_sync(0xffffffffu, ok)) return;
+        const long long t0 = clock64();
+        for (;;) {
+            if (!ok) ok = mbar_try_wait(bar(b), parity);
+            if (__all_sync(0xffffffffu, ok)) return;
+            if (__any_sync(0xffffffffu, *dead || clock64() - t0 > WAIT_CYCLES)) {
+                *dead = 1;
+                *a.status = 32;
+                return;
+            }
+        }
+    };
+    auto given_up = [&]() { return __any_sync(0xffffffffu, *dead) != 0; };
+    if (tid < C::BARS) {
+        const int b = tid;
+        int n = 1;
+        if (b < C::B_KEMPTY || (b >= C::B_VFULL && b < C::B_VEMPTY) || (b >= C::B_META && b < C::B_RFULL)) n = C::CODES ? 4 : 1;
+        if ((b >= C::B_REMPTY && b < C::B_S) || (b >= C::B_P && b < C::B_O)) n = 4;
+        mbar_init(bar(b), n);
+    }
+    if (tid == 0) *dead = 0;
+    mbar_init_fence();
+    if (warp == 8) tmem_alloc<false>(base + C::O_TMEM, 512);
+    tc_fence_before();
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + C::O_TMEM);
+
+    WorkShape w;
+    const int parts = (a.group + 127) / 128;   // parts of a cache head's query heads
+    w.group = (a.group + parts - 1) / parts;
+    w.tokens = 2 * (128 / w.group);
+    w.vheads = a.c.kv_heads * parts;
+    w.tile = BN;
+    w.window = a.window;
+    w.sinks = a.sinks;
+    long long chunk;
+    Walk walk = find_work(a.s, w, reinterpret_cast<WorkShared*>(smem + C::O_Q), 2, &chunk, a.status);
+    __syncthreads();
+    const int shift = a.c.page_shift;
+    const float scale2 = a.scale * 1.4426950408889634f;
+    int4* const info = a.items + blockIdx.x;   // for the kernel that joins the parts: what this block has begun and not finished
+    if (tid == 0) *info = make_int4(-1, 0, 0, 0);
+    Segment sg;
+
+    if (warp < 8) {
+        // ---- softmax of query tile i ----
+        const int i = warp >> 2, r = tid & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + T_S + i * BN + lanes, to = tmem + T_O + i * D + lanes;
+        const uint32_t qtile = base + C::O_Q + i * C::TILE;
+        uint32_t s_phase = 0, o_phase = 0;
+        int kt = 0;   // key tiles of the block so far
+        while (walk.next(a.s, w, &sg)) {
+            const ItemRows rows(sg, w);
+            const TileRange tr = sg.tiles(w);
+            const int kv_head = sg.vhead / parts, g = r % w.group, t = rows.first(i) + r / w.group, hg = (sg.vhead % parts) * w.group + g;
+            const bool on = r < rows.per * w.group && t <= rows.last(i) && hg < a.group;
+            const int row = sg.row0 + t, head = kv_head * a.group + hg, pos = on ? sg.len - sg.n + t : -1, lo = window_begin(pos < 0 ? 0 : pos, w.window);
+            // positions of the tile's first and last token
+            const int pmin = sg.len - sg.n + rows.first(i), pmax = sg.len - sg.n + rows.last(i), lo_max = window_begin(pmax < 0 ? 0 : pmax, w.window);
+            {
+                const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)row * a.q_stride + (int64_t)head * D);
+#pragma unroll
+                for (int ch = 0; ch < D / 8; ++ch) st_shared16(operand_at(qtile, r, ch), on ? src[ch] : make_uint4(0, 0, 0, 0));
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::B_Q + i));
+            }
+            float m = -INFINITY, l = 0.f;
+            bool first = true;
+            for (int j = rows.turns ? i : 0; j < sg.count; j += rows.turns ? 2 : 1) {
+                const int mt = (kt + j) % C::META;
+                wait(C::B_META + mt, ((kt + j) / C::META) & 1);
+                wait(C::B_S + i, s_phase);
+                s_phase ^= 1;
+                tc_fence_after();
+                const int k0 = sg.p1(w) < 0 ? 0 : tr.tile_at(sg.first + j) * BN;
+                const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + (kt + j) % C::HERE * 4);
+                const bool edge = here != 0xFFu || k0 + BN - 1 > pmin || (k0 < lo_max && k0 + BN > w.sinks);
+                const float4* ab = reinterpret_cast<const float4*>(smem + C::O_META + mt * C::META_BYTES);         // (a, b) of two keys
+                const float4* inv = reinterpret_cast<const float4*>(smem + C::O_META + mt * C::META_BYTES + BN * 8);
+                // score in powers of two, -infinity where the row does not see the key
+                auto score = [&](float s, float fa, float fb, int key) {
+                    float x = C::CODES ? fmaf(s, fa, fb) : s * scale2;
+                    if (edge && (!key_visible(k0 + key, pos, w.window, w.sinks) || !(here >> (key >> 4) & 1u))) x = -INFINITY;
+                    return x;
+                };
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int cb = 0; cb < 4; ++cb) {
+                    float s[32];
+                    tmem_ld32(ts + cb * 32, s);
+#pragma unroll
+                    for (int x = 0; x < 32; x += 2) {
+                        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (C::CODES) f = ab[(cb * 32 + x) / 2];
+                        top = fmaxf(top, fmaxf(score(s[x], f.x, f.y, cb * 32 + x), score(s[x + 1], f.z, f.w, cb * 32 + x + 1)));
+                    }
+                }
+                if (first) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
+                    // (the scores came after the product before, so the sums are complete)
+                    const float up = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2(m - up);
+                    m = up;
+                    l *= f;
+#pragma unroll 1
+                    for (int cb = 0; cb < D / 16; ++cb) {
+                        uint32_t o[16];
+                        tmem_ld16(to + cb * 16, o);
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                        tmem_st16(to + cb * 16, o);
+                    }
+                    tmem_wait_st();
+                }
+                first = false;
+                const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+                for (int cb = 0; cb < 4; ++cb) {
+                    float s[32];
+                    tmem_ld32(ts + cb * 32, s);
+                    uint32_t p[16];
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) {
+                        float4 f = make_float4(0.f, 0.f, 0.f, 0.f), f2 = f, n = f;
+                        if (C::CODES) {
+                            f = ab[(cb * 32 + x) / 2];
+                            f2 = ab[(cb * 32 + x) / 2 + 1];
+                            n = inv[(cb * 32 + x) / 4];
+                        }
+                        const float fa[4] = {f.x, f.z, f2.x, f2.z}, fb[4] = {f.y, f.w, f2.y, f2.w}, fn[4] = {n.x, n.y, n.z, n.w};
+                        float e[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) {
+                            const float sc = score(s[x + y], fa[y], fb[y], cb * 32 + x + y);
+                            e[y] = ex2(sc - ref);
+                            if (!C::CODES) l += e[y];
+                            else if (!edge || sc != -INFINITY) l = fmaf(e[y], fn[y], l);
+                        }
+                        p[x / 2] = floats_half2(e[0], e[1]);
+                        p[x / 2 + 1] = floats_half2(e[2], e[3]);
+                    }
+                    tmem_st16(ts + cb * 16, p);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::B_P + i));
+            }
+            kt += sg.count;
+
+            // ---- the segment's result ----
+            const bool mine = rows.turns ? i < sg.count : true;   // this tile has had keys
+            if (mine) {
+                wait(C::B_O + i, o_phase);
+                o_phase ^= 1;
+            }
+            float f0 = 1.f, f1 = 0.f;   // factors of this tile's sums and, where the tiles take turns, of the other's
+            if (rows.turns) {
+                float2* sums = reinterpret_cast<float2*>(smem + C::O_SUMS);
+                if (i == 1) sums[r] = make_float2(m, l);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                if (i == 0) {
+                    const float2 o = sums[r];
+                    const float up = fmaxf(m, o.x);
+                    f0 = m == -INFINITY ? 0.f : ex2(m - up);
+                    f1 = o.x == -INFINITY ? 0.f : ex2(o.x - up);
+                    l = l * f0 + o.y * f1;
+                    m = up;
+                }
+            }
+            tc_fence_after();
+            if (i == 0 || !rows.turns) {
+                const bool both = rows.turns && sg.count > 1, whole = sg.count == sg.total;
+                const float scale_out = whole ? 1.f / l : 1.f;
+                float4* part = reinterpret_cast<float4*>(a.parts) + (int64_t)(2 * blockIdx.x + (sg.first == 0 ? 1 : 0)) * (ATTN_CHUNK_PART / 16);
+                uint16_t* out = a.out + (int64_t)row * a.o_stride + (int64_t)head * D;
+                bool fine = l > 0.f && l < INFINITY;
+#pragma unroll 1
+                for (int pass = whole ? 0 : 1; pass < 2; ++pass) {   // whole items: first whether all is finite
+#pragma unroll 1
+                    for (int cb = 0; cb < D / 16; ++cb) {
+                        uint32_t o[16];
+                        float v[16];
+                        tmem_ld16(to + cb * 16, o);
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(o[x]) * f0;
+                        if (both) {
+                            tmem_ld16(to + D + cb * 16, o);
+#pragma unroll
+                            for (int x = 0; x < 16; ++x) v[x] = fmaf(__uint_as_float(o[x]), f1, v[x]);
+                        }
+                        if (!whole) {
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) part[(cb * 4 + x) * 256 + i * 128 + r] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+                            continue;
+                        }
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) {
+                            v[x] *= scale_out;
+                            fine = fine && fabsf(v[x]) < INFINITY;
+                        }
+                        if (pass == 1 && on && fine) {
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                                reinterpret_cast<uint4*>(out)[cb * 2 + x] = make_uint4(floats_half2(v[8 * x], v[8 * x + 1]), floats_half2(v[8 * x + 2], v[8 * x + 3]),
+                                                                                      floats_half2(v[8 * x + 4], v[8 * x + 5]), floats_half2(v[8 * x + 6], v[8 * x + 7]));
+                        }
+                    }
+                }
+                if (!whole) {
+                    reinterpret_cast<float2*>(part + 64 * D)[i * 128 + r] = make_float2(m, l);
+                    if (sg.first == 0 && tid == 0) *info = make_int4(sg.seq, sg.vhead, sg.qt, (int)((sg.unit0 + sg.total - 1) / chunk));
+                } else {
+                    // rows that are not finite, or see nothing: from the formula once more, which does not touch hidden cells
+                    for (unsigned left = __ballot_sync(0xffffffffu, on && !fine); left; left &= left - 1) {
+                        const int from = __ffs(left) - 1;
+                        const int r2 = __shfl_sync(0xffffffffu, row, from), h2 = __shfl_sync(0xffffffffu, head, from), p2 = __shfl_sync(0xffffffffu, pos, from);
+                        if (!attend_row<FMT, D>(a, sg.seq, sg.len, p2, r2, h2) && lane == 0) *a.status = STATUS_BAD_TABLE;
+                    }
+                }
+            }
+            tc_fence_before();
+            if (rows.turns) asm volatile("bar.sync 1, 256;" ::: "memory");   // (the other tile's sums have been read)
+        }
+    } else if (warp == 8) {
+        // ---- products ----
+        const bool issuer = elect_one();
+        const uint32_t id_s = instr_desc_f16(BN, 128), id_o = instr_desc_f16(D, 128) | IDESC_B_MN;
+        int kt = 0;
+        uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+        while (walk.next(a.s, w, &sg)) {
+            const bool turns = ItemRows(sg, w).turns;
+            const int n = sg.count;
+            auto second = [&](int i, int j) {   // out += weights V of tile j
+                wait(C::B_P + i, p_phase[i]);
+                p_phase[i] ^= 1;
+                const int slot = (kt + j) % C::RING;
+                wait(C::B_VFULL + slot, ((kt + j) / C::RING) & 1);
+                tc_fence_after();
+                if (issuer) {
+                    const uint32_t lo = desc_lo_mn(base + C::O_V + slot * C::TILE, BN * 128), ts = tmem + T_S + i * BN, to = tmem + T_O + i * D;
+                    const bool begin = turns ? j == i : j == 0;
+#pragma unroll
+                    for (int k = 0; k < BN / 16; ++k) umma_f16_ts<false>(to, ts + k * 8, desc_of(lo + k * 128), id_o, !(begin && k == 0));
+                    if (turns || i == 1) umma_commit<false>(bar(C::B_VEMPTY + slot));
+                }
+                __syncwarp();
+            };
+            for (int v = 0; v < (turns ? n : 2 * n); ++v) {
+                const int j = turns ? v : v >> 1, i = v & 1, before = turns ? j - 2 : j - 1;
+                if (before >= 0) second(i, before);
+                const int slot = (kt + j) % C::RING;
+                if (turns || i == 0) wait(C::B_KFULL + slot, ((kt + j) / C::RING) & 1);
+                if (before < 0) {
+                    wait(C::B_Q + i, q_phase[i]);
+                    q_phase[i] ^= 1;
+                }
+                tc_fence_after();
+                if (issuer) {
+                    const uint32_t qa = smem_desc_lo(base + C::O_Q + i * C::TILE), kb = smem_desc_lo(base + C::O_K + slot * C::TILE), ts = tmem + T_S + i * BN;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint32_t at = (k >> 2) * (BN * 128 / 16) + (k & 3) * 2;
+                        umma_f16<false>(ts, desc_of(qa + at), desc_of(kb + at), id_s, k > 0);
+                    }
+                    umma_commit<false>(bar(C::B_S + i));
+                    if (turns || i == 1) umma_commit<false>(bar(C::B_KEMPTY + slot));
+                }
+                __syncwarp();
+            }
+            if (turns && n == 1) {   // the second query tile has no keys: its queries' barrier moves on all the same
+                wait(C::B_Q + 1, q_phase[1]);
+                q_phase[1] ^= 1;
+            }
+            for (int e = 0; e < (turns && n == 1 ? 1 : 2); ++e) {   // what is still out, in the order of the values
+                const int tile = turns ? max(n - 2, 0) + e : n - 1, i = turns ? tile & 1 : e;
+                second(i, tile);
+                if (issuer) umma_commit<false>(bar(C::B_O + i));
+                __syncwarp();
+            }
+            kt += n;
+        }
+        if (issuer) umma_commit<false>(bar(C::B_DONE));
+        __syncwarp();
+        mbar_wait_bounded(bar(C::B_DONE), 0);
+    } else if (warp == 9) {
+        // ---- copies ----
+        const int box_keys = C::CODES ? min(C::RAW_KEYS, 1 << shift) : min(BN, 1 << shift), box_shift = 31 - __clz(box_keys), boxes = BN >> box_shift;
+        const uint64_t pol = l2_policy_evict_normal();
+        int kt = 0, raw = 0;
+        while (walk.next(a.s, w, &sg)) {
+            const TileRange tr = sg.tiles(w);
+            const int p0 = sg.p0(w), p1 = sg.p1(w), lo0 = window_begin(p0 < 0 ? 0 : p0, w.window), kv_head = sg.vhead / parts, n = sg.count;
+            auto key_of = [&](int j) { return p1 < 0 ? 0 : tr.tile_at(sg.first + j) * BN; };
+            // the page of box `lane` of tile j: -1 where no row sees any of it, -2 where the table is wrong
+            auto page_of = [&](int j) {
+                if (j >= n || lane >= boxes) return -1;
+                const int key = key_of(j) + lane * box_keys;
+                if (key > p1 || (key + box_keys <= lo0 && key >= w.sinks)) return -1;
+                const int page = a.s.page_table[(int64_t)sg.seq * a.s.table_stride + (key >> shift)];
+                return page_ok(page, a.c.num_pages) ? page : -2;
+            };
+            auto cells = [&](int j, int page) { return cell_row(page, kv_head, (key_of(j) + lane * box_keys) & ((1 << shift) - 1), a.c.kv_heads, shift); };
+            // 16-key granules of a tile that are copied
+            auto granules = [&](unsigned here) {
+                unsigned m = 0;
+                for (int b = 0; b < boxes; ++b) m |= (here >> b & 1u) ? ((1u << (box_keys / 16)) - 1u) << (b * (box_keys / 16)) : 0u;
+                return m;
+            };
+            auto copy = [&](int j, int page, bool value) {
+                if (page == -2) *a.status = STATUS_BAD_TABLE;
+                const bool in = page >= 0;
+                const unsigned here = __ballot_sync(0xffffffffu, in);
+                const int64_t row = in ? cells(j, page) : 0;
+                const int tile = kt + j;
+                if (!value && lane == 0) *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + (tile % C::HERE) * 4) = granules(here);
+                if (!C::CODES) {
+                    const int slot = tile % C::RING, full = (value ? C::B_VFULL : C::B_KFULL) + slot;
+                    wait((value ? C::B_VEMPTY : C::B_KEMPTY) + slot, ((tile / C::RING) & 1) ^ 1);
+                    if (given_up()) return;
+                    const uint32_t dst = base + (value ? C::O_V : C::O_K) + slot * C::TILE;
+                    // values that no row sees must not be NaN: their weights are 0.  Such a tile is put right here before it is handed on.
+                    const int k0 = key_of(j);
+                    const bool fix = value && (k0 + BN - 1 > p1 || (k0 < lo0 && k0 + BN > w.sinks) || granules(here) != 0xFFu);
+                    const uint32_t to = bar(fix ? C::B_FIX : full);
+                    if (lane == 0) mbar_arrive_expect_tx(to, (uint32_t)(__popc(here) * box_keys * D * 2));
+                    __syncwarp();
+                    if (in) {
+#pragma unroll
+                        for (int h = 0; h < C::HALVES; ++h)
+                            tma_load_2d(dst + h * (BN * 128) + lane * box_keys * 128, value ? &maps.v_tile : &maps.k_tile, h * 64, (int)row, to, pol);
+                    }
+                    if (fix) {
+                        wait(C::B_FIX, raw & 1);
+                        ++raw;
+                        const unsigned m = granules(here);
+                        for (int x = lane; x < BN * (D / 8); x += 32) {
+                            const int rr = x / (D / 8), key = k0 + rr;
+                            if (key > p1 || (key < lo0 && key >= w.sinks) || !(m >> (rr >> 4) & 1u)) st_shared16(operand_at(dst, rr, x % (D / 8)), make_uint4(0, 0, 0, 0));
+                        }
+                        fence_async_smem();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(bar(full));
+                    }
+                    if (!value && lane == 0) mbar_arrive(bar(C::B_META + tile % C::META));
+                } else {
+                    for (int half = 0; half < 2; ++half) {
+                        const int st = raw % RAWS;
+                        wait(C::B_REMPTY + st, ((raw / RAWS) & 1) ^ 1);
+                        if (given_up()) return;
+                        const bool now = in && (lane >> (6 - box_shift)) == half;   // boxes of this half of the keys
+                        const int cnt = __popc(__ballot_sync(0xffffffffu, now));
+                        const uint32_t full = bar(C::B_RFULL + st), dst = base + C::O_RAW + st * C::RAW_STAGE, at = lane * box_keys - half * C::RAW_KEYS;
+                        if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(cnt * box_keys * (D + (value ? 0 : 4))));
+                        __syncwarp();
+                        if (now) {
+                            bulk_g2s(dst + at * D, (const uint8_t*)(value ? a.c.v : a.c.k) + row * D, box_keys * D, full, pol);
+                            if (!value) {
+                                bulk_g2s(dst + C::RAW + at * 2, a.c.k_scale + row, box_keys * 2, full, pol);
+                                bulk_g2s(dst + C::RAW + 128 + at * 2, a.c.v_scale + row, box_keys * 2, full, pol);
+                            }
+                        }
+                        ++raw;
+                    }
+                }
+            };
+            // in the order in which they are used: K 0, K 1, then V j and K j + 2
+            int pages[3] = {page_of(0), page_of(1), page_of(2)};
+            copy(0, pages[0], false);
+            if (n > 1) copy(1, pages[1], false);
+            for (int j = 0; j < n; ++j) {
+                const int next = page_of(j + 3);
+                copy(j, pages[0], true);
+                if (j + 2 < n) copy(j + 2, pages[2], false);
+                pages[0] = pages[1];
+                pages[1] = pages[2];
+                pages[2] = next;
+            }
+            kt += n;
+        }
+        if (given_up()) {   // what was asked for must land before the block's memory is given back
+            if (C::CODES)
+                for (int i = raw < RAWS ? 0 : raw - RAWS; i < raw; ++i) mbar_wait_bounded(bar(C::B_RFULL + i % RAWS), (i / RAWS) & 1);
+            else
+                for (const long long t0 = clock64(); clock64() - t0 < WAIT_CYCLES;) {}   // (copies that a broken order left on either ring: time enough for any)
+        }
+    } else if (C::CODES) {
+        // ---- codes to operands ----
+        const int x0 = (warp - 10) * 32 + lane;
+        int kt = 0, raw = 0;
+        while (walk.next(a.s, w, &sg)) {
+            const TileRange tr = sg.tiles(w);
+            const int p0 = sg.p0(w), p1 = sg.p1(w), lo0 = window_begin(p0 < 0 ? 0 : p0, w.window), n = sg.count;
+            auto expand = [&](int j, bool value) {
+                const int tile = kt + j, slot = tile % C::RING, mt = tile % C::META;
+                const int k0 = p1 < 0 ? 0 : tr.tile_at(sg.first + j) * BN;
+                wait((value ? C::B_VEMPTY : C::B_KEMPTY) + slot, ((tile / C::RING) & 1) ^ 1);
+                const uint32_t dst = base + (value ? C::O_V : C::O_K) + slot * C::TILE;
+                for (int half = 0; half < 2; ++half) {
+                    const int st = raw % RAWS;
+                    wait(C::B_RFULL + st, (raw / RAWS) & 1);
+                    ++raw;
+                    const uint8_t* src = smem + C::O_RAW + st * C::RAW_STAGE;
+                    const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + tile % C::HERE * 4);
+                    const bool fix = value && (k0 + BN - 1 > p1 || (k0 < lo0 && k0 + BN > w.sinks) || here != 0xFFu);
+#pragma unroll 4
+                    for (int x = x0; x < C::RAW / 16; x += 128) {
+                        const int rr = half * C::RAW_KEYS + x / (D / 16), piece = x % (D / 16), key = k0 + rr;
+                        uint4 q = reinterpret_cast<const uint4*>(src)[x];
+                        // values that no row sees must not be NaN: their weights are 0
+                        if (fix && (key > p1 || (key < lo0 && key >= w.sinks) || !(here >> (rr >> 4) & 1u))) q = make_uint4(0, 0, 0, 0);
+                        uint4 lo, hi;
+                        codes_to_half2x2<FMT>(q.x, lo.x, lo.y);
+                        codes_to_half2x2<FMT>(q.y, lo.z, lo.w);
+                        codes_to_half2x2<FMT>(q.z, hi.x, hi.y);
+                        codes_to_half2x2<FMT>(q.w, hi.z, hi.w);
+                        // (the two columns of 64 dims share banks: neighbours take opposite pieces first)
+                        const bool swap = D == 128 && (piece & 4);
+                        st_shared16(operand_at(dst, rr, 2 * piece + (swap ? 1 : 0)), swap ? hi : lo);
+                        st_shared16(operand_at(dst, rr, 2 * piece + (swap ? 0 : 1)), swap ? lo : hi);
+                    }
+                    if (!value && x0 < C::RAW_KEYS) {
+                        const float ks = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW)[x0]), vs = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW + 128)[x0]);
+                        const int key = half * C::RAW_KEYS + x0;
+                        const float b = lg2(vs);
+                        reinterpret_cast<float2*>(smem + C::O_META + mt * C::META_BYTES)[key] = make_float2(ks * scale2, b);
+                        reinterpret_cast<float*>(smem + C::O_META + mt * C::META_BYTES + BN * 8)[key] = ex2(-b);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(C::B_REMPTY + st));
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar((value ? C::B_VFULL : C::B_KFULL) + slot));
+                    if (!value) mbar_arrive(bar(C::B_META + mt));
+                }
+            };
+            expand(0, false);
+            if (n > 1) expand(1, false);
+            for (int j = 0; j < n; ++j) {
+                expand(j, true);
+                if (j + 2 < n) expand(j + 2, false);
+            }
+            kt += n;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tmem_dealloc<false>(tmem, 512);
+}
+
+// Joins the parts of items that blocks share: block (b, y) the rows 32 y .. of the item that block b of the kernel above began and did not finish.
+constexpr int JOIN_THREADS = 256;
+template <int FMT, int D>
+__global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const AttnArgs a) {
+    pdl_launch_dependents();
+    pdl_wait_prior_grid();
+    const int b0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int4 it = a.items[b0];
+    if (it.x < 0) return;
+    WorkShape w;
+    const int parts = (a.group + 127) / 128;
+    w.group = (a.group + parts - 1) / parts;
+    w.tokens = 2 * (128 / w.group);
+    const SeqWork q = load_seq(a.s, w, it.x);
+    const int t0 = it.z * w.tokens, t1 = min(t0 + w.tokens, q.n) - 1, per = w.tokens / 2, r = blockIdx.y * 32 + lane, i = r >> 7;
+    const int t = t0 + i * per + (r & 127) / w.group, hg = (it.y % parts) * w.group + (r & 127) % w.group;
+    const bool on = (r & 127) < per * w.group && t <= min(t1, t0 + (i + 1) * per - 1) && hg < a.group;
+    if (!__syncthreads_or(on)) return;
+    const int row = q.row0 + t, head = it.y / parts * a.group + hg, pos = q.len - q.n + t;
+    const float4* base = reinterpret_cast<const float4*>(a.parts);
+    auto part = [&](int b) { return base + (int64_t)(2 * b + (b == b0 ? 1 : 0)) * (ATTN_CHUNK_PART / 16); };
+    float m = -INFINITY;
+    for (int b = b0; b <= it.w; ++b) m = fmaxf(m, reinterpret_cast<const float2*>(part(b) + 64 * D)[r].x);
+    constexpr int N = D / 32;   // quads of dims of a warp
+    float4 o[N] = {};
+    float l = 0.f;
+#pragma unroll 2
+    for (int b = b0; b <= it.w; ++b) {
+        const float4* p = part(b);
+        const float2 s = reinterpret_cast<const float2*>(p + 64 * D)[r];
+        float4 v[N];
+#pragma unroll
+        for (int x = 0; x < N; ++x) v[x] = p[(warp * N + x) * 256 + r];
+        const float f = s.x == -INFINITY ? 0.f : exp2f(s.x - m);
+        l += s.y * f;
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            o[x].x += v[x].x * f;
+            o[x].y += v[x].y * f;
+            o[x].z += v[x].z * f;
+            o[x].w += v[x].w * f;
+        }
+    }
+    const float inv = 1.f / l;
+    bool fine = l > 0.f && l < INFINITY;
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        o[x].x *= inv;
+        o[x].y *= inv;
+        o[x].z *= inv;
+        o[x].w *= inv;
+        fine = fine && fabsf(o[x].x) < INFINITY && fabsf(o[x].y) < INFINITY && fabsf(o[x].z) < INFINITY && fabsf(o[x].w) < INFINITY;
+    }
+    __shared__ unsigned bad[JOIN_THREADS / 32];
+    const unsigned mine = __ballot_sync(0xffffffffu, on && !fine);
+    if (lane == 0) bad[warp] = mine;
+    __syncthreads();
+    unsigned again = 0;
+#pragma unroll
+    for (int x = 0; x < JOIN_THREADS / 32; ++x) again |= bad[x];
+    if (on && !(again >> lane & 1u)) {
+        uint2* out = reinterpret_cast<uint2*>(a.out + (int64_t)row * a.o_stride + (int64_t)head * D) + warp * N;
+#pragma unroll
+        for (int x = 0; x < N; ++x) out[x] = make_uint2(floats_half2(o[x].x, o[x].y), floats_half2(o[x].z, o[x].w));
+    }
+    int k = 0;   // rows that are not finite, or see nothing: from the formula once more, a warp each
+    for (unsigned left = again; left; left &= left - 1, ++k) {
+        const int from = __ffs(left) - 1;
+        const int r2 = __shfl_sync(0xffffffffu, row, from), h2 = __shfl_sync(0xffffffffu, head, from), p2 = __shfl_sync(0xffffffffu, pos, from);
+        if (k % (JOIN_THREADS / 32) == warp && !attend_row<FMT, D>(a, it.x, q.len, p2, r2, h2) && lane == 0) *a.status = STATUS_BAD_TABLE;
+    }
+}
+
+template <int FMT, int D>
+cudaError_t launch(const AttnArgs& a, const AttnMaps& maps, int blocks, cudaStream_t st, bool pdl) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(Chunk<FMT, D>::THREADS);
+    cfg.dynamicSmemBytes = Chunk<FMT, D>::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, attention_chunk_kernel<FMT, D>, maps, a);
+    if (e != cudaSuccess) return e;
+    cfg.gridDim = dim3((unsigned)blocks, 8);
+    cfg.blockDim = dim3(JOIN_THREADS);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, attention_join_kernel<FMT, D>, a);
+}
+
+template <int FMT, int D>
+cudaError_t configure() {
+    return cudaFuncSetAttribute(attention_chunk_kernel<FMT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Chunk<FMT, D>::SMEM);
+}
+
+}  // namespace
+
+cudaError_t attention_chunk_configure() {
+    cudaError_t e;
+    if ((e = configure<KV_FP16, 64>()) != cudaSuccess || (e = configure<KV_FP16, 128>()) != cudaSuccess || (e = configure<KV_INT8, 64>()) != cudaSuccess ||
+        (e = configure<KV_INT8, 128>()) != cudaSuccess || (e = configure<KV_FP8, 64>()) != cudaSuccess)
+        return e;
+    return configure<KV_FP8, 128>();
+}
+
+cudaError_t launch_attention_chunk(const AttnArgs& a, const AttnMaps& maps, int sm_count, cudaStream_t st, bool pdl) {
+    const int blocks = sm_count < ATTN_MAX_BLOCKS ? sm_count : ATTN_MAX_BLOCKS;
+    if (a.c.fmt == KV_FP16) return a.c.dim == 64 ? launch<KV_FP16, 64>(a, maps, blocks, st, pdl) : launch<KV_FP16, 128>(a, maps, blocks, st, pdl);
+    if (a.c.fmt == KV_INT8) return a.c.dim == 64 ? launch<KV_INT8, 64>(a, maps, blocks, st, pdl) : launch<KV_INT8, 128>(a, maps, blocks, st, pdl);
+    return a.c.dim == 64 ? launch<KV_FP8, 64>(a, maps, blocks, st, pdl) : launch<KV_FP8, 128>(a, maps, blocks, st, pdl);
+}
+
+}  // namespace nnb

@@ -10,11 +10,15 @@ namespace nnb {
 struct AttnMaps {
     alignas(64) CUtensorMap k;
     alignas(64) CUtensorMap v;
+    alignas(64) CUtensorMap k_tile;   // fp16: for the operands of the tensor cores
+    alignas(64) CUtensorMap v_tile;
 };
-bool encode_attention_maps(const KvView& c, AttnMaps* decode);
+bool encode_attention_maps(const KvView& c, AttnMaps* maps);
 
 int attention_decode_keys(int fmt, int dim);   // keys of a stage: what a copy takes, if a page is that long
 cudaError_t attention_decode_configure();
 cudaError_t launch_attention_decode(const AttnArgs& a, const AttnMaps& maps, int sm_count, cudaStream_t st, bool pdl);
+cudaError_t attention_chunk_configure();
+cudaError_t launch_attention_chunk(const AttnArgs& a, const AttnMaps& maps, int sm_count, cudaStream_t st, bool pdl);
 
 }  // namespace nnb

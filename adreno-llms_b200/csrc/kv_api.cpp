@@ -33,17 +33,17 @@ static size_t cache_bytes(const KvView& v) {
 
 // The partial results of items that several blocks share: one buffer for all calls of the context, which run one after the other.
 static int attention_workspace(nn_context* c) {
-    if (c->attn_parts) return NN_OK;
+    if (c->attn_work) return NN_OK;
     if (c->capturing) return NN_FAIL(NN_ERR_UNSUPPORTED, "nn_kv_cache_create: the context's first cache cannot be made while a plan is being recorded");
     CUDA_TRY(attention_configure());
-    void* parts = nullptr;
-    CUDA_TRY(cudaMalloc(&parts, ATTN_PARTS_BYTES + ATTN_COUNTER_BYTES));
-    const cudaError_t e = cudaMemset((char*)parts + ATTN_PARTS_BYTES, 0, ATTN_COUNTER_BYTES);
+    void* work = nullptr;
+    CUDA_TRY(cudaMalloc(&work, attention_workspace_bytes(c->sm_count)));
+    const cudaError_t e = cudaMemset(work, 0, ATTN_HEAD_BYTES);
     if (e != cudaSuccess) {
-        cudaFree(parts);
+        cudaFree(work);
         return NN_FAIL(NN_ERR_CUDA, "nn_kv_cache_create: %s", cudaGetErrorString(e));
     }
-    c->attn_parts = parts;
+    c->attn_work = work;
     return NN_OK;
 }
 
@@ -158,7 +158,7 @@ static int take_batch(nn_context* c, const nn_kv_cache* h, const nn_kv_batch* b,
 // Last of the checks (the others need no GPU).  The calling thread may have another device current.
 static int make_current(nn_context* c, const nn_kv_cache* h, const char* who) {
     if (!c) return NN_FAIL(NN_ERR_ARG, "%s: null context", who);
-    if (!c->attn_parts) {   // a context that has made no cache of its own
+    if (!c->attn_work) {   // a context that has made no cache of its own
         const int rc = attention_workspace(c);
         if (rc) return rc;
     }
@@ -290,8 +290,9 @@ extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b,
     if ((rc = make_current(c, h, who))) return rc;
     a.status = c->status_dev;
     ProfScope prof(c, [&] { return std::string("attention_") + kv_name(a.c.fmt) + "_seqs" + std::to_string(b->num_seqs) + "_rows" + std::to_string(b->num_rows); });
-    a.parts = c->attn_parts;
-    a.counters = (unsigned*)((char*)c->attn_parts + ATTN_PARTS_BYTES);
+    a.counters = (unsigned*)c->attn_work;
+    a.items = (int4*)((char*)c->attn_work + ATTN_COUNTER_BYTES);
+    a.parts = (char*)c->attn_work + ATTN_HEAD_BYTES;
     const cudaError_t e = launch_attention(a, h->maps, b->max_new, c->sm_count, c->stream, c->use_pdl);
     if (e != cudaSuccess) return NN_FAIL(NN_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     c->in_flight.wrote(out, rows_bytes(ro, b->num_rows));
