@@ -16,6 +16,8 @@
 //   * warps 10-13, 8-bit cells only: codes to fp16 operands, and the keys' factors.
 // The exponentials bound it next to the products: 128 x 128 scores take 1024 clocks of the SM's exponential units and D * 8 clocks of
 // its tensor cores for both products.
+#include <type_traits>
+
 #include "attention_maps.h"
 #include "attention_row.cuh"
 #include "attention_work.cuh"
@@ -42,7 +44,7 @@ struct Chunk {
     static constexpr int THREADS = CODES ? 448 : 320;
     // shared memory
     static constexpr int O_Q = 0, O_K = O_Q + 2 * TILE, O_V = O_K + RING * TILE, O_RAW = O_V + RING * TILE, O_META = O_RAW + RAWS * RAW_STAGE;
-    static constexpr int META_BYTES = CODES ? BN * 12 : 0;       // a: factor of the score, b: its summand, 1 / scale of the value
+    static constexpr int META_BYTES = CODES ? BN * 12 : 0;       // factors of the scores, their summands, 1 / scale of the values
     static constexpr int O_HERE = O_META + META * META_BYTES, O_SUMS = O_HERE + HERE * 4, O_BARS = O_SUMS + BN * 8;
     static constexpr int B_KFULL = 0, B_KEMPTY = B_KFULL + RING, B_VFULL = B_KEMPTY + RING, B_VEMPTY = B_VFULL + RING, B_META = B_VEMPTY + RING,
                          B_RFULL = B_META + META, B_REMPTY = B_RFULL + RAWS, B_Q = B_REMPTY + RAWS, B_S = B_Q + 2, B_P = B_S + 2, B_O = B_P + 2, B_FIX = B_O + 2, B_DONE = B_FIX + 1,
@@ -64,8 +66,8 @@ __device__ __forceinline__ float lg2(float x) {
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {
-    uint32_t u[32];
+// 32 columns of this thread's lane; the registers are valid after tmem_wait_ld32.
+__device__ __forceinline__ void tmem_ld32_begin(uint32_t taddr, uint32_t (&u)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
@@ -73,14 +75,50 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&r)[32]) {
           "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]), "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]),
           "=r"(u[23]), "=r"(u[24]), "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
         : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t (&u)[32]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]), "+r"(u[9]), "+r"(u[10]), "+r"(u[11]),
                    "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15]), "+r"(u[16]), "+r"(u[17]), "+r"(u[18]), "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]),
                    "+r"(u[23]), "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]), "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])
                  :: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) r[i] = __uint_as_float(u[i]);
 }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&u)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]),
+          "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]),
+          "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
+        : "memory");
+}
+
+// Two 32-bit values in one instruction
+__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t pair(float a, float b) { return pair(__float_as_uint(a), __float_as_uint(b)); }
+__device__ __forceinline__ void unpair(uint64_t d, uint32_t& a, uint32_t& b) { asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Bits [0, n) of 32
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+
 // An operand whose N dimension lies together (V: dims of a key): tiles of 64 dims x 8 keys; the leading offset is the distance of
 // two 64-dim columns, the stride that of two groups of 8 keys (1024 bytes).
 __device__ __forceinline__ uint32_t desc_lo_mn(uint32_t saddr, uint32_t column_bytes) { return ((saddr >> 4) & 0x3FFFu) | ((column_bytes >> 4) << 16); }
@@ -203,26 +241,50 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 const int k0 = sg.p1(w) < 0 ? 0 : tr.tile_at(sg.first + j) * BN;
                 const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + (kt + j) % C::HERE * 4);
                 const bool edge = here != 0xFFu || k0 + BN - 1 > pmin || (k0 < lo_max && k0 + BN > w.sinks);
-                const float4* ab = reinterpret_cast<const float4*>(smem + C::O_META + mt * C::META_BYTES);         // (a, b) of two keys
-                const float4* inv = reinterpret_cast<const float4*>(smem + C::O_META + mt * C::META_BYTES + BN * 8);
-                // score in powers of two, -infinity where the row does not see the key
-                auto score = [&](float s, float fa, float fb, int key) {
-                    float x = C::CODES ? fmaf(s, fa, fb) : s * scale2;
-                    if (edge && (!key_visible(k0 + key, pos, w.window, w.sinks) || !(here >> (key >> 4) & 1u))) x = -INFINITY;
-                    return x;
-                };
+                const float4* fa = reinterpret_cast<const float4*>(smem + C::O_META + mt * C::META_BYTES);   // factors of four keys' scores
+                const float4 *fb = fa + BN / 4, *inv = fb + BN / 4;                                         // their summands; 1 / scale of the values
+                // First pass: the maximum.  Scores that do not go on as they are go back to their place: with their factors as powers of two, and
+                // -infinity where the row does not see the key.
                 float top = -INFINITY;
-#pragma unroll 1
-                for (int cb = 0; cb < 4; ++cb) {
-                    float s[32];
-                    tmem_ld32(ts + cb * 32, s);
+                auto find_top = [&](auto masked_) {
+                    constexpr bool masked = decltype(masked_)::value;
+                    uint32_t s[2][32];
+                    tmem_ld32_begin(ts, s[0]);
 #pragma unroll
-                    for (int x = 0; x < 32; x += 2) {
-                        float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (C::CODES) f = ab[(cb * 32 + x) / 2];
-                        top = fmaxf(top, fmaxf(score(s[x], f.x, f.y, cb * 32 + x), score(s[x + 1], f.z, f.w, cb * 32 + x + 1)));
+                    for (int cb = 0; cb < 4; ++cb) {
+                        uint32_t(&v)[32] = s[cb & 1];
+                        tmem_wait_ld32(v);
+                        if (cb < 3) tmem_ld32_begin(ts + (cb + 1) * 32, s[(cb + 1) & 1]);
+                        if (C::CODES) {
+#pragma unroll
+                            for (int x = 0; x < 8; ++x) {
+                                const float4 f = fa[cb * 8 + x], b = fb[cb * 8 + x];
+                                unpair(fma2(pair(v[4 * x], v[4 * x + 1]), pair(f.x, f.y), pair(b.x, b.y)), v[4 * x], v[4 * x + 1]);
+                                unpair(fma2(pair(v[4 * x + 2], v[4 * x + 3]), pair(f.z, f.w), pair(b.z, b.w)), v[4 * x + 2], v[4 * x + 3]);
+                            }
+                        }
+                        if (masked) {
+                            const int at = k0 + cb * 32;
+                            uint32_t seen = low_bits(pos + 1 - at) & (~low_bits(lo - at) | low_bits(w.sinks - at));
+                            seen &= ((here >> (2 * cb) & 1u) ? 0xFFFFu : 0u) | ((here >> (2 * cb + 1) & 1u) ? 0xFFFF0000u : 0u);
+#pragma unroll
+                            for (int x = 0; x < 32; ++x)
+                                if (!(seen >> x & 1u)) v[x] = 0xFF800000u;
+                        }
+                        if (C::CODES || masked) tmem_st32(ts + cb * 32, v);
+                        float t0 = top, t1 = -INFINITY;
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4) {
+                            t0 = max3(t0, __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
+                            t1 = max3(t1, __uint_as_float(v[x + 2]), __uint_as_float(v[x + 3]));
+                        }
+                        top = fmaxf(t0, t1);
                     }
-                }
+                    if (C::CODES || masked) tmem_wait_st();
+                };
+                if (edge) find_top(std::true_type());
+                else find_top(std::false_type());
+                if (!C::CODES) top *= scale2;
                 if (first) {
                     m = top;
                 } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
@@ -241,33 +303,46 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     tmem_wait_st();
                 }
                 first = false;
-                const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-                for (int cb = 0; cb < 4; ++cb) {
-                    float s[32];
-                    tmem_ld32(ts + cb * 32, s);
-                    uint32_t p[16];
+                // Second pass: the weights
+                {
+                    const float ref = m == -INFINITY ? 0.f : -m;
+                    const uint64_t ref2 = pair(ref, ref), mul2 = pair(scale2, scale2);
+                    uint64_t sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+                    uint32_t s[2][32];
+                    tmem_ld32_begin(ts, s[0]);
 #pragma unroll
-                    for (int x = 0; x < 32; x += 4) {
-                        float4 f = make_float4(0.f, 0.f, 0.f, 0.f), f2 = f, n = f;
-                        if (C::CODES) {
-                            f = ab[(cb * 32 + x) / 2];
-                            f2 = ab[(cb * 32 + x) / 2 + 1];
-                            n = inv[(cb * 32 + x) / 4];
-                        }
-                        const float fa[4] = {f.x, f.z, f2.x, f2.z}, fb[4] = {f.y, f.w, f2.y, f2.w}, fn[4] = {n.x, n.y, n.z, n.w};
-                        float e[4];
+                    for (int cb = 0; cb < 4; ++cb) {
+                        uint32_t(&v)[32] = s[cb & 1];
+                        tmem_wait_ld32(v);
+                        if (cb < 3) tmem_ld32_begin(ts + (cb + 1) * 32, s[(cb + 1) & 1]);
+                        uint32_t p[16];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            const float sc = score(s[x + y], fa[y], fb[y], cb * 32 + x + y);
-                            e[y] = ex2(sc - ref);
-                            if (!C::CODES) l += e[y];
-                            else if (!edge || sc != -INFINITY) l = fmaf(e[y], fn[y], l);
+                        for (int x = 0; x < 8; ++x) {
+                            float e[4];
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint64_t sc = pair(v[4 * x + 2 * h], v[4 * x + 2 * h + 1]);
+                                uint32_t u0, u1;
+                                unpair(C::CODES ? add2(sc, ref2) : fma2(sc, mul2, ref2), u0, u1);
+                                e[2 * h] = ex2(__uint_as_float(u0));
+                                e[2 * h + 1] = ex2(__uint_as_float(u1));
+                            }
+                            if (C::CODES) {
+                                const float4 n = inv[cb * 8 + x];
+                                sum2[0] = fma2(pair(e[0], e[1]), pair(n.x, n.y), sum2[0]);
+                                sum2[1] = fma2(pair(e[2], e[3]), pair(n.z, n.w), sum2[1]);
+                            } else {
+                                sum2[0] = add2(sum2[0], pair(e[0], e[1]));
+                                sum2[1] = add2(sum2[1], pair(e[2], e[3]));
+                            }
+                            p[2 * x] = floats_half2(e[0], e[1]);
+                            p[2 * x + 1] = floats_half2(e[2], e[3]);
                         }
-                        p[x / 2] = floats_half2(e[0], e[1]);
-                        p[x / 2 + 1] = floats_half2(e[2], e[3]);
+                        tmem_st16(ts + cb * 16, p);
                     }
-                    tmem_st16(ts + cb * 16, p);
+                    uint32_t u0, u1;
+                    unpair(add2(sum2[0], sum2[1]), u0, u1);
+                    l += __uint_as_float(u0) + __uint_as_float(u1);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -550,9 +625,13 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     if (!value && x0 < C::RAW_KEYS) {
                         const float ks = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW)[x0]), vs = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW + 128)[x0]);
                         const int key = half * C::RAW_KEYS + x0;
-                        const float b = lg2(vs);
-                        reinterpret_cast<float2*>(smem + C::O_META + mt * C::META_BYTES)[key] = make_float2(ks * scale2, b);
-                        reinterpret_cast<float*>(smem + C::O_META + mt * C::META_BYTES + BN * 8)[key] = ex2(-b);
+                        // (the scales of keys that no row sees may be anything)
+                        const bool seen = k0 + key <= p1 && (k0 + key >= lo0 || k0 + key < w.sinks) && (here >> (key >> 4) & 1u);
+                        const float b = seen ? lg2(vs) : 0.f;
+                        float* meta = reinterpret_cast<float*>(smem + C::O_META + mt * C::META_BYTES) + key;
+                        meta[0] = seen ? ks * scale2 : 1.f;
+                        meta[BN] = b;
+                        meta[2 * BN] = ex2(-b);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar(C::B_REMPTY + st));
