@@ -7,13 +7,14 @@
 // An item is up to 256 query rows: two tiles of 128, each new tokens times the query heads of a cache head, so that a cell is
 // fetched once for all heads that share it.  With no more than 128 rows the two tiles hold the same rows and take the key tiles in turn.
 // A block is one of each SM:
-//   * warps 0-3 and 4-7: the softmax of one query tile each, a thread per row: scores come from tensor memory, the weights go back there
-//     as fp16 in the scores' place (the A operand of the second product).  The sums of outputs stay in tensor memory and
-//     are scaled again only when a row's maximum has grown by more than 2^8.
-//   * warp 8: issues all tcgen05.mma: scores = Q K^T (both K-major), out += weights V (V as it lies in the cache, MN-major).  While one
+//   * warps 0-7 and 8-15: the softmax of one query tile each, two threads per row, 64 keys each (one thread per row left two warps to a
+//     scheduler, which were idle half of the time on each other's latencies: 3500 clocks for a pair of tiles of 64 dims, ... here): scores come
+//     from tensor memory, the weights go back there as fp16 in the scores' place (the A operand of the second product).  The sums of outputs stay
+//     in tensor memory and are scaled again only when a row's maximum has grown by more than 2^8.
+//   * warp 16: issues all tcgen05.mma: scores = Q K^T (both K-major), out += weights V (V as it lies in the cache, MN-major).  While one
 //     query tile is in its softmax the other one has the tensor cores.
-//   * warp 9: tensor copies (fp16: straight into the operands; 8-bit: codes into a ring of half tiles).
-//   * warps 10-13, 8-bit cells only: codes to fp16 operands, and the keys' factors.
+//   * warp 17: tensor copies (fp16: straight into the operands; 8-bit: codes into a ring of half tiles).
+//   * warps 20-23, 8-bit cells only: codes to fp16 operands, and the keys' factors.
 // The exponentials bound it next to the products: 128 x 128 scores take 1024 clocks of the SM's exponential units and D * 8 clocks of
 // its tensor cores for both products.
 #include <type_traits>
@@ -41,11 +42,11 @@ struct Chunk {
     static constexpr int RAW_KEYS = 64, RAW = RAW_KEYS * D;      // half tiles of codes
     static constexpr int RAW_STAGE = RAW + 256;                  // with the scales of keys and values
     static constexpr int RAWS = CODES ? (D == 64 ? 6 : 3) : 0;
-    static constexpr int THREADS = CODES ? 448 : 320;
+    static constexpr int THREADS = CODES ? 768 : 640;
     // shared memory
     static constexpr int O_Q = 0, O_K = O_Q + 2 * TILE, O_V = O_K + RING * TILE, O_RAW = O_V + RING * TILE, O_META = O_RAW + RAWS * RAW_STAGE;
     static constexpr int META_BYTES = CODES ? BN * 12 : 0;       // factors of the scores, their summands, 1 / scale of the values
-    static constexpr int O_HERE = O_META + META * META_BYTES, O_SUMS = O_HERE + HERE * 4, O_BARS = O_SUMS + BN * 8;
+    static constexpr int O_HERE = O_META + META * META_BYTES, O_SUMS = O_HERE + HERE * 4, O_BARS = O_SUMS + 5 * BN * 4;
     static constexpr int B_KFULL = 0, B_KEMPTY = B_KFULL + RING, B_VFULL = B_KEMPTY + RING, B_VEMPTY = B_VFULL + RING, B_META = B_VEMPTY + RING,
                          B_RFULL = B_META + META, B_REMPTY = B_RFULL + RAWS, B_Q = B_REMPTY + RAWS, B_S = B_Q + 2, B_P = B_S + 2, B_O = B_P + 2, B_FIX = B_O + 2, B_DONE = B_FIX + 1,
                          BARS = B_DONE + 1;
@@ -147,6 +148,15 @@ struct ItemRows {
     __device__ __forceinline__ int last(int i) const { return turns ? t1 : min(t1, t0 + (i + 1) * per - 1); }
 };
 
+// Two warps (named barrier `id`): wait for each other; and whether any of their threads says yes.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ bool pair_any(int id, bool yes) {
+    int r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, %2, 64, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"((int)yes), "r"(id) : "memory");
+    return r != 0;
+}
+
 template <int FMT, int D>
 __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_kernel(const __grid_constant__ AttnMaps maps, const AttnArgs a) {
     using C = Chunk<FMT, D>;
@@ -177,12 +187,13 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         const int b = tid;
         int n = 1;
         if (b < C::B_KEMPTY || (b >= C::B_VFULL && b < C::B_VEMPTY) || (b >= C::B_META && b < C::B_RFULL)) n = C::CODES ? 4 : 1;
-        if ((b >= C::B_REMPTY && b < C::B_S) || (b >= C::B_P && b < C::B_O)) n = 4;
+        if (b >= C::B_REMPTY && b < C::B_Q) n = 4;
+        if ((b >= C::B_Q && b < C::B_S) || (b >= C::B_P && b < C::B_O)) n = 8;
         mbar_init(bar(b), n);
     }
     if (tid == 0) *dead = 0;
     mbar_init_fence();
-    if (warp == 8) tmem_alloc<false>(base + C::O_TMEM, 512);
+    if (warp == 16) tmem_alloc<false>(base + C::O_TMEM, 512);
     tc_fence_before();
     pdl_launch_dependents();
     pdl_wait_prior_grid();
@@ -207,10 +218,13 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     if (tid == 0) *info = make_int4(-1, 0, 0, 0);
     Segment sg;
 
-    if (warp < 8) {
-        // ---- softmax of query tile i ----
-        const int i = warp >> 2, r = tid & 127;
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + T_S + i * BN + lanes, to = tmem + T_O + i * D + lanes;
+    if (warp < 16) {
+        // ---- softmax of query tile i, keys 64 c .. of a tile; row r ----
+        const int i = warp >> 3, c = warp >> 2 & 1, r = tid & 127, pair_bar = 1 + i * 4 + (warp & 3);
+        // What the threads of a row tell each other: [tile][half of the keys][row], and behind it the references of the second tile.
+        volatile float* const said = reinterpret_cast<volatile float*>(smem + C::O_SUMS) + r;
+        volatile float *const other = said + (i * 2 + (c ^ 1)) * BN, *const own = said + (i * 2 + c) * BN;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + T_S + i * BN + c * 64 + lanes, to = tmem + T_O + i * D + c * (D / 2) + lanes;
         const uint32_t qtile = base + C::O_Q + i * C::TILE;
         uint32_t s_phase = 0, o_phase = 0;
         int kt = 0;   // key tiles of the block so far
@@ -225,7 +239,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             {
                 const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)row * a.q_stride + (int64_t)head * D);
 #pragma unroll
-                for (int ch = 0; ch < D / 8; ++ch) st_shared16(operand_at(qtile, r, ch), on ? src[ch] : make_uint4(0, 0, 0, 0));
+                for (int ch = c * (D / 16); ch < (c + 1) * (D / 16); ++ch) st_shared16(operand_at(qtile, r, ch), on ? src[ch] : make_uint4(0, 0, 0, 0));
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(C::B_Q + i));
@@ -241,20 +255,18 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 const int k0 = sg.p1(w) < 0 ? 0 : tr.tile_at(sg.first + j) * BN;
                 const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + (kt + j) % C::HERE * 4);
                 const bool edge = here != 0xFFu || k0 + BN - 1 > pmin || (k0 < lo_max && k0 + BN > w.sinks);
-                const float4* fa = reinterpret_cast<const float4*>(smem + C::O_META + mt * C::META_BYTES);   // factors of four keys' scores
-                const float4 *fb = fa + BN / 4, *inv = fb + BN / 4;                                         // their summands; 1 / scale of the values
+                const float4* fa = reinterpret_cast<const float4*>(smem + C::O_META + mt * C::META_BYTES) + c * 16;   // factors of four keys' scores
+                const float4 *fb = fa + BN / 4, *inv = fb + BN / 4;                                                  // their summands; 1 / scale of the values
                 // First pass: the maximum.  Scores that do not go on as they are go back to their place: with their factors as powers of two, and
                 // -infinity where the row does not see the key.
                 float top = -INFINITY;
                 auto find_top = [&](auto masked_) {
                     constexpr bool masked = decltype(masked_)::value;
-                    uint32_t s[2][32];
-                    tmem_ld32_begin(ts, s[0]);
 #pragma unroll
-                    for (int cb = 0; cb < 4; ++cb) {
-                        uint32_t(&v)[32] = s[cb & 1];
+                    for (int cb = 0; cb < 2; ++cb) {
+                        uint32_t v[32];
+                        tmem_ld32_begin(ts + cb * 32, v);
                         tmem_wait_ld32(v);
-                        if (cb < 3) tmem_ld32_begin(ts + (cb + 1) * 32, s[(cb + 1) & 1]);
                         if (C::CODES) {
 #pragma unroll
                             for (int x = 0; x < 8; ++x) {
@@ -264,9 +276,10 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                             }
                         }
                         if (masked) {
-                            const int at = k0 + cb * 32;
+                            const int at = k0 + c * 64 + cb * 32;
                             uint32_t seen = low_bits(pos + 1 - at) & (~low_bits(lo - at) | low_bits(w.sinks - at));
-                            seen &= ((here >> (2 * cb) & 1u) ? 0xFFFFu : 0u) | ((here >> (2 * cb + 1) & 1u) ? 0xFFFF0000u : 0u);
+                            const unsigned there = here >> (4 * c + 2 * cb);
+                            seen &= ((there & 1u) ? 0xFFFFu : 0u) | ((there & 2u) ? 0xFFFF0000u : 0u);
 #pragma unroll
                             for (int x = 0; x < 32; ++x)
                                 if (!(seen >> x & 1u)) v[x] = 0xFF800000u;
@@ -285,22 +298,24 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 if (edge) find_top(std::true_type());
                 else find_top(std::false_type());
                 if (!C::CODES) top *= scale2;
-                if (first) {
-                    m = top;
-                } else if (__any_sync(0xffffffffu, top > m + 8.f)) {
-                    // (the scores came after the product before, so the sums are complete)
-                    const float up = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2(m - up);
+                // Both threads of a row keep the same reference: they agree whether some row of their two warps wants another one.
+                if (pair_any(pair_bar, first || top > m + 8.f)) {
+                    *own = top;
+                    pair_sync(pair_bar);
+                    const float up = fmaxf(m, fmaxf(top, *other)), f = m == -INFINITY ? 0.f : ex2(m - up);
                     m = up;
-                    l *= f;
+                    if (!first) {   // (the scores came after the product before, so the sums are complete)
+                        l *= f;
 #pragma unroll 1
-                    for (int cb = 0; cb < D / 16; ++cb) {
-                        uint32_t o[16];
-                        tmem_ld16(to + cb * 16, o);
+                        for (int cb = 0; cb < D / 32; ++cb) {
+                            uint32_t o[16];
+                            tmem_ld16(to + cb * 16, o);
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                        tmem_st16(to + cb * 16, o);
+                            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                            tmem_st16(to + cb * 16, o);
+                        }
+                        tmem_wait_st();
                     }
-                    tmem_wait_st();
                 }
                 first = false;
                 // Second pass: the weights
@@ -308,14 +323,11 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     const float ref = m == -INFINITY ? 0.f : -m;
                     const uint64_t ref2 = pair(ref, ref), mul2 = pair(scale2, scale2);
                     uint64_t sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-                    uint32_t s[2][32];
-                    tmem_ld32_begin(ts, s[0]);
 #pragma unroll
-                    for (int cb = 0; cb < 4; ++cb) {
-                        uint32_t(&v)[32] = s[cb & 1];
+                    for (int cb = 0; cb < 2; ++cb) {
+                        uint32_t v[32], p[16];
+                        tmem_ld32_begin(ts + cb * 32, v);
                         tmem_wait_ld32(v);
-                        if (cb < 3) tmem_ld32_begin(ts + (cb + 1) * 32, s[(cb + 1) & 1]);
-                        uint32_t p[16];
 #pragma unroll
                         for (int x = 0; x < 8; ++x) {
                             float e[4];
@@ -358,30 +370,35 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 o_phase ^= 1;
             }
             float f0 = 1.f, f1 = 0.f;   // factors of this tile's sums and, where the tiles take turns, of the other's
-            if (rows.turns) {
-                float2* sums = reinterpret_cast<float2*>(smem + C::O_SUMS);
-                if (i == 1) sums[r] = make_float2(m, l);
-                asm volatile("bar.sync 1, 256;" ::: "memory");
-                if (i == 0) {
-                    const float2 o = sums[r];
-                    const float up = fmaxf(m, o.x);
-                    f0 = m == -INFINITY ? 0.f : ex2(m - up);
-                    f1 = o.x == -INFINITY ? 0.f : ex2(o.x - up);
-                    l = l * f0 + o.y * f1;
-                    m = up;
-                }
+            *own = l;
+            if (rows.turns && i == 1) said[4 * BN] = m;
+            if (rows.turns) asm volatile("bar.sync 9, 512;" ::: "memory");
+            else pair_sync(pair_bar);
+            l += *other;
+            if (rows.turns && i == 0) {
+                const float m1 = said[4 * BN], up = fmaxf(m, m1);
+                f0 = m == -INFINITY ? 0.f : ex2(m - up);
+                f1 = m1 == -INFINITY ? 0.f : ex2(m1 - up);
+                l = l * f0 + (said[2 * BN] + said[3 * BN]) * f1;
+                m = up;
             }
             tc_fence_after();
             if (i == 0 || !rows.turns) {
                 const bool both = rows.turns && sg.count > 1, whole = sg.count == sg.total;
                 const float scale_out = whole ? 1.f / l : 1.f;
                 float4* part = reinterpret_cast<float4*>(a.parts) + (int64_t)(2 * blockIdx.x + (sg.first == 0 ? 1 : 0)) * (ATTN_CHUNK_PART / 16);
-                uint16_t* out = a.out + (int64_t)row * a.o_stride + (int64_t)head * D;
+                uint16_t* out = a.out + (int64_t)row * a.o_stride + (int64_t)head * D + c * (D / 2);
                 bool fine = l > 0.f && l < INFINITY;
 #pragma unroll 1
-                for (int pass = whole ? 0 : 1; pass < 2; ++pass) {   // whole items: first whether all is finite
+                for (int pass = whole ? 0 : 1; pass < 2; ++pass) {   // whole items: first whether all of the row is finite
+                    if (whole && pass == 1) {
+                        pair_sync(pair_bar);   // (the sums have been read)
+                        *own = fine ? 0.f : 1.f;
+                        pair_sync(pair_bar);
+                        fine = fine && *other == 0.f;
+                    }
 #pragma unroll 1
-                    for (int cb = 0; cb < D / 16; ++cb) {
+                    for (int cb = 0; cb < D / 32; ++cb) {
                         uint32_t o[16];
                         float v[16];
                         tmem_ld16(to + cb * 16, o);
@@ -394,7 +411,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                         }
                         if (!whole) {
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) part[(cb * 4 + x) * 256 + i * 128 + r] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+                            for (int x = 0; x < 4; ++x) part[(c * (D / 8) + cb * 4 + x) * 256 + i * 128 + r] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
                             continue;
                         }
 #pragma unroll
@@ -411,11 +428,11 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     }
                 }
                 if (!whole) {
-                    reinterpret_cast<float2*>(part + 64 * D)[i * 128 + r] = make_float2(m, l);
+                    if (c == 0) reinterpret_cast<float2*>(part + 64 * D)[i * 128 + r] = make_float2(m, l);
                     if (sg.first == 0 && tid == 0) *info = make_int4(sg.seq, sg.vhead, sg.qt, (int)((sg.unit0 + sg.total - 1) / chunk));
                 } else {
                     // rows that are not finite, or see nothing: from the formula once more, which does not touch hidden cells
-                    for (unsigned left = __ballot_sync(0xffffffffu, on && !fine); left; left &= left - 1) {
+                    for (unsigned left = c == 0 ? __ballot_sync(0xffffffffu, on && !fine) : 0u; left; left &= left - 1) {
                         const int from = __ffs(left) - 1;
                         const int r2 = __shfl_sync(0xffffffffu, row, from), h2 = __shfl_sync(0xffffffffu, head, from), p2 = __shfl_sync(0xffffffffu, pos, from);
                         if (!attend_row<FMT, D>(a, sg.seq, sg.len, p2, r2, h2) && lane == 0) *a.status = STATUS_BAD_TABLE;
@@ -423,9 +440,11 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 }
             }
             tc_fence_before();
-            if (rows.turns) asm volatile("bar.sync 1, 256;" ::: "memory");   // (the other tile's sums have been read)
+            // (what the threads have told each other has been read)
+            if (rows.turns) asm volatile("bar.sync 9, 512;" ::: "memory");
+            else pair_sync(pair_bar);
         }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
         // ---- products ----
         const bool issuer = elect_one();
         const uint32_t id_s = instr_desc_f16(BN, 128), id_o = instr_desc_f16(D, 128) | IDESC_B_MN;
@@ -435,25 +454,25 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             const bool turns = ItemRows(sg, w).turns;
             const int n = sg.count;
             auto second = [&](int i, int j) {   // out += weights V of tile j
+                const int slot = (kt + j) % C::RING;
+                if (turns || i == 0) wait(C::B_VFULL + slot, ((kt + j) / C::RING) & 1);
                 wait(C::B_P + i, p_phase[i]);
                 p_phase[i] ^= 1;
-                const int slot = (kt + j) % C::RING;
-                wait(C::B_VFULL + slot, ((kt + j) / C::RING) & 1);
                 tc_fence_after();
                 if (issuer) {
                     const uint32_t lo = desc_lo_mn(base + C::O_V + slot * C::TILE, BN * 128), ts = tmem + T_S + i * BN, to = tmem + T_O + i * D;
                     const bool begin = turns ? j == i : j == 0;
 #pragma unroll
-                    for (int k = 0; k < BN / 16; ++k) umma_f16_ts<false>(to, ts + k * 8, desc_of(lo + k * 128), id_o, !(begin && k == 0));
+                    for (int k = 0; k < BN / 16; ++k) umma_f16_ts<false>(to, ts + (k >> 2) * 64 + (k & 3) * 8, desc_of(lo + k * 128), id_o, !(begin && k == 0));
                     if (turns || i == 1) umma_commit<false>(bar(C::B_VEMPTY + slot));
                 }
                 __syncwarp();
             };
             for (int v = 0; v < (turns ? n : 2 * n); ++v) {
                 const int j = turns ? v : v >> 1, i = v & 1, before = turns ? j - 2 : j - 1;
-                if (before >= 0) second(i, before);
                 const int slot = (kt + j) % C::RING;
                 if (turns || i == 0) wait(C::B_KFULL + slot, ((kt + j) / C::RING) & 1);
+                if (before >= 0) second(i, before);
                 if (before < 0) {
                     wait(C::B_Q + i, q_phase[i]);
                     q_phase[i] ^= 1;
@@ -486,7 +505,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         if (issuer) umma_commit<false>(bar(C::B_DONE));
         __syncwarp();
         mbar_wait_bounded(bar(C::B_DONE), 0);
-    } else if (warp == 9) {
+    } else if (warp == 17) {
         // ---- copies ----
         const int box_keys = C::CODES ? min(C::RAW_KEYS, 1 << shift) : min(BN, 1 << shift), box_shift = 31 - __clz(box_keys), boxes = BN >> box_shift;
         const uint64_t pol = l2_policy_evict_normal();
@@ -587,9 +606,9 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             else
                 for (const long long t0 = clock64(); clock64() - t0 < WAIT_CYCLES;) {}   // (copies that a broken order left on either ring: time enough for any)
         }
-    } else if (C::CODES) {
+    } else if (C::CODES && warp >= 20) {
         // ---- codes to operands ----
-        const int x0 = (warp - 10) * 32 + lane;
+        const int x0 = (warp - 20) * 32 + lane;
         int kt = 0, raw = 0;
         while (walk.next(a.s, w, &sg)) {
             const TileRange tr = sg.tiles(w);
@@ -655,7 +674,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 8) tmem_dealloc<false>(tmem, 512);
+    if (warp == 16) tmem_dealloc<false>(tmem, 512);
 }
 
 // Joins the parts of items that blocks share: block (b, y) the rows 32 y .. of the item that block b of the kernel above began and did not finish.
