@@ -608,7 +608,11 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         }
     } else if (C::CODES && warp >= 20) {
         // ---- codes to operands ----
-        const int x0 = (warp - 20) * 32 + lane;
+        // A thread takes the same 16 codes of every ROWS-th key: its place in a row of operands, and so the swizzle, stays.
+        constexpr int ROWS = 128 / (D / 16), PIECES = C::RAW_KEYS / ROWS, BATCH = PIECES < 4 ? PIECES : 4;
+        const int x0 = (warp - 20) * 32 + lane, row0 = x0 / (D / 16), piece = x0 % (D / 16);
+        const bool swap = D == 128 && (piece & 4);   // (the two columns of 64 dims share banks: neighbours take opposite pieces first)
+        const uint32_t off0 = operand_at(0, row0, 2 * piece + (swap ? 1 : 0)), off1 = operand_at(0, row0, 2 * piece + (swap ? 0 : 1));
         int kt = 0, raw = 0;
         while (walk.next(a.s, w, &sg)) {
             const TileRange tr = sg.tiles(w);
@@ -625,22 +629,30 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     const uint8_t* src = smem + C::O_RAW + st * C::RAW_STAGE;
                     const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + tile % C::HERE * 4);
                     const bool fix = value && (k0 + BN - 1 > p1 || (k0 < lo0 && k0 + BN > w.sinks) || here != 0xFFu);
-#pragma unroll 4
-                    for (int x = x0; x < C::RAW / 16; x += 128) {
-                        const int rr = half * C::RAW_KEYS + x / (D / 16), piece = x % (D / 16), key = k0 + rr;
-                        uint4 q = reinterpret_cast<const uint4*>(src)[x];
-                        // values that no row sees must not be NaN: their weights are 0
-                        if (fix && (key > p1 || (key < lo0 && key >= w.sinks) || !(here >> (rr >> 4) & 1u))) q = make_uint4(0, 0, 0, 0);
-                        uint4 lo, hi;
-                        codes_to_half2x2<FMT>(q.x, lo.x, lo.y);
-                        codes_to_half2x2<FMT>(q.y, lo.z, lo.w);
-                        codes_to_half2x2<FMT>(q.z, hi.x, hi.y);
-                        codes_to_half2x2<FMT>(q.w, hi.z, hi.w);
-                        // (the two columns of 64 dims share banks: neighbours take opposite pieces first)
-                        const bool swap = D == 128 && (piece & 4);
-                        st_shared16(operand_at(dst, rr, 2 * piece + (swap ? 1 : 0)), swap ? hi : lo);
-                        st_shared16(operand_at(dst, rr, 2 * piece + (swap ? 0 : 1)), swap ? lo : hi);
-                    }
+                    const uint32_t to = dst + half * (C::RAW_KEYS * 128);
+                    auto pieces = [&](auto fixed) {
+#pragma unroll
+                        for (int b = 0; b < PIECES; b += BATCH) {
+                            uint4 q[BATCH];
+#pragma unroll
+                            for (int y = 0; y < BATCH; ++y) q[y] = reinterpret_cast<const uint4*>(src)[x0 + (b + y) * 128];
+#pragma unroll
+                            for (int y = 0; y < BATCH; ++y) {
+                                // values that no row sees must not be NaN: their weights are 0
+                                const int rr = half * C::RAW_KEYS + row0 + (b + y) * ROWS, key = k0 + rr;
+                                if (decltype(fixed)::value && (key > p1 || (key < lo0 && key >= w.sinks) || !(here >> (rr >> 4) & 1u))) q[y] = make_uint4(0, 0, 0, 0);
+                                uint4 lo, hi;
+                                codes_to_half2x2<FMT>(q[y].x, lo.x, lo.y);
+                                codes_to_half2x2<FMT>(q[y].y, lo.z, lo.w);
+                                codes_to_half2x2<FMT>(q[y].z, hi.x, hi.y);
+                                codes_to_half2x2<FMT>(q[y].w, hi.z, hi.w);
+                                st_shared16(to + off0 + (b + y) * (ROWS * 128), swap ? hi : lo);
+                                st_shared16(to + off1 + (b + y) * (ROWS * 128), swap ? lo : hi);
+                            }
+                        }
+                    };
+                    if (fix) pieces(std::true_type());
+                    else pieces(std::false_type());
                     if (!value && x0 < C::RAW_KEYS) {
                         const float ks = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW)[x0]), vs = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW + 128)[x0]);
                         const int key = half * C::RAW_KEYS + x0;
