@@ -13,7 +13,7 @@
 //     in tensor memory and are scaled again only when a row's maximum has grown by more than 2^8.
 //   * warp 16: issues all tcgen05.mma: scores = Q K^T (both K-major), out += weights V (V as it lies in the cache, MN-major).  While one
 //     query tile is in its softmax the other one has the tensor cores.
-//   * warp 17: tensor copies (fp16: straight into the operands; 8-bit: codes into a ring of half tiles).
+//   * warp 17: tensor copies (fp16: straight into the operands; 8-bit: codes into a ring of parts of tiles).
 //   * warps 20-23, 8-bit cells only: codes to fp16 operands, and the keys' factors.
 // The exponentials bound it next to the products: 128 x 128 scores take 1024 clocks of the SM's exponential units and D * 8 clocks of
 // its tensor cores for both products.
@@ -29,6 +29,12 @@ namespace {
 
 constexpr int BN = 128;   // keys of a tile
 
+// Where a warp is in its block's work.  It lies in shared memory: two dozen registers less in the softmax's loops.
+struct Steps {
+    Walk walk;
+    Segment sg;
+};
+
 template <int FMT, int D>
 struct Chunk {
     static constexpr bool CODES = FMT != KV_FP16;
@@ -39,19 +45,20 @@ struct Chunk {
     // of tile t - RING - 2 is.  (Its copies begin up to two tiles earlier.)
     static constexpr int META = D == 64 ? 8 : 4;
     static constexpr int HERE = 8;                               // which keys of a tile were copied: noted when its copies begin
-    static constexpr int RAW_KEYS = 64, RAW = RAW_KEYS * D;      // half tiles of codes
-    static constexpr int RAW_STAGE = RAW + 256;                  // with the scales of keys and values
-    static constexpr int RAWS = CODES ? (D == 64 ? 6 : 3) : 0;
+    static constexpr int RAW_KEYS = 32, RAW = RAW_KEYS * D;      // codes arrive in parts of a tile, one for each expanding warp
+    static constexpr int RAW_STAGE = RAW + 4 * RAW_KEYS;         // with the scales of keys and values
+    static constexpr int RAWS = CODES ? (D == 64 ? 12 : 4) : 0; // a stage is always the same warp's: whose turn it is shows in one bit
     static constexpr int THREADS = CODES ? 768 : 640;
     // shared memory
     static constexpr int O_Q = 0, O_K = O_Q + 2 * TILE, O_V = O_K + RING * TILE, O_RAW = O_V + RING * TILE, O_META = O_RAW + RAWS * RAW_STAGE;
     static constexpr int META_BYTES = CODES ? BN * 12 : 0;       // factors of the scores, their summands, 1 / scale of the values
-    static constexpr int O_HERE = O_META + META * META_BYTES, O_SUMS = O_HERE + HERE * 4, O_BARS = O_SUMS + 5 * BN * 4;
+    static constexpr int O_HERE = O_META + META * META_BYTES, O_SUMS = O_HERE + HERE * 4, O_WALK = O_SUMS + 5 * BN * 4, O_BARS = O_WALK + THREADS / 32 * (int)sizeof(Steps);
     static constexpr int B_KFULL = 0, B_KEMPTY = B_KFULL + RING, B_VFULL = B_KEMPTY + RING, B_VEMPTY = B_VFULL + RING, B_META = B_VEMPTY + RING,
                          B_RFULL = B_META + META, B_REMPTY = B_RFULL + RAWS, B_Q = B_REMPTY + RAWS, B_S = B_Q + 2, B_P = B_S + 2, B_O = B_P + 2, B_FIX = B_O + 2, B_DONE = B_FIX + 1,
                          BARS = B_DONE + 1;
     static constexpr int O_TMEM = O_BARS + BARS * 8, O_DEAD = O_TMEM + 4, BYTES = O_DEAD + 4, SMEM = BYTES + 1024;
     static_assert(SMEM <= 227 * 1024, "shared memory");
+    static_assert(RAWS % (BN / RAW_KEYS) == 0, "a stage belongs to one part of a tile");
     static_assert(O_BARS % 8 == 0 && O_RAW % 128 == 0 && RAW_STAGE % 16 == 0 && O_META % 16 == 0, "alignment");
     static_assert(sizeof(WorkShared) <= 2 * TILE, "the work list lies where the queries will");
 };
@@ -187,8 +194,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         const int b = tid;
         int n = 1;
         if (b < C::B_KEMPTY || (b >= C::B_VFULL && b < C::B_VEMPTY) || (b >= C::B_META && b < C::B_RFULL)) n = C::CODES ? 4 : 1;
-        if (b >= C::B_REMPTY && b < C::B_Q) n = 4;
-        if ((b >= C::B_Q && b < C::B_S) || (b >= C::B_P && b < C::B_O)) n = 8;
+                if ((b >= C::B_Q && b < C::B_S) || (b >= C::B_P && b < C::B_O)) n = 8;
         mbar_init(bar(b), n);
     }
     if (tid == 0) *dead = 0;
@@ -210,13 +216,23 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     w.window = a.window;
     w.sinks = a.sinks;
     long long chunk;
-    Walk walk = find_work(a.s, w, reinterpret_cast<WorkShared*>(smem + C::O_Q), 2, &chunk, a.status);
+    Steps& steps = reinterpret_cast<Steps*>(smem + C::O_WALK)[warp];
+    Segment& sg = steps.sg;
+    {
+        const Walk walk = find_work(a.s, w, reinterpret_cast<WorkShared*>(smem + C::O_Q), 2, &chunk, a.status);
+        if (lane == 0) steps.walk = walk;
+    }
     __syncthreads();
+    auto next_segment = [&]() {
+        int more = 0;
+        __syncwarp();
+        if (lane == 0) more = steps.walk.next(a.s, w, &steps.sg);
+        return __shfl_sync(0xffffffffu, more, 0) != 0;
+    };
     const int shift = a.c.page_shift;
     const float scale2 = a.scale * 1.4426950408889634f;
     int4* const info = a.items + blockIdx.x;   // for the kernel that joins the parts: what this block has begun and not finished
     if (tid == 0) *info = make_int4(-1, 0, 0, 0);
-    Segment sg;
 
     if (warp < 16) {
         // ---- softmax of query tile i, keys 64 c .. of a tile; row r ----
@@ -228,7 +244,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         const uint32_t qtile = base + C::O_Q + i * C::TILE;
         uint32_t s_phase = 0, o_phase = 0;
         int kt = 0;   // key tiles of the block so far
-        while (walk.next(a.s, w, &sg)) {
+        while (next_segment()) {
             const ItemRows rows(sg, w);
             const TileRange tr = sg.tiles(w);
             const int kv_head = sg.vhead / parts, g = r % w.group, t = rows.first(i) + r / w.group, hg = (sg.vhead % parts) * w.group + g;
@@ -450,7 +466,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         const uint32_t id_s = instr_desc_f16(BN, 128), id_o = instr_desc_f16(D, 128) | IDESC_B_MN;
         int kt = 0;
         uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-        while (walk.next(a.s, w, &sg)) {
+        while (next_segment()) {
             const bool turns = ItemRows(sg, w).turns;
             const int n = sg.count;
             auto second = [&](int i, int j) {   // out += weights V of tile j
@@ -507,10 +523,10 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         mbar_wait_bounded(bar(C::B_DONE), 0);
     } else if (warp == 17) {
         // ---- copies ----
-        const int box_keys = C::CODES ? min(C::RAW_KEYS, 1 << shift) : min(BN, 1 << shift), box_shift = 31 - __clz(box_keys), boxes = BN >> box_shift;
+        const int box_keys = C::CODES ? min((int)C::RAW_KEYS, 1 << shift) : min(BN, 1 << shift), box_shift = 31 - __clz(box_keys), boxes = BN >> box_shift;
         const uint64_t pol = l2_policy_evict_normal();
         int kt = 0, raw = 0;
-        while (walk.next(a.s, w, &sg)) {
+        while (next_segment()) {
             const TileRange tr = sg.tiles(w);
             const int p0 = sg.p0(w), p1 = sg.p1(w), lo0 = window_begin(p0 < 0 ? 0 : p0, w.window), kv_head = sg.vhead / parts, n = sg.count;
             auto key_of = [&](int j) { return p1 < 0 ? 0 : tr.tile_at(sg.first + j) * BN; };
@@ -566,24 +582,26 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     }
                     if (!value && lane == 0) mbar_arrive(bar(C::B_META + tile % C::META));
                 } else {
-                    for (int half = 0; half < 2; ++half) {
-                        const int st = raw % RAWS;
-                        wait(C::B_REMPTY + st, ((raw / RAWS) & 1) ^ 1);
-                        if (given_up()) return;
-                        const bool now = in && (lane >> (6 - box_shift)) == half;   // boxes of this half of the keys
-                        const int cnt = __popc(__ballot_sync(0xffffffffu, now));
-                        const uint32_t full = bar(C::B_RFULL + st), dst = base + C::O_RAW + st * C::RAW_STAGE, at = lane * box_keys - half * C::RAW_KEYS;
-                        if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(cnt * box_keys * (D + (value ? 0 : 4))));
-                        __syncwarp();
-                        if (now) {
-                            bulk_g2s(dst + at * D, (const uint8_t*)(value ? a.c.v : a.c.k) + row * D, box_keys * D, full, pol);
-                            if (!value) {
-                                bulk_g2s(dst + C::RAW + at * 2, a.c.k_scale + row, box_keys * 2, full, pol);
-                                bulk_g2s(dst + C::RAW + 128 + at * 2, a.c.v_scale + row, box_keys * 2, full, pol);
-                            }
-                        }
-                        ++raw;
+                    // A lane for each box, in the part of the tile that it lies in.
+                    const int part = lane * box_keys / C::RAW_KEYS, per = C::RAW_KEYS / box_keys, at = lane * box_keys % C::RAW_KEYS, st = (raw + part) % RAWS;
+                    const bool leads = lane < boxes && at == 0;
+                    const uint32_t full = bar(C::B_RFULL + st), dst = base + C::O_RAW + st * C::RAW_STAGE;
+                    const bool late = leads && !mbar_wait_bounded(bar(C::B_REMPTY + st), (((raw + part) / RAWS) & 1) ^ 1);
+                    if (__any_sync(0xffffffffu, late)) {
+                        *dead = 1;
+                        *a.status = 32;
                     }
+                    if (given_up()) return;
+                    if (leads) mbar_arrive_expect_tx(full, (uint32_t)(__popc(here >> lane & ((1u << per) - 1u)) * box_keys * (D + (value ? 0 : 4))));
+                    __syncwarp();
+                    if (in) {
+                        bulk_g2s(dst + at * D, (const uint8_t*)(value ? a.c.v : a.c.k) + row * D, box_keys * D, full, pol);
+                        if (!value) {
+                            bulk_g2s(dst + C::RAW + at * 2, a.c.k_scale + row, box_keys * 2, full, pol);
+                            bulk_g2s(dst + C::RAW + 2 * C::RAW_KEYS + at * 2, a.c.v_scale + row, box_keys * 2, full, pol);
+                        }
+                    }
+                    raw += BN / C::RAW_KEYS;
                 }
             };
             // in the order in which they are used: K 0, K 1, then V j and K j + 2
@@ -608,13 +626,19 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         }
     } else if (C::CODES && warp >= 20) {
         // ---- codes to operands ----
-        // A thread takes the same 16 codes of every ROWS-th key: its place in a row of operands, and so the swizzle, stays.
-        constexpr int ROWS = 128 / (D / 16), PIECES = C::RAW_KEYS / ROWS, BATCH = PIECES < 4 ? PIECES : 4;
-        const int x0 = (warp - 20) * 32 + lane, row0 = x0 / (D / 16), piece = x0 % (D / 16);
+        // Each warp has a part of every tile.  A thread takes the same 16 codes of every ROWS-th key: its place in a row of operands, and so the
+        // swizzle, stays.
+        constexpr int ROWS = 32 / (D / 16), PIECES = C::RAW_KEYS / ROWS, PERIOD = 8 / ROWS;   // (the swizzle comes round after 8 rows)
+        const int part = warp - 20, row0 = lane / (D / 16), piece = lane % (D / 16);
         const bool swap = D == 128 && (piece & 4);   // (the two columns of 64 dims share banks: neighbours take opposite pieces first)
-        const uint32_t off0 = operand_at(0, row0, 2 * piece + (swap ? 1 : 0)), off1 = operand_at(0, row0, 2 * piece + (swap ? 0 : 1));
+        uint32_t off0[PERIOD], off1[PERIOD];
+#pragma unroll
+        for (int y = 0; y < PERIOD; ++y) {
+            off0[y] = operand_at(0, part * C::RAW_KEYS + row0 + y * ROWS, 2 * piece + (swap ? 1 : 0));
+            off1[y] = operand_at(0, part * C::RAW_KEYS + row0 + y * ROWS, 2 * piece + (swap ? 0 : 1));
+        }
         int kt = 0, raw = 0;
-        while (walk.next(a.s, w, &sg)) {
+        while (next_segment()) {
             const TileRange tr = sg.tiles(w);
             const int p0 = sg.p0(w), p1 = sg.p1(w), lo0 = window_begin(p0 < 0 ? 0 : p0, w.window), n = sg.count;
             auto expand = [&](int j, bool value) {
@@ -622,51 +646,49 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 const int k0 = p1 < 0 ? 0 : tr.tile_at(sg.first + j) * BN;
                 wait((value ? C::B_VEMPTY : C::B_KEMPTY) + slot, ((tile / C::RING) & 1) ^ 1);
                 const uint32_t dst = base + (value ? C::O_V : C::O_K) + slot * C::TILE;
-                for (int half = 0; half < 2; ++half) {
-                    const int st = raw % RAWS;
-                    wait(C::B_RFULL + st, (raw / RAWS) & 1);
-                    ++raw;
-                    const uint8_t* src = smem + C::O_RAW + st * C::RAW_STAGE;
-                    const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + tile % C::HERE * 4);
-                    const bool fix = value && (k0 + BN - 1 > p1 || (k0 < lo0 && k0 + BN > w.sinks) || here != 0xFFu);
-                    const uint32_t to = dst + half * (C::RAW_KEYS * 128);
-                    auto pieces = [&](auto fixed) {
+                const int st = (raw + part) % RAWS;
+                wait(C::B_RFULL + st, ((raw + part) / RAWS) & 1);
+                raw += BN / C::RAW_KEYS;
+                const uint8_t* src = smem + C::O_RAW + st * C::RAW_STAGE;
+                const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + tile % C::HERE * 4);
+                const bool fix = value && (k0 + BN - 1 > p1 || (k0 < lo0 && k0 + BN > w.sinks) || here != 0xFFu);
+                auto pieces = [&](auto fixed) {
 #pragma unroll
-                        for (int b = 0; b < PIECES; b += BATCH) {
-                            uint4 q[BATCH];
+                    for (int b = 0; b < PIECES; b += 4) {
+                        uint4 q[4];
 #pragma unroll
-                            for (int y = 0; y < BATCH; ++y) q[y] = reinterpret_cast<const uint4*>(src)[x0 + (b + y) * 128];
+                        for (int y = 0; y < 4; ++y) q[y] = reinterpret_cast<const uint4*>(src)[lane + (b + y) * 32];
 #pragma unroll
-                            for (int y = 0; y < BATCH; ++y) {
-                                // values that no row sees must not be NaN: their weights are 0
-                                const int rr = half * C::RAW_KEYS + row0 + (b + y) * ROWS, key = k0 + rr;
-                                if (decltype(fixed)::value && (key > p1 || (key < lo0 && key >= w.sinks) || !(here >> (rr >> 4) & 1u))) q[y] = make_uint4(0, 0, 0, 0);
-                                uint4 lo, hi;
-                                codes_to_half2x2<FMT>(q[y].x, lo.x, lo.y);
-                                codes_to_half2x2<FMT>(q[y].y, lo.z, lo.w);
-                                codes_to_half2x2<FMT>(q[y].z, hi.x, hi.y);
-                                codes_to_half2x2<FMT>(q[y].w, hi.z, hi.w);
-                                st_shared16(to + off0 + (b + y) * (ROWS * 128), swap ? hi : lo);
-                                st_shared16(to + off1 + (b + y) * (ROWS * 128), swap ? lo : hi);
-                            }
+                        for (int y = 0; y < 4; ++y) {
+                            // values that no row sees must not be NaN: their weights are 0
+                            const int rr = part * C::RAW_KEYS + row0 + (b + y) * ROWS, key = k0 + rr;
+                            if (decltype(fixed)::value && (key > p1 || (key < lo0 && key >= w.sinks) || !(here >> (rr >> 4) & 1u))) q[y] = make_uint4(0, 0, 0, 0);
+                            uint4 lo, hi;
+                            codes_to_half2x2<FMT>(q[y].x, lo.x, lo.y);
+                            codes_to_half2x2<FMT>(q[y].y, lo.z, lo.w);
+                            codes_to_half2x2<FMT>(q[y].z, hi.x, hi.y);
+                            codes_to_half2x2<FMT>(q[y].w, hi.z, hi.w);
+                            const uint32_t to = dst + (b + y) / PERIOD * (8 * 128);
+                            st_shared16(to + off0[(b + y) % PERIOD], swap ? hi : lo);
+                            st_shared16(to + off1[(b + y) % PERIOD], swap ? lo : hi);
                         }
-                    };
-                    if (fix) pieces(std::true_type());
-                    else pieces(std::false_type());
-                    if (!value && x0 < C::RAW_KEYS) {
-                        const float ks = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW)[x0]), vs = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW + 128)[x0]);
-                        const int key = half * C::RAW_KEYS + x0;
-                        // (the scales of keys that no row sees may be anything)
-                        const bool seen = k0 + key <= p1 && (k0 + key >= lo0 || k0 + key < w.sinks) && (here >> (key >> 4) & 1u);
-                        const float b = seen ? lg2(vs) : 0.f;
-                        float* meta = reinterpret_cast<float*>(smem + C::O_META + mt * C::META_BYTES) + key;
-                        meta[0] = seen ? ks * scale2 : 1.f;
-                        meta[BN] = b;
-                        meta[2 * BN] = ex2(-b);
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(C::B_REMPTY + st));
+                };
+                if (fix) pieces(std::true_type());
+                else pieces(std::false_type());
+                if (!value) {
+                    const float ks = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW)[lane]), vs = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW + 2 * C::RAW_KEYS)[lane]);
+                    const int key = part * C::RAW_KEYS + lane;
+                    // (the scales of keys that no row sees may be anything)
+                    const bool seen = k0 + key <= p1 && (k0 + key >= lo0 || k0 + key < w.sinks) && (here >> (key >> 4) & 1u);
+                    const float b = seen ? lg2(vs) : 0.f;
+                    float* meta = reinterpret_cast<float*>(smem + C::O_META + mt * C::META_BYTES) + key;
+                    meta[0] = seen ? ks * scale2 : 1.f;
+                    meta[BN] = b;
+                    meta[2 * BN] = ex2(-b);
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(C::B_REMPTY + st));
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {
