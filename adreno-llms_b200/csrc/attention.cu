@@ -35,7 +35,7 @@ cudaError_t attention_configure() {
 }
 
 cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl) {
-    if (a.group <= 16 && (long long)a.group * max_new <= 16) return launch_attention_decode(a, maps, sm_count, st, pdl);
+    if (a.group <= 16 && (long long)a.group * max_new <= 16) return launch_attention_decode(a, maps, max_new, sm_count, st, pdl);
     return launch_attention_chunk(a, maps, sm_count, st, pdl);
 }
 

@@ -67,7 +67,7 @@ struct AttnMaps;
 cudaError_t attention_configure();
 cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl);
 constexpr int ATTN_MAX_BLOCKS = 256;
-constexpr size_t ATTN_DECODE_PART = 17 * 512, ATTN_CHUNK_PART = 256 * 128 * 4 + 256 * 8;   // two per block
+constexpr size_t ATTN_DECODE_PART = 18 * 512, ATTN_CHUNK_PART = 256 * 128 * 4 + 256 * 8;   // two per block
 // The workspace: counters, items, parts.
 constexpr size_t ATTN_COUNTER_BYTES = ATTN_MAX_BLOCKS * sizeof(unsigned), ATTN_HEAD_BYTES = ATTN_COUNTER_BYTES + ATTN_MAX_BLOCKS * sizeof(int4);
 inline size_t attention_workspace_bytes(int sm_count) { return ATTN_HEAD_BYTES + 2 * (size_t)(sm_count < ATTN_MAX_BLOCKS ? sm_count : ATTN_MAX_BLOCKS) * ATTN_CHUNK_PART; }

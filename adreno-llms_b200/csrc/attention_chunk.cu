@@ -60,7 +60,6 @@ struct Chunk {
     static_assert(SMEM <= 227 * 1024, "shared memory");
     static_assert(RAWS % (BN / RAW_KEYS) == 0, "a stage belongs to one part of a tile");
     static_assert(O_BARS % 8 == 0 && O_RAW % 128 == 0 && RAW_STAGE % 16 == 0 && O_META % 16 == 0, "alignment");
-    static_assert(sizeof(WorkShared) <= 2 * TILE, "the work list lies where the queries will");
 };
 constexpr int T_S = 0, T_O = 256;   // tensor memory: two tiles of scores (and weights), two of outputs
 
@@ -219,10 +218,9 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     Steps& steps = reinterpret_cast<Steps*>(smem + C::O_WALK)[warp];
     Segment& sg = steps.sg;
     {
-        const Walk walk = find_work(a.s, w, reinterpret_cast<WorkShared*>(smem + C::O_Q), 2, &chunk, a.status);
+        const Walk walk = find_work(a.s, w, 2, &chunk, a.status);
         if (lane == 0) steps.walk = walk;
     }
-    __syncthreads();
     auto next_segment = [&]() {
         int more = 0;
         __syncwarp();

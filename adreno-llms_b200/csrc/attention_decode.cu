@@ -1,4 +1,4 @@
-// Attention of few new tokens: at most 16 query rows (new tokens times query heads to a cache head) read a cache head together.
+// Attention of few new tokens: up to 8 or 16 query rows (new tokens times query heads to a cache head) read a cache head together.
 //
 //   t_k = scale log2(e) q.k,  w_k = 2^(t_k - m),  out = sum w_k v_k / sum w_k          m: the running maximum of t
 //
@@ -6,10 +6,14 @@
 // scale its weight: t'_k = t_k + log2(scale_v), w'_k = 2^(t'_k - m'), out = sum w'_k code_k / sum w'_k / scale_v, so that the weights
 // that are rounded to fp16 for the second product are at most 1 and no rounding is added.
 //
-// Bound by the bytes of the cache: every cell is read once, for all rows, and a cell does 4 rows flops per byte.  So: eight warps per block and
+// Bound by the bytes of the cache: every cell is read once, for all rows, and a cell does 4 rows flops per byte.  So: twelve warps per block and
 // one block per SM, each warp with a ring of its own of 8 KB stages that tensor copies fill (16 to 64 keys with their values),
 // no synchronisation between warps along the keys; the units of all sequences and heads are dealt out evenly (attention_work.cuh).
-// Both products are mma.sync: 16 rows are an eighth of a tcgen05 tile's, and a warp keeps scores, weights and sums in registers.
+//
+// Next to the bytes it is bound by instructions: 8 KB have 354 clocks of the SM, 1416 instructions of its four schedulers, and e4m3 codes took 1344
+// as the rows of m16n8k16 products.  So keys and dims are the products' rows and the queries their 8 columns (the few rows waste no half of a
+// product, a score or a sum): S^T = K Q^T and O^T += V^T W^T, codes converted in registers on the way, the weights turned around by movmatrix.
+// (tcgen05 would want the codes as fp16 in shared memory, four times their traffic there.)
 #include "attention_maps.h"
 #include "attention_row.cuh"
 #include "attention_work.cuh"
@@ -17,25 +21,26 @@
 namespace nnb {
 namespace {
 
-constexpr int WARPS = 8, STAGES = 3, STAGE = 8192, PART = STAGE / 2;
-constexpr int MERGE_BYTES = 17408;   // two warps' sums of 128 dims with their maxima (four of 64)
+constexpr int WARPS = 12, STAGES = 2, STAGE = 8192, PART = STAGE / 2, THREADS = WARPS * 32;
 
 template <int FMT, int D>
 struct Shape {
     static constexpr int EB = kv_cell_bytes(FMT), ROW = D * EB, KT = PART / ROW;   // bytes of a cell row, keys of a stage
-    static constexpr int NT = KT / 8, DT = D / 8;                                  // 8-key and 8-dim tiles
-    static constexpr int DUMP = (DT + 1) * 512;                                    // a warp's partial result
-    static constexpr int DUMPS = MERGE_BYTES / DUMP;                               // that fit the merge buffer
+    static constexpr int KG = KT / 16, DG = D / 16;                                // groups of 16 keys, of 16 dims
 };
-
-constexpr int S_RING = 0, S_SCALE = WARPS * STAGES * STAGE, S_MERGE = S_SCALE + WARPS * STAGES * 256, S_BARS = S_MERGE + MERGE_BYTES,
-              S_HERE = S_BARS + WARPS * STAGES * 8, S_FLAG = S_HERE + WARPS * STAGES * 4,
-              SMEM_BYTES = S_FLAG + 16 + 1024;
+constexpr int S_RING = 0, S_SCALE = WARPS * STAGES * STAGE, S_MERGE = S_SCALE + WARPS * STAGES * 256, S_BARS = S_MERGE + 2 * (int)ATTN_DECODE_PART,
+              S_HERE = S_BARS + WARPS * STAGES * 8, S_FLAG = S_HERE + WARPS * STAGES * 4, SMEM_BYTES = S_FLAG + 32 + 1024;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
-static_assert(sizeof(WorkShared) <= MERGE_BYTES, "the work list lies in the merge buffer");
+static_assert((int)ATTN_DECODE_PART <= STAGES * STAGE, "a warp's result fits its ring");
 
 __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
+}
+// 8 x 8 values of 16 bits turned around: rows lane / 4, columns 2 (lane % 4) ..
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -48,6 +53,22 @@ __device__ __forceinline__ float lg2(float x) {
     return y;
 }
 
+// Bytes 0 and 2, and bytes 1 and 3, of four codes as half2, exact.
+template <int FMT>
+__device__ __forceinline__ void codes_even_odd(uint32_t w, uint32_t& even, uint32_t& odd) {
+    if (FMT == KV_INT8) {   // the bytes, their sign bit turned over, as the low mantissa bits of 1024.0h, less 1152
+        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const uint32_t e = (w & 0x00FF00FFu) ^ 0x64806480u, o = (w >> 8 & 0x00FF00FFu) ^ 0x64806480u;
+        const __half2 he = __hsub2(*reinterpret_cast<const __half2*>(&e), bias), ho = __hsub2(*reinterpret_cast<const __half2*>(&o), bias);
+        even = *reinterpret_cast<const uint32_t*>(&he);
+        odd = *reinterpret_cast<const uint32_t*>(&ho);
+    } else {
+        const uint32_t p = __byte_perm(w, 0u, 0x3120);
+        even = e4m3x2_to_half2(p & 0xFFFFu);
+        odd = e4m3x2_to_half2(p >> 16);
+    }
+}
+
 // Address of 16 bytes of a cell row in a stage's half, as the tensor copies' swizzle leaves them: 64-byte rows, or 128-byte rows (256-byte ones as two halves).
 template <int FMT, int D>
 __device__ __forceinline__ uint32_t chunk_at(uint32_t base, int row, int chunk) {
@@ -56,87 +77,131 @@ __device__ __forceinline__ uint32_t chunk_at(uint32_t base, int row, int chunk) 
     return base + (chunk >> 3) * (S::KT * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
-// A warp's running result for its rows lane / 4 and lane / 4 + 8.  Of 16 dims (8-bit cells) or two tiles of 8 (fp16): the accumulator
-// layout of the products, which only the last step turns into dims.
-template <int D>
+// A warp's running result: for each tile b of 8 query rows, rows 8 b + 2 (lane % 4) and + 1, and of the sums two dims of each 16:
+// lane / 4 and + 8 (fp16), 2 (lane / 4) and + 1 (8-bit): o[b][g] = {first dim, row 0; row 1; second dim, row 0; row 1}.
+template <int D, int NB>
 struct State {
-    float m[2], l[2];
-    float o[D / 8][4];
+    float m[NB][2], l[NB][2];
+    float4 o[NB][D / 16];
     __device__ __forceinline__ void clear() {
-        m[0] = m[1] = -INFINITY;
-        l[0] = l[1] = 0.f;
 #pragma unroll
-        for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        for (int b = 0; b < NB; ++b) {
+            m[b][0] = m[b][1] = -INFINITY;
+            l[b][0] = l[b][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[b][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
     }
     // (the sums of the weights are kept per lane along the keys)
     __device__ __forceinline__ void close() {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[b][h] += __shfl_xor_sync(0xffffffffu, l[b][h], d);
+    }
+    // A partial result: [NB] maxima and sums, [NB][D / 16] quads, each of 32 lanes.
+    __device__ __forceinline__ void store(float4* p) const {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            p[b * 32 + lane] = make_float4(m[b][0], l[b][0], m[b][1], l[b][1]);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) p[(NB + b * (D / 16) + i) * 32 + lane] = o[b][i];
         }
     }
-    // A partial result is [1 + D / 8][32 lanes] float4: maxima and sums, rows lane / 4, rows lane / 4 + 8 (only with `two`).
-    __device__ __forceinline__ void store(float4* p, bool two) const {
-        const int lane = threadIdx.x & 31;
-        p[lane] = make_float4(m[0], l[0], m[1], l[1]);
+    __device__ __forceinline__ void rescale(int b, float f0, float f1) {
+        l[b][0] *= f0;
+        l[b][1] *= f1;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) p[(1 + i) * 32 + lane] = make_float4(o[2 * i][0], o[2 * i][1], o[2 * i + 1][0], o[2 * i + 1][1]);
-        if (two)
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) p[(1 + D / 16 + i) * 32 + lane] = make_float4(o[2 * i][2], o[2 * i][3], o[2 * i + 1][2], o[2 * i + 1][3]);
+        for (int i = 0; i < D / 16; ++i) {
+            o[b][i].x *= f0;
+            o[b][i].y *= f1;
+            o[b][i].z *= f0;
+            o[b][i].w *= f1;
+        }
     }
-    __device__ __forceinline__ void add(const float4* p, bool two) {
+    __device__ __forceinline__ void add(const float4* p) {
         const int lane = threadIdx.x & 31;
-        const float4 h = p[lane];
-        float4 v[D / 16];
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) v[i] = p[(1 + i) * 32 + lane];
-        const float hm[2] = {h.x, h.z}, hl[2] = {h.y, h.w};
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            if (r == 1) {
-                if (!two) break;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) v[i] = p[(1 + D / 16 + i) * 32 + lane];
-            }
-            const float up = fmaxf(m[r], hm[r]);
-            const float a = m[r] == -INFINITY ? 0.f : ex2(m[r] - up), b = hm[r] == -INFINITY ? 0.f : ex2(hm[r] - up);
-            m[r] = up;
-            l[r] = l[r] * a + hl[r] * b;
+        for (int b = 0; b < NB; ++b) {
+            const float4 h = p[b * 32 + lane];
+            const float u0 = fmaxf(m[b][0], h.x), u1 = fmaxf(m[b][1], h.z);
+            rescale(b, m[b][0] == -INFINITY ? 0.f : ex2(m[b][0] - u0), m[b][1] == -INFINITY ? 0.f : ex2(m[b][1] - u1));
+            const float f0 = h.x == -INFINITY ? 0.f : ex2(h.x - u0), f1 = h.z == -INFINITY ? 0.f : ex2(h.z - u1);
+            m[b][0] = u0;
+            m[b][1] = u1;
+            l[b][0] += h.y * f0;
+            l[b][1] += h.w * f1;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-                o[2 * i][2 * r] = o[2 * i][2 * r] * a + v[i].x * b;
-                o[2 * i][2 * r + 1] = o[2 * i][2 * r + 1] * a + v[i].y * b;
-                o[2 * i + 1][2 * r] = o[2 * i + 1][2 * r] * a + v[i].z * b;
-                o[2 * i + 1][2 * r + 1] = o[2 * i + 1][2 * r + 1] * a + v[i].w * b;
+                const float4 v = p[(NB + b * (D / 16) + i) * 32 + lane];
+                o[b][i].x += v.x * f0;
+                o[b][i].y += v.y * f1;
+                o[b][i].z += v.z * f0;
+                o[b][i].w += v.w * f1;
             }
         }
     }
 };
 
-// The warps' results added up, in a fixed order, into warp 0's.
-template <int FMT, int D>
-__device__ __forceinline__ void merge_warps(State<D>& st, uint8_t* buf, int warp, bool two) {
-    using S = Shape<FMT, D>;
+// The warps' results added up, in a fixed order, into warp 0's, two at a time in `buf`: while other warps' rings hold the next segment's keys.
+template <int D, int NB>
+__device__ __forceinline__ void merge_warps(State<D, NB>& st, uint8_t* buf, int warp) {
 #pragma unroll 1
-    for (int half = WARPS / 2; half > 0; half >>= 1) {
+    for (int n = WARPS; n > 1; n = (n + 1) / 2) {
+        const int half = (n + 1) / 2;   // warps half .. n - 1 are added to 0 ..
 #pragma unroll 1
-        for (int s0 = 0; s0 < half; s0 += S::DUMPS) {
-            const int at = warp % half - s0;
-            const bool in = warp < 2 * half && at >= 0 && at < S::DUMPS;
-            float4* p = reinterpret_cast<float4*>(buf + (in ? at : 0) * S::DUMP);
-            if (in && warp >= half) st.store(p, two);
+        for (int s0 = 0; s0 < n - half; s0 += 2) {
+            const int to = warp < half ? warp - s0 : warp - half - s0;
+            const bool in = warp < n && to >= 0 && to < 2 && to + s0 < n - half;
+            float4* p = reinterpret_cast<float4*>(buf + (in ? to : 0) * ATTN_DECODE_PART);
+            if (in && warp >= half) st.store(p);
             __syncthreads();
-            if (in && warp < half) st.add(p, two);
+            if (in && warp < half) st.add(p);
             __syncthreads();
         }
     }
 }
 
-template <int FMT, int D>
-__global__ void __launch_bounds__(WARPS * 32, 1) attention_decode_kernel(const __grid_constant__ AttnMaps maps, const AttnArgs a) {
+// A quad of a partial result with its two rows' maxima and sums.
+struct Quad {
+    float4 v, h;
+};
+// Quad k of the NB * quads of this lane over `count` partial results, in order; `at(i)`: the i-th of them.
+template <int NB, class At>
+__device__ __forceinline__ Quad add_up(int k, int quads, int count, At&& at) {
+    const int lane = threadIdx.x & 31, b = k / quads;
+    Quad q;
+    q.v = make_float4(0.f, 0.f, 0.f, 0.f);
+    q.h = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+    constexpr int N = 4;   // (loads of so many at once)
+    for (int i0 = 0; i0 < count; i0 += N) {
+        float4 h[N], v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float4* p = at(min(i0 + i, count - 1));
+            h[i] = p[b * 32 + lane];
+            v[i] = p[(NB + k) * 32 + lane];
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (i0 + i >= count) h[i].x = h[i].z = -INFINITY;
+            const float u0 = fmaxf(q.h.x, h[i].x), u1 = fmaxf(q.h.z, h[i].z);
+            const float a0 = q.h.x == -INFINITY ? 0.f : ex2(q.h.x - u0), a1 = q.h.z == -INFINITY ? 0.f : ex2(q.h.z - u1);
+            const float f0 = h[i].x == -INFINITY ? 0.f : ex2(h[i].x - u0), f1 = h[i].z == -INFINITY ? 0.f : ex2(h[i].z - u1);
+            q.h = make_float4(u0, q.h.y * a0 + h[i].y * f0, u1, q.h.w * a1 + h[i].w * f1);
+            q.v = make_float4(q.v.x * a0 + v[i].x * f0, q.v.y * a1 + v[i].y * f1, q.v.z * a0 + v[i].z * f0, q.v.w * a1 + v[i].w * f1);
+        }
+    }
+    return q;
+}
+
+template <int FMT, int D, int NB>
+__global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __grid_constant__ AttnMaps maps, const AttnArgs a) {
     using S = Shape<FMT, D>;
+    constexpr bool CODES = FMT != KV_FP16;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t base = smem_u32(smem);
@@ -144,68 +209,74 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_decode_kernel(const _
     const uint32_t ring = base + S_RING + warp * (STAGES * STAGE), scales = base + S_SCALE + warp * (STAGES * 256), bars = base + S_BARS + warp * (STAGES * 8);
     if (lane < STAGES) mbar_init(bars + lane * 8, 1);
     mbar_init_fence();
+    __syncwarp();
     pdl_launch_dependents();
     pdl_wait_prior_grid();
 
     WorkShape w;
     w.group = a.group;
-    w.tokens = 16 / a.group;
+    w.tokens = 8 * NB / a.group;
     w.vheads = a.c.kv_heads;
     w.tile = S::KT;
     w.window = a.window;
     w.sinks = a.sinks;
-    const bool two = w.group * w.tokens > 8;
     long long chunk;
-    Walk walk = find_work(a.s, w, reinterpret_cast<WorkShared*>(smem + S_MERGE), WARPS, &chunk, a.status);
-    __syncthreads();
+    Walk walk = find_work(a.s, w, WARPS, &chunk, a.status);
     if (walk.u >= walk.end) return;
 
     const int shift = a.c.page_shift, box = min(S::KT, 1 << shift), nbox = S::KT / box, box_shift = 31 - __clz(box), nbox_shift = 31 - __clz(nbox);
     const float scale2 = a.scale * 1.4426950408889634f;
 
-    // ---- this warp's copies, `ahead` stages in front of its products ----
+    // ---- this warp's copies, a ring in front of its products ----
     Walk pw = walk;
-    Segment ps;
-    bool pmore = pw.next(a.s, w, &ps);
+    const int* ptable = a.s.page_table;
+    int phead = 0, pcount = 0, pfirst = 0, psink = 0, pskip = 0, plast = -1, plo = 0;   // the segment: its key tiles, its last position, its window
     int pslice = warp, issued = 0, page_base = 0, page_reg = -1;
-    bool fresh = true;   // page numbers of a new segment
+    bool pmore = true;
     auto issue = [&]() {   // the next stage's copies, if there is one
-        while (pmore && pslice >= ps.count) {
-            pmore = pw.next(a.s, w, &ps);
+        bool fresh = false;
+        while (pmore && pslice >= pcount) {
+            Segment s;
+            pmore = pw.next(a.s, w, &s);
+            if (!pmore) return;
+            const TileRange tr = s.tiles(w);
+            ptable = a.s.page_table + (int64_t)s.seq * a.s.table_stride;
+            phead = s.vhead;
+            pcount = s.count;
+            pfirst = s.first;
+            psink = tr.sink_tiles;
+            pskip = tr.first - tr.sink_tiles;
+            plast = s.p1(w);
+            plo = window_begin(max(s.p0(w), 0), w.window);
             pslice = warp;
             fresh = true;
         }
         if (!pmore) return;
-        const TileRange tr = ps.tiles(w);
-        const int p0 = ps.p0(w), p1 = ps.p1(w), lo = window_begin(p0 < 0 ? 0 : p0, w.window);
-        // page numbers of this warp's next boxes, one per lane
-        const int j = (pslice / WARPS) * nbox;   // boxes of this warp's stages in the segment are numbered in order
+        auto key_at = [&](int slice) { return (pfirst + slice + (pfirst + slice < psink ? 0 : pskip)) * S::KT; };
+        // page numbers of this warp's next boxes, one per lane: those of its stages in the segment are numbered in order
+        const int j = (pslice / WARPS) << nbox_shift;
         if (fresh || j + nbox > page_base + 32) {
             page_base = j;
-            const int slice = ps.first + ((j + lane) >> nbox_shift) * WARPS + warp;
+            const int slice = ((j + lane) >> nbox_shift) * WARPS + warp, key = key_at(slice) + ((j + lane) & (nbox - 1)) * box;
             page_reg = -1;
-            if (slice < ps.first + ps.count && p1 >= 0) {
-                const int key = tr.tile_at(slice) * S::KT + ((j + lane) & (nbox - 1)) * box;
-                if (key <= p1 && (key + box > lo || key < w.sinks)) {
-                    const int page = a.s.page_table[(int64_t)ps.seq * a.s.table_stride + (key >> shift)];
-                    page_reg = page_ok(page, a.c.num_pages) ? page : -2;
-                    if (page_reg == -2) *a.status = STATUS_BAD_TABLE;
-                }
+            if (slice < pcount && key <= plast && (key + box > plo || key < w.sinks)) {
+                const int page = ptable[key >> shift];
+                page_reg = page_ok(page, a.c.num_pages) ? page : -1;
+                if (page_reg < 0) *a.status = STATUS_BAD_TABLE;
             }
-            fresh = false;
         }
         const int page = __shfl_sync(0xffffffffu, page_reg, (j - page_base + lane) & 31);
         const bool mine = lane < nbox && page >= 0;
         const int stage = issued % STAGES;
         const uint32_t bar = bars + stage * 8, dst = ring + stage * STAGE, sdst = scales + stage * 256;
         const unsigned here = __ballot_sync(0xffffffffu, mine);   // the boxes that are copied: the others' keys count as hidden
-        const int boxes = __popc(here);
-        if (lane == 0) reinterpret_cast<unsigned*>(smem + S_HERE)[warp * STAGES + stage] = here;
-        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)(boxes * box * (2 * S::ROW + (FMT == KV_FP16 ? 0 : 4))));
+        if (lane == 0) {
+            reinterpret_cast<unsigned*>(smem + S_HERE)[warp * STAGES + stage] = here;
+            mbar_arrive_expect_tx(bar, (uint32_t)(__popc(here) * box * (2 * S::ROW + (CODES ? 4 : 0))));
+        }
         __syncwarp();
         if (mine) {
-            const int slot = (p1 < 0 ? 0 : tr.tile_at(ps.first + pslice) * S::KT + lane * box) & ((1 << shift) - 1);
-            const int64_t row = cell_row(page, ps.vhead, slot, a.c.kv_heads, shift);
+            const int64_t row = cell_row(page, phead, (key_at(pslice) + lane * box) & ((1 << shift) - 1), a.c.kv_heads, shift);
             const uint64_t pol = l2_policy_evict_normal();
             constexpr int HALVES = S::ROW > 128 ? 2 : 1, W = S::ROW / HALVES;
 #pragma unroll
@@ -213,7 +284,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_decode_kernel(const _
                 tma_load_2d(dst + h * (S::KT * W) + lane * box * W, &maps.k, h * 64, (int)row, bar, pol);
                 tma_load_2d(dst + PART + h * (S::KT * W) + lane * box * W, &maps.v, h * 64, (int)row, bar, pol);
             }
-            if (FMT != KV_FP16) {
+            if (CODES) {
                 bulk_g2s(sdst + lane * box * 2, a.c.k_scale + row, box * 2, bar, pol);
                 bulk_g2s(sdst + 128 + lane * box * 2, a.c.v_scale + row, box * 2, bar, pol);
             }
@@ -221,38 +292,41 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_decode_kernel(const _
         pslice += WARPS;
         ++issued;
     };
+#pragma unroll 1
     for (int i = 0; i < STAGES; ++i) issue();
 
     int used = 0;
     bool dead = false;
     Segment sg;
     while (walk.next(a.s, w, &sg)) {
-        // ---- the rows of the item: lane / 4 and lane / 4 + 8 ----
         const int p0 = sg.p0(w), p1 = sg.p1(w), lo0 = window_begin(p0 < 0 ? 0 : p0, w.window), lo1 = window_begin(p1 < 0 ? 0 : p1, w.window);
         const TileRange tr = sg.tiles(w);
-        int row[2], head[2], pos[2];
+        // row r of the item: its row of the operands (-1: none), its head, its position
+        auto row_of = [&](int r) {
+            const int t = sg.qt * w.tokens + r / w.group;
+            return r < w.tokens * w.group && t < sg.n ? sg.row0 + t : -1;
+        };
+        auto head_of = [&](int r) { return sg.vhead * w.group + r % w.group; };
+        auto pos_of = [&](int r) { return sg.len - sg.n + sg.qt * w.tokens + r / w.group; };
+        int pos[NB][2];   // of this lane's rows of scores
+        uint32_t q[NB][S::DG][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = quad + 8 * h, t = sg.qt * w.tokens + r / w.group;
-            const bool on = r < w.tokens * w.group && t < sg.n;
-            row[h] = on ? sg.row0 + t : -1;
-            head[h] = sg.vhead * w.group + r % w.group;
-            pos[h] = on ? sg.len - sg.n + t : -1;
-        }
-        uint32_t q[D / 16][4];
+        for (int b = 0; b < NB; ++b) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(a.q + (int64_t)(row[h] < 0 ? 0 : row[h]) * a.q_stride + (int64_t)head[h] * D);
+            for (int h = 0; h < 2; ++h) pos[b][h] = row_of(8 * b + 2 * c + h) >= 0 ? pos_of(8 * b + 2 * c + h) : -1;
+            const int row = row_of(8 * b + quad);
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(a.q + (int64_t)max(row, 0) * a.q_stride + (int64_t)head_of(8 * b + quad) * D);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k) {   // fp16 cells: dims 2c, 2c + 1 and 8 behind; 8-bit cells: the four dims 4c .. that a word of codes holds
+            for (int k = 0; k < S::DG; ++k) {   // fp16: dims 2c and 2c + 1, and 8 behind; codes: the dims 4c .. that a word of them holds
                 uint2 x = make_uint2(0, 0);
-                if (row[h] >= 0) x = FMT == KV_FP16 ? make_uint2(src[8 * k + c], src[8 * k + c + 4]) : *reinterpret_cast<const uint2*>(src + 8 * k + 2 * c);
-                q[k][h] = x.x;
-                q[k][2 + h] = x.y;
+                if (row >= 0) x = CODES ? *reinterpret_cast<const uint2*>(src + 8 * k + 2 * c) : make_uint2(src[8 * k + c], src[8 * k + c + 4]);
+                q[b][k][0] = x.x;
+                q[b][k][1] = x.y;
             }
         }
-        State<D> st;
+        State<D, NB> st;
         st.clear();
+#pragma unroll 1
         for (int slice = warp; slice < sg.count; slice += WARPS) {
             const int stage = used % STAGES;
             if (!dead && !mbar_wait_bounded_warp(bars + stage * 8, (used / STAGES) & 1)) {
@@ -265,118 +339,127 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_decode_kernel(const _
             const unsigned here = reinterpret_cast<const unsigned*>(smem + S_HERE)[warp * STAGES + stage];
             // some row does not see all of the keys
             const bool edge = here != (1u << nbox) - 1u || k0 + S::KT - 1 > p0 || (k0 < lo1 && k0 + S::KT > w.sinks);
+            // a key that some row sees
+            auto seen_by_some = [&](int x) { return k0 + x <= p1 && (k0 + x >= lo0 || k0 + x < w.sinks) && (here >> (x >> box_shift) & 1u); };
             if (edge) {   // values that no row sees: whatever lies there, their weight is 0 and they must not be NaN
                 for (int i = lane; i < S::KT * (S::ROW / 16); i += 32) {
-                    const int r = i / (S::ROW / 16), key = k0 + r;
-                    if (key > p1 || (key < lo0 && key >= w.sinks) || !(here >> (r >> box_shift) & 1u))
+                    const int r = i / (S::ROW / 16);
+                    if (!seen_by_some(r))
                         asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_at<FMT, D>(vb, r, i % (S::ROW / 16))), "r"(0) : "memory");
                 }
                 __syncwarp();
             }
-            float s[S::NT][4];
+            // ---- scores: rows are keys quad and quad + 8 of 16, columns the queries ----
+            float s[NB][S::KG][4];
 #pragma unroll
-            for (int n = 0; n < S::NT; ++n) {
-                s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+            for (int t = 0; t < S::KG; ++t) {
 #pragma unroll
-                for (int j = 0; j < S::ROW / 64; ++j) {   // four 16-byte pieces of 8 keys
+                for (int b = 0; b < NB; ++b) s[b][t][0] = s[b][t][1] = s[b][t][2] = s[b][t][3] = 0.f;
+                const int krow = 16 * t + (lane & 15);
+#pragma unroll
+                for (int j = 0; j < S::ROW / 32; ++j) {   // 32 bytes of 16 keys
                     uint32_t r[4];
-                    ldsm_x4(chunk_at<FMT, D>(kb, n * 8 + (lane & 7), 4 * j + (lane >> 3)), r[0], r[1], r[2], r[3]);
-                    if (FMT == KV_FP16) {
-                        mma_16816(s[n], q[2 * j][0], q[2 * j][1], q[2 * j][2], q[2 * j][3], r[0], r[1]);
-                        mma_16816(s[n], q[2 * j + 1][0], q[2 * j + 1][1], q[2 * j + 1][2], q[2 * j + 1][3], r[2], r[3]);
+                    ldsm_x4(chunk_at<FMT, D>(kb, krow, 2 * j + (lane >> 4)), r[0], r[1], r[2], r[3]);
+                    if (!CODES) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) mma_16816(s[b][t], r[0], r[1], r[2], r[3], q[b][j][0], q[b][j][1]);
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t b0, b1;
-                            codes_to_half2x2<FMT>(r[i], b0, b1);
-                            mma_16816(s[n], q[4 * j + i][0], q[4 * j + i][1], q[4 * j + i][2], q[4 * j + i][3], b0, b1);
+                        for (int x = 0; x < 2; ++x) {
+                            uint32_t a0, a1, a2, a3;
+                            codes_to_half2x2<FMT>(r[2 * x], a0, a2);
+                            codes_to_half2x2<FMT>(r[2 * x + 1], a1, a3);
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) mma_16816(s[b][t], a0, a1, a2, a3, q[b][2 * j + x][0], q[b][2 * j + x][1]);
                         }
                     }
                 }
             }
-            // scores as powers of two, with the scales of the two keys of this lane
-            float inv[S::NT][2];
-            float top[2] = {-INFINITY, -INFINITY};
+            // ---- as powers of two, with the factors of this lane's keys; the maximum ----
+            float inv[S::KG][2];
+            float top[NB][2];
 #pragma unroll
-            for (int n = 0; n < S::NT; ++n) {
-                float ka = scale2, kc = scale2, ba = 0.f, bc = 0.f;
-                if (FMT != KV_FP16) {
-                    uint32_t ks, vs;
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(ks) : "r"(sb + (n * 8 + 2 * c) * 2));
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vs) : "r"(sb + 128 + (n * 8 + 2 * c) * 2));
-                    const float2 kf = half2_floats(ks), vf = half2_floats(vs);
-                    ka = scale2 * kf.x;
-                    kc = scale2 * kf.y;
-                    ba = lg2(vf.x);
-                    bc = lg2(vf.y);
-                    inv[n][0] = ex2(-ba);
-                    inv[n][1] = ex2(-bc);
-                }
-                s[n][0] = FMT == KV_FP16 ? s[n][0] * ka : fmaf(s[n][0], ka, ba);
-                s[n][1] = FMT == KV_FP16 ? s[n][1] * kc : fmaf(s[n][1], kc, bc);
-                s[n][2] = FMT == KV_FP16 ? s[n][2] * ka : fmaf(s[n][2], ka, ba);
-                s[n][3] = FMT == KV_FP16 ? s[n][3] * kc : fmaf(s[n][3], kc, bc);
-                if (edge) {
-                    const int key = k0 + n * 8 + 2 * c;
-                    const bool there = here >> ((n * 8) >> box_shift) & 1u;
+            for (int b = 0; b < NB; ++b) top[b][0] = top[b][1] = -INFINITY;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!there || !key_visible(key + (i & 1), pos[i >> 1], w.window, w.sinks)) s[n][i] = -INFINITY;
-                }
-                top[0] = fmaxf(top[0], fmaxf(s[n][0], s[n][1]));
-                top[1] = fmaxf(top[1], fmaxf(s[n][2], s[n][3]));
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-            }
-            if (__any_sync(0xffffffffu, top[0] > st.m[0] || top[1] > st.m[1])) {
+            for (int t = 0; t < S::KG; ++t) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const float up = fmaxf(st.m[h], top[h]), f = st.m[h] == -INFINITY ? 0.f : ex2(st.m[h] - up);
-                    st.m[h] = up;
-                    st.l[h] *= f;
-#pragma unroll
-                    for (int i = 0; i < S::DT; ++i) {
-                        st.o[i][2 * h] *= f;
-                        st.o[i][2 * h + 1] *= f;
+                    const int x = 16 * t + 8 * h + quad;
+                    float fa = scale2, fb = 0.f;
+                    if (CODES) {
+                        uint16_t ks, vs;
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(ks) : "r"(sb + x * 2));
+                        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(vs) : "r"(sb + 128 + x * 2));
+                        // (the scale of a cell that no row sees may be anything)
+                        const bool seen = !edge || seen_by_some(x);
+                        fa = seen ? scale2 * half_float(ks) : 1.f;
+                        fb = seen ? lg2(half_float(vs)) : 0.f;
+                        inv[t][h] = ex2(-fb);
                     }
-                }
-            }
-            const float ref[2] = {st.m[0] == -INFINITY ? 0.f : st.m[0], st.m[1] == -INFINITY ? 0.f : st.m[1]};
-            uint32_t p[S::NT][2];
 #pragma unroll
-            for (int n = 0; n < S::NT; ++n) {
-                float e[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    e[i] = ex2(s[n][i] - ref[i >> 1]);
-                    if (FMT == KV_FP16) st.l[i >> 1] += e[i];
-                    else if (!edge || s[n][i] != -INFINITY) st.l[i >> 1] = fmaf(e[i], inv[n][i & 1], st.l[i >> 1]);   // (the scale of a cell that is not there may be anything)
-                }
-                p[n][0] = floats_half2(e[0], e[1]);
-                p[n][1] = floats_half2(e[2], e[3]);
-            }
-#pragma unroll
-            for (int j = 0; j < S::KT / 16; ++j) {
-                const uint32_t a0 = p[2 * j][0], a1 = p[2 * j][1], a2 = p[2 * j + 1][0], a3 = p[2 * j + 1][1];
-#pragma unroll
-                for (int d = 0; d < S::ROW / 32; ++d) {   // two 16-byte pieces of 16 keys
-                    uint32_t r[4];
-                    ldsm_x4_t(chunk_at<FMT, D>(vb, 16 * j + ((lane >> 3) & 1) * 8 + (lane & 7), 2 * d + (lane >> 4)), r[0], r[1], r[2], r[3]);
-                    if (FMT == KV_FP16) {
-                        mma_16816(st.o[2 * d], a0, a1, a2, a3, r[0], r[1]);
-                        mma_16816(st.o[2 * d + 1], a0, a1, a2, a3, r[2], r[3]);
-                    } else {
-                        // a word holds dims 2 quad and 2 quad + 1 of two keys: one product for the even dims, one for the odd ones
+                    for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            uint32_t e0, o0, e1, o1;
-                            codes_to_half2x2<FMT>(__byte_perm(r[2 * i], 0u, 0x3120), e0, o0);
-                            codes_to_half2x2<FMT>(__byte_perm(r[2 * i + 1], 0u, 0x3120), e1, o1);
-                            mma_16816(st.o[4 * d + 2 * i], a0, a1, a2, a3, e0, e1);
-                            mma_16816(st.o[4 * d + 2 * i + 1], a0, a1, a2, a3, o0, o1);
+                            float& y = s[b][t][2 * h + i];
+                            y = CODES ? fmaf(y, fa, fb) : y * fa;
+                            if (edge && !(key_visible(k0 + x, pos[b][i], w.window, w.sinks) && (here >> (x >> box_shift) & 1u))) y = -INFINITY;
+                            top[b][i] = fmaxf(top[b][i], y);
+                        }
+                }
+            }
+            bool grows = false;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top[b][i] = fmaxf(top[b][i], __shfl_xor_sync(0xffffffffu, top[b][i], d));
+                    grows |= top[b][i] > st.m[b][i];
+                }
+            if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const float u0 = fmaxf(st.m[b][0], top[b][0]), u1 = fmaxf(st.m[b][1], top[b][1]);
+                    st.rescale(b, st.m[b][0] == -INFINITY ? 0.f : ex2(st.m[b][0] - u0), st.m[b][1] == -INFINITY ? 0.f : ex2(st.m[b][1] - u1));
+                    st.m[b][0] = u0;
+                    st.m[b][1] = u1;
+                }
+            }
+            // ---- weights, and their product with the values: rows are dims ----
+            uint32_t p[NB][S::KG][2];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                const float r0 = st.m[b][0] == -INFINITY ? 0.f : st.m[b][0], r1 = st.m[b][1] == -INFINITY ? 0.f : st.m[b][1];
+#pragma unroll
+                for (int t = 0; t < S::KG; ++t)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float e0 = ex2(s[b][t][2 * h] - r0), e1 = ex2(s[b][t][2 * h + 1] - r1);
+                        st.l[b][0] = CODES ? fmaf(e0, inv[t][h], st.l[b][0]) : st.l[b][0] + e0;
+                        st.l[b][1] = CODES ? fmaf(e1, inv[t][h], st.l[b][1]) : st.l[b][1] + e1;
+                        p[b][t][h] = turned(floats_half2(e0, e1));
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < S::KG; ++t) {
+                // 16 keys, 32 bytes: matrices of 8 keys x 16 bytes.  fp16: a0 (dims 0-7, keys 0-7), a1 (dims 8-15), a2 and a3 keys 8-15.  Codes: two
+                // pieces of 16 dims; a word holds two dims of two keys
+                const int vrow = 16 * t + (lane & 7) + (CODES ? (lane & 8) : (lane >> 4) * 8), vpiece = CODES ? lane >> 4 : lane >> 3 & 1;
+#pragma unroll
+                for (int j = 0; j < S::ROW / 32; ++j) {
+                    uint32_t r[4];
+                    ldsm_x4_t(chunk_at<FMT, D>(vb, vrow, 2 * j + vpiece), r[0], r[1], r[2], r[3]);
+                    if (!CODES) {
+#pragma unroll
+                        for (int b = 0; b < NB; ++b) mma_16816(reinterpret_cast<float(&)[4]>(st.o[b][j]), r[0], r[1], r[2], r[3], p[b][t][0], p[b][t][1]);
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            uint32_t a0, a1, a2, a3;
+                            codes_even_odd<FMT>(r[2 * x], a0, a1);
+                            codes_even_odd<FMT>(r[2 * x + 1], a2, a3);
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) mma_16816(reinterpret_cast<float(&)[4]>(st.o[b][2 * j + x]), a0, a1, a2, a3, p[b][t][0], p[b][t][1]);
                         }
                     }
                 }
@@ -386,101 +469,145 @@ __global__ void __launch_bounds__(WARPS * 32, 1) attention_decode_kernel(const _
             if (!dead) issue();
         }
 
-        // ---- the block's result of this segment, in warp 0 ----
+        // ---- the block's result of this segment: each warp's, or (where the rings are in use) their sum, and from there by all threads ----
         st.close();
-        merge_warps<FMT, D>(st, smem + S_MERGE, warp, two);
+        const bool last = walk.u >= walk.end;
+        const uint8_t* dumps = smem + (last ? S_RING : S_MERGE);
+        int parts = last ? min(WARPS, sg.count) : 1;   // (warps that have had a slice)
+        if (!last) merge_warps<D, NB>(st, smem + S_MERGE, warp);
+        if (warp < parts) st.store(reinterpret_cast<float4*>(smem + (last ? S_RING : S_MERGE) + warp * (STAGES * STAGE)));
+        unsigned* const bad = reinterpret_cast<unsigned*>(smem + S_FLAG) + 4;   // rows that are not finite, or see nothing
+        volatile int* const flag = reinterpret_cast<volatile int*>(smem + S_FLAG);
+        if (tid == 0) *bad = 0u;
+        __syncthreads();
+        constexpr int QUADS = D / 16, ALL = NB * QUADS, SHARE = WARPS / ALL > 0 ? WARPS / ALL : 1;   // warps to a quad of the joined parts
+        int stride = STAGES * STAGE;
         bool whole = sg.count == sg.total;
         if (!whole) {   // one of several blocks: the last to arrive adds the parts up, in the blocks' order
-            const int b0 = (int)(sg.unit0 / chunk), b1 = (int)((sg.unit0 + sg.total - 1) / chunk);
-            volatile int* flag = reinterpret_cast<volatile int*>(smem + S_FLAG);
-            float4* parts = reinterpret_cast<float4*>(a.parts);
-            if (warp == 0) {
-                st.store(parts + (int64_t)(2 * blockIdx.x + (sg.first == 0 ? 1 : 0)) * (ATTN_DECODE_PART / 16), two);
-                __threadfence();
-                __syncwarp();
-                if (lane == 0) {
-                    const unsigned before = atomicAdd(a.counters + b0, 1u);
-                    const bool last = before == (unsigned)(b1 - b0);
-                    if (last) a.counters[b0] = 0u;
-                    *flag = last;
-                }
+            float4* const slots = reinterpret_cast<float4*>(a.parts);
+            const int b0 = (int)quotient(sg.unit0, chunk), b1 = (int)quotient(sg.unit0 + sg.total - 1, chunk);
+            float4* const slot = slots + (int64_t)(2 * blockIdx.x + (sg.first == 0 ? 1 : 0)) * (ATTN_DECODE_PART / 16);
+            for (int k = warp; k < ALL; k += WARPS) {
+                const Quad x = add_up<NB>(k, QUADS, parts, [&](int i) { return reinterpret_cast<const float4*>(dumps + i * stride); });
+                slot[(NB + k) * 32 + lane] = x.v;
+                if (k % QUADS == 0) slot[k / QUADS * 32 + lane] = x.h;
+            }
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                const bool done = atomicAdd(a.counters + b0, 1u) == (unsigned)(b1 - b0);
+                if (done) a.counters[b0] = 0u;
+                *flag = done;
             }
             __syncthreads();
             whole = *flag != 0;
             if (whole) {
                 __threadfence();
-                st.clear();
-                for (int b = b0 + warp; b <= b1; b += WARPS) st.add(parts + (int64_t)(2 * b + (b == b0 ? 1 : 0)) * (ATTN_DECODE_PART / 16), two);
-                merge_warps<FMT, D>(st, smem + S_MERGE, warp, two);
+                const int n = b1 - b0 + 1, per = (n + SHARE - 1) / SHARE;
+                float4* const mid = reinterpret_cast<float4*>(smem + S_MERGE);
+#pragma unroll 1
+                for (int x = warp; x < ALL * SHARE; x += WARPS) {
+                    const int k = x % ALL, lo = x / ALL * per;
+                    const Quad y = add_up<NB>(k, QUADS, min(per, n - lo), [&](int i) {
+                        const int b = b0 + lo + i;
+                        return const_cast<const float4*>(slots) + (int64_t)(2 * b + (b == b0 ? 1 : 0)) * (ATTN_DECODE_PART / 16);
+                    });
+                    float4* const d = mid + x / ALL * ((NB + ALL) * 32);
+                    d[(NB + k) * 32 + lane] = y.v;
+                    if (k % QUADS == 0) d[k / QUADS * 32 + lane] = y.h;
+                }
+                __syncthreads();
+                dumps = smem + S_MERGE;
+                parts = SHARE;
+                stride = (NB + ALL) * 512;
+            }
+        }
+        static_assert(SHARE * (NB + ALL) * 512 <= 2 * (int)ATTN_DECODE_PART && (NB + ALL) * 512 <= (int)ATTN_DECODE_PART, "partial results");
+        if (whole) {
+            constexpr int N = (ALL + WARPS - 1) / WARPS;
+            Quad x[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int k = warp + i * WARPS;
+                if (k < ALL) {
+                    x[i] = add_up<NB>(k, QUADS, parts, [&](int y) { return reinterpret_cast<const float4*>(dumps + y * stride); });
+                    float4& v = x[i].v;
+                    const float f0 = 1.f / x[i].h.y, f1 = 1.f / x[i].h.w;
+                    v = make_float4(v.x * f0, v.y * f1, v.z * f0, v.w * f1);
+                    const bool fine0 = x[i].h.y > 0.f && x[i].h.y < INFINITY && fabsf(v.x) < INFINITY && fabsf(v.z) < INFINITY;
+                    const bool fine1 = x[i].h.w > 0.f && x[i].h.w < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.w) < INFINITY;
+                    const int r = k / QUADS * 8 + 2 * c;
+                    if (!fine0 || !fine1) atomicOr(bad, (fine0 ? 0u : 1u << r) | (fine1 ? 0u : 2u << r));
+                }
             }
             __syncthreads();
-        }
-        if (whole && warp == 0) {
-            unsigned again[2];   // rows that are not finite, or see nothing: from the formula once more, which does not touch hidden cells
+            const unsigned again = *bad;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float f = 1.f / st.l[h];
-                bool fine = st.l[h] > 0.f && st.l[h] < INFINITY;
+            for (int i = 0; i < N; ++i) {
+                const int k = warp + i * WARPS;
 #pragma unroll
-                for (int i = 0; i < S::DT; ++i) {
-                    st.o[i][2 * h] *= f;
-                    st.o[i][2 * h + 1] *= f;
-                    fine = fine && fabsf(st.o[i][2 * h]) < INFINITY && fabsf(st.o[i][2 * h + 1]) < INFINITY;
-                }
-                unsigned bad = __ballot_sync(0xffffffffu, !fine && row[h] >= 0);
-                bad |= bad >> 1;
-                bad |= bad >> 2;
-                again[h] = bad & 0x11111111u;
-                if (row[h] >= 0 && !(again[h] >> (lane & 28) & 1u)) {
-                    uint32_t* out = reinterpret_cast<uint32_t*>(a.out + (int64_t)row[h] * a.o_stride + (int64_t)head[h] * D);
-#pragma unroll
-                    for (int i = 0; i < S::DT; ++i) {
-                        if (FMT == KV_FP16) out[4 * i + c] = floats_half2(st.o[i][2 * h], st.o[i][2 * h + 1]);
-                        else if (i % 2 == 0)   // dims 4c .. of 16: even, odd, even, odd
-                            *reinterpret_cast<uint2*>(out + 4 * i + 2 * c) = make_uint2(floats_half2(st.o[i][2 * h], st.o[i + 1][2 * h]),
-                                                                                      floats_half2(st.o[i][2 * h + 1], st.o[i + 1][2 * h + 1]));
+                for (int h = 0; h < 2; ++h) {
+                    const int r = k / QUADS * 8 + 2 * c + h, row = k < ALL ? row_of(r) : -1;
+                    if (row < 0 || (again >> r & 1u)) continue;
+                    uint16_t* out = a.out + (int64_t)row * a.o_stride + (int64_t)head_of(r) * D + k % QUADS * 16;
+                    const uint32_t two = floats_half2(h ? x[i].v.y : x[i].v.x, h ? x[i].v.w : x[i].v.z);
+                    if (CODES) {
+                        reinterpret_cast<uint32_t*>(out)[quad] = two;
+                    } else {
+                        out[quad] = (uint16_t)two;
+                        out[quad + 8] = (uint16_t)(two >> 16);
                     }
                 }
             }
-#pragma unroll 1
-            for (int h = 0; h < 2; ++h)
-                for (unsigned left = again[h]; left; left &= left - 1) {
-                    const int from = __ffs(left) - 1;
-                    const int r = __shfl_sync(0xffffffffu, row[h], from), hd = __shfl_sync(0xffffffffu, head[h], from), ps2 = __shfl_sync(0xffffffffu, pos[h], from);
-                    if (!attend_row<FMT, D>(a, sg.seq, sg.len, ps2, r, hd) && lane == 0) *a.status = STATUS_BAD_TABLE;
-                }
+            // ... from the formula once more, which does not touch hidden cells; a warp each
+            int turn = 0;
+            for (unsigned left = again; left; left &= left - 1) {
+                const int r = __ffs(left) - 1, row = row_of(r);
+                if (row < 0 || turn++ % WARPS != warp) continue;
+                if (!attend_row<FMT, D>(a, sg.seq, sg.len, pos_of(r), row, head_of(r)) && lane == 0) *a.status = STATUS_BAD_TABLE;
+            }
         }
+        if (!last) __syncthreads();   // (the buffers are free again)
     }
     // (after a wait that ran out: what was asked for must land before the block's memory is given back)
     if (dead)
         for (int i = issued < STAGES ? 0 : issued - STAGES; i < issued; ++i) mbar_wait_bounded_warp(bars + (i % STAGES) * 8, (i / STAGES) & 1);
 }
 
+template <int FMT, int D, int NB>
+cudaError_t configure() {
+    return cudaFuncSetAttribute(attention_decode_kernel<FMT, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+}
+template <int FMT, int D>
+cudaError_t configure() {
+    const cudaError_t e = configure<FMT, D, 1>();
+    return e != cudaSuccess ? e : configure<FMT, D, 2>();
+}
+template <int FMT, int D>
+auto kernel(bool one_tile) {
+    return one_tile ? attention_decode_kernel<FMT, D, 1> : attention_decode_kernel<FMT, D, 2>;
+}
+
 }  // namespace
 
 cudaError_t attention_decode_configure() {
-    cudaError_t e = cudaSuccess;
-    auto one = [&](auto* k) {
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
-    };
-    one(attention_decode_kernel<KV_FP16, 64>);
-    one(attention_decode_kernel<KV_FP16, 128>);
-    one(attention_decode_kernel<KV_INT8, 64>);
-    one(attention_decode_kernel<KV_INT8, 128>);
-    one(attention_decode_kernel<KV_FP8, 64>);
-    one(attention_decode_kernel<KV_FP8, 128>);
-    return e;
+    cudaError_t e;
+    if ((e = configure<KV_FP16, 64>()) != cudaSuccess || (e = configure<KV_FP16, 128>()) != cudaSuccess || (e = configure<KV_INT8, 64>()) != cudaSuccess ||
+        (e = configure<KV_INT8, 128>()) != cudaSuccess || (e = configure<KV_FP8, 64>()) != cudaSuccess)
+        return e;
+    return configure<KV_FP8, 128>();
 }
 
 int attention_decode_keys(int fmt, int dim) { return PART / (dim * kv_cell_bytes(fmt)); }
 
-cudaError_t launch_attention_decode(const AttnArgs& a, const AttnMaps& maps, int sm_count, cudaStream_t st, bool pdl) {
-    auto k = a.c.fmt == KV_FP16 ? (a.c.dim == 64 ? attention_decode_kernel<KV_FP16, 64> : attention_decode_kernel<KV_FP16, 128>)
-             : a.c.fmt == KV_INT8 ? (a.c.dim == 64 ? attention_decode_kernel<KV_INT8, 64> : attention_decode_kernel<KV_INT8, 128>)
-                                  : (a.c.dim == 64 ? attention_decode_kernel<KV_FP8, 64> : attention_decode_kernel<KV_FP8, 128>);
+cudaError_t launch_attention_decode(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl) {
+    const bool one = (long long)a.group * max_new <= 8;   // one tile of 8 rows
+    auto k = a.c.fmt == KV_FP16 ? (a.c.dim == 64 ? kernel<KV_FP16, 64>(one) : kernel<KV_FP16, 128>(one))
+             : a.c.fmt == KV_INT8 ? (a.c.dim == 64 ? kernel<KV_INT8, 64>(one) : kernel<KV_INT8, 128>(one))
+                                  : (a.c.dim == 64 ? kernel<KV_FP8, 64>(one) : kernel<KV_FP8, 128>(one));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(sm_count < ATTN_MAX_BLOCKS ? sm_count : ATTN_MAX_BLOCKS));
-    cfg.blockDim = dim3(WARPS * 32);
+    cfg.blockDim = dim3(THREADS);
     cfg.dynamicSmemBytes = SMEM_BYTES;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];

@@ -48,16 +48,32 @@ __device__ __forceinline__ int item_tiles(const SeqWork& q, const WorkShape& w, 
     const int p0 = q.len - q.n + qt * w.tokens, p1 = q.len - q.n + min((qt + 1) * w.tokens, q.n) - 1;
     return max(1, visible_tiles(p0, p1, w.window, w.sinks, w.tile).tiles());
 }
-// Key tiles of all query tiles of a sequence; by a whole warp.
+// Key tiles of all query tiles of a sequence; by each lane for one of its own.  (`deep`: some lane's sequence has many query tiles: the warp
+// goes through them together.)
 __device__ __forceinline__ long long seq_tiles(const SeqWork& q, const WorkShape& w) {
+    const int lane = threadIdx.x & 31;
     long long t = 0;
-    for (int i = threadIdx.x & 31; i < q.tiles_q; i += 32) t += item_tiles(q, w, i);
-    if (q.tiles_q > 1) {   // (uniform)
+    const bool deep = q.tiles_q > 4;
+    if (!deep)
+        for (int i = 0; i < q.tiles_q; ++i) t += item_tiles(q, w, i);
+    for (unsigned left = __ballot_sync(0xffffffffu, deep); left; left &= left - 1) {
+        const int from = __ffs(left) - 1;
+        SeqWork o;
+        o.row0 = 0;
+        o.n = __shfl_sync(0xffffffffu, q.n, from);
+        o.len = __shfl_sync(0xffffffffu, q.len, from);
+        o.tiles_q = __shfl_sync(0xffffffffu, q.tiles_q, from);
+        long long x = 0;
+        for (int i = lane; i < o.tiles_q; i += 32) x += item_tiles(o, w, i);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        return t;
+        for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+        if (lane == from) t = x;
     }
-    return __shfl_sync(0xffffffffu, t, 0);
+    return t;
+}
+// (the quotient of 64-bit numbers takes a few hundred clocks; they nearly always fit 32 bits)
+__device__ __forceinline__ long long quotient(long long x, long long y) {
+    return ((x | y) >> 31) == 0 ? (long long)((unsigned)x / (unsigned)y) : x / y;
 }
 
 // Where a block's units are.  Copies of a walk go on independently; next() is called by whole warps.
@@ -97,91 +113,82 @@ struct Walk {
     }
 };
 
-struct WorkShared {
-    static constexpr int SEQS = 256;
-    SeqWork q[SEQS];
-    long long units[SEQS];
-};
-
-// The walk of this block, by all its threads.  `least`: the fewest units that are worth a block.  *chunk: units of a block.
-// (Two passes over the sequences: how many units there are, then where this block's begin.  The first of up to 256 sequences keeps
-// everything in shared memory for the second.)
-__device__ __forceinline__ Walk find_work(const KvSeqs& s, const WorkShape& w, WorkShared* sh, int least, long long* chunk, int* status) {
-    const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x / 32, warp = tid / 32;
+// The walk of this block, found by each warp for itself: two passes over the sequences, one per lane, how many units there are and where this
+// block's begin.  `least`: the fewest units that are worth a block.  *chunk: units of a block.
+__device__ __forceinline__ Walk find_work(const KvSeqs& s, const WorkShape& w, int least, long long* chunk, int* status) {
+    const int lane = threadIdx.x & 31;
     Walk k;
     k.u = k.end = 0;
     k.seq = k.vhead = k.qt = k.first = 0;
     k.q = SeqWork{0, 0, 0, 0};
-    long long total = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        long long base = 0;
-        for (int c0 = 0; c0 < s.num_seqs; c0 += WorkShared::SEQS) {
-            const int cnt = min(WorkShared::SEQS, s.num_seqs - c0);
-            if (pass == 0 || s.num_seqs > WorkShared::SEQS) {
-                __syncthreads();
-                for (int i = tid; i < cnt; i += blockDim.x) {
-                    bool bad;
-                    sh->q[i] = load_seq(s, w, c0 + i, &bad);
-                    if (bad) *status = STATUS_BAD_TABLE;
-                }
-                __syncthreads();
-                for (int i = warp; i < cnt; i += warps) {
-                    const long long t = seq_tiles(sh->q[i], w);
-                    if (lane == 0) sh->units[i] = t * w.vheads;
-                }
-                __syncthreads();
-            }
-            for (int i0 = 0; i0 < cnt; i0 += 32) {
-                const long long mine = i0 + lane < cnt ? sh->units[i0 + lane] : 0;
-                long long upto = mine;
+    SeqWork q = k.q;
+    long long mine = 0, total = 0;
+    auto load = [&](int i0) {
+        bool bad = false;
+        q = SeqWork{0, 0, 0, 0};
+        if (i0 + lane < s.num_seqs) q = load_seq(s, w, i0 + lane, &bad);
+        if (bad) *status = STATUS_BAD_TABLE;
+        mine = seq_tiles(q, w) * w.vheads;
+    };
+    for (int i0 = 0; i0 < s.num_seqs; i0 += 32) {
+        load(i0);
+        long long t = mine;
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += x;
-                }
-                if (pass == 1) {
-                    const unsigned hit = __ballot_sync(0xffffffffu, base + upto > k.u);
-                    if (hit) {   // the sequence of the block's first unit
-                        const int l = __ffs(hit) - 1;
-                        const long long before = base + __shfl_sync(0xffffffffu, upto - mine, l);
-                        const long long per_head = __shfl_sync(0xffffffffu, mine, l) / w.vheads;
-                        long long rest = k.u - before;
-                        k.seq = c0 + i0 + l;
-                        k.q = sh->q[i0 + l];
-                        k.vhead = (int)(rest / per_head);
-                        rest -= k.vhead * per_head;
-                        for (int q0 = 0;; q0 += 32) {   // and its query tile
-                            long long n = q0 + lane < k.q.tiles_q ? item_tiles(k.q, w, q0 + lane) : 0, run = n;
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        total += t;
+    }
+    const long long c = quotient(total + gridDim.x - 1, gridDim.x);
+    *chunk = c < least ? least : c;
+    k.u = blockIdx.x * *chunk;
+    k.end = min(total, k.u + *chunk);
+    if (k.u >= total) {
+        k.u = k.end = 0;
+        return k;
+    }
+    long long base = 0;
+    for (int i0 = 0; i0 < s.num_seqs; i0 += 32) {
+        if (s.num_seqs > 32) load(i0);
+        long long upto = mine;
 #pragma unroll
-                            for (int o = 1; o < 32; o <<= 1) {
-                                const long long x = __shfl_up_sync(0xffffffffu, run, o);
-                                if (lane >= o) run += x;
-                            }
-                            const unsigned in = __ballot_sync(0xffffffffu, run > rest);
-                            if (in || q0 + 32 >= k.q.tiles_q) {
-                                const int j = in ? __ffs(in) - 1 : 0;
-                                k.qt = q0 + j;
-                                k.first = (int)(rest - __shfl_sync(0xffffffffu, run - n, j));
-                                break;
-                            }
-                            rest -= __shfl_sync(0xffffffffu, run, 31);
-                        }
-                        return k;
-                    }
-                }
-                base += __shfl_sync(0xffffffffu, upto, 31);
-            }
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
         }
-        if (pass == 0) {
-            total = base;
-            long long c = (total + gridDim.x - 1) / gridDim.x;
-            *chunk = c < least ? least : c;
-            k.u = blockIdx.x * *chunk;
-            k.end = min(total, k.u + *chunk);
-            if (k.u >= total) {
-                k.u = k.end = 0;
+        const unsigned hit = __ballot_sync(0xffffffffu, base + upto > k.u);
+        if (!hit) {
+            base += __shfl_sync(0xffffffffu, upto, 31);
+            continue;
+        }
+        const int l = __ffs(hit) - 1;   // the sequence of the block's first unit
+        long long rest = k.u - base - __shfl_sync(0xffffffffu, upto - mine, l);
+        const long long per_head = quotient(__shfl_sync(0xffffffffu, mine, l), w.vheads);
+        k.seq = i0 + l;
+        k.q.row0 = __shfl_sync(0xffffffffu, q.row0, l);
+        k.q.n = __shfl_sync(0xffffffffu, q.n, l);
+        k.q.len = __shfl_sync(0xffffffffu, q.len, l);
+        k.q.tiles_q = __shfl_sync(0xffffffffu, q.tiles_q, l);
+        k.vhead = (int)quotient(rest, per_head);
+        rest -= k.vhead * per_head;
+        if (k.q.tiles_q == 1) {
+            k.first = (int)rest;
+            return k;
+        }
+        for (int q0 = 0;; q0 += 32) {   // and its query tile
+            const long long n = q0 + lane < k.q.tiles_q ? item_tiles(k.q, w, q0 + lane) : 0;
+            long long run = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, run, o);
+                if (lane >= o) run += x;
+            }
+            const unsigned in = __ballot_sync(0xffffffffu, run > rest);
+            if (in || q0 + 32 >= k.q.tiles_q) {
+                const int j = in ? __ffs(in) - 1 : 0;
+                k.qt = q0 + j;
+                k.first = (int)(rest - __shfl_sync(0xffffffffu, run - n, j));
                 return k;
             }
+            rest -= __shfl_sync(0xffffffffu, run, 31);
         }
     }
     return k;
