@@ -34,8 +34,19 @@ cudaError_t attention_configure() {
     return e != cudaSuccess ? e : attention_chunk_configure();
 }
 
+// Few rows to a cache head go to the kernel that is bound by the cache's bytes, ...
+static bool few_rows(const AttnArgs& a, int max_new) { return a.group <= 16 && (long long)a.group * max_new <= 64; }
+
+bool attention_countable(const AttnArgs& a, int max_new) {
+    const bool few = few_rows(a, max_new);
+    const long long tile = few ? attention_decode_keys(a.c.fmt, a.c.dim) : 128;
+    const long long parts = few ? 1 : (a.group + 127) / 128, group = (a.group + parts - 1) / parts, tokens = few ? 8 / a.group > 0 ? 8 / a.group : 1 : 2 * (128 / group);
+    const double items = (double)a.c.kv_heads * parts * ((double)a.s.num_rows / tokens + a.s.num_seqs);
+    return items * ((double)a.s.max_len / tile + 2) < (double)(1 << 30);
+}
+
 cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl) {
-    if (a.group <= 16 && (long long)a.group * max_new <= 16) return launch_attention_decode(a, maps, max_new, sm_count, st, pdl);
+    if (few_rows(a, max_new)) return launch_attention_decode(a, maps, max_new, sm_count, st, pdl);
     return launch_attention_chunk(a, maps, sm_count, st, pdl);
 }
 

@@ -66,6 +66,7 @@ struct AttnArgs {
 struct AttnMaps;
 cudaError_t attention_configure();
 cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl);
+bool attention_countable(const AttnArgs& a, int max_new);   // whether the call's tiles of work surely stay below 2^30
 constexpr int ATTN_MAX_BLOCKS = 256;
 constexpr size_t ATTN_DECODE_PART = 18 * 512, ATTN_CHUNK_PART = 256 * 128 * 4 + 256 * 8;   // two per block
 // The workspace: counters, items, parts.

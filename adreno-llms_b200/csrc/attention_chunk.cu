@@ -214,11 +214,10 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     w.tile = BN;
     w.window = a.window;
     w.sinks = a.sinks;
-    long long chunk;
     Steps& steps = reinterpret_cast<Steps*>(smem + C::O_WALK)[warp];
     Segment& sg = steps.sg;
     {
-        const Walk walk = find_work(a.s, w, 2, &chunk, a.status);
+        const Walk walk = find_work(a.s, &w, 2, a.status);
         if (lane == 0) steps.walk = walk;
     }
     auto next_segment = [&]() {
@@ -443,7 +442,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 }
                 if (!whole) {
                     if (c == 0) reinterpret_cast<float2*>(part + 64 * D)[i * 128 + r] = make_float2(m, l);
-                    if (sg.first == 0 && tid == 0) *info = make_int4(sg.seq, sg.vhead, sg.qt, (int)((sg.unit0 + sg.total - 1) / chunk));
+                    if (sg.first == 0 && tid == 0) *info = make_int4(sg.seq, sg.vhead, sg.qt, (int)((sg.unit0 + sg.total - 1) / w.chunk));
                 } else {
                     // rows that are not finite, or see nothing: from the formula once more, which does not touch hidden cells
                     for (unsigned left = c == 0 ? __ballot_sync(0xffffffffu, on && !fine) : 0u; left; left &= left - 1) {

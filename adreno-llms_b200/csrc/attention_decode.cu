@@ -220,8 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
     w.tile = S::KT;
     w.window = a.window;
     w.sinks = a.sinks;
-    long long chunk;
-    Walk walk = find_work(a.s, w, WARPS, &chunk, a.status);
+    Walk walk = find_work(a.s, &w, WARPS, a.status);
     if (walk.u >= walk.end) return;
 
     const int shift = a.c.page_shift, box = min(S::KT, 1 << shift), nbox = S::KT / box, box_shift = 31 - __clz(box), nbox_shift = 31 - __clz(nbox);
@@ -292,8 +291,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
         pslice += WARPS;
         ++issued;
     };
-#pragma unroll 1
-    for (int i = 0; i < STAGES; ++i) issue();
 
     int used = 0;
     bool dead = false;
@@ -328,6 +325,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
         st.clear();
 #pragma unroll 1
         for (int slice = warp; slice < sg.count; slice += WARPS) {
+#pragma unroll 1
+            while (!dead && pmore && issued < used + STAGES) issue();
             const int stage = used % STAGES;
             if (!dead && !mbar_wait_bounded_warp(bars + stage * 8, (used / STAGES) & 1)) {
                 dead = true;
@@ -466,7 +465,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
             }
             if (edge) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // (the zeros above, before a copy lands there)
             __syncwarp();
-            if (!dead) issue();
         }
 
         // ---- the block's result of this segment: each warp's, or (where the rings are in use) their sum, and from there by all threads ----
@@ -485,7 +483,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
         bool whole = sg.count == sg.total;
         if (!whole) {   // one of several blocks: the last to arrive adds the parts up, in the blocks' order
             float4* const slots = reinterpret_cast<float4*>(a.parts);
-            const int b0 = (int)quotient(sg.unit0, chunk), b1 = (int)quotient(sg.unit0 + sg.total - 1, chunk);
+            const int b0 = (int)(sg.unit0 / w.chunk), b1 = (int)((sg.unit0 + sg.total - 1) / w.chunk);
             float4* const slot = slots + (int64_t)(2 * blockIdx.x + (sg.first == 0 ? 1 : 0)) * (ATTN_DECODE_PART / 16);
             for (int k = warp; k < ALL; k += WARPS) {
                 const Quad x = add_up<NB>(k, QUADS, parts, [&](int i) { return reinterpret_cast<const float4*>(dumps + i * stride); });

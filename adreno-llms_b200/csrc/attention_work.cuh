@@ -5,6 +5,8 @@
 // sequence, head and query tile, their key tiles are strung together, and block b takes units [b * chunk, (b + 1) * chunk) of that string:
 // every block has the same number, whatever the lengths are, and all lengths stay on the device, so that a recorded call takes new ones.
 // A piece of an item in one block is a segment; the blocks of an item that is cut leave partial results to be joined.
+// Where there are at least twice as many blocks as items, each item is filled up to whole chunks, so that no block has parts of two: it
+// would only have two segments to finish, one after the other.
 #pragma once
 #include "kv_cells.cuh"
 
@@ -16,6 +18,9 @@ struct WorkShape {
     int vheads;    // items side by side: cache heads (times the parts of a head's query heads)
     int tile;      // keys of a unit
     int window, sinks;
+    unsigned chunk;   // units of a block, and whether items are filled up to it
+    bool pad;
+    __device__ __forceinline__ unsigned padded(unsigned tiles) const { return pad ? (tiles + chunk - 1) / chunk * chunk : tiles; }
 };
 
 struct SeqWork {
@@ -27,7 +32,7 @@ struct Segment {
     int row0, n, len;       // of the sequence
     int first, count;       // key tiles [first, first + count) of the item
     int total;              // key tiles of the item
-    long long unit0;        // number of the item's first unit
+    unsigned unit0;         // number of the item's first unit
     // positions of the item's first and last token
     __device__ __forceinline__ int p0(const WorkShape& w) const { return len - n + qt * w.tokens; }
     __device__ __forceinline__ int p1(const WorkShape& w) const { return len - n + min((qt + 1) * w.tokens, n) - 1; }
@@ -48,14 +53,14 @@ __device__ __forceinline__ int item_tiles(const SeqWork& q, const WorkShape& w, 
     const int p0 = q.len - q.n + qt * w.tokens, p1 = q.len - q.n + min((qt + 1) * w.tokens, q.n) - 1;
     return max(1, visible_tiles(p0, p1, w.window, w.sinks, w.tile).tiles());
 }
-// Key tiles of all query tiles of a sequence; by each lane for one of its own.  (`deep`: some lane's sequence has many query tiles: the warp
-// goes through them together.)
-__device__ __forceinline__ long long seq_tiles(const SeqWork& q, const WorkShape& w) {
+// Units of all query tiles of a sequence; by each lane for one of its own.  (Where some lane's sequence has many, the warp goes through them
+// together.)
+__device__ __forceinline__ unsigned seq_tiles(const SeqWork& q, const WorkShape& w) {
     const int lane = threadIdx.x & 31;
-    long long t = 0;
+    unsigned t = 0;
     const bool deep = q.tiles_q > 4;
     if (!deep)
-        for (int i = 0; i < q.tiles_q; ++i) t += item_tiles(q, w, i);
+        for (int i = 0; i < q.tiles_q; ++i) t += w.padded(item_tiles(q, w, i));
     for (unsigned left = __ballot_sync(0xffffffffu, deep); left; left &= left - 1) {
         const int from = __ffs(left) - 1;
         SeqWork o;
@@ -63,22 +68,17 @@ __device__ __forceinline__ long long seq_tiles(const SeqWork& q, const WorkShape
         o.n = __shfl_sync(0xffffffffu, q.n, from);
         o.len = __shfl_sync(0xffffffffu, q.len, from);
         o.tiles_q = __shfl_sync(0xffffffffu, q.tiles_q, from);
-        long long x = 0;
-        for (int i = lane; i < o.tiles_q; i += 32) x += item_tiles(o, w, i);
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+        unsigned x = 0;
+        for (int i = lane; i < o.tiles_q; i += 32) x += w.padded(item_tiles(o, w, i));
+        x = __reduce_add_sync(0xffffffffu, x);
         if (lane == from) t = x;
     }
     return t;
 }
-// (the quotient of 64-bit numbers takes a few hundred clocks; they nearly always fit 32 bits)
-__device__ __forceinline__ long long quotient(long long x, long long y) {
-    return ((x | y) >> 31) == 0 ? (long long)((unsigned)x / (unsigned)y) : x / y;
-}
 
 // Where a block's units are.  Copies of a walk go on independently; next() is called by whole warps.
 struct Walk {
-    long long u, end;      // the next unit, and the block's last one + 1
+    unsigned u, end;      // the next unit, and the block's last one + 1
     int seq, vhead, qt, first;
     SeqWork q;
 
@@ -105,53 +105,51 @@ struct Walk {
         out->first = first;
         out->total = total;
         out->unit0 = u - first;
-        out->count = (int)min((long long)(total - first), end - u);
-        u += out->count;
+        out->count = (int)min((unsigned)(total - first), end - u);
+        u = w.pad ? end : u + out->count;
         first = 0;
         ++qt;
         return true;
     }
 };
 
-// The walk of this block, found by each warp for itself: two passes over the sequences, one per lane, how many units there are and where this
-// block's begin.  `least`: the fewest units that are worth a block.  *chunk: units of a block.
-__device__ __forceinline__ Walk find_work(const KvSeqs& s, const WorkShape& w, int least, long long* chunk, int* status) {
+// The walk of this block, found by each warp for itself: the sequences, one per lane, how many units there are and where this block's begin.
+// `least`: the fewest units that are worth a block.  w->chunk and w->pad are set.  (The host has seen to it that units are fewer than 2^31.)
+__device__ __forceinline__ Walk find_work(const KvSeqs& s, WorkShape* w, unsigned least, int* status) {
     const int lane = threadIdx.x & 31;
     Walk k;
     k.u = k.end = 0;
     k.seq = k.vhead = k.qt = k.first = 0;
     k.q = SeqWork{0, 0, 0, 0};
     SeqWork q = k.q;
-    long long mine = 0, total = 0;
+    unsigned total = 0, items = 0;
+    w->pad = false;
+    w->chunk = 1;
     auto load = [&](int i0) {
         bool bad = false;
         q = SeqWork{0, 0, 0, 0};
-        if (i0 + lane < s.num_seqs) q = load_seq(s, w, i0 + lane, &bad);
+        if (i0 + lane < s.num_seqs) q = load_seq(s, *w, i0 + lane, &bad);
         if (bad) *status = STATUS_BAD_TABLE;
-        mine = seq_tiles(q, w) * w.vheads;
     };
     for (int i0 = 0; i0 < s.num_seqs; i0 += 32) {
         load(i0);
-        long long t = mine;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        total += t;
+        total += __reduce_add_sync(0xffffffffu, seq_tiles(q, *w));
+        items += __reduce_add_sync(0xffffffffu, (unsigned)q.tiles_q);
     }
-    const long long c = quotient(total + gridDim.x - 1, gridDim.x);
-    *chunk = c < least ? least : c;
-    k.u = blockIdx.x * *chunk;
-    k.end = min(total, k.u + *chunk);
-    if (k.u >= total) {
-        k.u = k.end = 0;
-        return k;
-    }
-    long long base = 0;
+    total *= w->vheads;
+    items *= w->vheads;
+    w->pad = 2 * items <= gridDim.x;
+    const unsigned blocks = w->pad ? gridDim.x - items : gridDim.x;   // (filled up, items take up to one more block each)
+    w->chunk = max(least, (total + blocks - 1) / blocks);
+    k.u = blockIdx.x * w->chunk;
+    unsigned base = 0;
     for (int i0 = 0; i0 < s.num_seqs; i0 += 32) {
         if (s.num_seqs > 32) load(i0);
-        long long upto = mine;
+        const unsigned mine = seq_tiles(q, *w) * w->vheads;
+        unsigned upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            const unsigned x = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += x;
         }
         const unsigned hit = __ballot_sync(0xffffffffu, base + upto > k.u);
@@ -160,37 +158,39 @@ __device__ __forceinline__ Walk find_work(const KvSeqs& s, const WorkShape& w, i
             continue;
         }
         const int l = __ffs(hit) - 1;   // the sequence of the block's first unit
-        long long rest = k.u - base - __shfl_sync(0xffffffffu, upto - mine, l);
-        const long long per_head = quotient(__shfl_sync(0xffffffffu, mine, l), w.vheads);
+        unsigned rest = k.u - base - __shfl_sync(0xffffffffu, upto - mine, l);
+        const unsigned per_head = __shfl_sync(0xffffffffu, mine, l) / w->vheads;
         k.seq = i0 + l;
         k.q.row0 = __shfl_sync(0xffffffffu, q.row0, l);
         k.q.n = __shfl_sync(0xffffffffu, q.n, l);
         k.q.len = __shfl_sync(0xffffffffu, q.len, l);
         k.q.tiles_q = __shfl_sync(0xffffffffu, q.tiles_q, l);
-        k.vhead = (int)quotient(rest, per_head);
+        k.vhead = (int)(rest / per_head);
         rest -= k.vhead * per_head;
-        if (k.q.tiles_q == 1) {
-            k.first = (int)rest;
-            return k;
-        }
-        for (int q0 = 0;; q0 += 32) {   // and its query tile
-            const long long n = q0 + lane < k.q.tiles_q ? item_tiles(k.q, w, q0 + lane) : 0;
-            long long run = n;
+        if (k.q.tiles_q > 1) {
+            for (int q0 = 0;; q0 += 32) {   // and its query tile
+                const unsigned n = q0 + lane < k.q.tiles_q ? w->padded(item_tiles(k.q, *w, q0 + lane)) : 0u;
+                unsigned run = n;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= o) run += x;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned x = __shfl_up_sync(0xffffffffu, run, o);
+                    if (lane >= o) run += x;
+                }
+                const unsigned in = __ballot_sync(0xffffffffu, run > rest);
+                if (in || q0 + 32 >= k.q.tiles_q) {
+                    const int j = in ? __ffs(in) - 1 : 0;
+                    k.qt = q0 + j;
+                    rest -= __shfl_sync(0xffffffffu, run - n, j);
+                    break;
+                }
+                rest -= __shfl_sync(0xffffffffu, run, 31);
             }
-            const unsigned in = __ballot_sync(0xffffffffu, run > rest);
-            if (in || q0 + 32 >= k.q.tiles_q) {
-                const int j = in ? __ffs(in) - 1 : 0;
-                k.qt = q0 + j;
-                k.first = (int)(rest - __shfl_sync(0xffffffffu, run - n, j));
-                return k;
-            }
-            rest -= __shfl_sync(0xffffffffu, run, 31);
         }
+        k.first = (int)rest;
+        k.end = w->pad ? k.u + w->chunk : min(total, k.u + w->chunk);
+        return k;
     }
+    k.u = k.end = 0;   // no units for this block
     return k;
 }
 

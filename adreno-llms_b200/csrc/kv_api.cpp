@@ -287,6 +287,8 @@ extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b,
     a.scale = scale;
     a.window = window;
     a.sinks = window ? sinks : 0;   // (without a window all keys up to the row's own are visible)
+    if (!attention_countable(a, b->max_new))
+        return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: num_seqs=%d num_rows=%d max_len=%d: more than 2^30 tiles of work", who, b->num_seqs, b->num_rows, b->max_len);
     if ((rc = make_current(c, h, who))) return rc;
     a.status = c->status_dev;
     ProfScope prof(c, [&] { return std::string("attention_") + kv_name(a.c.fmt) + "_seqs" + std::to_string(b->num_seqs) + "_rows" + std::to_string(b->num_rows); });
