@@ -35,7 +35,13 @@ cudaError_t attention_configure() {
 }
 
 // Few rows to a cache head go to the kernel that is bound by the cache's bytes, ...
-static bool few_rows(const AttnArgs& a, int max_new) { return a.group <= 16 && (long long)a.group * max_new <= 64; }
+static bool few_rows(const AttnArgs& a, int max_new) {
+    const long long rows = (long long)a.group * max_new;
+    if (a.group > 16 || rows > 64) return false;
+    if (rows <= 16) return true;
+    if (a.c.dim != 64) return false;
+    return rows <= 32 || (double)a.s.num_seqs * a.s.max_len * a.c.kv_heads <= 65536.0;
+}
 
 bool attention_countable(const AttnArgs& a, int max_new) {
     const bool few = few_rows(a, max_new);

@@ -53,34 +53,34 @@ __device__ __forceinline__ uint2 encode8(const float (&f)[8], float scale) {
     return make_uint2(w[0], w[1]);
 }
 
-constexpr int WRITE_THREADS = 128;
+// A warp per row, or four where the rows are few (SPREAD); blocks of four warps.
+constexpr int WARPS = 4;
 
-// One block per row.
-template <int FMT, int D>
-__global__ void __launch_bounds__(WRITE_THREADS) kv_write_kernel(const KvWriteArgs a) {
-    constexpr int LANES = D / 16;
+template <int FMT, int D, bool SPREAD>
+__global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs a) {
+    constexpr int LANES = D / 16, HEADS = 32 / LANES * (SPREAD ? WARPS : 1);   // threads of a head's row; heads at a time
+    constexpr int AHEAD = SPREAD ? 1 : 3;                                      // loads of so many heads in flight
     pdl_launch_dependents();
     pdl_wait_prior_grid();
-    const int r = blockIdx.x;
-    const int seq = seq_of_row(a.s, r);
-    if (seq >= a.s.num_seqs || r < a.s.row_start[0]) return;   // a row behind the last sequence
-    const SeqExtent e = seq_extent(a.s.row_start[seq], a.s.row_start[seq + 1], a.s.kv_len[seq], a.s.num_rows, a.s.max_len);
-    const int pos = e.len - (e.row1 - r);
-    if (e.bad || pos < 0 || r < e.row0 || r >= e.row1 || (a.rotary && pos >= a.table_len)) {
-        if (threadIdx.x == 0) *a.status = STATUS_BAD_TABLE;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = SPREAD ? blockIdx.x : blockIdx.x * WARPS + warp;
+    if (r >= a.s.num_rows) return;
+    const RowPlace at = place_of_row(a.s, r);
+    if (at.none) return;
+    if (at.bad || (a.rotary && at.pos >= a.table_len)) {
+        if (lane == 0) *a.status = STATUS_BAD_TABLE;
         return;
     }
-    const int page = a.s.page_table[(int64_t)seq * a.s.table_stride + (pos >> a.c.page_shift)];
+    const int page = a.s.page_table[(int64_t)at.seq * a.s.table_stride + (at.pos >> a.c.page_shift)], slot = at.pos & ((1 << a.c.page_shift) - 1);
     const bool cell = page_ok(page, a.c.num_pages);
-    if (!cell && threadIdx.x == 0) *a.status = STATUS_BAD_TABLE;
-    const int j = threadIdx.x % LANES;
+    if (!cell && lane == 0) *a.status = STATUS_BAD_TABLE;
+    const int j = lane % LANES;
     int pa, pb;
     piece_pair(j, a.rotary, pa, pb);
     const bool turns = j < a.rotary / 16;
     float c[8], s[8];
     if (turns) {
-        const float4* ct = reinterpret_cast<const float4*>(a.cos + (int64_t)pos * (a.rotary / 2) + 8 * j);
-        const float4* st = reinterpret_cast<const float4*>(a.sin + (int64_t)pos * (a.rotary / 2) + 8 * j);
+        const float4* ct = reinterpret_cast<const float4*>(a.cos + (int64_t)at.pos * (a.rotary / 2) + 8 * j);
+        const float4* st = reinterpret_cast<const float4*>(a.sin + (int64_t)at.pos * (a.rotary / 2) + 8 * j);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const float4 x = ct[i], y = st[i];
@@ -88,16 +88,27 @@ __global__ void __launch_bounds__(WRITE_THREADS) kv_write_kernel(const KvWriteAr
             s[4 * i] = y.x, s[4 * i + 1] = y.y, s[4 * i + 2] = y.z, s[4 * i + 3] = y.w;
         }
     }
-    const int nq = a.q ? a.q_heads : 0, heads = nq + 2 * a.c.kv_heads;
-    for (int h0 = 0; h0 < heads; h0 += WRITE_THREADS / LANES) {   // (whole warps stay together for the shuffles)
-        const int h = h0 + threadIdx.x / LANES;
-        const bool on = h < heads, is_q = h < nq, is_k = !is_q && h < nq + a.c.kv_heads;
-        const int hc = is_k ? h - nq : h - nq - a.c.kv_heads;
-        const uint16_t* src = is_q ? a.q + r * a.q_stride + (int64_t)h * D : (is_k ? a.k + r * a.k_stride : a.v + r * a.v_stride) + (int64_t)hc * D;
-        float x[8], y[8];
-        if (on) {
-            unpack8(reinterpret_cast<const uint4*>(src)[pa], x);
-            unpack8(reinterpret_cast<const uint4*>(src)[pb], y);
+    const int nq = a.q ? a.q_heads : 0, heads = nq + 2 * a.c.kv_heads, first = (SPREAD ? threadIdx.x : lane) / LANES;
+    for (int h0 = 0; h0 < heads; h0 += HEADS * AHEAD) {   // (whole warps stay together for the shuffles)
+        uint4 in[AHEAD][2];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int h = h0 + u * HEADS + first;
+            in[u][0] = in[u][1] = make_uint4(0, 0, 0, 0);
+            if (h < heads) {
+                const uint16_t* src = h < nq ? a.q + r * a.q_stride + (int64_t)h * D
+                                             : h < nq + a.c.kv_heads ? a.k + r * a.k_stride + (int64_t)(h - nq) * D : a.v + r * a.v_stride + (int64_t)(h - nq - a.c.kv_heads) * D;
+                in[u][0] = reinterpret_cast<const uint4*>(src)[pa];
+                in[u][1] = reinterpret_cast<const uint4*>(src)[pb];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int h = h0 + u * HEADS + first;
+            const bool on = h < heads, is_q = h < nq, is_k = !is_q && h < nq + a.c.kv_heads;
+            float x[8], y[8];
+            unpack8(in[u][0], x);
+            unpack8(in[u][1], y);
             if (turns && (is_q || is_k)) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -107,104 +118,108 @@ __global__ void __launch_bounds__(WRITE_THREADS) kv_write_kernel(const KvWriteAr
                     y[i] = __half2float(__float2half_rn(t2));
                 }
             }
-            if (is_q) {
+            if (is_q) {   // (h < nq <= heads)
                 uint4* dst = reinterpret_cast<uint4*>(a.q_out + r * a.qo_stride + (int64_t)h * D);
                 dst[pa] = pack8(x);
                 dst[pb] = pack8(y);
             }
-        }
-        if (FMT == KV_FP16) {
-            if (on && !is_q && cell) {
-                const int64_t at = cell_row(page, hc, pos & ((1 << a.c.page_shift) - 1), a.c.kv_heads, a.c.page_shift);
-                uint4* dst = reinterpret_cast<uint4*>((uint16_t*)(is_k ? a.c.k : a.c.v) + at * D);
-                dst[pa] = pack8(x);
-                dst[pb] = pack8(y);
-            }
-        } else {
-            float most = 0.f;
-            bool nan = false;
-            if (on) {
+            const bool store = on && !is_q && cell;
+            const int64_t row = store ? cell_row(page, is_k ? h - nq : h - nq - a.c.kv_heads, slot, a.c.kv_heads, a.c.page_shift) : 0;
+            if (FMT == KV_FP16) {
+                if (store) {
+                    uint4* dst = reinterpret_cast<uint4*>((uint16_t*)(is_k ? a.c.k : a.c.v) + row * D);
+                    dst[pa] = pack8(x);
+                    dst[pb] = pack8(y);
+                }
+            } else if (__any_sync(0xffffffffu, store)) {
+                float most = 0.f;
+                bool nan = false;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     most = fmaxf(most, fmaxf(fabsf(x[i]), fabsf(y[i])));
                     nan |= x[i] != x[i] || y[i] != y[i];
                 }
-            }
-            if (nan) most = INFINITY;
+                if (nan) most = INFINITY;
 #pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            if (on && !is_q && cell) {
-                const int64_t at = cell_row(page, hc, pos & ((1 << a.c.page_shift) - 1), a.c.kv_heads, a.c.page_shift);
-                const uint16_t sc = row_scale(most, kv_max_code(FMT));
-                const float f = half_float(sc);
-                uint2* dst = reinterpret_cast<uint2*>((uint8_t*)(is_k ? a.c.k : a.c.v) + at * D);
-                const bool whole = sc != 0x7FFF;
-                dst[pa] = whole ? encode8<FMT>(x, f) : make_uint2(0, 0);
-                dst[pb] = whole ? encode8<FMT>(y, f) : make_uint2(0, 0);
-                if (j == 0) (is_k ? a.c.k_scale : a.c.v_scale)[at] = sc;
+                for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                if (store) {
+                    const uint16_t sc = row_scale(most, kv_max_code(FMT));
+                    const float f = half_float(sc);
+                    const bool whole = sc != 0x7FFF;
+                    uint2* dst = reinterpret_cast<uint2*>((uint8_t*)(is_k ? a.c.k : a.c.v) + row * D);
+                    dst[pa] = whole ? encode8<FMT>(x, f) : make_uint2(0, 0);
+                    dst[pb] = whole ? encode8<FMT>(y, f) : make_uint2(0, 0);
+                    if (j == 0) (is_k ? a.c.k_scale : a.c.v_scale)[row] = sc;
+                }
             }
         }
     }
 }
 
-constexpr int READ_THREADS = 128;
-
-// One block per row: a thread takes 16 bytes of the cache at a time.
-template <int FMT, int D>
-__global__ void __launch_bounds__(READ_THREADS) kv_read_kernel(const KvReadArgs a) {
+// A thread takes 16 bytes of the cache at a time, with four loads in flight.
+template <int FMT, int D, bool SPREAD>
+__global__ void __launch_bounds__(WARPS * 32) kv_read_kernel(const KvReadArgs a) {
     constexpr int PIECE = FMT == KV_FP16 ? 8 : 16, LANES = D / PIECE;   // values of a piece, pieces of a head's row
+    constexpr int STEP = 32 * (SPREAD ? WARPS : 1), AHEAD = SPREAD ? 1 : 4;
     pdl_launch_dependents();
     pdl_wait_prior_grid();
-    const int r = blockIdx.x;
-    const int seq = seq_of_row(a.s, r);
-    if (seq >= a.s.num_seqs || r < a.s.row_start[0]) return;
-    const SeqExtent e = seq_extent(a.s.row_start[seq], a.s.row_start[seq + 1], a.s.kv_len[seq], a.s.num_rows, a.s.max_len);
-    const int pos = e.len - (e.row1 - r);
-    if (r < e.row0 || r >= e.row1) {
-        if (threadIdx.x == 0) *a.status = STATUS_BAD_TABLE;
-        return;
-    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = SPREAD ? blockIdx.x : blockIdx.x * WARPS + warp;
+    if (r >= a.s.num_rows) return;
+    const RowPlace at = place_of_row(a.s, r);
+    if (at.none) return;
     int page = -1;
-    if (!e.bad && pos >= 0) page = a.s.page_table[(int64_t)seq * a.s.table_stride + (pos >> a.c.page_shift)];
+    if (!at.bad) page = a.s.page_table[(int64_t)at.seq * a.s.table_stride + (at.pos >> a.c.page_shift)];
     const bool cell = page_ok(page, a.c.num_pages);
-    if (!cell && threadIdx.x == 0) *a.status = STATUS_BAD_TABLE;
-    for (int i = threadIdx.x; i < 2 * a.c.kv_heads * LANES; i += READ_THREADS) {
-        const int head = (i / LANES) % a.c.kv_heads, piece = i % LANES;
-        const bool is_k = i / LANES < a.c.kv_heads;
-        uint16_t* out = (is_k ? a.k_out + r * a.k_stride : a.v_out + r * a.v_stride) + (int64_t)head * D + piece * PIECE;
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;   // (a row without a cell reads as zeros)
-        if (cell) {
-            const int64_t at = cell_row(page, head, pos & ((1 << a.c.page_shift) - 1), a.c.kv_heads, a.c.page_shift);
-            const uint4 raw = reinterpret_cast<const uint4*>((const uint8_t*)(is_k ? a.c.k : a.c.v) + at * (D * kv_cell_bytes(FMT)))[piece];
-            if (FMT == KV_FP16) {
-                lo = raw;
-            } else {
-                const float sc = half_float((is_k ? a.c.k_scale : a.c.v_scale)[at]);
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-                uint32_t h[8];
+    if (!cell && lane == 0) *a.status = STATUS_BAD_TABLE;
+    const int slot = at.pos & ((1 << a.c.page_shift) - 1), all = 2 * a.c.kv_heads * LANES;
+    for (int i0 = SPREAD ? threadIdx.x : lane; i0 < all; i0 += STEP * AHEAD) {
+        uint4 raw[AHEAD];
+        uint16_t scale[AHEAD];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    codes_to_half2x2<FMT>(w[q], h[2 * q], h[2 * q + 1]);
-#pragma unroll
-                    for (int p = 2 * q; p < 2 * q + 2; ++p) {
-                        const float2 f = half2_floats(h[p]);
-                        h[p] = floats_half2(f.x * sc, f.y * sc);
-                    }
-                }
-                lo = make_uint4(h[0], h[1], h[2], h[3]);
-                hi = make_uint4(h[4], h[5], h[6], h[7]);
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = i0 + u * STEP, head = i / LANES % a.c.kv_heads;
+            const bool is_k = i / LANES < a.c.kv_heads;
+            raw[u] = make_uint4(0, 0, 0, 0);   // (a row without a cell reads as zeros)
+            scale[u] = 0;
+            if (cell && i < all) {
+                const int64_t row = cell_row(page, head, slot, a.c.kv_heads, a.c.page_shift);
+                raw[u] = reinterpret_cast<const uint4*>((const uint8_t*)(is_k ? a.c.k : a.c.v) + row * (D * kv_cell_bytes(FMT)))[i % LANES];
+                if (FMT != KV_FP16) scale[u] = (is_k ? a.c.k_scale : a.c.v_scale)[row];
             }
         }
-        reinterpret_cast<uint4*>(out)[0] = lo;
-        if (FMT != KV_FP16) reinterpret_cast<uint4*>(out)[1] = hi;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = i0 + u * STEP, head = i / LANES % a.c.kv_heads;
+            if (i >= all) break;
+            const bool is_k = i / LANES < a.c.kv_heads;
+            uint4* out = reinterpret_cast<uint4*>((is_k ? a.k_out + r * a.k_stride : a.v_out + r * a.v_stride) + (int64_t)head * D + i % LANES * PIECE);
+            if (FMT == KV_FP16) {
+                out[0] = raw[u];
+                continue;
+            }
+            const float sc = half_float(scale[u]);
+            const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+            uint32_t h[8];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                codes_to_half2x2<FMT>(w[q], h[2 * q], h[2 * q + 1]);
+#pragma unroll
+                for (int p = 2 * q; p < 2 * q + 2; ++p) {
+                    const float2 f = half2_floats(h[p]);
+                    h[p] = floats_half2(f.x * sc, f.y * sc);
+                }
+            }
+            out[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            out[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
     }
 }
 
 template <class Args>
-cudaError_t launch(void (*kernel)(const Args), const Args& a, int grid, int threads, cudaStream_t st, bool pdl) {
+cudaError_t launch(void (*kernel)(const Args), const Args& a, int grid, cudaStream_t st, bool pdl) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3((unsigned)threads);
+    cfg.blockDim = dim3(WARPS * 32);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -214,20 +229,33 @@ cudaError_t launch(void (*kernel)(const Args), const Args& a, int grid, int thre
     return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+// A row in four warps is ready sooner, a row in one moves more bytes at a time: with one a call of 8192 rows of 48 heads of 128 dims takes .. us, with four
+// .., and one row of 15 heads of 64 dims .. and .. us.
+constexpr int SPREAD_ROWS = 592;   // (four blocks for each SM)
+
+template <int FMT, int D>
+cudaError_t write_rows(const KvWriteArgs& a, cudaStream_t st, bool pdl) {
+    if (a.s.num_rows <= SPREAD_ROWS) return launch(kv_write_kernel<FMT, D, true>, a, a.s.num_rows, st, pdl);
+    return launch(kv_write_kernel<FMT, D, false>, a, (a.s.num_rows - 1) / WARPS + 1, st, pdl);
+}
+template <int FMT, int D>
+cudaError_t read_rows(const KvReadArgs& a, cudaStream_t st, bool pdl) {
+    if (a.s.num_rows <= SPREAD_ROWS) return launch(kv_read_kernel<FMT, D, true>, a, a.s.num_rows, st, pdl);
+    return launch(kv_read_kernel<FMT, D, false>, a, (a.s.num_rows - 1) / WARPS + 1, st, pdl);
+}
+
 }  // namespace
 
 cudaError_t launch_kv_write(const KvWriteArgs& a, cudaStream_t st, bool pdl) {
-    auto k = a.c.fmt == KV_FP16 ? (a.c.dim == 64 ? kv_write_kernel<KV_FP16, 64> : kv_write_kernel<KV_FP16, 128>)
-             : a.c.fmt == KV_INT8 ? (a.c.dim == 64 ? kv_write_kernel<KV_INT8, 64> : kv_write_kernel<KV_INT8, 128>)
-                                  : (a.c.dim == 64 ? kv_write_kernel<KV_FP8, 64> : kv_write_kernel<KV_FP8, 128>);
-    return launch(k, a, a.s.num_rows, WRITE_THREADS, st, pdl);
+    if (a.c.fmt == KV_FP16) return a.c.dim == 64 ? write_rows<KV_FP16, 64>(a, st, pdl) : write_rows<KV_FP16, 128>(a, st, pdl);
+    if (a.c.fmt == KV_INT8) return a.c.dim == 64 ? write_rows<KV_INT8, 64>(a, st, pdl) : write_rows<KV_INT8, 128>(a, st, pdl);
+    return a.c.dim == 64 ? write_rows<KV_FP8, 64>(a, st, pdl) : write_rows<KV_FP8, 128>(a, st, pdl);
 }
 
 cudaError_t launch_kv_read(const KvReadArgs& a, cudaStream_t st, bool pdl) {
-    auto k = a.c.fmt == KV_FP16 ? (a.c.dim == 64 ? kv_read_kernel<KV_FP16, 64> : kv_read_kernel<KV_FP16, 128>)
-             : a.c.fmt == KV_INT8 ? (a.c.dim == 64 ? kv_read_kernel<KV_INT8, 64> : kv_read_kernel<KV_INT8, 128>)
-                                  : (a.c.dim == 64 ? kv_read_kernel<KV_FP8, 64> : kv_read_kernel<KV_FP8, 128>);
-    return launch(k, a, a.s.num_rows, READ_THREADS, st, pdl);
+    if (a.c.fmt == KV_FP16) return a.c.dim == 64 ? read_rows<KV_FP16, 64>(a, st, pdl) : read_rows<KV_FP16, 128>(a, st, pdl);
+    if (a.c.fmt == KV_INT8) return a.c.dim == 64 ? read_rows<KV_INT8, 64>(a, st, pdl) : read_rows<KV_INT8, 128>(a, st, pdl);
+    return a.c.dim == 64 ? read_rows<KV_FP8, 64>(a, st, pdl) : read_rows<KV_FP8, 128>(a, st, pdl);
 }
 
 }  // namespace nnb

@@ -44,14 +44,30 @@ __device__ __forceinline__ uint16_t row_scale(float most, float Q) {
     return s;
 }
 
-// The sequence of row r: how many end at or before it.  By all threads of the block; every thread has the result.
-__device__ __forceinline__ int seq_of_row(const KvSeqs& s, int r) {
-    int before = 0;
-    for (int i0 = 0; i0 < s.num_seqs; i0 += blockDim.x) {
-        const int i = i0 + threadIdx.x;
-        before += __syncthreads_count(i < s.num_seqs && s.row_start[i + 1] <= r);
+// Where a row of a call belongs.  By a whole warp.
+struct RowPlace {
+    bool none;   // behind the last sequence, or before the first
+    bool bad;    // its sequence's numbers are out of range
+    int seq, pos;
+};
+__device__ __forceinline__ RowPlace place_of_row(const KvSeqs& s, int r) {
+    const int lane = threadIdx.x & 31;
+    RowPlace p;
+    p.seq = 0;   // how many sequences end at or before it
+    for (int i0 = 0; i0 < s.num_seqs; i0 += 32) {
+        const int i = i0 + lane;
+        const unsigned before = __ballot_sync(0xffffffffu, i < s.num_seqs && s.row_start[i + 1] <= r);
+        p.seq += __popc(before);
+        if (before != 0xffffffffu) break;   // (they ascend)
     }
-    return before;
+    p.none = p.seq >= s.num_seqs || (p.seq == 0 && r < s.row_start[0]);
+    p.bad = false;
+    p.pos = 0;
+    if (p.none) return p;
+    const SeqExtent e = seq_extent(s.row_start[p.seq], s.row_start[p.seq + 1], s.kv_len[p.seq], s.num_rows, s.max_len);
+    p.pos = e.len - (e.row1 - r);
+    p.bad = e.bad || p.pos < 0 || r < e.row0 || r >= e.row1;
+    return p;
 }
 
 }  // namespace nnb
