@@ -14,7 +14,7 @@
 //   * warp 16: issues all tcgen05.mma: scores = Q K^T (both K-major), out += weights V (V as it lies in the cache, MN-major).  While one
 //     query tile is in its softmax the other one has the tensor cores.
 //   * warp 17: tensor copies (fp16: straight into the operands; 8-bit: codes into a ring of parts of tiles).
-//   * warps 20-23, 8-bit cells only: codes to fp16 operands, and the keys' factors.
+//   * warps 18 and 19 (cells of 128 dims: 20-23), 8-bit cells only: codes to fp16 operands, and the keys' factors.
 // The exponentials bound it next to the products: 128 x 128 scores take 1024 clocks of the SM's exponential units and D * 8 clocks of
 // its tensor cores for both products.
 #include <type_traits>
@@ -48,7 +48,8 @@ struct Chunk {
     static constexpr int RAW_KEYS = 32, RAW = RAW_KEYS * D;      // codes arrive in parts of a tile, one for each expanding warp
     static constexpr int RAW_STAGE = RAW + 4 * RAW_KEYS;         // with the scales of keys and values
     static constexpr int RAWS = CODES ? (D == 64 ? 12 : 4) : 0; // a stage is always the same warp's: whose turn it is shows in one bit
-    static constexpr int THREADS = CODES ? 768 : 640;
+    static constexpr int EXPANDERS = D == 64 ? 2 : 4;            // warps that expand codes
+    static constexpr int FIRST_EXPANDER = EXPANDERS == 2 ? 18 : 20, THREADS = CODES && EXPANDERS == 4 ? 768 : 640;
     // shared memory
     static constexpr int O_Q = 0, O_K = O_Q + 2 * TILE, O_V = O_K + RING * TILE, O_RAW = O_V + RING * TILE, O_META = O_RAW + RAWS * RAW_STAGE;
     static constexpr int META_BYTES = CODES ? BN * 12 : 0;       // factors of the scores, their summands, 1 / scale of the values
@@ -90,16 +91,6 @@ __device__ __forceinline__ void tmem_wait_ld32(uint32_t (&u)[32]) {
                    "+r"(u[23]), "+r"(u[24]), "+r"(u[25]), "+r"(u[26]), "+r"(u[27]), "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])
                  :: "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&u)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-        ::"r"(taddr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7]), "r"(u[8]), "r"(u[9]), "r"(u[10]), "r"(u[11]),
-          "r"(u[12]), "r"(u[13]), "r"(u[14]), "r"(u[15]), "r"(u[16]), "r"(u[17]), "r"(u[18]), "r"(u[19]), "r"(u[20]), "r"(u[21]), "r"(u[22]),
-          "r"(u[23]), "r"(u[24]), "r"(u[25]), "r"(u[26]), "r"(u[27]), "r"(u[28]), "r"(u[29]), "r"(u[30]), "r"(u[31])
-        : "memory");
-}
-
 // Two 32-bit values in one instruction
 __device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) {
     uint64_t d;
@@ -123,6 +114,10 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+template <int N>
+__device__ __forceinline__ void set_registers_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void set_registers_fewer() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 // Bits [0, n) of 32
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
 
@@ -192,7 +187,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     if (tid < C::BARS) {
         const int b = tid;
         int n = 1;
-        if (b < C::B_KEMPTY || (b >= C::B_VFULL && b < C::B_VEMPTY) || (b >= C::B_META && b < C::B_RFULL)) n = C::CODES ? 4 : 1;
+        if (b < C::B_KEMPTY || (b >= C::B_VFULL && b < C::B_VEMPTY) || (b >= C::B_META && b < C::B_RFULL)) n = C::CODES ? C::EXPANDERS : 1;
                 if ((b >= C::B_Q && b < C::B_S) || (b >= C::B_P && b < C::B_O)) n = 8;
         mbar_init(bar(b), n);
     }
@@ -231,6 +226,10 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     int4* const info = a.items + blockIdx.x;   // for the kernel that joins the parts: what this block has begun and not finished
     if (tid == 0) *info = make_int4(-1, 0, 0, 0);
 
+    // Registers of a thread: more for the four groups of four warps that do the softmax, fewer for the others.  The shares add up to what the block
+    // was launched with, 5 x 96 or 6 x 80.
+    if (warp < 16) set_registers_more<C::THREADS == 640 ? 104 : 88>();
+    else set_registers_fewer<64>();
     if (warp < 16) {
         // ---- softmax of query tile i, keys 64 c .. of a tile; row r ----
         const int i = warp >> 3, c = warp >> 2 & 1, r = tid & 127, pair_bar = 1 + i * 4 + (warp & 3);
@@ -270,46 +269,38 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 const bool edge = here != 0xFFu || k0 + BN - 1 > pmin || (k0 < lo_max && k0 + BN > w.sinks);
                 const float4* fa = reinterpret_cast<const float4*>(smem + C::O_META + mt * C::META_BYTES) + c * 16;   // factors of four keys' scores
                 const float4 *fb = fa + BN / 4, *inv = fb + BN / 4;                                                  // their summands; 1 / scale of the values
-                // First pass: the maximum.  Scores that do not go on as they are go back to their place: with their factors as powers of two, and
-                // -infinity where the row does not see the key.
-                float top = -INFINITY;
-                auto find_top = [&](auto masked_) {
-                    constexpr bool masked = decltype(masked_)::value;
+                uint32_t v[2][32];
+                tmem_ld32_begin(ts, v[0]);
+                tmem_ld32_begin(ts + 32, v[1]);
+                // Scores as powers of two (fp16: times 1 / scale2 still), -infinity where the row does not see the key; their maximum.
+                float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-                    for (int cb = 0; cb < 2; ++cb) {
-                        uint32_t v[32];
-                        tmem_ld32_begin(ts + cb * 32, v);
-                        tmem_wait_ld32(v);
-                        if (C::CODES) {
+                for (int cb = 0; cb < 2; ++cb) {
+                    tmem_wait_ld32(v[cb]);
+                    if (C::CODES) {
 #pragma unroll
-                            for (int x = 0; x < 8; ++x) {
-                                const float4 f = fa[cb * 8 + x], b = fb[cb * 8 + x];
-                                unpair(fma2(pair(v[4 * x], v[4 * x + 1]), pair(f.x, f.y), pair(b.x, b.y)), v[4 * x], v[4 * x + 1]);
-                                unpair(fma2(pair(v[4 * x + 2], v[4 * x + 3]), pair(f.z, f.w), pair(b.z, b.w)), v[4 * x + 2], v[4 * x + 3]);
-                            }
+                        for (int x = 0; x < 8; ++x) {
+                            const float4 f = fa[cb * 8 + x], b = fb[cb * 8 + x];
+                            unpair(fma2(pair(v[cb][4 * x], v[cb][4 * x + 1]), pair(f.x, f.y), pair(b.x, b.y)), v[cb][4 * x], v[cb][4 * x + 1]);
+                            unpair(fma2(pair(v[cb][4 * x + 2], v[cb][4 * x + 3]), pair(f.z, f.w), pair(b.z, b.w)), v[cb][4 * x + 2], v[cb][4 * x + 3]);
                         }
-                        if (masked) {
-                            const int at = k0 + c * 64 + cb * 32;
-                            uint32_t seen = low_bits(pos + 1 - at) & (~low_bits(lo - at) | low_bits(w.sinks - at));
-                            const unsigned there = here >> (4 * c + 2 * cb);
-                            seen &= ((there & 1u) ? 0xFFFFu : 0u) | ((there & 2u) ? 0xFFFF0000u : 0u);
-#pragma unroll
-                            for (int x = 0; x < 32; ++x)
-                                if (!(seen >> x & 1u)) v[x] = 0xFF800000u;
-                        }
-                        if (C::CODES || masked) tmem_st32(ts + cb * 32, v);
-                        float t0 = top, t1 = -INFINITY;
-#pragma unroll
-                        for (int x = 0; x < 32; x += 4) {
-                            t0 = max3(t0, __uint_as_float(v[x]), __uint_as_float(v[x + 1]));
-                            t1 = max3(t1, __uint_as_float(v[x + 2]), __uint_as_float(v[x + 3]));
-                        }
-                        top = fmaxf(t0, t1);
                     }
-                    if (C::CODES || masked) tmem_wait_st();
-                };
-                if (edge) find_top(std::true_type());
-                else find_top(std::false_type());
+                    if (edge) {
+                        const int at = k0 + c * 64 + cb * 32;
+                        uint32_t seen = low_bits(pos + 1 - at) & (~low_bits(lo - at) | low_bits(w.sinks - at));
+                        const unsigned there = here >> (4 * c + 2 * cb);
+                        seen &= ((there & 1u) ? 0xFFFFu : 0u) | ((there & 2u) ? 0xFFFF0000u : 0u);
+#pragma unroll
+                        for (int x = 0; x < 32; ++x)
+                            if (!(seen >> x & 1u)) v[cb][x] = 0xFF800000u;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4) {
+                        t0 = max3(t0, __uint_as_float(v[cb][x]), __uint_as_float(v[cb][x + 1]));
+                        t1 = max3(t1, __uint_as_float(v[cb][x + 2]), __uint_as_float(v[cb][x + 3]));
+                    }
+                }
+                float top = fmaxf(t0, t1);
                 if (!C::CODES) top *= scale2;
                 // Both threads of a row keep the same reference: they agree whether some row of their two warps wants another one.
                 if (pair_any(pair_bar, first || top > m + 8.f)) {
@@ -331,40 +322,38 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     }
                 }
                 first = false;
-                // Second pass: the weights
-                {
-                    const float ref = m == -INFINITY ? 0.f : -m;
-                    const uint64_t ref2 = pair(ref, ref), mul2 = pair(scale2, scale2);
-                    uint64_t sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+                // the weights
+                const float ref = m == -INFINITY ? 0.f : -m;
+                const uint64_t ref2 = pair(ref, ref), mul2 = pair(scale2, scale2);
+                uint64_t sum2[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-                    for (int cb = 0; cb < 2; ++cb) {
-                        uint32_t v[32], p[16];
-                        tmem_ld32_begin(ts + cb * 32, v);
-                        tmem_wait_ld32(v);
+                for (int cb = 0; cb < 2; ++cb) {
+                    uint32_t p[16];
 #pragma unroll
-                        for (int x = 0; x < 8; ++x) {
-                            float e[4];
+                    for (int x = 0; x < 8; ++x) {
+                        float e[4];
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const uint64_t sc = pair(v[4 * x + 2 * h], v[4 * x + 2 * h + 1]);
-                                uint32_t u0, u1;
-                                unpair(C::CODES ? add2(sc, ref2) : fma2(sc, mul2, ref2), u0, u1);
-                                e[2 * h] = ex2(__uint_as_float(u0));
-                                e[2 * h + 1] = ex2(__uint_as_float(u1));
-                            }
-                            if (C::CODES) {
-                                const float4 n = inv[cb * 8 + x];
-                                sum2[0] = fma2(pair(e[0], e[1]), pair(n.x, n.y), sum2[0]);
-                                sum2[1] = fma2(pair(e[2], e[3]), pair(n.z, n.w), sum2[1]);
-                            } else {
-                                sum2[0] = add2(sum2[0], pair(e[0], e[1]));
-                                sum2[1] = add2(sum2[1], pair(e[2], e[3]));
-                            }
-                            p[2 * x] = floats_half2(e[0], e[1]);
-                            p[2 * x + 1] = floats_half2(e[2], e[3]);
+                        for (int h = 0; h < 2; ++h) {
+                            const uint64_t sc = pair(v[cb][4 * x + 2 * h], v[cb][4 * x + 2 * h + 1]);
+                            uint32_t u0, u1;
+                            unpair(C::CODES ? add2(sc, ref2) : fma2(sc, mul2, ref2), u0, u1);
+                            e[2 * h] = ex2(__uint_as_float(u0));
+                            e[2 * h + 1] = ex2(__uint_as_float(u1));
                         }
-                        tmem_st16(ts + cb * 16, p);
+                        if (C::CODES) {
+                            const float4 n = inv[cb * 8 + x];
+                            sum2[0] = fma2(pair(e[0], e[1]), pair(n.x, n.y), sum2[0]);
+                            sum2[1] = fma2(pair(e[2], e[3]), pair(n.z, n.w), sum2[1]);
+                        } else {
+                            sum2[0] = add2(sum2[0], pair(e[0], e[1]));
+                            sum2[1] = add2(sum2[1], pair(e[2], e[3]));
+                        }
+                        p[2 * x] = floats_half2(e[0], e[1]);
+                        p[2 * x + 1] = floats_half2(e[2], e[3]);
                     }
+                    tmem_st16(ts + cb * 16, p);
+                }
+                {
                     uint32_t u0, u1;
                     unpair(add2(sum2[0], sum2[1]), u0, u1);
                     l += __uint_as_float(u0) + __uint_as_float(u1);
@@ -621,18 +610,18 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             else
                 for (const long long t0 = clock64(); clock64() - t0 < WAIT_CYCLES;) {}   // (copies that a broken order left on either ring: time enough for any)
         }
-    } else if (C::CODES && warp >= 20) {
+    } else if (C::CODES && warp >= C::FIRST_EXPANDER) {
         // ---- codes to operands ----
-        // Each warp has a part of every tile.  A thread takes the same 16 codes of every ROWS-th key: its place in a row of operands, and so the
+        // Each warp has every other part of a tile.  A thread takes the same 16 codes of every ROWS-th key: its place in a row of operands, and so the
         // swizzle, stays.
         constexpr int ROWS = 32 / (D / 16), PIECES = C::RAW_KEYS / ROWS, PERIOD = 8 / ROWS;   // (the swizzle comes round after 8 rows)
-        const int part = warp - 20, row0 = lane / (D / 16), piece = lane % (D / 16);
+        const int row0 = lane / (D / 16), piece = lane % (D / 16);
         const bool swap = D == 128 && (piece & 4);   // (the two columns of 64 dims share banks: neighbours take opposite pieces first)
         uint32_t off0[PERIOD], off1[PERIOD];
 #pragma unroll
         for (int y = 0; y < PERIOD; ++y) {
-            off0[y] = operand_at(0, part * C::RAW_KEYS + row0 + y * ROWS, 2 * piece + (swap ? 1 : 0));
-            off1[y] = operand_at(0, part * C::RAW_KEYS + row0 + y * ROWS, 2 * piece + (swap ? 0 : 1));
+            off0[y] = operand_at(0, row0 + y * ROWS, 2 * piece + (swap ? 1 : 0));
+            off1[y] = operand_at(0, row0 + y * ROWS, 2 * piece + (swap ? 0 : 1));
         }
         int kt = 0, raw = 0;
         while (next_segment()) {
@@ -643,49 +632,51 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 const int k0 = p1 < 0 ? 0 : tr.tile_at(sg.first + j) * BN;
                 wait((value ? C::B_VEMPTY : C::B_KEMPTY) + slot, ((tile / C::RING) & 1) ^ 1);
                 const uint32_t dst = base + (value ? C::O_V : C::O_K) + slot * C::TILE;
-                const int st = (raw + part) % RAWS;
-                wait(C::B_RFULL + st, ((raw + part) / RAWS) & 1);
-                raw += BN / C::RAW_KEYS;
-                const uint8_t* src = smem + C::O_RAW + st * C::RAW_STAGE;
-                const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + tile % C::HERE * 4);
-                const bool fix = value && (k0 + BN - 1 > p1 || (k0 < lo0 && k0 + BN > w.sinks) || here != 0xFFu);
-                auto pieces = [&](auto fixed) {
+                for (int part = warp - C::FIRST_EXPANDER; part < BN / C::RAW_KEYS; part += C::EXPANDERS) {
+                    const int st = (raw + part) % RAWS;
+                    wait(C::B_RFULL + st, ((raw + part) / RAWS) & 1);
+                    const uint8_t* src = smem + C::O_RAW + st * C::RAW_STAGE;
+                    const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + tile % C::HERE * 4);
+                    const bool fix = value && (k0 + BN - 1 > p1 || (k0 < lo0 && k0 + BN > w.sinks) || here != 0xFFu);
+                    auto pieces = [&](auto fixed) {
 #pragma unroll
-                    for (int b = 0; b < PIECES; b += 4) {
-                        uint4 q[4];
+                        for (int b = 0; b < PIECES; b += 4) {
+                            uint4 q[4];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) q[y] = reinterpret_cast<const uint4*>(src)[lane + (b + y) * 32];
+                            for (int y = 0; y < 4; ++y) q[y] = reinterpret_cast<const uint4*>(src)[lane + (b + y) * 32];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) {
-                            // values that no row sees must not be NaN: their weights are 0
-                            const int rr = part * C::RAW_KEYS + row0 + (b + y) * ROWS, key = k0 + rr;
-                            if (decltype(fixed)::value && (key > p1 || (key < lo0 && key >= w.sinks) || !(here >> (rr >> 4) & 1u))) q[y] = make_uint4(0, 0, 0, 0);
-                            uint4 lo, hi;
-                            codes_to_half2x2<FMT>(q[y].x, lo.x, lo.y);
-                            codes_to_half2x2<FMT>(q[y].y, lo.z, lo.w);
-                            codes_to_half2x2<FMT>(q[y].z, hi.x, hi.y);
-                            codes_to_half2x2<FMT>(q[y].w, hi.z, hi.w);
-                            const uint32_t to = dst + (b + y) / PERIOD * (8 * 128);
-                            st_shared16(to + off0[(b + y) % PERIOD], swap ? hi : lo);
-                            st_shared16(to + off1[(b + y) % PERIOD], swap ? lo : hi);
+                            for (int y = 0; y < 4; ++y) {
+                                // values that no row sees must not be NaN: their weights are 0
+                                const int rr = part * C::RAW_KEYS + row0 + (b + y) * ROWS, key = k0 + rr;
+                                if (decltype(fixed)::value && (key > p1 || (key < lo0 && key >= w.sinks) || !(here >> (rr >> 4) & 1u))) q[y] = make_uint4(0, 0, 0, 0);
+                                uint4 lo, hi;
+                                codes_to_half2x2<FMT>(q[y].x, lo.x, lo.y);
+                                codes_to_half2x2<FMT>(q[y].y, lo.z, lo.w);
+                                codes_to_half2x2<FMT>(q[y].z, hi.x, hi.y);
+                                codes_to_half2x2<FMT>(q[y].w, hi.z, hi.w);
+                                const uint32_t to = dst + part * (C::RAW_KEYS * 128) + (b + y) / PERIOD * (8 * 128);
+                                st_shared16(to + off0[(b + y) % PERIOD], swap ? hi : lo);
+                                st_shared16(to + off1[(b + y) % PERIOD], swap ? lo : hi);
+                            }
                         }
+                    };
+                    if (fix) pieces(std::true_type());
+                    else pieces(std::false_type());
+                    if (!value) {
+                        const float ks = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW)[lane]), vs = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW + 2 * C::RAW_KEYS)[lane]);
+                        const int key = part * C::RAW_KEYS + lane;
+                        // (the scales of keys that no row sees may be anything)
+                        const bool seen = k0 + key <= p1 && (k0 + key >= lo0 || k0 + key < w.sinks) && (here >> (key >> 4) & 1u);
+                        const float b = seen ? lg2(vs) : 0.f;
+                        float* meta = reinterpret_cast<float*>(smem + C::O_META + mt * C::META_BYTES) + key;
+                        meta[0] = seen ? ks * scale2 : 1.f;
+                        meta[BN] = b;
+                        meta[2 * BN] = ex2(-b);
                     }
-                };
-                if (fix) pieces(std::true_type());
-                else pieces(std::false_type());
-                if (!value) {
-                    const float ks = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW)[lane]), vs = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW + 2 * C::RAW_KEYS)[lane]);
-                    const int key = part * C::RAW_KEYS + lane;
-                    // (the scales of keys that no row sees may be anything)
-                    const bool seen = k0 + key <= p1 && (k0 + key >= lo0 || k0 + key < w.sinks) && (here >> (key >> 4) & 1u);
-                    const float b = seen ? lg2(vs) : 0.f;
-                    float* meta = reinterpret_cast<float*>(smem + C::O_META + mt * C::META_BYTES) + key;
-                    meta[0] = seen ? ks * scale2 : 1.f;
-                    meta[BN] = b;
-                    meta[2 * BN] = ex2(-b);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(C::B_REMPTY + st));
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(C::B_REMPTY + st));
+                raw += BN / C::RAW_KEYS;
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) {

@@ -4,7 +4,7 @@
 //   y1 = half(x1 c - x2 s), y2 = half(x2 c + x1 s)      dims i and i + rotary / 2 of queries and keys, c and s of the row's position;
 //                                                       products and sums are rounded to 32 bits one by one
 //   scale = the smallest fp16 with scale * Q >= max|y|  over the row's dims; Q = 127 or 448, the largest code (row_scale)
-//   code = rint(y / scale), or y / scale in e4m3        the division and the rounding exact, so that equal rows give equal codes
+//   code = rint(y / scale), or y / scale in e4m3        rounded to nearest even, as of the exact quotient
 //   read back: half(code * scale)                       the product is exact in 32 bits
 //
 // Both are bound by the bytes they move, a short call by its chain of dependent loads (row starts, page number, cell).
@@ -35,18 +35,27 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 }
 
 template <int FMT>
-__device__ __forceinline__ uint2 encode8(const float (&f)[8], float scale) {
+__device__ __forceinline__ uint2 encode8(const float (&f)[8], float scale, float inverse) {
+    // The quotient by the reciprocal, corrected by its remainder, which the fused multiply-add gives exactly (P. Markstein, IBM J. Res. Dev. 34,
+    // 1990): off by less than 2^-23 of it, and exact where it is a number of 24 bits.  The values that lie between two codes are (at most 9
+    // bits), and value and scale have 11 bits, so that a quotient is such a value or 2^-20 of it away.
+    float t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float q = f[i] * inverse;
+        t[i] = copysignf(fmaf(fmaf(-q, scale, f[i]), inverse, q), f[i]);   // (-0 would lose its sign)
+    }
     uint32_t w[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (FMT == KV_INT8) {
             uint32_t u = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) u |= ((uint32_t)__float2int_rn(__fdiv_rn(f[4 * h + i], scale)) & 0xFFu) << (8 * i);
+            for (int i = 0; i < 4; ++i) u |= ((uint32_t)__float2int_rn(t[4 * h + i]) & 0xFFu) << (8 * i);
             w[h] = u;
         } else {
-            const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f[4 * h], scale), __fdiv_rn(f[4 * h + 1], scale)), __NV_SATFINITE, __NV_E4M3);
-            const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f[4 * h + 2], scale), __fdiv_rn(f[4 * h + 3], scale)), __NV_SATFINITE, __NV_E4M3);
+            const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * h], t[4 * h + 1]), __NV_SATFINITE, __NV_E4M3);
+            const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(t[4 * h + 2], t[4 * h + 3]), __NV_SATFINITE, __NV_E4M3);
             w[h] = (uint32_t)lo | ((uint32_t)hi << 16);
         }
     }
@@ -144,11 +153,11 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
                 for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 if (store) {
                     const uint16_t sc = row_scale(most, kv_max_code(FMT));
-                    const float f = half_float(sc);
+                    const float f = half_float(sc), inverse = __frcp_rn(f);
                     const bool whole = sc != 0x7FFF;
                     uint2* dst = reinterpret_cast<uint2*>((uint8_t*)(is_k ? a.c.k : a.c.v) + row * D);
-                    dst[pa] = whole ? encode8<FMT>(x, f) : make_uint2(0, 0);
-                    dst[pb] = whole ? encode8<FMT>(y, f) : make_uint2(0, 0);
+                    dst[pa] = whole ? encode8<FMT>(x, f, inverse) : make_uint2(0, 0);
+                    dst[pb] = whole ? encode8<FMT>(y, f, inverse) : make_uint2(0, 0);
                     if (j == 0) (is_k ? a.c.k_scale : a.c.v_scale)[row] = sc;
                 }
             }
