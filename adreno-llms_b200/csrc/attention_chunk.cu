@@ -209,6 +209,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     w.tile = BN;
     w.window = a.window;
     w.sinks = a.sinks;
+    w.extra = 3;
     Steps& steps = reinterpret_cast<Steps*>(smem + C::O_WALK)[warp];
     Segment& sg = steps.sg;
     {

@@ -220,6 +220,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
     w.tile = S::KT;
     w.window = a.window;
     w.sinks = a.sinks;
+    w.extra = 8;
     Walk walk = find_work(a.s, &w, WARPS, a.status);
     if (walk.u >= walk.end) return;
 
