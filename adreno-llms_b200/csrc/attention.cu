@@ -7,13 +7,13 @@ namespace nnb {
 namespace {
 
 bool encode_cells(CUtensorMap* map, const KvView& c, void* base, int box_rows) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    if (!encode) {
+    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || !fn || q != cudaDriverEntryPointSuccess) return false;
-        encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
-    }
+        const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+        return (PFN_cuTensorMapEncodeTiled_v12000)(found ? fn : nullptr);
+    }();
+    if (!encode) return false;
     const int eb = kv_cell_bytes(c.fmt), row = c.dim * eb, cols = row > 128 ? 128 / eb : c.dim;   // (boxes of 128 bytes at most)
     const cuuint64_t dims[2] = {(cuuint64_t)c.dim, ((cuuint64_t)c.num_pages * c.kv_heads) << c.page_shift}, strides[1] = {(cuuint64_t)row};
     const cuuint32_t box[2] = {(cuuint32_t)cols, (cuuint32_t)box_rows}, one[2] = {1, 1};
@@ -48,11 +48,12 @@ bool attention_countable(const AttnArgs& a, int max_new) {
     const long long tile = few ? attention_decode_keys(a.c.fmt, a.c.dim) : 128;
     const long long parts = few ? 1 : (a.group + 127) / 128, group = (a.group + parts - 1) / parts, tokens = few ? 8 / a.group > 0 ? 8 / a.group : 1 : 2 * (128 / group);
     const double items = (double)a.c.kv_heads * parts * ((double)a.s.num_rows / tokens + a.s.num_seqs);
-    return items * ((double)a.s.max_len / tile + 2) < (double)(1 << 30);
+    return items * ((double)a.s.max_len / tile + 2 + (few ? ATTN_DECODE_EXTRA : ATTN_CHUNK_EXTRA)) < (double)(1 << 30);
 }
 
-cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl) {
-    if (few_rows(a, max_new)) return launch_attention_decode(a, maps, max_new, sm_count, st, pdl);
+cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl, int* kernels) {
+    *kernels = few_rows(a, max_new) ? 1 : 2;
+    if (*kernels == 1) return launch_attention_decode(a, maps, max_new, sm_count, st, pdl);
     return launch_attention_chunk(a, maps, sm_count, st, pdl);
 }
 

@@ -65,9 +65,10 @@ struct AttnArgs {
 };
 struct AttnMaps;
 cudaError_t attention_configure();
-cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl);
+cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl, int* kernels);   // *kernels: launches
 bool attention_countable(const AttnArgs& a, int max_new);   // whether the call's tiles of work surely stay below 2^30
 constexpr int ATTN_MAX_BLOCKS = 256;
+constexpr int ATTN_DECODE_EXTRA = 8, ATTN_CHUNK_EXTRA = 3;   // what an item costs besides its key tiles, in units of them
 constexpr size_t ATTN_DECODE_PART = 18 * 512, ATTN_CHUNK_PART = 256 * 128 * 4 + 256 * 8;   // two per block
 // The workspace: counters, items, parts.
 constexpr size_t ATTN_COUNTER_BYTES = ATTN_MAX_BLOCKS * sizeof(unsigned), ATTN_HEAD_BYTES = ATTN_COUNTER_BYTES + ATTN_MAX_BLOCKS * sizeof(int4);

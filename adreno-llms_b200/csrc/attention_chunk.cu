@@ -31,7 +31,7 @@ constexpr int BN = 128;   // keys of a tile
 
 // Where a warp is in its block's work.  It lies in shared memory: two dozen registers less in the softmax's loops.
 struct Steps {
-    Walk walk;
+    Walk walk, begin;
     Segment sg;
 };
 
@@ -57,7 +57,7 @@ struct Chunk {
     static constexpr int B_KFULL = 0, B_KEMPTY = B_KFULL + RING, B_VFULL = B_KEMPTY + RING, B_VEMPTY = B_VFULL + RING, B_META = B_VEMPTY + RING,
                          B_RFULL = B_META + META, B_REMPTY = B_RFULL + RAWS, B_Q = B_REMPTY + RAWS, B_S = B_Q + 2, B_P = B_S + 2, B_O = B_P + 2, B_FIX = B_O + 2, B_DONE = B_FIX + 1,
                          BARS = B_DONE + 1;
-    static constexpr int O_TMEM = O_BARS + BARS * 8, O_DEAD = O_TMEM + 4, BYTES = O_DEAD + 4, SMEM = BYTES + 1024;
+    static constexpr int O_TMEM = O_BARS + BARS * 8, O_DEAD = O_TMEM + 4, BYTES = O_DEAD + 8, SMEM = BYTES + 1024;
     static_assert(SMEM <= 227 * 1024, "shared memory");
     static_assert(RAWS % (BN / RAW_KEYS) == 0, "a stage belongs to one part of a tile");
     static_assert(O_BARS % 8 == 0 && O_RAW % 128 == 0 && RAW_STAGE % 16 == 0 && O_META % 16 == 0, "alignment");
@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     auto bar = [&](int i) { return bars + (uint32_t)i * 8; };
     volatile int* dead = reinterpret_cast<volatile int*>(smem + C::O_DEAD);
+    volatile int* some_again = dead + 1;   // some row of the block's whole items has to be computed once more
     // Waits of whole warps.  When one runs out the block carries on without waiting: what it computes is void, and ends.
     auto wait = [&](int b, uint32_t parity) {
         uint32_t ok = mbar_try_wait(bar(b), parity);
@@ -188,14 +189,13 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         const int b = tid;
         int n = 1;
         if (b < C::B_KEMPTY || (b >= C::B_VFULL && b < C::B_VEMPTY) || (b >= C::B_META && b < C::B_RFULL)) n = C::CODES ? C::EXPANDERS : 1;
-                if ((b >= C::B_Q && b < C::B_S) || (b >= C::B_P && b < C::B_O)) n = 8;
+        if ((b >= C::B_Q && b < C::B_S) || (b >= C::B_P && b < C::B_O)) n = 8;
         mbar_init(bar(b), n);
     }
-    if (tid == 0) *dead = 0;
+    if (tid == 0) *dead = *some_again = 0;
     mbar_init_fence();
     if (warp == 16) tmem_alloc<false>(base + C::O_TMEM, 512);
     tc_fence_before();
-    pdl_launch_dependents();
     pdl_wait_prior_grid();
     __syncthreads();
     tc_fence_after();
@@ -209,12 +209,12 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     w.tile = BN;
     w.window = a.window;
     w.sinks = a.sinks;
-    w.extra = 3;
+    w.extra = ATTN_CHUNK_EXTRA;
     Steps& steps = reinterpret_cast<Steps*>(smem + C::O_WALK)[warp];
     Segment& sg = steps.sg;
     {
         const Walk walk = find_work(a.s, &w, 2, a.status);
-        if (lane == 0) steps.walk = walk;
+        if (lane == 0) steps.walk = steps.begin = walk;
     }
     auto next_segment = [&]() {
         int more = 0;
@@ -434,11 +434,10 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     if (c == 0) reinterpret_cast<float2*>(part + 64 * D)[i * 128 + r] = make_float2(m, l);
                     if (sg.first == 0 && tid == 0) *info = make_int4(sg.seq, sg.vhead, sg.qt, (int)((sg.unit0 + sg.total - 1) / w.chunk));
                 } else {
-                    // rows that are not finite, or see nothing: from the formula once more, which does not touch hidden cells
-                    for (unsigned left = c == 0 ? __ballot_sync(0xffffffffu, on && !fine) : 0u; left; left &= left - 1) {
-                        const int from = __ffs(left) - 1;
-                        const int r2 = __shfl_sync(0xffffffffu, row, from), h2 = __shfl_sync(0xffffffffu, head, from), p2 = __shfl_sync(0xffffffffu, pos, from);
-                        if (!attend_row<FMT, D>(a, sg.seq, sg.len, p2, r2, h2) && lane == 0) *a.status = STATUS_BAD_TABLE;
+                    // rows that are not finite, or see nothing, are marked by a NaN
+                    if (c == 0 && on && !fine) {
+                        *out = 0x7FFF;
+                        *some_again = 1;
                     }
                 }
             }
@@ -446,6 +445,26 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             // (what the threads have told each other has been read)
             if (rows.turns) asm volatile("bar.sync 9, 512;" ::: "memory");
             else pair_sync(pair_bar);
+        }
+        // Marked rows: from the formula once more, which does not use hidden cells.  Behind the loop: no wait of another warp runs out meanwhile, and
+        // this takes no registers from it (int8 cells of 128 dims, 2048 tokens of 32 heads to 16384 positions: 675 us, 800 with this inside).
+        asm volatile("bar.sync 9, 512;" ::: "memory");
+        if (*some_again) {
+            __syncwarp();
+            if (lane == 0) steps.walk = steps.begin;
+            while (next_segment()) {
+                if (sg.count != sg.total) continue;
+                const ItemRows rows(sg, w);
+                const int kv_head = sg.vhead / parts, x = warp >> 1, rr = (x & 3) * 32 + lane, g = rr % w.group, t = rows.first(x >> 2) + rr / w.group;
+                const int hg = (sg.vhead % parts) * w.group + g, row = sg.row0 + t, head = kv_head * a.group + hg, pos = sg.len - sg.n + t;
+                const bool on = !(rows.turns && x >= 4) && rr < rows.per * w.group && t <= rows.last(x >> 2) && hg < a.group;
+                const bool marked = on && (*reinterpret_cast<const volatile uint16_t*>(a.out + (int64_t)row * a.o_stride + (int64_t)head * D) & 0x7FFF) > 0x7C00;
+                for (unsigned left = __ballot_sync(0xffffffffu, marked) & (warp & 1 ? 0xAAAAAAAAu : 0x55555555u); left; left &= left - 1) {
+                    const int from = __ffs(left) - 1;
+                    const int r2 = __shfl_sync(0xffffffffu, row, from), h2 = __shfl_sync(0xffffffffu, head, from), p2 = __shfl_sync(0xffffffffu, pos, from);
+                    if (!attend_row<FMT, D>(a, sg.seq, sg.len, p2, r2, h2) && lane == 0) *a.status = STATUS_BAD_TABLE;
+                }
+            }
         }
     } else if (warp == 16) {
         // ---- products ----
@@ -505,6 +524,8 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             }
             kt += n;
         }
+        // Not earlier: waits of the next launch have a limit, which counts from its beginning, and this kernel may run for longer than that.
+        pdl_launch_dependents();
         if (issuer) umma_commit<false>(bar(C::B_DONE));
         __syncwarp();
         mbar_wait_bounded(bar(C::B_DONE), 0);
@@ -668,7 +689,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                         const int key = part * C::RAW_KEYS + lane;
                         // (the scales of keys that no row sees may be anything)
                         const bool seen = k0 + key <= p1 && (k0 + key >= lo0 || k0 + key < w.sinks) && (here >> (key >> 4) & 1u);
-                        const float b = seen ? lg2(vs) : 0.f;
+                        const float b = seen ? fmaf(ks, 0.f, lg2(vs)) : 0.f;   // (an infinite scale as a NaN: the formula knows what codes of 0 make of it)
                         float* meta = reinterpret_cast<float*>(smem + C::O_META + mt * C::META_BYTES) + key;
                         meta[0] = seen ? ks * scale2 : 1.f;
                         meta[BN] = b;
@@ -704,7 +725,6 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
 constexpr int JOIN_THREADS = 256;
 template <int FMT, int D>
 __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const AttnArgs a) {
-    pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int b0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int4 it = a.items[b0];
@@ -765,6 +785,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Attn
 #pragma unroll
         for (int x = 0; x < N; ++x) out[x] = make_uint2(floats_half2(o[x].x, o[x].y), floats_half2(o[x].z, o[x].w));
     }
+    if (!again) pdl_launch_dependents();   // (the rest may take long)
     int k = 0;   // rows that are not finite, or see nothing: from the formula once more, a warp each
     for (unsigned left = again; left; left &= left - 1, ++k) {
         const int from = __ffs(left) - 1;

@@ -210,7 +210,6 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
     if (lane < STAGES) mbar_init(bars + lane * 8, 1);
     mbar_init_fence();
     __syncwarp();
-    pdl_launch_dependents();
     pdl_wait_prior_grid();
 
     WorkShape w;
@@ -220,7 +219,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
     w.tile = S::KT;
     w.window = a.window;
     w.sinks = a.sinks;
-    w.extra = 8;
+    w.extra = ATTN_DECODE_EXTRA;
     Walk walk = find_work(a.s, &w, WARPS, a.status);
     if (walk.u >= walk.end) return;
 
@@ -238,7 +237,11 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
         while (pmore && pslice >= pcount) {
             Segment s;
             pmore = pw.next(a.s, w, &s);
-            if (!pmore) return;
+            if (!pmore) {
+                // Not earlier: waits of the next launch have a limit, which counts from its beginning, and this kernel may run for longer than that.
+                pdl_launch_dependents();
+                return;
+            }
             const TileRange tr = s.tiles(w);
             ptable = a.s.page_table + (int64_t)s.seq * a.s.table_stride;
             phead = s.vhead;
@@ -392,8 +395,9 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
                         asm volatile("ld.shared.u16 %0, [%1];" : "=h"(vs) : "r"(sb + 128 + x * 2));
                         // (the scale of a cell that no row sees may be anything)
                         const bool seen = !edge || seen_by_some(x);
-                        fa = seen ? scale2 * half_float(ks) : 1.f;
-                        fb = seen ? lg2(half_float(vs)) : 0.f;
+                        const float k = half_float(ks);
+                        fa = seen ? scale2 * k : 1.f;
+                        fb = seen ? fmaf(k, 0.f, lg2(half_float(vs))) : 0.f;   // (an infinite scale as a NaN: the formula knows what codes of 0 make of it)
                         inv[t][h] = ex2(-fb);
                     }
 #pragma unroll

@@ -43,9 +43,11 @@ struct Segment {
     __device__ __forceinline__ TileRange tiles(const WorkShape& w) const { return visible_tiles(p0(w), p1(w), w.window, w.sinks, w.tile); }
 };
 
-__device__ __forceinline__ SeqWork load_seq(const KvSeqs& s, const WorkShape& w, int i, bool* bad = nullptr) {
-    const SeqExtent e = seq_extent(s.row_start[i], s.row_start[i + 1], s.kv_len[i], s.num_rows, s.max_len);
+__device__ __forceinline__ SeqWork load_seq(const KvSeqs& s, const WorkShape& w, int i, bool* bad = nullptr, bool* descends = nullptr) {
+    const int start = s.row_start[i], end = s.row_start[i + 1];
+    const SeqExtent e = seq_extent(start, end, s.kv_len[i], s.num_rows, s.max_len);
     if (bad) *bad = e.bad;
+    if (descends) *descends = end < start;
     SeqWork q;
     q.row0 = e.row0;
     q.n = e.row1 - e.row0;
@@ -125,7 +127,8 @@ struct Walk {
 };
 
 // The walk of this block, found by each warp for itself: the sequences, one per lane, how many units there are and where this block's begin.
-// `least`: the fewest units that are worth a block.  w->chunk and w->pad are set.  (The host has seen to it that units are fewer than 2^31.)
+// `least`: the fewest units that are worth a block.  w->chunk and w->pad are set.
+// The host has seen to it that units are fewer than 2^31 as long as no row belongs to two sequences: row starts that do not ascend are no work at all.
 __device__ __forceinline__ Walk find_work(const KvSeqs& s, WorkShape* w, unsigned least, int* status) {
     const int lane = threadIdx.x & 31;
     Walk k;
@@ -138,17 +141,20 @@ __device__ __forceinline__ Walk find_work(const KvSeqs& s, WorkShape* w, unsigne
     w->extra = 0;
     w->pad = false;
     w->chunk = 1;
+    bool disorder = false;
     auto load = [&](int i0) {
-        bool bad = false;
+        bool bad = false, descends = false;
         q = SeqWork{0, 0, 0, 0};
-        if (i0 + lane < s.num_seqs) q = load_seq(s, *w, i0 + lane, &bad);
+        if (i0 + lane < s.num_seqs) q = load_seq(s, *w, i0 + lane, &bad, &descends);
         if (bad) *status = STATUS_BAD_TABLE;
+        disorder |= descends;
     };
     for (int i0 = 0; i0 < s.num_seqs; i0 += 32) {
         load(i0);
         total += __reduce_add_sync(0xffffffffu, seq_tiles(q, *w));
         items += __reduce_add_sync(0xffffffffu, (unsigned)q.tiles_q);
     }
+    if (__any_sync(0xffffffffu, disorder)) return k;
     total *= w->vheads;
     items *= w->vheads;
     w->pad = 2 * items <= gridDim.x;

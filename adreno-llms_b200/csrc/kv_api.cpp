@@ -38,13 +38,43 @@ static int attention_workspace(nn_context* c) {
     CUDA_TRY(attention_configure());
     void* work = nullptr;
     CUDA_TRY(cudaMalloc(&work, attention_workspace_bytes(c->sm_count)));
-    const cudaError_t e = cudaMemset(work, 0, ATTN_HEAD_BYTES);
+    const cudaError_t e = cudaMemsetAsync(work, 0, ATTN_HEAD_BYTES, c->stream);
     if (e != cudaSuccess) {
         cudaFree(work);
         return NN_FAIL(NN_ERR_CUDA, "nn_kv_cache_create: %s", cudaGetErrorString(e));
     }
     c->attn_work = work;
     return NN_OK;
+}
+
+// Rows of `width` values at a distance of `stride`.
+struct Rows {
+    const uint16_t* p;
+    int64_t stride, width;
+};
+static size_t rows_bytes(const Rows& r, int rows) { return ((size_t)(rows - 1) * r.stride + r.width) * 2; }
+
+// Whether two sets of rows share memory.  Of equal stride they may be columns of one buffer (q, k and v of a fused projection).
+static bool rows_overlap(const Rows& a, const Rows& b, int rows) {
+    const char *pa = (const char*)a.p, *pb = (const char*)b.p;
+    if (pa >= pb + rows_bytes(b, rows) || pb >= pa + rows_bytes(a, rows)) return false;
+    if (a.stride != b.stride) return true;
+    const int64_t pitch = a.stride * 2;
+    int64_t d = (int64_t)((intptr_t)pb - (intptr_t)pa) % pitch;
+    if (d < 0) d += pitch;
+    return d < a.width * 2 || d + b.width * 2 > pitch;
+}
+static bool share(const void* p, size_t np, const void* q, size_t nq) { return p && q && (const char*)p < (const char*)q + nq && (const char*)q < (const char*)p + np; }
+static size_t scale_bytes(const KvView& v) { return cache_bytes(v) / ((size_t)v.dim * kv_cell_bytes(v.fmt)) * 2; }
+static bool rows_over_cache(const Rows& r, int rows, const KvView& v) {
+    const size_t n = rows_bytes(r, rows), nc = cache_bytes(v), ns = scale_bytes(v);
+    return share(r.p, n, v.k, nc) || share(r.p, n, v.v, nc) || share(r.p, n, v.k_scale, ns) || share(r.p, n, v.v_scale, ns);
+}
+// (what a call writes must not be what tells it where to)
+static bool rows_over_batch(const Rows& r, const nn_kv_batch* b) {
+    const size_t n = rows_bytes(r, b->num_rows);
+    return share(r.p, n, b->row_start, 4 * ((size_t)b->num_seqs + 1)) || share(r.p, n, b->kv_len, 4 * (size_t)b->num_seqs) ||
+           share(r.p, n, b->page_table, 4 * (size_t)b->num_seqs * b->table_stride);
 }
 
 extern "C" int nn_kv_cache_create(nn_context* c, int format, int num_pages, int page_size, int kv_heads, int head_dim, nn_buf k, nn_buf v,
@@ -74,6 +104,9 @@ extern "C" int nn_kv_cache_create(nn_context* c, int format, int num_pages, int 
     for (w.page_shift = 0; (1 << w.page_shift) < page_size;) ++w.page_shift;
     w.kv_heads = kv_heads;
     w.dim = head_dim;
+    const size_t n = cache_bytes(w), ns = scale_bytes(w);
+    if (share(k, n, v, n) || share(k_scale, ns, v_scale, ns) || share(k, n, k_scale, ns) || share(k, n, v_scale, ns) || share(v, n, k_scale, ns) || share(v, n, v_scale, ns))
+        return NN_FAIL(NN_ERR_ARG, "nn_kv_cache_create: the buffers overlap");
     AttnMaps maps = {};
     if (c) {
         CUDA_TRY(cudaSetDevice(c->device));
@@ -90,30 +123,6 @@ extern "C" int nn_kv_cache_create(nn_context* c, int format, int num_pages, int 
 extern "C" int nn_kv_cache_free(nn_kv_cache* h) {
     delete h;
     return NN_OK;
-}
-
-// Rows of `width` values at a distance of `stride`.
-struct Rows {
-    const uint16_t* p;
-    int64_t stride, width;
-};
-static size_t rows_bytes(const Rows& r, int rows) { return ((size_t)(rows - 1) * r.stride + r.width) * 2; }
-
-// Whether two sets of rows share memory.  Of equal stride they may be columns of one buffer (q, k and v of a fused projection).
-static bool rows_overlap(const Rows& a, const Rows& b, int rows) {
-    const char *pa = (const char*)a.p, *pb = (const char*)b.p;
-    if (pa >= pb + rows_bytes(b, rows) || pb >= pa + rows_bytes(a, rows)) return false;
-    if (a.stride != b.stride) return true;
-    const int64_t pitch = a.stride * 2;
-    int64_t d = (int64_t)((intptr_t)pb - (intptr_t)pa) % pitch;
-    if (d < 0) d += pitch;
-    return d < a.width * 2 || d + b.width * 2 > pitch;
-}
-static bool rows_over_cache(const Rows& r, int rows, const KvView& v) {
-    const char *p = (const char*)r.p, *end = p + rows_bytes(r, rows);
-    const size_t n = cache_bytes(v), ns = n / ((size_t)v.dim * kv_cell_bytes(v.fmt)) * 2;
-    auto hit = [&](const void* q, size_t bytes) { return q && p < (const char*)q + bytes && (const char*)q < end; };
-    return hit(v.k, n) || hit(v.v, n) || hit(v.k_scale, ns) || hit(v.v_scale, ns);
 }
 
 // The rows of one operand: `stride` 0 stands for dense rows.
@@ -189,14 +198,16 @@ static int kv_write(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf 
     if (q) {
         if ((rc = take_rows(q, q_stride, q_heads, D, who, "q", &rq)) || (rc = take_rows(q_out, q_out_stride, q_heads, D, who, "q_out", &ro))) return rc;
         if (!(rq.p == ro.p && rq.stride == ro.stride) && rows_overlap(rq, ro, b->num_rows)) return NN_FAIL(NN_ERR_ARG, "%s: q_out overlaps q without being q", who);
-        if (rows_overlap(ro, rk, b->num_rows) || rows_overlap(ro, rv, b->num_rows) || rows_over_cache(ro, b->num_rows, a.c))
-            return NN_FAIL(NN_ERR_ARG, "%s: q_out overlaps k, v or the cache", who);
+        if (rows_overlap(ro, rk, b->num_rows) || rows_overlap(ro, rv, b->num_rows) || rows_over_cache(ro, b->num_rows, a.c) || rows_over_batch(ro, b))
+            return NN_FAIL(NN_ERR_ARG, "%s: q_out overlaps k, v, the cache or the batch", who);
     }
     if (rows_over_cache(rk, b->num_rows, a.c) || rows_over_cache(rv, b->num_rows, a.c)) return NN_FAIL(NN_ERR_ARG, "%s: k or v lies in the cache", who);
     if (rotary_dim) {
         if (rotary_dim < 0 || rotary_dim > D || rotary_dim % 16 != 0) return NN_FAIL(NN_ERR_ARG, "%s: rotary_dim=%d: a multiple of 16, at most %d", who, rotary_dim, D);
         if (!cos_f32 || !sin_f32 || !aligned(cos_f32, 16) || !aligned(sin_f32, 16)) return NN_FAIL(NN_ERR_ARG, "%s: cos and sin must be there and 16-byte aligned", who);
         if (table_len <= 0) return NN_FAIL(NN_ERR_ARG, "%s: table_len=%d", who, table_len);
+        const size_t n = rows_bytes(ro, b->num_rows), table = (size_t)table_len * (rotary_dim / 2) * 4;
+        if (q && (share(ro.p, n, cos_f32, table) || share(ro.p, n, sin_f32, table))) return NN_FAIL(NN_ERR_ARG, "%s: q_out overlaps cos or sin", who);
     }
     a.q = rq.p;
     a.q_out = const_cast<uint16_t*>(ro.p);
@@ -216,7 +227,7 @@ static int kv_write(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf 
     ProfScope prof(c, [&] { return std::string("kv_write_") + kv_name(a.c.fmt) + "_rows" + std::to_string(b->num_rows) + (rotary_dim ? "_rope" : ""); });
     const cudaError_t e = launch_kv_write(a, c->stream, c->use_pdl);
     if (e != cudaSuccess) return NN_FAIL(NN_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
-    const size_t n = cache_bytes(a.c), ns = n / ((size_t)D * kv_cell_bytes(a.c.fmt)) * 2;
+    const size_t n = cache_bytes(a.c), ns = scale_bytes(a.c);
     if (q) c->in_flight.wrote(q_out, rows_bytes(ro, b->num_rows));
     c->in_flight.wrote(a.c.k, n);
     c->in_flight.wrote(a.c.v, n);
@@ -246,8 +257,8 @@ extern "C" int nn_kv_read(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, n
     a.c = h->view;
     Rows rk, rv;
     if ((rc = take_rows(k_out, k_stride, a.c.kv_heads, a.c.dim, who, "k_out", &rk)) || (rc = take_rows(v_out, v_stride, a.c.kv_heads, a.c.dim, who, "v_out", &rv))) return rc;
-    if (rows_overlap(rk, rv, b->num_rows) || rows_over_cache(rk, b->num_rows, a.c) || rows_over_cache(rv, b->num_rows, a.c))
-        return NN_FAIL(NN_ERR_ARG, "%s: k_out, v_out and the cache overlap", who);
+    if (rows_overlap(rk, rv, b->num_rows) || rows_over_cache(rk, b->num_rows, a.c) || rows_over_cache(rv, b->num_rows, a.c) || rows_over_batch(rk, b) || rows_over_batch(rv, b))
+        return NN_FAIL(NN_ERR_ARG, "%s: k_out, v_out, the cache and the batch overlap", who);
     a.k_out = const_cast<uint16_t*>(rk.p);
     a.v_out = const_cast<uint16_t*>(rv.p);
     a.k_stride = rk.stride;
@@ -275,7 +286,8 @@ extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b,
     if (q_heads <= 0 || q_heads % a.c.kv_heads != 0) return NN_FAIL(NN_ERR_ARG, "%s: q_heads=%d is not a multiple of the cache's %d heads", who, q_heads, a.c.kv_heads);
     Rows rq, ro;
     if ((rc = take_rows(q, q_stride, q_heads, a.c.dim, who, "q", &rq)) || (rc = take_rows(out, out_stride, q_heads, a.c.dim, who, "out", &ro))) return rc;
-    if (rows_overlap(rq, ro, b->num_rows) || rows_over_cache(ro, b->num_rows, a.c)) return NN_FAIL(NN_ERR_ARG, "%s: out overlaps q or the cache", who);
+    if (rows_overlap(rq, ro, b->num_rows) || rows_over_cache(ro, b->num_rows, a.c) || rows_over_batch(ro, b))
+        return NN_FAIL(NN_ERR_ARG, "%s: out overlaps q, the cache or the batch", who);
     if (!(scale > 0.f) || !std::isfinite(scale)) return NN_FAIL(NN_ERR_ARG, "%s: scale=%g: finite and positive", who, (double)scale);
     if (window < 0 || sinks < 0) return NN_FAIL(NN_ERR_ARG, "%s: window=%d sinks=%d", who, window, sinks);
     a.q = rq.p;
@@ -295,9 +307,10 @@ extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b,
     a.counters = (unsigned*)c->attn_work;
     a.items = (int4*)((char*)c->attn_work + ATTN_COUNTER_BYTES);
     a.parts = (char*)c->attn_work + ATTN_HEAD_BYTES;
-    const cudaError_t e = launch_attention(a, h->maps, b->max_new, c->sm_count, c->stream, c->use_pdl);
+    int kernels = 0;
+    const cudaError_t e = launch_attention(a, h->maps, b->max_new, c->sm_count, c->stream, c->use_pdl, &kernels);
     if (e != cudaSuccess) return NN_FAIL(NN_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     c->in_flight.wrote(out, rows_bytes(ro, b->num_rows));
-    c->launches++;
+    c->launches += kernels;
     return NN_OK;
 }

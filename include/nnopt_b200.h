@@ -185,14 +185,17 @@ int nn_linear_argmax(nn_context* ctx, int N, int K, nn_buf x, nn_buf W, nn_buf l
  *   A batch describes the sequences of a call in device memory that the call reads when it runs, so that a recorded
  *   step takes new lengths at every replay:
  *     row_start   int32 [num_seqs + 1], ascending: rows row_start[s] .. row_start[s + 1] - 1 of the call's operands are the new
- *                 tokens of sequence s (none, one or many).  Rows behind row_start[num_seqs] are neither read nor written.
+ *                 tokens of sequence s (none, one or many).  Rows behind row_start[num_seqs] and before row_start[0] are neither read
+ *                 nor written.
  *     kv_len      int32 [num_seqs]: positions of the sequence, its new tokens included: the last row has position kv_len - 1.
  *     page_table  int32 [num_seqs][table_stride]: position p lies in page page_table[s][p / page_size], slot p % page_size.
- *                 Entries behind the last position are not read.
+ *                 Entries behind the last position are not read.  Sequences may share pages that none of them writes in the call (a
+ *                 common prefix); what two rows write to one cell is either of them, or of both.
  *   and bounds for the host: num_rows rows in every operand; max_new, the most new rows of a sequence (it picks the kernel: a
  *   longer one is served all the same); max_len, beyond which no sequence is (at most table_stride * page_size, and 2^30).
- *   A page number, length or position that is out of range makes the next nn_sync return NN_ERR_ARG; rows and keys that it concerns
- *   are left out, nothing out of bounds is touched.
+ *   A page number, length or position that is out of range makes the next nn_sync return NN_ERR_ARG, and nothing out of bounds is
+ *   touched: the cells that it concerns are not written, are zeros for nn_kv_read and hidden for nn_attention (whose rows of a sequence
+ *   with a bad length, and of all sequences where row_start does not ascend, hold no result).  (nn_attention accepts positions below 0.)
  *   Operands are fp16 rows of [heads][head_dim], 16-byte aligned; strides count values from row to row (a multiple of 8;
  *   0: dense), so that q, k and v may be columns of one buffer.
  *

@@ -56,8 +56,10 @@ def attend(q, k, v, positions, scale, window, sinks):
             w /= w.sum()
             out[i] = w @ v[key]
             spread[i] = w @ np.abs(v[key])
-            most[i] = np.abs(v[key]).max()
-            steep[i] = scale * (np.abs(k[key]) @ np.abs(q[i])).max()
+            # (rows that see what is not finite are computed with weights of 32 bits; a key at an infinite distance has the weight 0 without an error)
+            most[i] = np.abs(v[key], where=np.isfinite(v[key]), out=np.zeros_like(v[key])).max()
+            far = np.abs(k[key]) @ np.abs(q[i])
+            steep[i] = scale * np.where(np.isfinite(far), far, 0).max()
     return out, spread, most, steep
 
 

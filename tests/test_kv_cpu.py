@@ -69,6 +69,8 @@ def _create(nnb, L, fmt=0, pages=4, page=16, heads=2, dim=64, k=BUF, v=2 * BUF, 
     (dict(dim=80), "UNSUPPORTED", b"head_dim"), (dict(dim=256), "UNSUPPORTED", b"head_dim"), (dict(pages=1 << 27, heads=8), "UNSUPPORTED", b"cells"),
     (dict(k=None), "ARG", b"null pages"), (dict(v=None), "ARG", b"null pages"), (dict(k=BUF + 8), "ARG", b"aligned"),
     (dict(fmt=1), "ARG", b"scale"), (dict(fmt=2, ks=BUF), "ARG", b"scale"), (dict(vs=BUF), "ARG", b"no scale"), (dict(fmt=1, ks=BUF, vs=BUF + 2), "ARG", b"aligned"),
+    (dict(v=BUF + 4 * 16 * 2 * 64 * 2 - 16), "ARG", b"overlap"), (dict(v=BUF - 16), "ARG", b"overlap"), (dict(fmt=1, ks=3 * BUF, vs=3 * BUF + 240), "ARG", b"overlap"),
+    (dict(fmt=2, ks=BUF + 16, vs=3 * BUF), "ARG", b"overlap"), (dict(fmt=2, ks=3 * BUF, vs=2 * BUF), "ARG", b"overlap"),
 ])
 def test_cache_refusals(nnb, built_lib, change, code, text):
     rc, _ = _create(nnb, built_lib, **change)
@@ -107,7 +109,7 @@ NO_CONTEXT = b"null context"
 @pytest.mark.parametrize("change,text", [
     ({}, NO_CONTEXT), (dict(num_seqs=0), NO_CONTEXT), (dict(num_rows=0, row_start=None), NO_CONTEXT), (dict(num_seqs=-1), b"num_seqs"), (dict(num_rows=-1), b"num_rows"),
     (dict(max_new=0), b"max_new"), (dict(max_len=0), b"max_len"), (dict(table_stride=0), b"table_stride"), (dict(max_len=129), b"page table row"),
-    (dict(max_len=128), NO_CONTEXT), (dict(table_stride=1 << 30, max_len=1 << 30), NO_CONTEXT),
+    (dict(max_len=128), NO_CONTEXT), (dict(table_stride=1 << 30, max_len=1 << 30, page_table=1 << 40), NO_CONTEXT),
     (dict(row_start=None), b"null row_start"), (dict(kv_len=None), b"null row_start"), (dict(page_table=None), b"null row_start"), (dict(kv_len=4 * BUF + 2), b"4-byte"),
 ])
 def test_batch_refusals(nnb, built_lib, call, change, text):
@@ -125,7 +127,9 @@ def test_batch_refusals(nnb, built_lib, call, change, text):
     (_attention, dict(scale=0.0), b"scale"), (_attention, dict(scale=-1.0), b"scale"), (_attention, dict(scale=float("inf")), b"scale"), (_attention, dict(scale=float("nan")), b"scale"),
     (_attention, dict(window=-1), b"window"), (_attention, dict(sinks=-1), b"sinks"), (_attention, dict(out=Q), b"overlaps"), (_attention, dict(out=Q + 16), b"overlaps"),
     (_attention, dict(out=Q + 6 * 512), NO_CONTEXT), (_attention, dict(out=Q + 512, qs=512, os_=512), NO_CONTEXT), (_attention, dict(out=Q + 496, qs=512, os_=512), b"overlaps"),
-    (_attention, dict(out=BUF), b"overlaps"),
+    (_attention, dict(out=BUF), b"overlaps"), (_attention, dict(out=3 * BUF), b"overlaps"), (_attention, dict(out=4 * BUF), b"overlaps"),
+    (_attention, dict(out=5 * BUF + 48), b"overlaps"), (_attention, dict(out=5 * BUF + 64), NO_CONTEXT), (_rope, dict(qo=5 * BUF), b"overlaps"), (_read, dict(k=4 * BUF), b"overlap"),
+    (_rope, dict(qo=8 * BUF), b"q_out overlaps cos"), (_rope, dict(qo=9 * BUF + 12784), b"q_out overlaps cos"), (_rope, dict(qo=9 * BUF + 12800), NO_CONTEXT),
     (_rope, dict(rot=0), b"rotary_dim"), (_rope, dict(rot=8), b"rotary_dim"), (_rope, dict(rot=80), b"rotary_dim"), (_rope, dict(cos=None), b"cos"), (_rope, dict(sin=9 * BUF + 4), b"cos"),
     (_rope, dict(n=0), b"table_len"), (_rope, dict(q=None), b"q_heads"), (_rope, dict(q_heads=0), b"q_heads"), (_rope, dict(qo=None), b"q_heads"),
     (_rope, dict(q_heads=0, q=None, qo=None), NO_CONTEXT), (_rope, dict(qo=Q + 16), b"q_out overlaps"), (_rope, dict(qo=K), b"q_out overlaps"), (_rope, dict(qo=2 * BUF), b"q_out overlaps"),
