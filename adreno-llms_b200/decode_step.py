@@ -3,8 +3,8 @@
 Mirrors the call points of the reference's decode loop
 (src/models/smollm2-135m-instruct/src/model.cpp:88-239): per layer a fused QKV
 launch, o_proj + residual, fused gate/up/SiLU, down + residual, then the lm_head
-GEMV and the arg-max.  The operators between the projections (norms, RoPE,
-attention) are not on this path.  Two wirings:
+GEMV and the arg-max.  The rotation, the key/value cache and the attention between
+q/k/v and o_proj are part of it where `attention` is given.  Two wirings:
 
   fixed inputs   each projection reads a fixed N(0,1) activation buffer, as in a host
                  program whose own kernels sit between the projections; only the in-place
@@ -21,13 +21,69 @@ stream from HBM rather than L2.
 """
 import numpy as np
 
-from . import QuantWeight
+from . import KVBatch, QuantWeight
 from . import synth
+
+
+class Attention:
+    """What a decode step keeps for the attention of its M sequences, one new token each: per layer a paged cache with
+    random contents up to `lengths`, and one batch for all layers.  cache: "fp16", "int8" or "fp8"."""
+
+    def __init__(self, ctx, shape, M, lengths, cache="int8", page=64, max_len=0, head_dim=64, window=0, sinks=0, rope_base=10000.0, seed=7, host=None):
+        self.ctx, self.D, self.cache, self.window, self.sinks = ctx, head_dim, cache, window, sinks
+        self.q_heads, self.kv_heads = shape.q_dim // head_dim, shape.kv_dim // head_dim
+        self.max_len = max_len or max(lengths) + 16
+        per_seq = -(-self.max_len // page)
+        rng = np.random.default_rng(seed)
+        self.table = rng.permutation(M * per_seq).astype(np.int32).reshape(M, per_seq)
+        angle = np.arange(self.max_len)[:, None] * rope_base ** (-np.arange(0, head_dim, 2) / head_dim)
+        self.cos_host, self.sin_host = np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+        self.cos, self.sin = ctx.upload(self.cos_host), ctx.upload(self.sin_host)
+        self.row_start, self.kv_len, self.table_dev = ctx.upload(np.arange(M + 1, dtype=np.int32)), ctx.alloc(4 * M), ctx.upload(self.table)
+        self.batch = KVBatch(M, M, 1, self.max_len, per_seq, self.row_start, self.kv_len, self.table_dev)
+        self.out = ctx.alloc(M * shape.q_dim * 2)
+        self.caches, self.buffers = [], []
+        cells = M * per_seq * page * self.kv_heads
+        starts = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+        fill = KVBatch(M, int(starts[-1]), max(1, max(lengths)), self.max_len, per_seq, ctx.upload(starts), ctx.upload(np.asarray(lengths, np.int32)), self.table_dev)
+        for layer in range(shape.layers):
+            bufs = [ctx.alloc(cells * head_dim * (2 if cache == "fp16" else 1)) for _ in range(2)]
+            bufs += [None, None] if cache == "fp16" else [ctx.alloc(cells * 2) for _ in range(2)]
+            self.buffers.append(bufs)
+            self.caches.append(ctx.kv_cache(cache, M * per_seq, page, self.kv_heads, head_dim, *bufs))
+            if starts[-1]:
+                rows = [rng.standard_normal((int(starts[-1]), shape.kv_dim)).astype(np.float16) for _ in range(2)]
+                up = [ctx.upload(r.view(np.uint16)) for r in rows]
+                ctx.kv_write(self.caches[-1], fill, up[0], 0, up[1], 0)
+                ctx.sync()
+                for b in up:
+                    ctx.free(b)
+                if host is not None:
+                    host[f"cache.{layer}"] = rows
+        self.set_lengths(lengths)
+
+    def set_lengths(self, lengths):
+        """Positions that the sequences have before the next step's token."""
+        self.lengths = np.asarray(lengths, np.int32).copy()
+        self.ctx.upload(self.lengths + 1, self.kv_len)
+
+    def advance(self):
+        self.set_lengths(self.lengths + 1)
+
+    def enqueue(self, layer, q, k, v):
+        c = self.ctx
+        c.rope_kv_write(self.caches[layer], self.batch, self.cos, self.sin, self.max_len, self.D, self.q_heads, q, 0, q, 0, k, 0, v, 0)
+        c.attention(self.caches[layer], self.batch, self.q_heads, q, 0, self.out, 0, self.D ** -0.5, self.window, self.sinks)
+
+    def close(self):
+        for cache in self.caches:
+            cache.close()
 
 
 class DecodeStep:
     def __init__(self, ctx, shape: synth.ModelShape, fmt: str, M: int = 1, n_sets: int = 1, seed: int = 1235,
-                 vocab_rows=None, keep_host=False, only=None, comm=None, norm=False, gather_logits=False, chained=False, qkv_bias=False):
+                 vocab_rows=None, keep_host=False, only=None, comm=None, norm=False, gather_logits=False, chained=False, qkv_bias=False,
+                 attention=None):
         self.ctx, self.shape, self.fmt, self.M = ctx, shape, fmt, M
         # with a communicator the lm_head rows are this rank's shard and the projection
         # stores into every rank's gather buffer (one buffer per weight set, so that
@@ -55,6 +111,10 @@ class DecodeStep:
             self.gamma = ctx.upload(g.view(np.uint16))
             if self.host is not None:
                 self.host["gamma"] = g
+        # attention: keyword arguments of Attention (at least lengths=[...], one per row); o_proj then reads its output
+        if attention and not chained:
+            raise ValueError("attention needs a chained step")
+        self.attention = Attention(ctx, shape, M, host=self.host, **attention) if attention else None
         # qkv_bias=True: Qwen's q/k/v bias rows (src/models/qwen2-5-0-5b/src/layers/attention.cpp:413-469), one set per layer
         self.qkv_bias = None
         if qkv_bias:
@@ -115,7 +175,7 @@ class DecodeStep:
         c, s, M, sh = self.ctx, self.sets[set_index], self.M, self.shape
         ch = self.chained
         x_qkv = self.resid if (ch or self.norm) else self.x_h
-        x_o = self.q if ch else self.x_attn
+        x_o = self.attention.out if self.attention else self.q if ch else self.x_attn
         x_down = self.act if ch else self.x_act
         x_head = self.resid if ch else self.x_h
         for kind, layer, ws in self.ops:
@@ -135,6 +195,8 @@ class DecodeStep:
             elif kind == "qkv":
                 c.linear_qkv(M, sh.hidden, x_qkv, w[0], sh.q_dim, w[1], sh.kv_dim, w[2], sh.kv_dim, self.q, self.k, self.v)
             elif kind == "o_add":
+                if self.attention:
+                    self.attention.enqueue(layer, self.q, self.k, self.v)
                 c.linear_add(M, sh.hidden, sh.q_dim, x_o, w[0], self.resid)
             elif kind == "gate_up":
                 c.fused_gate_up_silu(M, sh.ffn, sh.hidden, x_qkv, w[0], w[1], self.act)

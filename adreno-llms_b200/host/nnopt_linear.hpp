@@ -53,6 +53,17 @@ inline bool lm_head_argmax_m1(nn_context* queue, int vocab, int hidden, nn_buf x
     return nn_linear_argmax(queue, vocab, hidden, x, W, logits, token_out) == NN_OK;
 }
 
+// src/models/smollm2-135m-instruct/src/layers/attention.cpp:724-769: rotation of q (in place) and k, k and v into the cache, and the
+// attention of one new token per sequence over it.  The reference keeps one contiguous cache of one sequence; here it is a
+// paged one of `batch->num_seqs` sequences (nn_kv_cache), and cos / sin are tables by position.
+inline bool fused_rope_kvwrite_m1(nn_context* queue, nn_kv_cache* cache, const nn_kv_batch* batch, nn_buf cos_f32, nn_buf sin_f32, int table_len, int head_dim,
+                                  int q_heads, nn_buf q_inout, nn_buf k, nn_buf v) {
+    return nn_rope_kv_write(queue, cache, batch, cos_f32, sin_f32, table_len, head_dim, q_heads, q_inout, 0, q_inout, 0, k, 0, v, 0) == NN_OK;
+}
+inline bool fused_decode_attn_m1(nn_context* queue, nn_kv_cache* cache, const nn_kv_batch* batch, int q_heads, nn_buf q, nn_buf out, float scale) {
+    return nn_attention(queue, cache, batch, q_heads, q, 0, out, 0, scale, 0, 0) == NN_OK;
+}
+
 // RMSNorm::forward (src/models/smollm2-135m-instruct/src/layers/layer_norm.cpp:76-126) and the norm fused
 // into the projection that consumes it.
 inline bool rmsnorm_forward(nn_context* queue, int rows, int cols, nn_buf x, nn_buf weight, float eps, nn_buf out) {

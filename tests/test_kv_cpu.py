@@ -141,3 +141,27 @@ def test_operand_refusals(nnb, built_lib, call, change, text):
     rc, h = _create(nnb, built_lib)
     assert call(built_lib, h, _batch(nnb), **change) == nnb.NN_ERR_ARG and text in built_lib.nn_last_error(), built_lib.nn_last_error()
     built_lib.nn_kv_cache_free(h)
+
+
+MIRROR = r"""
+#include "nnopt_linear.hpp"
+int main() {
+    nn_kv_cache* cache = nullptr;
+    if (nn_kv_cache_create(nullptr, NN_KV_FP16, 4, 16, 2, 64, (nn_buf)0x100000, (nn_buf)0x200000, nullptr, nullptr, &cache) != NN_OK) return 1;
+    nn_kv_batch b = {1, 1, 1, 64, 4, (nn_buf)0x300000, (nn_buf)0x400000, (nn_buf)0x500000};
+    nn_buf q = (nn_buf)0x4000000, k = (nn_buf)0x5000000, v = (nn_buf)0x6000000, out = (nn_buf)0x7000000, cos = (nn_buf)0x8000000, sin = (nn_buf)0x9000000;
+    // (without a context every call is refused)
+    if (nnopt::fused_rope_kvwrite_m1(nullptr, cache, &b, cos, sin, 64, 64, 4, q, k, v)) return 2;
+    if (nnopt::fused_decode_attn_m1(nullptr, cache, &b, 4, q, out, 0.125f)) return 3;
+    return nn_kv_cache_free(cache) == NN_OK ? 0 : 4;
+}
+"""
+
+
+def test_cpp_mirror_of_rotation_and_attention(built_lib, tmp_path):
+    src, exe = tmp_path / "mirror.cpp", tmp_path / "mirror"
+    src.write_text(MIRROR)
+    base = os.path.join(REPO, "adreno-llms_b200")
+    subprocess.check_call(["g++", "-std=c++17", "-Wall", "-Werror", "-I", os.path.join(base, "host"), str(src), "-o", str(exe), "-L" + os.path.join(base, "lib"),
+                           "-lnnopt_b200", "-Wl,-rpath," + os.path.join(base, "lib")])
+    assert subprocess.run([str(exe)]).returncode == 0
