@@ -32,7 +32,7 @@ constexpr int BN = 128;   // keys of a tile
 // Where a warp is in its block's work.  It lies in shared memory: two dozen registers less in the softmax's loops.
 struct Steps {
     Walk walk, begin;
-    Segment sg;
+    Segment sg, next;   // (the softmax warps fetch the next one's queries early)
 };
 
 template <int FMT, int D>
@@ -216,12 +216,13 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         const Walk walk = find_work(a.s, &w, 2, a.status);
         if (lane == 0) steps.walk = steps.begin = walk;
     }
-    auto next_segment = [&]() {
+    auto next_into = [&](Segment* to) {
         int more = 0;
         __syncwarp();
-        if (lane == 0) more = steps.walk.next(a.s, w, &steps.sg);
+        if (lane == 0) more = steps.walk.next(a.s, w, to);
         return __shfl_sync(0xffffffffu, more, 0) != 0;
     };
+    auto next_segment = [&]() { return next_into(&steps.sg); };
     const int shift = a.c.page_shift;
     const float scale2 = a.scale * 1.4426950408889634f;
     int4* const info = a.items + blockIdx.x;   // for the kernel that joins the parts: what this block has begun and not finished
@@ -241,7 +242,24 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         const uint32_t qtile = base + C::O_Q + i * C::TILE;
         uint32_t s_phase = 0, o_phase = 0;
         int kt = 0;   // key tiles of the block so far
-        while (next_segment()) {
+        // This thread's half of its row of a segment's queries, to where the products take them from.
+        auto queries = [&](const Segment& s) {
+            const ItemRows rows(s, w);
+            const int kv_head = s.vhead / parts, g = r % w.group, t = rows.first(i) + r / w.group, hg = (s.vhead % parts) * w.group + g;
+            const bool on = r < rows.per * w.group && t <= rows.last(i) && hg < a.group;
+            const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)(s.row0 + t) * a.q_stride + (int64_t)(kv_head * a.group + hg) * D) + c * (D / 16);
+            uint4 v[D / 16];
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) v[x] = on ? src[x] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) st_shared16(operand_at(qtile, r, c * (D / 16) + x), v[x]);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(C::B_Q + i));
+        };
+        bool more = next_segment();
+        if (more) queries(sg);
+        while (more) {
             const ItemRows rows(sg, w);
             const TileRange tr = sg.tiles(w);
             const int kv_head = sg.vhead / parts, g = r % w.group, t = rows.first(i) + r / w.group, hg = (sg.vhead % parts) * w.group + g;
@@ -249,14 +267,6 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             const int row = sg.row0 + t, head = kv_head * a.group + hg, pos = on ? sg.len - sg.n + t : -1, lo = window_begin(pos < 0 ? 0 : pos, w.window);
             // positions of the tile's first and last token
             const int pmin = sg.len - sg.n + rows.first(i), pmax = sg.len - sg.n + rows.last(i), lo_max = window_begin(pmax < 0 ? 0 : pmax, w.window);
-            {
-                const uint4* src = reinterpret_cast<const uint4*>(a.q + (int64_t)row * a.q_stride + (int64_t)head * D);
-#pragma unroll
-                for (int ch = c * (D / 16); ch < (c + 1) * (D / 16); ++ch) st_shared16(operand_at(qtile, r, ch), on ? src[ch] : make_uint4(0, 0, 0, 0));
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(C::B_Q + i));
-            }
             float m = -INFINITY, l = 0.f;
             bool first = true;
             for (int j = rows.turns ? i : 0; j < sg.count; j += rows.turns ? 2 : 1) {
@@ -368,6 +378,9 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
 
             // ---- the segment's result ----
             const bool mine = rows.turns ? i < sg.count : true;   // this tile has had keys
+            // The next segment's queries: the products have taken this one's, as the scores of its last tile have come, and go on meanwhile.
+            more = next_into(&steps.next);
+            if (more && mine) queries(steps.next);
             if (mine) {
                 wait(C::B_O + i, o_phase);
                 o_phase ^= 1;
@@ -393,48 +406,43 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 uint16_t* out = a.out + (int64_t)row * a.o_stride + (int64_t)head * D + c * (D / 2);
                 bool fine = l > 0.f && l < INFINITY;
 #pragma unroll 1
-                for (int pass = whole ? 0 : 1; pass < 2; ++pass) {   // whole items: first whether all of the row is finite
-                    if (whole && pass == 1) {
-                        pair_sync(pair_bar);   // (the sums have been read)
-                        *own = fine ? 0.f : 1.f;
-                        pair_sync(pair_bar);
-                        fine = fine && *other == 0.f;
+                for (int cb = 0; cb < D / 32; ++cb) {
+                    uint32_t o[16];
+                    float v[16];
+                    tmem_ld16(to + cb * 16, o);
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(o[x]) * f0;
+                    if (both) {
+                        tmem_ld16(to + D + cb * 16, o);
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) v[x] = fmaf(__uint_as_float(o[x]), f1, v[x]);
                     }
-#pragma unroll 1
-                    for (int cb = 0; cb < D / 32; ++cb) {
-                        uint32_t o[16];
-                        float v[16];
-                        tmem_ld16(to + cb * 16, o);
+                    if (!whole) {
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) v[x] = __uint_as_float(o[x]) * f0;
-                        if (both) {
-                            tmem_ld16(to + D + cb * 16, o);
+                        for (int x = 0; x < 4; ++x) part[(c * (D / 8) + cb * 4 + x) * 256 + i * 128 + r] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+                        continue;
+                    }
 #pragma unroll
-                            for (int x = 0; x < 16; ++x) v[x] = fmaf(__uint_as_float(o[x]), f1, v[x]);
-                        }
-                        if (!whole) {
+                    for (int x = 0; x < 16; ++x) {
+                        v[x] *= scale_out;
+                        fine = fine && fabsf(v[x]) < INFINITY;
+                    }
+                    if (on) {
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) part[(c * (D / 8) + cb * 4 + x) * 256 + i * 128 + r] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
-                            continue;
-                        }
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) {
-                            v[x] *= scale_out;
-                            fine = fine && fabsf(v[x]) < INFINITY;
-                        }
-                        if (pass == 1 && on && fine) {
-#pragma unroll
-                            for (int x = 0; x < 2; ++x)
-                                reinterpret_cast<uint4*>(out)[cb * 2 + x] = make_uint4(floats_half2(v[8 * x], v[8 * x + 1]), floats_half2(v[8 * x + 2], v[8 * x + 3]),
-                                                                                      floats_half2(v[8 * x + 4], v[8 * x + 5]), floats_half2(v[8 * x + 6], v[8 * x + 7]));
-                        }
+                        for (int x = 0; x < 2; ++x)
+                            reinterpret_cast<uint4*>(out)[cb * 2 + x] = make_uint4(floats_half2(v[8 * x], v[8 * x + 1]), floats_half2(v[8 * x + 2], v[8 * x + 3]),
+                                                                                  floats_half2(v[8 * x + 4], v[8 * x + 5]), floats_half2(v[8 * x + 6], v[8 * x + 7]));
                     }
                 }
                 if (!whole) {
                     if (c == 0) reinterpret_cast<float2*>(part + 64 * D)[i * 128 + r] = make_float2(m, l);
                     if (sg.first == 0 && tid == 0) *info = make_int4(sg.seq, sg.vhead, sg.qt, (int)((sg.unit0 + sg.total - 1) / w.chunk));
                 } else {
-                    // rows that are not finite, or see nothing, are marked by a NaN
+                    // rows that are not finite in either half, or see nothing, are marked by a NaN
+                    pair_sync(pair_bar);   // (the sums have been read)
+                    *own = fine ? 0.f : 1.f;
+                    pair_sync(pair_bar);
+                    fine = fine && *other == 0.f;
                     if (c == 0 && on && !fine) {
                         *out = 0x7FFF;
                         *some_again = 1;
@@ -445,6 +453,11 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             // (what the threads have told each other has been read)
             if (rows.turns) asm volatile("bar.sync 9, 512;" ::: "memory");
             else pair_sync(pair_bar);
+            // (without keys of its own, this tile's barrier must not get two segments ahead of the products)
+            if (more && !mine) queries(steps.next);
+            __syncwarp();
+            if (lane == 0) sg = steps.next;
+            __syncwarp();
         }
         // Marked rows: from the formula once more, which does not use hidden cells.  Behind the loop: no wait of another warp runs out meanwhile, and
         // this takes no registers from it (int8 cells of 128 dims, 2048 tokens of 32 heads to 16384 positions: 675 us, 800 with this inside).

@@ -176,7 +176,8 @@ __device__ __forceinline__ Quad add_up(int k, int quads, int count, At&& at) {
     Quad q;
     q.v = make_float4(0.f, 0.f, 0.f, 0.f);
     q.h = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
-    constexpr int N = 4;   // (loads of so many at once)
+    constexpr int N = 4;   // (so many at once: their loads and exponentials do not wait for one another)
+#pragma unroll 1
     for (int i0 = 0; i0 < count; i0 += N) {
         float4 h[N], v[N];
 #pragma unroll
@@ -185,14 +186,22 @@ __device__ __forceinline__ Quad add_up(int k, int quads, int count, At&& at) {
             h[i] = p[b * 32 + lane];
             v[i] = p[(NB + k) * 32 + lane];
         }
+        float u0 = q.h.x, u1 = q.h.z;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             if (i0 + i >= count) h[i].x = h[i].z = -INFINITY;
-            const float u0 = fmaxf(q.h.x, h[i].x), u1 = fmaxf(q.h.z, h[i].z);
-            const float a0 = q.h.x == -INFINITY ? 0.f : ex2(q.h.x - u0), a1 = q.h.z == -INFINITY ? 0.f : ex2(q.h.z - u1);
-            const float f0 = h[i].x == -INFINITY ? 0.f : ex2(h[i].x - u0), f1 = h[i].z == -INFINITY ? 0.f : ex2(h[i].z - u1);
-            q.h = make_float4(u0, q.h.y * a0 + h[i].y * f0, u1, q.h.w * a1 + h[i].w * f1);
-            q.v = make_float4(q.v.x * a0 + v[i].x * f0, q.v.y * a1 + v[i].y * f1, q.v.z * a0 + v[i].z * f0, q.v.w * a1 + v[i].w * f1);
+            u0 = fmaxf(u0, h[i].x);
+            u1 = fmaxf(u1, h[i].z);
+        }
+        const float r0 = u0 == -INFINITY ? 0.f : u0, r1 = u1 == -INFINITY ? 0.f : u1, a0 = ex2(q.h.x - r0), a1 = ex2(q.h.z - r1);
+        q.h = make_float4(u0, q.h.y * a0, u1, q.h.w * a1);
+        q.v = make_float4(q.v.x * a0, q.v.y * a1, q.v.z * a0, q.v.w * a1);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float f0 = ex2(h[i].x - r0), f1 = ex2(h[i].z - r1);
+            q.h.y = fmaf(h[i].y, f0, q.h.y);
+            q.h.w = fmaf(h[i].w, f1, q.h.w);
+            q.v = make_float4(fmaf(v[i].x, f0, q.v.x), fmaf(v[i].y, f1, q.v.y), fmaf(v[i].z, f0, q.v.z), fmaf(v[i].w, f1, q.v.w));
         }
     }
     return q;
@@ -207,7 +216,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
     const uint32_t base = smem_u32(smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), quad = lane >> 2, c = lane & 3;
     const uint32_t ring = base + S_RING + warp * (STAGES * STAGE), scales = base + S_SCALE + warp * (STAGES * 256), bars = base + S_BARS + warp * (STAGES * 8);
-    if (lane < STAGES) mbar_init(bars + lane * 8, 1);
+    if (lane < STAGES) mbar_init(bars + lane * 8, CODES ? 33 : 1);   // (the tensor copies' lane, and each lane's copy of scales)
     mbar_init_fence();
     __syncwarp();
     pdl_wait_prior_grid();
@@ -227,13 +236,28 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
     const float scale2 = a.scale * 1.4426950408889634f;
 
     // ---- this warp's copies, a ring in front of its products ----
+    Segment sg;
+    bool more = walk.next(a.s, w, &sg);
     Walk pw = walk;
-    const int* ptable = a.s.page_table;
+    const int* ptable = nullptr;
     int phead = 0, pcount = 0, pfirst = 0, psink = 0, pskip = 0, plast = -1, plo = 0;   // the segment: its key tiles, its last position, its window
-    int pslice = warp, issued = 0, page_base = 0, page_reg = -1;
-    bool pmore = true;
+    int pslice = 0, issued = 0, page_base = 0, page_reg = -1;
+    bool pmore = more;
+    auto copy_from = [&](const Segment& s) {
+        const TileRange tr = s.tiles(w);
+        ptable = a.s.page_table + (int64_t)s.seq * a.s.table_stride;
+        phead = s.vhead;
+        pcount = s.count;
+        pfirst = s.first;
+        psink = tr.sink_tiles;
+        pskip = tr.first - tr.sink_tiles;
+        plast = s.p1(w);
+        plo = window_begin(max(s.p0(w), 0), w.window);
+        pslice = warp;
+        page_base = -64;   // (no page numbers yet)
+    };
+    if (more) copy_from(sg);
     auto issue = [&]() {   // the next stage's copies, if there is one
-        bool fresh = false;
         while (pmore && pslice >= pcount) {
             Segment s;
             pmore = pw.next(a.s, w, &s);
@@ -242,23 +266,13 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
                 pdl_launch_dependents();
                 return;
             }
-            const TileRange tr = s.tiles(w);
-            ptable = a.s.page_table + (int64_t)s.seq * a.s.table_stride;
-            phead = s.vhead;
-            pcount = s.count;
-            pfirst = s.first;
-            psink = tr.sink_tiles;
-            pskip = tr.first - tr.sink_tiles;
-            plast = s.p1(w);
-            plo = window_begin(max(s.p0(w), 0), w.window);
-            pslice = warp;
-            fresh = true;
+            copy_from(s);
         }
         if (!pmore) return;
         auto key_at = [&](int slice) { return (pfirst + slice + (pfirst + slice < psink ? 0 : pskip)) * S::KT; };
         // page numbers of this warp's next boxes, one per lane: those of its stages in the segment are numbered in order
         const int j = (pslice / WARPS) << nbox_shift;
-        if (fresh || j + nbox > page_base + 32) {
+        if (j + nbox > page_base + 32) {
             page_base = j;
             const int slice = ((j + lane) >> nbox_shift) * WARPS + warp, key = key_at(slice) + ((j + lane) & (nbox - 1)) * box;
             page_reg = -1;
@@ -275,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
         const unsigned here = __ballot_sync(0xffffffffu, mine);   // the boxes that are copied: the others' keys count as hidden
         if (lane == 0) {
             reinterpret_cast<unsigned*>(smem + S_HERE)[warp * STAGES + stage] = here;
-            mbar_arrive_expect_tx(bar, (uint32_t)(__popc(here) * box * (2 * S::ROW + (CODES ? 4 : 0))));
+            mbar_arrive_expect_tx(bar, (uint32_t)(__popc(here) * box * 2 * S::ROW));
         }
         __syncwarp();
         if (mine) {
@@ -287,10 +301,15 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
                 tma_load_2d(dst + h * (S::KT * W) + lane * box * W, &maps.k, h * 64, (int)row, bar, pol);
                 tma_load_2d(dst + PART + h * (S::KT * W) + lane * box * W, &maps.v, h * 64, (int)row, bar, pol);
             }
-            if (CODES) {
-                bulk_g2s(sdst + lane * box * 2, a.c.k_scale + row, box * 2, bar, pol);
-                bulk_g2s(sdst + 128 + lane * box * 2, a.c.v_scale + row, box * 2, bar, pol);
+        }
+        if (CODES) {   // 8 scales to a lane, plain asynchronous copies (with bulk ones, 64 sequences of 8192 positions, e4m3 of 128 dims: 149 us,
+            // 146 so)
+            const int x = lane % (S::KT / 8) * 8, from = __shfl_sync(0xffffffffu, page, x >> box_shift);
+            if (lane < S::KT / 4 && from >= 0) {
+                const int64_t row = cell_row(from, phead, (key_at(pslice) + x) & ((1 << shift) - 1), a.c.kv_heads, shift);
+                cp_async_16(sdst + (lane < S::KT / 8 ? 0 : 128) + x * 2, (lane < S::KT / 8 ? a.c.k_scale : a.c.v_scale) + row);
             }
+            cp_async_mbar_arrive_noinc(bar);
         }
         pslice += WARPS;
         ++issued;
@@ -298,17 +317,18 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
 
     int used = 0;
     bool dead = false;
-    Segment sg;
-    while (walk.next(a.s, w, &sg)) {
+    for (; more; more = walk.next(a.s, w, &sg)) {
         const int p0 = sg.p0(w), p1 = sg.p1(w), lo0 = window_begin(p0 < 0 ? 0 : p0, w.window), lo1 = window_begin(p1 < 0 ? 0 : p1, w.window);
         const TileRange tr = sg.tiles(w);
-        // row r of the item: its row of the operands (-1: none), its head, its position
+        // row r of the item: its token, its row of the operands (-1: none), its head, its position
+        const int thirds = (256 + w.group - 1) / w.group;
+        auto token_of = [&](int r) { return r * thirds >> 8; };   // r / w.group, for r and w.group up to 16
         auto row_of = [&](int r) {
-            const int t = sg.qt * w.tokens + r / w.group;
+            const int t = sg.qt * w.tokens + token_of(r);
             return r < w.tokens * w.group && t < sg.n ? sg.row0 + t : -1;
         };
-        auto head_of = [&](int r) { return sg.vhead * w.group + r % w.group; };
-        auto pos_of = [&](int r) { return sg.len - sg.n + sg.qt * w.tokens + r / w.group; };
+        auto head_of = [&](int r) { return sg.vhead * w.group + r - token_of(r) * w.group; };
+        auto pos_of = [&](int r) { return sg.len - sg.n + sg.qt * w.tokens + token_of(r); };
         int pos[NB][2];   // of this lane's rows of scores
         uint32_t q[NB][S::DG][2];
 #pragma unroll

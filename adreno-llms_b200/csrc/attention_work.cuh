@@ -52,7 +52,7 @@ __device__ __forceinline__ SeqWork load_seq(const KvSeqs& s, const WorkShape& w,
     q.row0 = e.row0;
     q.n = e.row1 - e.row0;
     q.len = e.len;
-    q.tiles_q = (q.n + w.tokens - 1) / w.tokens;
+    q.tiles_q = q.n <= w.tokens ? (q.n > 0) : (q.n + w.tokens - 1) / w.tokens;   // (a division costs as much as a load from the L2)
     return q;
 }
 __device__ __forceinline__ int item_tiles(const SeqWork& q, const WorkShape& w, int qt) {
@@ -149,9 +149,11 @@ __device__ __forceinline__ Walk find_work(const KvSeqs& s, WorkShape* w, unsigne
         if (bad) *status = STATUS_BAD_TABLE;
         disorder |= descends;
     };
+    unsigned tiles = 0;
     for (int i0 = 0; i0 < s.num_seqs; i0 += 32) {
         load(i0);
-        total += __reduce_add_sync(0xffffffffu, seq_tiles(q, *w));
+        tiles = seq_tiles(q, *w);
+        total += __reduce_add_sync(0xffffffffu, tiles);
         items += __reduce_add_sync(0xffffffffu, (unsigned)q.tiles_q);
     }
     if (__any_sync(0xffffffffu, disorder)) return k;
@@ -168,7 +170,11 @@ __device__ __forceinline__ Walk find_work(const KvSeqs& s, WorkShape* w, unsigne
     unsigned base = 0;
     for (int i0 = 0; i0 < s.num_seqs; i0 += 32) {
         if (s.num_seqs > 32) load(i0);
-        const unsigned mine = seq_tiles(q, *w) * w->vheads;
+        // (of a head; what has been counted above serves where items are not filled up, or are one to a sequence)
+        const unsigned head = s.num_seqs <= 32 && !w->pad                                             ? tiles + q.tiles_q * w->extra
+                              : s.num_seqs <= 32 && __all_sync(0xffffffffu, q.tiles_q <= 1) ? (q.tiles_q ? w->units(tiles) : 0u)
+                                                                                            : seq_tiles(q, *w);
+        const unsigned mine = head * w->vheads;
         unsigned upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -182,7 +188,7 @@ __device__ __forceinline__ Walk find_work(const KvSeqs& s, WorkShape* w, unsigne
         }
         const int l = __ffs(hit) - 1;   // the sequence of the block's first unit
         unsigned rest = k.u - base - __shfl_sync(0xffffffffu, upto - mine, l);
-        const unsigned per_head = __shfl_sync(0xffffffffu, mine, l) / w->vheads;
+        const unsigned per_head = __shfl_sync(0xffffffffu, head, l);
         k.seq = i0 + l;
         k.q.row0 = __shfl_sync(0xffffffffu, q.row0, l);
         k.q.n = __shfl_sync(0xffffffffu, q.n, l);
