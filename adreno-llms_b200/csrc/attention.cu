@@ -52,9 +52,9 @@ bool attention_countable(const AttnArgs& a, int max_new) {
 }
 
 cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl, int* kernels) {
-    *kernels = few_rows(a, max_new) ? 1 : 2;
-    if (*kernels == 1) return launch_attention_decode(a, maps, max_new, sm_count, st, pdl);
-    return launch_attention_chunk(a, maps, sm_count, st, pdl);
+    *kernels = 1;
+    if (few_rows(a, max_new)) return launch_attention_decode(a, maps, max_new, sm_count, st, pdl);
+    return launch_attention_chunk(a, maps, sm_count, st, pdl, kernels);
 }
 
 }  // namespace nnb

@@ -61,6 +61,7 @@ struct AttnArgs {
     int* status;
     unsigned* counters;      // blocks of a shared item that have arrived (0 between launches)
     int4* items;             // shared items, by the block that begins them
+    int join_here;           // (chunks) whether the last block to have a part of an item joins all of them
     void* parts;             // partial results of items that blocks share: the context's, for one call at a time
 };
 struct AttnMaps;

@@ -57,7 +57,7 @@ struct Chunk {
     static constexpr int B_KFULL = 0, B_KEMPTY = B_KFULL + RING, B_VFULL = B_KEMPTY + RING, B_VEMPTY = B_VFULL + RING, B_META = B_VEMPTY + RING,
                          B_RFULL = B_META + META, B_REMPTY = B_RFULL + RAWS, B_Q = B_REMPTY + RAWS, B_S = B_Q + 2, B_P = B_S + 2, B_O = B_P + 2, B_FIX = B_O + 2, B_DONE = B_FIX + 1,
                          BARS = B_DONE + 1;
-    static constexpr int O_TMEM = O_BARS + BARS * 8, O_DEAD = O_TMEM + 4, BYTES = O_DEAD + 8, SMEM = BYTES + 1024;
+    static constexpr int O_TMEM = O_BARS + BARS * 8, O_DEAD = O_TMEM + 4, BYTES = O_DEAD + 12, SMEM = BYTES + 1024;
     static_assert(SMEM <= 227 * 1024, "shared memory");
     static_assert(RAWS % (BN / RAW_KEYS) == 0, "a stage belongs to one part of a tile");
     static_assert(O_BARS % 8 == 0 && O_RAW % 128 == 0 && RAW_STAGE % 16 == 0 && O_META % 16 == 0, "alignment");
@@ -158,6 +158,75 @@ __device__ __forceinline__ bool pair_any(int id, bool yes) {
     return r != 0;
 }
 
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 9, 512;" ::: "memory"); }
+
+// The 512 threads of the softmax, after their part of an item that several blocks share has been written: where it is the last one to
+// arrive, adds all of them up, in the blocks' order.  True: some row of this thread's is not finite (it is marked).
+template <int D>
+__device__ __forceinline__ bool join_parts(const AttnArgs& a, const Segment& sg, const WorkShape& w, const ItemRows& rows, int parts, volatile int* joined) {
+    const int tid = threadIdx.x, b0 = (int)(sg.unit0 / w.chunk), b1 = (int)((sg.unit0 + sg.total - 1) / w.chunk), id = sg.first ? 1 : 2;
+    __threadfence();
+    softmax_sync();
+    if (tid == 0) {
+        const bool last = atomicAdd(a.counters + b0, 1u) == (unsigned)(b1 - b0);
+        if (last) {
+            a.counters[b0] = 0u;
+            *joined = *joined | id;
+        }
+    }
+    softmax_sync();
+    if (!(*joined & id)) return false;
+    __threadfence();
+    // a row to a thread, and half of its dims, or a quarter where there are 128 rows
+    const int r = rows.turns ? tid & 127 : tid & 255, i = r >> 7, rr = r & 127, t = rows.first(i) + rr / w.group, hg = (sg.vhead % parts) * w.group + rr % w.group;
+    const bool on = rr < rows.per * w.group && t <= rows.last(i) && hg < a.group;
+    const int quads = rows.turns ? D / 16 : D / 8, q0 = (rows.turns ? tid >> 7 : tid >> 8) * quads;
+    const float4* base = reinterpret_cast<const float4*>(a.parts);
+    auto part = [&](int b) { return base + (int64_t)(2 * b + (b == b0 ? 1 : 0)) * (ATTN_CHUNK_PART / 16); };
+    auto sums = [&](int b) { return reinterpret_cast<const float2*>(part(b) + 64 * D)[r]; };   // maximum and sum of the weights
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 4
+    for (int b = b0; b <= b1; ++b) m = fmaxf(m, sums(b).x);
+    const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+    for (int b = b0; b <= b1; ++b) {
+        const float2 x = sums(b);
+        l = fmaf(x.y, ex2(x.x - ref), l);
+    }
+    const float inv = 1.f / l;
+    bool fine = l > 0.f && l < INFINITY;
+    uint16_t* const out = a.out + (int64_t)(sg.row0 + t) * a.o_stride + (int64_t)(sg.vhead / parts * a.group + hg) * D;
+#pragma unroll 1
+    for (int q = q0; q < q0 + quads; q += 4) {
+        float4 o[4] = {};
+#pragma unroll 2
+        for (int b = b0; b <= b1; ++b) {
+            const float4* p = part(b) + q * 256 + r;
+            float4 v[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) v[x] = p[x * 256];
+            const float f = ex2(sums(b).x - ref);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[x] = make_float4(fmaf(v[x].x, f, o[x].x), fmaf(v[x].y, f, o[x].y), fmaf(v[x].z, f, o[x].z), fmaf(v[x].w, f, o[x].w));
+        }
+        uint32_t h[8];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const float y[4] = {o[x].x * inv, o[x].y * inv, o[x].z * inv, o[x].w * inv};
+            fine = fine && fabsf(y[0]) < INFINITY && fabsf(y[1]) < INFINITY && fabsf(y[2]) < INFINITY && fabsf(y[3]) < INFINITY;
+            h[2 * x] = floats_half2(y[0], y[1]);
+            h[2 * x + 1] = floats_half2(y[2], y[3]);
+        }
+        if (on) {
+            reinterpret_cast<uint4*>(out + 4 * q)[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            reinterpret_cast<uint4*>(out + 4 * q)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+    }
+    softmax_sync();
+    if (on && !fine) *out = 0x7FFF;
+    return on && !fine;
+}
+
 template <int FMT, int D>
 __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_kernel(const __grid_constant__ AttnMaps maps, const AttnArgs a) {
     using C = Chunk<FMT, D>;
@@ -168,7 +237,8 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     auto bar = [&](int i) { return bars + (uint32_t)i * 8; };
     volatile int* dead = reinterpret_cast<volatile int*>(smem + C::O_DEAD);
-    volatile int* some_again = dead + 1;   // some row of the block's whole items has to be computed once more
+    volatile int* some_again = dead + 1;   // some row of the items that the block has finished has to be computed once more
+    volatile int* joined = dead + 2;       // which of its parts of items the block has joined with the others: 1 its first one, 2 its last one
     // Waits of whole warps.  When one runs out the block carries on without waiting: what it computes is void, and ends.
     auto wait = [&](int b, uint32_t parity) {
         uint32_t ok = mbar_try_wait(bar(b), parity);
@@ -192,7 +262,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         if ((b >= C::B_Q && b < C::B_S) || (b >= C::B_P && b < C::B_O)) n = 8;
         mbar_init(bar(b), n);
     }
-    if (tid == 0) *dead = *some_again = 0;
+    if (tid == 0) *dead = *some_again = *joined = 0;
     mbar_init_fence();
     if (warp == 16) tmem_alloc<false>(base + C::O_TMEM, 512);
     tc_fence_before();
@@ -226,12 +296,13 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     const int shift = a.c.page_shift;
     const float scale2 = a.scale * 1.4426950408889634f;
     int4* const info = a.items + blockIdx.x;   // for the kernel that joins the parts: what this block has begun and not finished
-    if (tid == 0) *info = make_int4(-1, 0, 0, 0);
+    if (tid == 0 && !a.join_here) *info = make_int4(-1, 0, 0, 0);
 
     // Registers of a thread: more for the four groups of four warps that do the softmax, fewer for the others.  The shares add up to what the block
-    // was launched with, 5 x 96 or 6 x 80.
-    if (warp < 16) set_registers_more<C::THREADS == 640 ? 104 : 88>();
-    else set_registers_fewer<64>();
+    // was launched with: 4 x 104 + 64 = 5 x 96, 4 x 96 + 2 x 48 = 6 x 80.  (With 88 and 64 of the latter int8 cells, 2048 tokens of 32 heads of 128 dims to
+    // 16384 positions, took 734 us instead of 684.)
+    if (warp < 16) set_registers_more<C::THREADS == 640 ? 104 : 96>();
+    else set_registers_fewer<C::THREADS == 640 ? 64 : 48>();
     if (warp < 16) {
         // ---- softmax of query tile i, keys 64 c .. of a tile; row r ----
         const int i = warp >> 3, c = warp >> 2 & 1, r = tid & 127, pair_bar = 1 + i * 4 + (warp & 3);
@@ -388,7 +459,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             float f0 = 1.f, f1 = 0.f;   // factors of this tile's sums and, where the tiles take turns, of the other's
             *own = l;
             if (rows.turns && i == 1) said[4 * BN] = m;
-            if (rows.turns) asm volatile("bar.sync 9, 512;" ::: "memory");
+            if (rows.turns) softmax_sync();
             else pair_sync(pair_bar);
             l += *other;
             if (rows.turns && i == 0) {
@@ -436,7 +507,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 }
                 if (!whole) {
                     if (c == 0) reinterpret_cast<float2*>(part + 64 * D)[i * 128 + r] = make_float2(m, l);
-                    if (sg.first == 0 && tid == 0) *info = make_int4(sg.seq, sg.vhead, sg.qt, (int)((sg.unit0 + sg.total - 1) / w.chunk));
+                    if (!a.join_here && sg.first == 0 && tid == 0) *info = make_int4(sg.seq, sg.vhead, sg.qt, (int)((sg.unit0 + sg.total - 1) / w.chunk));
                 } else {
                     // rows that are not finite in either half, or see nothing, are marked by a NaN
                     pair_sync(pair_bar);   // (the sums have been read)
@@ -449,9 +520,10 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     }
                 }
             }
+            if (a.join_here && sg.count != sg.total && join_parts<D>(a, sg, w, rows, parts, joined)) *some_again = 1;
             tc_fence_before();
             // (what the threads have told each other has been read)
-            if (rows.turns) asm volatile("bar.sync 9, 512;" ::: "memory");
+            if (rows.turns) softmax_sync();
             else pair_sync(pair_bar);
             // (without keys of its own, this tile's barrier must not get two segments ahead of the products)
             if (more && !mine) queries(steps.next);
@@ -461,12 +533,15 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         }
         // Marked rows: from the formula once more, which does not use hidden cells.  Behind the loop: no wait of another warp runs out meanwhile, and
         // this takes no registers from it (int8 cells of 128 dims, 2048 tokens of 32 heads to 16384 positions: 675 us, 800 with this inside).
-        asm volatile("bar.sync 9, 512;" ::: "memory");
-        if (*some_again) {
+        softmax_sync();
+        if (!*some_again) {
+            // Not earlier: waits of the next launch have a limit, which counts from its beginning, and this kernel may run for longer than that.
+            pdl_launch_dependents();
+        } else {
             __syncwarp();
             if (lane == 0) steps.walk = steps.begin;
             while (next_segment()) {
-                if (sg.count != sg.total) continue;
+                if (sg.count != sg.total && !(*joined & (sg.first ? 1 : 2))) continue;
                 const ItemRows rows(sg, w);
                 const int kv_head = sg.vhead / parts, x = warp >> 1, rr = (x & 3) * 32 + lane, g = rr % w.group, t = rows.first(x >> 2) + rr / w.group;
                 const int hg = (sg.vhead % parts) * w.group + g, row = sg.row0 + t, head = kv_head * a.group + hg, pos = sg.len - sg.n + t;
@@ -537,8 +612,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             }
             kt += n;
         }
-        // Not earlier: waits of the next launch have a limit, which counts from its beginning, and this kernel may run for longer than that.
-        pdl_launch_dependents();
+        if (!a.join_here) pdl_launch_dependents();   // (the kernel that joins the parts: its wait has no limit)
         if (issuer) umma_commit<false>(bar(C::B_DONE));
         __syncwarp();
         mbar_wait_bounded(bar(C::B_DONE), 0);
@@ -808,7 +882,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Attn
 }
 
 template <int FMT, int D>
-cudaError_t launch(const AttnArgs& a, const AttnMaps& maps, int blocks, cudaStream_t st, bool pdl) {
+cudaError_t launch(const AttnArgs& a, const AttnMaps& maps, int blocks, cudaStream_t st, bool pdl, int* kernels) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(Chunk<FMT, D>::THREADS);
@@ -820,7 +894,8 @@ cudaError_t launch(const AttnArgs& a, const AttnMaps& maps, int blocks, cudaStre
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     cudaError_t e = cudaLaunchKernelEx(&cfg, attention_chunk_kernel<FMT, D>, maps, a);
-    if (e != cudaSuccess) return e;
+    *kernels = a.join_here ? 1 : 2;
+    if (e != cudaSuccess || a.join_here) return e;
     cfg.gridDim = dim3((unsigned)blocks, 8);
     cfg.blockDim = dim3(JOIN_THREADS);
     cfg.dynamicSmemBytes = 0;
@@ -842,11 +917,20 @@ cudaError_t attention_chunk_configure() {
     return configure<KV_FP8, 128>();
 }
 
-cudaError_t launch_attention_chunk(const AttnArgs& a, const AttnMaps& maps, int sm_count, cudaStream_t st, bool pdl) {
+// An item's parts are joined by the last block to have one, or, where there are several to an item, by a kernel of their own, in more blocks.
+// Here / apart, us: 2 x 4096 tokens under a window of 1024 (16 heads to 8 of 64 dims, fp16; items cut in 1 to 2 parts) 98.5 / 100.8; 16 x 64 tokens to 2048
+// (32 heads to 8 of 128 dims, e4m3; 1 to 2) 78.0 / 80.3; 8 x 20 to 4096 (28 to 4 of 128, fp16; 5) 34.9 / 33.1; 1 x 17 to 4096 (32 to 4 of 64; 32) 23.5 / 18.1;
+// 1 x 32 to 32768 (8 to 1 of 128; 148) 212 / 62.
+constexpr int PARTS_HERE = 2;
+
+cudaError_t launch_attention_chunk(const AttnArgs& given, const AttnMaps& maps, int sm_count, cudaStream_t st, bool pdl, int* kernels) {
     const int blocks = sm_count < ATTN_MAX_BLOCKS ? sm_count : ATTN_MAX_BLOCKS;
-    if (a.c.fmt == KV_FP16) return a.c.dim == 64 ? launch<KV_FP16, 64>(a, maps, blocks, st, pdl) : launch<KV_FP16, 128>(a, maps, blocks, st, pdl);
-    if (a.c.fmt == KV_INT8) return a.c.dim == 64 ? launch<KV_INT8, 64>(a, maps, blocks, st, pdl) : launch<KV_INT8, 128>(a, maps, blocks, st, pdl);
-    return a.c.dim == 64 ? launch<KV_FP8, 64>(a, maps, blocks, st, pdl) : launch<KV_FP8, 128>(a, maps, blocks, st, pdl);
+    AttnArgs a = given;
+    const int parts = (a.group + 127) / 128, tokens = 2 * (128 / ((a.group + parts - 1) / parts)), tiles = (a.s.num_rows - 1) / tokens + 1;
+    a.join_here = (long long)a.c.kv_heads * parts * (a.s.num_seqs > tiles ? a.s.num_seqs : tiles) * PARTS_HERE >= blocks;
+    if (a.c.fmt == KV_FP16) return a.c.dim == 64 ? launch<KV_FP16, 64>(a, maps, blocks, st, pdl, kernels) : launch<KV_FP16, 128>(a, maps, blocks, st, pdl, kernels);
+    if (a.c.fmt == KV_INT8) return a.c.dim == 64 ? launch<KV_INT8, 64>(a, maps, blocks, st, pdl, kernels) : launch<KV_INT8, 128>(a, maps, blocks, st, pdl, kernels);
+    return a.c.dim == 64 ? launch<KV_FP8, 64>(a, maps, blocks, st, pdl, kernels) : launch<KV_FP8, 128>(a, maps, blocks, st, pdl, kernels);
 }
 
 }  // namespace nnb

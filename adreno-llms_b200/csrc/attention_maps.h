@@ -19,6 +19,6 @@ int attention_decode_keys(int fmt, int dim);   // keys of a stage: what a copy t
 cudaError_t attention_decode_configure();
 cudaError_t launch_attention_decode(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl);
 cudaError_t attention_chunk_configure();
-cudaError_t launch_attention_chunk(const AttnArgs& a, const AttnMaps& maps, int sm_count, cudaStream_t st, bool pdl);
+cudaError_t launch_attention_chunk(const AttnArgs& a, const AttnMaps& maps, int sm_count, cudaStream_t st, bool pdl, int* kernels);
 
 }  // namespace nnb
