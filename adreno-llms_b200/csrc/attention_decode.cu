@@ -28,10 +28,9 @@ struct Shape {
     static constexpr int EB = kv_cell_bytes(FMT), ROW = D * EB, KT = PART / ROW;   // bytes of a cell row, keys of a stage
     static constexpr int KG = KT / 16, DG = D / 16;                                // groups of 16 keys, of 16 dims
 };
-constexpr int S_RING = 0, S_SCALE = WARPS * STAGES * STAGE, S_MERGE = S_SCALE + WARPS * STAGES * 256, S_BARS = S_MERGE + 2 * (int)ATTN_DECODE_PART,
+constexpr int S_RING = 0, S_SCALE = WARPS * STAGES * STAGE, S_MERGE = S_SCALE + WARPS * STAGES * 256, MERGE_BYTES = 25344, S_BARS = S_MERGE + MERGE_BYTES,
               S_HERE = S_BARS + WARPS * STAGES * 8, S_FLAG = S_HERE + WARPS * STAGES * 4, SMEM_BYTES = S_FLAG + 32 + 1024;
 static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
-static_assert((int)ATTN_DECODE_PART <= STAGES * STAGE, "a warp's result fits its ring");
 
 __device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3) : "r"(addr));
@@ -101,14 +100,14 @@ struct State {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) l[b][h] += __shfl_xor_sync(0xffffffffu, l[b][h], d);
     }
-    // A partial result: [NB] maxima and sums, [NB][D / 16] quads, each of 32 lanes.
+    // A partial result: maxima and sums of [NB][4] pairs of rows, [NB][D / 16] quads of 32 lanes.
     __device__ __forceinline__ void store(float4* p) const {
         const int lane = threadIdx.x & 31;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            p[b * 32 + lane] = make_float4(m[b][0], l[b][0], m[b][1], l[b][1]);
+            if (lane < 4) p[b * 4 + lane] = make_float4(m[b][0], l[b][0], m[b][1], l[b][1]);
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) p[(NB + b * (D / 16) + i) * 32 + lane] = o[b][i];
+            for (int i = 0; i < D / 16; ++i) p[NB * 4 + (b * (D / 16) + i) * 32 + lane] = o[b][i];
         }
     }
     __device__ __forceinline__ void rescale(int b, float f0, float f1) {
@@ -122,60 +121,17 @@ struct State {
             o[b][i].w *= f1;
         }
     }
-    __device__ __forceinline__ void add(const float4* p) {
-        const int lane = threadIdx.x & 31;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const float4 h = p[b * 32 + lane];
-            const float u0 = fmaxf(m[b][0], h.x), u1 = fmaxf(m[b][1], h.z);
-            rescale(b, m[b][0] == -INFINITY ? 0.f : ex2(m[b][0] - u0), m[b][1] == -INFINITY ? 0.f : ex2(m[b][1] - u1));
-            const float f0 = h.x == -INFINITY ? 0.f : ex2(h.x - u0), f1 = h.z == -INFINITY ? 0.f : ex2(h.z - u1);
-            m[b][0] = u0;
-            m[b][1] = u1;
-            l[b][0] += h.y * f0;
-            l[b][1] += h.w * f1;
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-                const float4 v = p[(NB + b * (D / 16) + i) * 32 + lane];
-                o[b][i].x += v.x * f0;
-                o[b][i].y += v.y * f1;
-                o[b][i].z += v.z * f0;
-                o[b][i].w += v.w * f1;
-            }
-        }
-    }
 };
-
-// The warps' results added up, in a fixed order, into warp 0's, two at a time in `buf`: while other warps' rings hold the next segment's keys.
-template <int D, int NB>
-__device__ __forceinline__ void merge_warps(State<D, NB>& st, uint8_t* buf, int warp) {
-#pragma unroll 1
-    for (int n = WARPS; n > 1; n = (n + 1) / 2) {
-        const int half = (n + 1) / 2;   // warps half .. n - 1 are added to 0 ..
-#pragma unroll 1
-        for (int s0 = 0; s0 < n - half; s0 += 2) {
-            const int to = warp < half ? warp - s0 : warp - half - s0;
-            const bool in = warp < n && to >= 0 && to < 2 && to + s0 < n - half;
-            float4* p = reinterpret_cast<float4*>(buf + (in ? to : 0) * ATTN_DECODE_PART);
-            if (in && warp >= half) st.store(p);
-            __syncthreads();
-            if (in && warp < half) st.add(p);
-            __syncthreads();
-        }
-    }
-}
 
 // A quad of a partial result with its two rows' maxima and sums.
 struct Quad {
     float4 v, h;
 };
-// Quad k of the NB * quads of this lane over `count` partial results, in order; `at(i)`: the i-th of them.
+__device__ __forceinline__ Quad no_quad() { return Quad{make_float4(0.f, 0.f, 0.f, 0.f), make_float4(-INFINITY, 0.f, -INFINITY, 0.f)}; }
+// q and quad k of the NB * quads of this lane of `count` partial results added up, in order; `at(i)`: the i-th of them.
 template <int NB, class At>
-__device__ __forceinline__ Quad add_up(int k, int quads, int count, At&& at) {
+__device__ __forceinline__ Quad add_up(Quad q, int k, int quads, int count, At&& at) {
     const int lane = threadIdx.x & 31, b = k / quads;
-    Quad q;
-    q.v = make_float4(0.f, 0.f, 0.f, 0.f);
-    q.h = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
     constexpr int N = 4;   // (so many at once: their loads and exponentials do not wait for one another)
 #pragma unroll 1
     for (int i0 = 0; i0 < count; i0 += N) {
@@ -183,8 +139,8 @@ __device__ __forceinline__ Quad add_up(int k, int quads, int count, At&& at) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float4* p = at(min(i0 + i, count - 1));
-            h[i] = p[b * 32 + lane];
-            v[i] = p[(NB + k) * 32 + lane];
+            h[i] = p[b * 4 + (lane & 3)];
+            v[i] = p[NB * 4 + k * 32 + lane];
         }
         float u0 = q.h.x, u1 = q.h.z;
 #pragma unroll
@@ -492,29 +448,43 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
             __syncwarp();
         }
 
-        // ---- the block's result of this segment: each warp's, or (where the rings are in use) their sum, and from there by all threads ----
+        // ---- the block's result of this segment: the warps' added up, as many at a time as there is room for (all of them where the rings are idle),
+        // a quad of it to a warp ----
         st.close();
         const bool last = walk.u >= walk.end;
-        const uint8_t* dumps = smem + (last ? S_RING : S_MERGE);
-        int parts = last ? min(WARPS, sg.count) : 1;   // (warps that have had a slice)
-        if (!last) merge_warps<D, NB>(st, smem + S_MERGE, warp);
-        if (warp < parts) st.store(reinterpret_cast<float4*>(smem + (last ? S_RING : S_MERGE) + warp * (STAGES * STAGE)));
+        constexpr int QUADS = D / 16, ALL = NB * QUADS, PARTIAL = NB * 64 + ALL * 512, N = (ALL + WARPS - 1) / WARPS;
+        constexpr int SHARE = WARPS / ALL > 0 ? WARPS / ALL : 1, ROOM = MERGE_BYTES / PARTIAL < WARPS ? MERGE_BYTES / PARTIAL : WARPS;
+        static_assert(PARTIAL <= (int)ATTN_DECODE_PART && PARTIAL <= STAGES * STAGE && SHARE * PARTIAL <= MERGE_BYTES, "partial results");
         unsigned* const bad = reinterpret_cast<unsigned*>(smem + S_FLAG) + 4;   // rows that are not finite, or see nothing
         volatile int* const flag = reinterpret_cast<volatile int*>(smem + S_FLAG);
         if (tid == 0) *bad = 0u;
-        __syncthreads();
-        constexpr int QUADS = D / 16, ALL = NB * QUADS, SHARE = WARPS / ALL > 0 ? WARPS / ALL : 1;   // warps to a quad of the joined parts
-        int stride = STAGES * STAGE;
+        const int with = min(WARPS, sg.count), room = last ? WARPS : ROOM, stride = last ? STAGES * STAGE : PARTIAL;   // (warps that have had a slice)
+        uint8_t* const dumps = smem + (last ? S_RING : S_MERGE);
+        Quad x[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = no_quad();
+#pragma unroll 1
+        for (int w0 = 0; w0 < with; w0 += room) {
+            if (w0) __syncthreads();
+            if (warp >= w0 && warp < min(w0 + room, with)) st.store(reinterpret_cast<float4*>(dumps + (warp - w0) * stride));
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (warp + i * WARPS < ALL)
+                    x[i] = add_up<NB>(x[i], warp + i * WARPS, QUADS, min(room, with - w0), [&](int y) { return reinterpret_cast<const float4*>(dumps + y * stride); });
+        }
         bool whole = sg.count == sg.total;
         if (!whole) {   // one of several blocks: the last to arrive adds the parts up, in the blocks' order
             float4* const slots = reinterpret_cast<float4*>(a.parts);
             const int b0 = (int)(sg.unit0 / w.chunk), b1 = (int)((sg.unit0 + sg.total - 1) / w.chunk);
             float4* const slot = slots + (int64_t)(2 * blockIdx.x + (sg.first == 0 ? 1 : 0)) * (ATTN_DECODE_PART / 16);
-            for (int k = warp; k < ALL; k += WARPS) {
-                const Quad x = add_up<NB>(k, QUADS, parts, [&](int i) { return reinterpret_cast<const float4*>(dumps + i * stride); });
-                slot[(NB + k) * 32 + lane] = x.v;
-                if (k % QUADS == 0) slot[k / QUADS * 32 + lane] = x.h;
-            }
+            auto put = [&](float4* d, int k, const Quad& y) {
+                d[NB * 4 + k * 32 + lane] = y.v;
+                if (k % QUADS == 0 && lane < 4) d[k / QUADS * 4 + lane] = y.h;
+            };
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (warp + i * WARPS < ALL) put(slot, warp + i * WARPS, x[i]);
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -527,33 +497,27 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
             if (whole) {
                 __threadfence();
                 const int n = b1 - b0 + 1, per = (n + SHARE - 1) / SHARE;
-                float4* const mid = reinterpret_cast<float4*>(smem + S_MERGE);
+                uint8_t* const mid = smem + S_MERGE;
 #pragma unroll 1
-                for (int x = warp; x < ALL * SHARE; x += WARPS) {
-                    const int k = x % ALL, lo = x / ALL * per;
-                    const Quad y = add_up<NB>(k, QUADS, min(per, n - lo), [&](int i) {
-                        const int b = b0 + lo + i;
-                        return const_cast<const float4*>(slots) + (int64_t)(2 * b + (b == b0 ? 1 : 0)) * (ATTN_DECODE_PART / 16);
-                    });
-                    float4* const d = mid + x / ALL * ((NB + ALL) * 32);
-                    d[(NB + k) * 32 + lane] = y.v;
-                    if (k % QUADS == 0) d[k / QUADS * 32 + lane] = y.h;
+                for (int y = warp; y < ALL * SHARE; y += WARPS) {
+                    const int k = y % ALL, lo = y / ALL * per;
+                    put(reinterpret_cast<float4*>(mid + y / ALL * PARTIAL), k, add_up<NB>(no_quad(), k, QUADS, min(per, n - lo), [&](int i) {
+                            const int b = b0 + lo + i;
+                            return const_cast<const float4*>(slots) + (int64_t)(2 * b + (b == b0 ? 1 : 0)) * (ATTN_DECODE_PART / 16);
+                        }));
                 }
                 __syncthreads();
-                dumps = smem + S_MERGE;
-                parts = SHARE;
-                stride = (NB + ALL) * 512;
+#pragma unroll
+                for (int i = 0; i < N; ++i)
+                    if (warp + i * WARPS < ALL)
+                        x[i] = add_up<NB>(no_quad(), warp + i * WARPS, QUADS, SHARE, [&](int y) { return reinterpret_cast<const float4*>(mid + y * PARTIAL); });
             }
         }
-        static_assert(SHARE * (NB + ALL) * 512 <= 2 * (int)ATTN_DECODE_PART && (NB + ALL) * 512 <= (int)ATTN_DECODE_PART, "partial results");
         if (whole) {
-            constexpr int N = (ALL + WARPS - 1) / WARPS;
-            Quad x[N];
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int k = warp + i * WARPS;
                 if (k < ALL) {
-                    x[i] = add_up<NB>(k, QUADS, parts, [&](int y) { return reinterpret_cast<const float4*>(dumps + y * stride); });
                     float4& v = x[i].v;
                     const float f0 = 1.f / x[i].h.y, f1 = 1.f / x[i].h.w;
                     v = make_float4(v.x * f0, v.y * f1, v.z * f0, v.w * f1);
