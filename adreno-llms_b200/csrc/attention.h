@@ -69,7 +69,9 @@ cudaError_t attention_configure();
 cudaError_t launch_attention(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl, int* kernels);   // *kernels: launches
 bool attention_countable(const AttnArgs& a, int max_new);   // whether the call's tiles of work surely stay below 2^30
 constexpr int ATTN_MAX_BLOCKS = 256;
-constexpr int ATTN_DECODE_EXTRA = 8, ATTN_CHUNK_EXTRA = 3;   // what an item costs besides its key tiles, in units of them
+// What an item costs besides its key tiles, in units of them (tiles of 8 KB, and of 128 keys).  With / without, us: 4096 tokens of 32 heads to 8 of 64 dims,
+// fp16 125 / 162; a token each of 64 sequences of up to 500 positions 30.6 / 34.9, of 64 of 8192 with 8 heads of 128 dims, e4m3, 146 / 150.
+constexpr int ATTN_DECODE_EXTRA = 8, ATTN_CHUNK_EXTRA = 3;
 constexpr size_t ATTN_DECODE_PART = 18 * 512, ATTN_CHUNK_PART = 256 * 128 * 4 + 256 * 8;   // two per block
 // The workspace: counters, items, parts.
 constexpr size_t ATTN_COUNTER_BYTES = ATTN_MAX_BLOCKS * sizeof(unsigned), ATTN_HEAD_BYTES = ATTN_COUNTER_BYTES + ATTN_MAX_BLOCKS * sizeof(int4);

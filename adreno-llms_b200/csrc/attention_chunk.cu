@@ -8,15 +8,17 @@
 // fetched once for all heads that share it.  With no more than 128 rows the two tiles hold the same rows and take the key tiles in turn.
 // A block is one of each SM:
 //   * warps 0-7 and 8-15: the softmax of one query tile each, two threads per row, 64 keys each (one thread per row left two warps to a
-//     scheduler, which were idle half of the time on each other's latencies: 3500 clocks for a pair of tiles of 64 dims, ... here): scores come
-//     from tensor memory, the weights go back there as fp16 in the scores' place (the A operand of the second product).  The sums of outputs stay
-//     in tensor memory and are scaled again only when a row's maximum has grown by more than 2^8.
+//     scheduler, which were idle half of the time on each other's latencies: 3500 clocks for a pair of tiles of 64 dims, 2650 here): scores come
+//     from tensor memory and stay in registers, the weights go back there as fp16 in the scores' place (the A operand of the second product).  The
+//     sums of outputs stay in tensor memory and are scaled again only when a row's maximum has grown by more than 2^8.
 //   * warp 16: issues all tcgen05.mma: scores = Q K^T (both K-major), out += weights V (V as it lies in the cache, MN-major).  While one
 //     query tile is in its softmax the other one has the tensor cores.
 //   * warp 17: tensor copies (fp16: straight into the operands; 8-bit: codes into a ring of parts of tiles).
 //   * warps 18 and 19 (cells of 128 dims: 20-23), 8-bit cells only: codes to fp16 operands, and the keys' factors.
-// The exponentials bound it next to the products: 128 x 128 scores take 1024 clocks of the SM's exponential units and D * 8 clocks of
-// its tensor cores for both products.
+// What bounds it: two tiles of 128 x 128 scores take 2048 clocks of the SM's exponential units and 16 D of its tensor cores.  2048 tokens of
+// 32 heads to 8, to 16384 positions: fp16 of 64 dims 354 us (700 TFLOP/s; the exponentials alone 270), of 128 dims 440 us (1170 TFLOP/s).
+// 8-bit cells (64 dims 440 to 460, 128 dims 610 to 640 us) are bound by what expands them: codes go through shared memory twice, and the factors of
+// 128 keys are read from there by every row.  (Without the conversion's arithmetic 128 dims took 606 us of 682.)
 #include <type_traits>
 
 #include "attention_maps.h"
@@ -705,6 +707,13 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             if (n > 1) copy(1, pages[1], false);
             for (int j = 0; j < n; ++j) {
                 const int next = page_of(j + 3);
+                // Cells of 128 dims leave room for four parts in flight, too few for the memory's latency: what comes next waits in the L2 (32 x 24 tokens to
+                // 8192 positions, 16 heads to 4: e4m3 180 -> 145 us, int8 186 -> 177).  With 64 dims there are twelve (93 -> 103 us with this).
+                if (C::CODES && D == 128 && next >= 0) {
+                    const int64_t row = cells(j + 3, next);
+                    bulk_prefetch_l2((const uint8_t*)a.c.k + row * D, box_keys * D);
+                    bulk_prefetch_l2((const uint8_t*)a.c.v + row * D, box_keys * D);
+                }
                 copy(j, pages[0], true);
                 if (j + 2 < n) copy(j + 2, pages[2], false);
                 pages[0] = pages[1];

@@ -111,6 +111,11 @@ __device__ __forceinline__ void bulk_g2s(uint32_t dst, const void* src, uint32_t
         : "memory");
 }
 
+// 16-byte aligned, a multiple of 16 bytes
+__device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
+
 // ---- tiled 2-D tensor copy global -> shared (TMA unit, 128-byte swizzle set in the map) ----
 // x = coordinate in the innermost dimension (elements; must cover a multiple of 16 bytes),
 // y = row.  The whole box is written (out-of-range parts as zeros) and counted on the mbarrier.
