@@ -180,7 +180,7 @@ int nn_linear_argmax(nn_context* ctx, int N, int K, nn_buf x, nn_buf W, nn_buf l
  *   [num_pages][kv_heads][page_size][head_dim] cells of 2 bytes (NN_KV_FP16) or 1, and with 8 bits two of fp16 scales
  *   [num_pages][kv_heads][page_size].  A cell row stands for code * scale.  The caller allocates them (16-byte
  *   aligned) and keeps them; the handle only describes them.  page_size 16, 32, 64, 128 or 256; head_dim 64 or 128.
- *   Pages need no initial contents.  Codes are those that nn_kv_write leaves (no e4m3 NaNs).
+ *   The buffers must not overlap.  Pages need no initial contents.  Codes are those that nn_kv_write leaves (no e4m3 NaNs).
  *
  *   A batch describes the sequences of a call in device memory that the call reads when it runs, so that a recorded
  *   step takes new lengths at every replay:

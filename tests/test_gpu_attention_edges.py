@@ -282,3 +282,45 @@ def test_a_cache_of_another_context(nnb, ctx):
     for b in bufs[0][1:]:
         ctx.free(b)
     c.close()
+
+
+@pytest.mark.parametrize("fmt,D", [("fp16", 64), ("int8", 128)])
+def test_recorded_calls_of_both_kinds_take_new_batches(nnb, ctx, fmt, D):
+    """A chunk, tokens and a read back in one recording, replayed while row starts and lengths change between replays (sequences without rows
+    too): the bits of separate calls, whose counters and partial results they share."""
+    lengths, hq, hk, rows, spare = [900, 333, 64, 2000], 8, 2, 220, 0x7E7E
+    c = ref.Cache(nnb, ctx, fmt, lengths, hk, D, 32, seed=33)
+    q = np.random.default_rng(34).standard_normal((rows, hq, D)).astype(np.float16)
+    qb, outs, reads = ctx.upload(q), [ctx.alloc(q.nbytes) for _ in range(2)], [ctx.alloc(rows * hk * D * 2) for _ in range(2)]
+    start, lens = ctx.alloc(4 * 5), ctx.alloc(4 * 4)
+    batches = [nnb.KVBatch(4, rows, m, c.table.shape[1] * 32, c.table.shape[1], start, lens, ctx.upload(c.table)) for m in (200, 1)]
+
+    def call():
+        for b, out in zip(batches, outs):
+            ctx.attention(c.handle, b, hq, qb, 0, out, 0, D ** -0.5)
+        ctx.kv_read(c.handle, batches[0], reads[0], 0, reads[1], 0)
+
+    def results():
+        return [ctx.download(b, (rows, w, D), np.uint16) for b, w in (*((o, hq) for o in outs), *((r, hk) for r in reads))]
+
+    ctx.plan_begin()
+    call()
+    plan = ctx.plan_end()
+    for new, now in (([200, 1, 0, 5], [900, 333, 64, 2000]), ([1, 1, 1, 1], [1, 200, 64, 1999]), ([0, 0, 0, 0], [5, 5, 5, 5]), ([0, 220, 0, 0], [9, 333, 0, 7]), ([3, 64, 64, 64], [700, 64, 64, 2000])):
+        ctx.upload(np.concatenate([[0], np.cumsum(new)]).astype(np.int32), start)
+        ctx.upload(np.asarray(now, np.int32), lens)
+        got = []
+        for replay in (False, True):
+            for b, w in (*((o, hq) for o in outs), *((r, hk) for r in reads)):
+                ctx.upload(np.full((rows, w, D), spare, np.uint16), b)
+            ctx.plan_launch(plan) if replay else call()
+            got.append(results())
+        for a, b in zip(*got):
+            assert np.array_equal(a, b)
+        total = sum(new)
+        for out in got[0][:2]:
+            assert (out[total:] == spare).all()
+            check_attention(c, out.view(np.float16), q, list(zip(new, now)), D ** -0.5, 0, 0, f"replay {new}")
+    c.close()
+    for b in (qb, *outs, *reads, start, lens):
+        ctx.free(b)
