@@ -756,12 +756,21 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     const uint8_t* src = smem + C::O_RAW + st * C::RAW_STAGE;
                     const unsigned here = *reinterpret_cast<volatile unsigned*>(smem + C::O_HERE + tile % C::HERE * 4);
                     const bool fix = value && (k0 + BN - 1 > p1 || (k0 < lo0 && k0 + BN > w.sinks) || here != 0xFFu);
+                    float ks = 0.f, vs = 0.f;
+                    if (!value) {
+                        ks = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW)[lane]);
+                        vs = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW + 2 * C::RAW_KEYS)[lane]);
+                    }
                     auto pieces = [&](auto fixed) {
 #pragma unroll
                         for (int b = 0; b < PIECES; b += 4) {
                             uint4 q[4];
 #pragma unroll
                             for (int y = 0; y < 4; ++y) q[y] = reinterpret_cast<const uint4*>(src)[lane + (b + y) * 32];
+                            if (b + 4 == PIECES) {   // all of the part has been read: the next one may come
+                                __syncwarp();
+                                if (lane == 0) mbar_arrive(bar(C::B_REMPTY + st));
+                            }
 #pragma unroll
                             for (int y = 0; y < 4; ++y) {
                                 // values that no row sees must not be NaN: their weights are 0
@@ -781,7 +790,6 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     if (fix) pieces(std::true_type());
                     else pieces(std::false_type());
                     if (!value) {
-                        const float ks = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW)[lane]), vs = half_float(reinterpret_cast<const uint16_t*>(src + C::RAW + 2 * C::RAW_KEYS)[lane]);
                         const int key = part * C::RAW_KEYS + lane;
                         // (the scales of keys that no row sees may be anything)
                         const bool seen = k0 + key <= p1 && (k0 + key >= lo0 || k0 + key < w.sinks) && (here >> (key >> 4) & 1u);
@@ -791,8 +799,6 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                         meta[BN] = b;
                         meta[2 * BN] = ex2(-b);
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(C::B_REMPTY + st));
                 }
                 raw += BN / C::RAW_KEYS;
                 fence_async_smem();
