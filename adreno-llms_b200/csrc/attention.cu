@@ -39,10 +39,10 @@ cudaError_t attention_configure() {
 //   rows   cells            1 x 2048        8 x 4096        32 x 8192 positions
 //   16     fp16 of 64      10.6 / 14.0     14.5 / 21.6     45.5 / 66.6
 //   16     fp16 of 128     16.4 / 16.1     23.2 / 26.3     88.4 / 82.8
-//   16     e4m3 of 128     17.3 / 19.5     26.4 / 35.0     97.4 / 145
+//   16     e4m3 of 128     17.3 / 19.5     26.4 / 35.0     97.4 / 132
 //   20     fp16 of 64      11.3 / 14.1     21.9 / 21.6     73.5 / 66.6
 //   20     int8 of 64      14.2 / 16.2     24.8 / 27.1     86.8 / 91.3
-//   20     e4m3 of 128     18.1 / 19.8     42.2 / 34.9      167 / 145
+//   20     e4m3 of 128     18.1 / 19.8     42.2 / 34.9      167 / 132
 //   64     fp16 of 64      12.2 / 14.0     30.3 / 22.4      133 / 67
 //   64     int8 of 64      14.9 / 16.7     34.6 / 27.8      159 / 92
 static bool few_rows(const AttnArgs& a, int max_new) {

@@ -17,8 +17,8 @@
 //   * warps 18 and 19 (cells of 128 dims: 20-23), 8-bit cells only: codes to fp16 operands, and the keys' factors.
 // What bounds it: two tiles of 128 x 128 scores take 2048 clocks of the SM's exponential units and 16 D of its tensor cores.  2048 tokens of
 // 32 heads to 8, to 16384 positions: fp16 of 64 dims 354 us (700 TFLOP/s; the exponentials alone 270), of 128 dims 440 us (1170 TFLOP/s).
-// 8-bit cells (64 dims 440 to 460, 128 dims 610 to 640 us) are bound by what expands them: codes go through shared memory twice, and the factors of
-// 128 keys are read from there by every row.  (Without the conversion's arithmetic 128 dims took 606 us of 682.)
+// 8-bit cells (64 dims 437 to 447, 128 dims 595 to 598 us) are bound by what expands them: codes go through shared memory twice, and the factors of
+// 128 keys are read from there by every row.
 #include <type_traits>
 
 #include "attention_maps.h"
@@ -767,7 +767,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                             uint4 q[4];
 #pragma unroll
                             for (int y = 0; y < 4; ++y) q[y] = reinterpret_cast<const uint4*>(src)[lane + (b + y) * 32];
-                            if (b + 4 == PIECES) {   // all of the part has been read: the next one may come
+                            if (b + 4 == PIECES) {   // all of the part has been read: the next one may come (given back at the end: int8, 128 dims, 641 us instead of 598)
                                 __syncwarp();
                                 if (lane == 0) mbar_arrive(bar(C::B_REMPTY + st));
                             }

@@ -240,7 +240,8 @@ cudaError_t launch(void (*kernel)(const Args), const Args& a, int grid, cudaStre
 
 // A row in four warps is ready sooner, a row in one has more loads in flight and fewer blocks to start.  Four warps / one, us, in a recorded chain of calls:
 // writes of 32 + 2 x 8 heads of 128 dims, fp16: 1 row 2.5 / 4.3, 1200 rows 5.1 / 7.9, 2400 rows 8.4 / 8.1, 8192 rows 35.4 / 34.0; of 9 + 2 x 3 heads of 64:
-// 1 row 1.9 / 2.1, 256 rows 2.4 / 2.3, 2400 rows 4.8 / 3.3.  Reads of 8 heads of 128 dims, int8: 1 row 1.8 / 2.9, 2400 rows 4.6 / 7.1, 65536 rows of 16 heads, e4m3,
+// 1 row 1.9 / 2.1, 256 rows 2.4 / 2.3, 2400 rows 4.8 / 3.3.  Reads of 3 heads of 64 dims, int8: 1200 rows 2.5 / 2.8, 2400 rows
+// 4.1 / 2.8; of 8 heads of 128 dims: 1 row 1.8 / 2.9, 2400 rows 4.6 / 7.1, 65536 rows of 16 heads, e4m3,
 // 135 / 143; but of 8 heads of 64, e4m3, 70 / 50, of 4 heads of 128, fp16, 71 / 43.
 constexpr int FEW_ROWS = 592;   // (four blocks for each SM)
 
@@ -253,7 +254,7 @@ cudaError_t write_rows(const KvWriteArgs& a, cudaStream_t st, bool pdl) {
 template <int FMT, int D>
 cudaError_t read_rows(const KvReadArgs& a, cudaStream_t st, bool pdl) {
     const bool wide = FMT != KV_FP16 && 2 * a.c.kv_heads * (D / 16) >= WARPS * 32;
-    if (a.s.num_rows <= FEW_ROWS || wide) return launch(kv_read_kernel<FMT, D, true>, a, a.s.num_rows, st, pdl);
+    if (a.s.num_rows <= 2 * FEW_ROWS || wide) return launch(kv_read_kernel<FMT, D, true>, a, a.s.num_rows, st, pdl);
     return launch(kv_read_kernel<FMT, D, false>, a, (a.s.num_rows - 1) / WARPS + 1, st, pdl);
 }
 
