@@ -292,6 +292,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
         int more = 0;
         __syncwarp();
         if (lane == 0) more = steps.walk.next(a.s, w, to);
+        __syncwarp();   // (the other lanes read the segment next: a shuffle orders registers alone)
         return __shfl_sync(0xffffffffu, more, 0) != 0;
     };
     auto next_segment = [&]() { return next_into(&steps.sg); };
@@ -689,6 +690,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                         *a.status = 32;
                     }
                     if (given_up()) return;
+                    __syncwarp();   // (what lane 0 has noted is read behind any of these barriers)
                     if (leads) mbar_arrive_expect_tx(full, (uint32_t)(__popc(here >> lane & ((1u << per) - 1u)) * box_keys * (D + (value ? 0 : 4))));
                     __syncwarp();
                     if (in) {
