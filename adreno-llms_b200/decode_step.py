@@ -31,7 +31,8 @@ class Attention:
 
     def __init__(self, ctx, shape, M, lengths, cache="int8", page=64, max_len=0, head_dim=64, window=0, sinks=0, rope_base=10000.0, seed=7, host=None):
         self.ctx, self.D, self.cache, self.window, self.sinks = ctx, head_dim, cache, window, sinks
-        self.q_heads, self.kv_heads = shape.q_dim // head_dim, shape.kv_dim // head_dim
+        self.q_heads, self.kv_heads, self.M = shape.q_dim // head_dim, shape.kv_dim // head_dim, M
+        self._one_per_row(lengths)
         self.max_len = max_len or max(lengths) + 16
         per_seq = -(-self.max_len // page)
         rng = np.random.default_rng(seed)
@@ -62,8 +63,13 @@ class Attention:
                     host[f"cache.{layer}"] = rows
         self.set_lengths(lengths)
 
+    def _one_per_row(self, lengths):
+        if len(lengths) != self.M:
+            raise ValueError(f"{len(lengths)} lengths for {self.M} sequences")
+
     def set_lengths(self, lengths):
         """Positions that the sequences have before the next step's token."""
+        self._one_per_row(lengths)
         self.lengths = np.asarray(lengths, np.int32).copy()
         self.ctx.upload(self.lengths + 1, self.kv_len)
 
