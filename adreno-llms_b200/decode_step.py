@@ -46,7 +46,8 @@ class Attention:
         self.caches, self.buffers = [], []
         cells = M * per_seq * page * self.kv_heads
         starts = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
-        fill = KVBatch(M, int(starts[-1]), max(1, max(lengths)), self.max_len, per_seq, ctx.upload(starts), ctx.upload(np.asarray(lengths, np.int32)), self.table_dev)
+        filled = [ctx.upload(starts), ctx.upload(np.asarray(lengths, np.int32))]
+        fill = KVBatch(M, int(starts[-1]), max(1, max(lengths)), self.max_len, per_seq, *filled, self.table_dev)
         for layer in range(shape.layers):
             bufs = [ctx.alloc(cells * head_dim * (2 if cache == "fp16" else 1)) for _ in range(2)]
             bufs += [None, None] if cache == "fp16" else [ctx.alloc(cells * 2) for _ in range(2)]
@@ -61,6 +62,8 @@ class Attention:
                     ctx.free(b)
                 if host is not None:
                     host[f"cache.{layer}"] = rows
+        for b in filled:
+            ctx.free(b)
         self.set_lengths(lengths)
 
     def _one_per_row(self, lengths):
@@ -82,8 +85,13 @@ class Attention:
         c.attention(self.caches[layer], self.batch, self.q_heads, q, 0, self.out, 0, self.D ** -0.5, self.window, self.sinks)
 
     def close(self):
+        """Gives the caches and all buffers back; a recording of the step must not be launched any more."""
         for cache in self.caches:
             cache.close()
+        mine = [self.cos, self.sin, self.row_start, self.kv_len, self.table_dev, self.out] if self.out else []
+        for b in (*mine, *(b for bufs in self.buffers for b in bufs if b)):
+            self.ctx.free(b)
+        self.out, self.caches, self.buffers = None, [], []
 
 
 class DecodeStep:

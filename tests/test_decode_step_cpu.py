@@ -57,3 +57,18 @@ def test_one_length_for_each_row(nnb, lengths):
     at.set_lengths([5, 0])
     at.advance()
     assert list(at.lengths) == [6, 1]
+
+
+@pytest.mark.parametrize("cache,lengths", [("fp16", [3, 40]), ("int8", [0, 0]), ("fp8", [17, 0])])
+def test_a_closed_attention_gives_its_buffers_back(nnb, cache, lengths):
+    synth, dstep = _modules()
+    c = Account()
+    mine = c.alloc(64)
+    at = dstep.Attention(c, synth.ModelShape("tiny", 128, 3, 128, 64, 256, 64), 2, lengths, cache=cache)
+    assert c.caches == 3
+    per_layer = 2 if cache == "fp16" else 4
+    assert len(c.size) == 1 + 3 * per_layer + 6     # cells and scales; cos, sin, row starts, lengths, pages, output: not what filled the cache
+    at.close()
+    assert list(c.size) == [mine] and c.caches == 0
+    at.close()                                      # (once more: nothing left to do)
+    assert list(c.size) == [mine] and c.caches == 0
