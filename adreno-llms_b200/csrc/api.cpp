@@ -160,12 +160,12 @@ extern "C" int nn_init(int device, nn_context** out) {
         delete c;
         return NN_FAIL(NN_ERR_CUDA, "nn_init: cudaStreamCreate failed");
     }
-    if (cudaHostAlloc((void**)&c->status_host, sizeof(int), cudaHostAllocMapped) != cudaSuccess ||
+    if (cudaHostAlloc((void**)&c->status_host, STATUS_WORDS * sizeof(int), cudaHostAllocMapped) != cudaSuccess ||
         cudaHostGetDevicePointer((void**)&c->status_dev, c->status_host, 0) != cudaSuccess) {
         delete c;
         return NN_FAIL(NN_ERR_CUDA, "nn_init: status word allocation failed");
     }
-    *c->status_host = 0;
+    for (int i = 0; i < STATUS_WORDS; ++i) c->status_host[i] = 0;
     // [0] nn_argmax's reduction word, [3] its block counter; [1] and [2] the fused arg-max's
     if (cudaMalloc((void**)&c->argmax_slot, 32) != cudaSuccess || cudaMemset(c->argmax_slot, 0, 32) != cudaSuccess) {
         delete c;
@@ -235,16 +235,16 @@ extern "C" int nn_sync(nn_context* c) {
     if (!c) return NN_FAIL(NN_ERR_ARG, "nn_sync: null context");
     CUDA_TRY(cudaStreamSynchronize(c->stream));
     c->in_flight.ordered();
-    if (*c->status_host != 0) {
-        const int s = *c->status_host;
-        *c->status_host = 0;
-        if (s == STATUS_BAD_TABLE)
-            return NN_FAIL(NN_ERR_ARG, "a page number, length or position of a key/value batch was out of range; the rows and keys it concerned were left out");
+    const int s = c->status_host[0], bad_table = c->status_host[STATUS_BAD_TABLE];
+    c->status_host[0] = c->status_host[STATUS_BAD_TABLE] = 0;
+    if (s != 0) {
         cudaMemsetAsync(c->argmax_slot, 0, 32, c->stream);  // a cut-short launch may have left its words set
         cudaMemsetAsync(c->sk_flags, 0, SK_MAX_BLOCKS * sizeof(unsigned), c->stream);
         if (c->attn_work) cudaMemsetAsync(c->attn_work, 0, ATTN_COUNTER_BYTES, c->stream);
-        return NN_FAIL(NN_ERR_TIMEOUT, "a device-side bounded wait ran out (status %d); results of the last calls are invalid", s);
+        return NN_FAIL(NN_ERR_TIMEOUT, "a device-side bounded wait ran out (status %d); results of the last calls are invalid%s", s,
+                       bad_table ? " (and a page number, length or position of a key/value batch was out of range)" : "");
     }
+    if (bad_table) return NN_FAIL(NN_ERR_ARG, "a page number, length or position of a key/value batch was out of range; the rows and keys it concerned were left out");
     return NN_OK;
 }
 

@@ -77,8 +77,8 @@ constexpr size_t ATTN_DECODE_PART = 18 * 512, ATTN_CHUNK_PART = 256 * 128 * 4 + 
 constexpr size_t ATTN_COUNTER_BYTES = ATTN_MAX_BLOCKS * sizeof(unsigned), ATTN_HEAD_BYTES = ATTN_COUNTER_BYTES + ATTN_MAX_BLOCKS * sizeof(int4);
 inline size_t attention_workspace_bytes(int sm_count) { return ATTN_HEAD_BYTES + 2 * (size_t)(sm_count < ATTN_MAX_BLOCKS ? sm_count : ATTN_MAX_BLOCKS) * ATTN_CHUNK_PART; }
 
-// What a kernel of these leaves in the context's status word when the tables or lengths that it was given are out of range
-// (nn_sync reports it as an argument error; other non-zero values are waits that ran out).
-constexpr int STATUS_BAD_TABLE = 1 << 20;
+// Which of the context's status words says that the tables or lengths that a kernel of these was given are out of range (nn_sync reports an argument
+// error).  Word 0 is for waits that ran out, of any kernel: neither hides the other.
+constexpr int STATUS_BAD_TABLE = 1, STATUS_WORDS = 2;
 
 }  // namespace nnb

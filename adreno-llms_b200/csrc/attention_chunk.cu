@@ -553,7 +553,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 for (unsigned left = __ballot_sync(0xffffffffu, marked) & (warp & 1 ? 0xAAAAAAAAu : 0x55555555u); left; left &= left - 1) {
                     const int from = __ffs(left) - 1;
                     const int r2 = __shfl_sync(0xffffffffu, row, from), h2 = __shfl_sync(0xffffffffu, head, from), p2 = __shfl_sync(0xffffffffu, pos, from);
-                    if (!attend_row<FMT, D>(a, sg.seq, sg.len, p2, r2, h2) && lane == 0) *a.status = STATUS_BAD_TABLE;
+                    if (!attend_row<FMT, D>(a, sg.seq, sg.len, p2, r2, h2) && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
                 }
             }
         }
@@ -644,7 +644,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 return m;
             };
             auto copy = [&](int j, int page, bool value) {
-                if (page == -2) *a.status = STATUS_BAD_TABLE;
+                if (page == -2) a.status[STATUS_BAD_TABLE] = 1;
                 const bool in = page >= 0;
                 const unsigned here = __ballot_sync(0xffffffffu, in);
                 const int64_t row = in ? cells(j, page) : 0;
@@ -894,7 +894,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Attn
     for (unsigned left = again; left; left &= left - 1, ++k) {
         const int from = __ffs(left) - 1;
         const int r2 = __shfl_sync(0xffffffffu, row, from), h2 = __shfl_sync(0xffffffffu, head, from), p2 = __shfl_sync(0xffffffffu, pos, from);
-        if (k % (JOIN_THREADS / 32) == warp && !attend_row<FMT, D>(a, it.x, q.len, p2, r2, h2) && lane == 0) *a.status = STATUS_BAD_TABLE;
+        if (k % (JOIN_THREADS / 32) == warp && !attend_row<FMT, D>(a, it.x, q.len, p2, r2, h2) && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
     }
 }
 

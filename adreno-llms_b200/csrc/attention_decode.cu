@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
             if (slice < pcount && key <= plast && (key + box > plo || key < w.sinks)) {
                 const int page = ptable[key >> shift];
                 page_reg = page_ok(page, a.c.num_pages) ? page : -1;
-                if (page_reg < 0) *a.status = STATUS_BAD_TABLE;
+                if (page_reg < 0) a.status[STATUS_BAD_TABLE] = 1;
             }
         }
         const int page = __shfl_sync(0xffffffffu, page_reg, (j - page_base + lane) & 31);
@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
             for (unsigned left = again; left; left &= left - 1) {
                 const int r = __ffs(left) - 1, row = row_of(r);
                 if (row < 0 || turn++ % WARPS != warp) continue;
-                if (!attend_row<FMT, D>(a, sg.seq, sg.len, pos_of(r), row, head_of(r)) && lane == 0) *a.status = STATUS_BAD_TABLE;
+                if (!attend_row<FMT, D>(a, sg.seq, sg.len, pos_of(r), row, head_of(r)) && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
             }
         }
         if (!last) __syncthreads();   // (the buffers are free again)

@@ -148,7 +148,7 @@ __device__ __forceinline__ Walk find_work(const KvSeqs& s, WorkShape* w, unsigne
         bool bad = false, descends = false;
         q = SeqWork{0, 0, 0, 0};
         if (i0 + lane < s.num_seqs) q = load_seq(s, *w, i0 + lane, &bad, &descends);
-        if (bad) *status = STATUS_BAD_TABLE;
+        if (bad) status[STATUS_BAD_TABLE] = 1;
         disorder |= descends;
     };
     unsigned tiles = 0;

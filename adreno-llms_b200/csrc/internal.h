@@ -43,7 +43,7 @@ struct nn_context {
     size_t l2_bytes = 0, hbm_bytes = 0, smem_limit = 0;
     cudaStream_t stream = nullptr;
     std::map<uintptr_t, QuantEntry> registry;  // keyed by weight device pointer
-    int* status_host = nullptr;                // mapped pinned word written by kernels
+    int* status_host = nullptr;                // mapped pinned words written by kernels: [0] a wait that ran out, [1] a bad page or length
     int* status_dev = nullptr;
     unsigned long long* argmax_slot = nullptr;
     void* stage_img = nullptr;      // staged activations of a batched call, written once per launch (stage_image.cu)

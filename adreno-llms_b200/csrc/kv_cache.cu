@@ -76,12 +76,12 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
     const RowPlace at = place_of_row(a.s, r);
     if (at.none) return;
     if (at.bad || (a.rotary && at.pos >= a.table_len)) {
-        if (lane == 0) *a.status = STATUS_BAD_TABLE;
+        if (lane == 0) a.status[STATUS_BAD_TABLE] = 1;
         return;
     }
     const int page = a.s.page_table[(int64_t)at.seq * a.s.table_stride + (at.pos >> a.c.page_shift)], slot = at.pos & ((1 << a.c.page_shift) - 1);
     const bool cell = page_ok(page, a.c.num_pages);
-    if (!cell && lane == 0) *a.status = STATUS_BAD_TABLE;
+    if (!cell && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
     const int j = lane % LANES;
     int pa, pb;
     piece_pair(j, a.rotary, pa, pb);
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_read_kernel(const KvReadArgs a)
     int page = -1;
     if (!at.bad) page = a.s.page_table[(int64_t)at.seq * a.s.table_stride + (at.pos >> a.c.page_shift)];
     const bool cell = page_ok(page, a.c.num_pages);
-    if (!cell && lane == 0) *a.status = STATUS_BAD_TABLE;
+    if (!cell && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
     const int slot = at.pos & ((1 << a.c.page_shift) - 1), all = 2 * a.c.kv_heads * LANES;
     for (int i0 = SPREAD ? threadIdx.x : lane; i0 < all; i0 += STEP * AHEAD) {
         uint4 raw[AHEAD];

@@ -60,7 +60,7 @@ const char* nn_version(void);
 int nn_init(int device_ordinal, nn_context** out_ctx);
 int nn_shutdown(nn_context* ctx); /* frees registry entries and library-owned buffers */
 void* nn_stream(nn_context* ctx); /* the cudaStream_t every call is ordered on */
-int nn_sync(nn_context* ctx);     /* host wait; also reports a recorded device-side timeout */
+int nn_sync(nn_context* ctx);     /* host wait; also reports a recorded device-side timeout, or a bad page or length of a key/value batch */
 int nn_device_info(nn_context* ctx, int* sm_count, size_t* l2_bytes, size_t* hbm_bytes);
 
 /* ---- buffers: clCreateBuffer / clEnqueueWriteBuffer / clEnqueueReadBuffer /
@@ -193,7 +193,7 @@ int nn_linear_argmax(nn_context* ctx, int N, int K, nn_buf x, nn_buf W, nn_buf l
  *                 common prefix); what two rows write to one cell is either of them, or of both.
  *   and bounds for the host: num_rows rows in every operand; max_new, the most new rows of a sequence (it picks the kernel: a
  *   longer one is served all the same); max_len, beyond which no sequence is (at most table_stride * page_size, and 2^30).
- *   A page number, length or position that is out of range makes the next nn_sync return NN_ERR_ARG, and nothing out of bounds is
+ *   A page number, length or position that is out of range makes the next nn_sync return NN_ERR_ARG (NN_ERR_TIMEOUT where a wait has run out too), and nothing out of bounds is
  *   touched: the cells that it concerns are not written, are zeros for nn_kv_read and hidden for nn_attention (whose rows of a sequence
  *   with a bad length, and of all sequences where row_start does not ascend, hold no result).  (nn_attention accepts positions below 0.)
  *   Operands are fp16 rows of [heads][head_dim], 16-byte aligned; strides count values from row to row (a multiple of 8;
