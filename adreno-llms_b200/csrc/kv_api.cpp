@@ -32,16 +32,18 @@ static size_t cache_bytes(const KvView& v) {
     } while (0)
 
 // The partial results of items that several blocks share: one buffer for all calls of the context, which run one after the other.
-static int attention_workspace(nn_context* c) {
+// Made with the context's first cache, or by its first nn_attention on the cache of another context; the context's device is current.
+static int attention_workspace(nn_context* c, const char* who) {
     if (c->attn_work) return NN_OK;
-    if (c->capturing) return NN_FAIL(NN_ERR_UNSUPPORTED, "nn_kv_cache_create: the context's first cache cannot be made while a plan is being recorded");
+    if (c->capturing)
+        return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: the attention's workspace cannot be made while a plan is being recorded (the context's first cache, or its first nn_attention, makes it)", who);
     CUDA_TRY(attention_configure());
     void* work = nullptr;
     CUDA_TRY(cudaMalloc(&work, attention_workspace_bytes(c->sm_count)));
     const cudaError_t e = cudaMemsetAsync(work, 0, ATTN_HEAD_BYTES, c->stream);
     if (e != cudaSuccess) {
         cudaFree(work);
-        return NN_FAIL(NN_ERR_CUDA, "nn_kv_cache_create: %s", cudaGetErrorString(e));
+        return NN_FAIL(NN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
     }
     c->attn_work = work;
     return NN_OK;
@@ -110,7 +112,7 @@ extern "C" int nn_kv_cache_create(nn_context* c, int format, int num_pages, int 
     AttnMaps maps = {};
     if (c) {
         CUDA_TRY(cudaSetDevice(c->device));
-        const int rc = attention_workspace(c);
+        const int rc = attention_workspace(c, "nn_kv_cache_create");
         if (rc) return rc;
         if (!encode_attention_maps(w, &maps)) return NN_FAIL(NN_ERR_CUDA, "nn_kv_cache_create: no tensor maps for these pages (k=%p v=%p)", k, v);
     }
@@ -167,10 +169,6 @@ static int take_batch(nn_context* c, const nn_kv_cache* h, const nn_kv_batch* b,
 // Last of the checks (the others need no GPU).  The calling thread may have another device current.
 static int make_current(nn_context* c, const nn_kv_cache* h, const char* who) {
     if (!c) return NN_FAIL(NN_ERR_ARG, "%s: null context", who);
-    if (!c->attn_work) {   // a context that has made no cache of its own
-        const int rc = attention_workspace(c);
-        if (rc) return rc;
-    }
     if (h->device != c->device) return NN_FAIL(NN_ERR_ARG, "%s: the cache was made for device %d, the context is of device %d", who, h->device, c->device);
     int now = -1;
     if (cudaGetDevice(&now) != cudaSuccess || now != c->device) {
@@ -301,7 +299,7 @@ extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b,
     a.sinks = window ? sinks : 0;   // (without a window all keys up to the row's own are visible)
     if (!attention_countable(a, b->max_new))
         return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: num_seqs=%d num_rows=%d max_len=%d: more than 2^30 tiles of work", who, b->num_seqs, b->num_rows, b->max_len);
-    if ((rc = make_current(c, h, who))) return rc;
+    if ((rc = make_current(c, h, who)) || (rc = attention_workspace(c, who))) return rc;
     a.status = c->status_dev;
     ProfScope prof(c, [&] { return std::string("attention_") + kv_name(a.c.fmt) + "_seqs" + std::to_string(b->num_seqs) + "_rows" + std::to_string(b->num_rows); });
     a.counters = (unsigned*)c->attn_work;
