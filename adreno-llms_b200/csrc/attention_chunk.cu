@@ -215,7 +215,7 @@ __device__ __forceinline__ bool join_parts(const AttnArgs& a, const Segment& sg,
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             const float y[4] = {o[x].x * inv, o[x].y * inv, o[x].z * inv, o[x].w * inv};
-            fine = fine && fabsf(y[0]) < INFINITY && fabsf(y[1]) < INFINITY && fabsf(y[2]) < INFINITY && fabsf(y[3]) < INFINITY;
+            fine = fine && fabsf(y[0]) < HALF_END && fabsf(y[1]) < HALF_END && fabsf(y[2]) < HALF_END && fabsf(y[3]) < HALF_END;
             h[2 * x] = floats_half2(y[0], y[1]);
             h[2 * x + 1] = floats_half2(y[2], y[3]);
         }
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
                         v[x] *= scale_out;
-                        fine = fine && fabsf(v[x]) < INFINITY;
+                        fine = fine && fabsf(v[x]) < HALF_END;
                     }
                     if (on) {
 #pragma unroll
@@ -875,7 +875,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Attn
         o[x].y *= inv;
         o[x].z *= inv;
         o[x].w *= inv;
-        fine = fine && fabsf(o[x].x) < INFINITY && fabsf(o[x].y) < INFINITY && fabsf(o[x].z) < INFINITY && fabsf(o[x].w) < INFINITY;
+        fine = fine && fabsf(o[x].x) < HALF_END && fabsf(o[x].y) < HALF_END && fabsf(o[x].z) < HALF_END && fabsf(o[x].w) < HALF_END;
     }
     __shared__ unsigned bad[JOIN_THREADS / 32];
     const unsigned mine = __ballot_sync(0xffffffffu, on && !fine);

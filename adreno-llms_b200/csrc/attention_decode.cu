@@ -525,8 +525,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
                     float4& v = x[i].v;
                     const float f0 = 1.f / x[i].h.y, f1 = 1.f / x[i].h.w;
                     v = make_float4(v.x * f0, v.y * f1, v.z * f0, v.w * f1);
-                    const bool fine0 = x[i].h.y > 0.f && x[i].h.y < INFINITY && fabsf(v.x) < INFINITY && fabsf(v.z) < INFINITY;
-                    const bool fine1 = x[i].h.w > 0.f && x[i].h.w < INFINITY && fabsf(v.y) < INFINITY && fabsf(v.w) < INFINITY;
+                    const bool fine0 = x[i].h.y > 0.f && x[i].h.y < INFINITY && fabsf(v.x) < HALF_END && fabsf(v.z) < HALF_END;
+                    const bool fine1 = x[i].h.w > 0.f && x[i].h.w < INFINITY && fabsf(v.y) < HALF_END && fabsf(v.w) < HALF_END;
                     const int r = k / QUADS * 8 + 2 * c;
                     if (!fine0 || !fine1) atomicOr(bad, (fine0 ? 0u : 1u << r) | (fine1 ? 0u : 2u << r));
                 }

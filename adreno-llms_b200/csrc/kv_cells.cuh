@@ -26,6 +26,9 @@ __device__ __forceinline__ void codes_to_half2x2(uint32_t w, uint32_t& h01, uint
 }
 __device__ __forceinline__ float2 half2_floats(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 __device__ __forceinline__ float half_float(uint16_t h) { return __half2float(__ushort_as_half(h)); }
+// From here on a value is an infinity as fp16.  (The attention's weights are rounded for their product with the values and not in their sum, so that a
+// result may pass the largest value by 2^-11 of it: such a row is computed once more, with weights of 32 bits.)
+constexpr float HALF_END = 65520.f;
 __device__ __forceinline__ uint32_t floats_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
