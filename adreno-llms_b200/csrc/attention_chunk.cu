@@ -1,8 +1,9 @@
 // Attention of many query rows to a cache head (chunks of new tokens, prompts, drafts): two products on the tensor cores per tile of keys.
 //
-//   t_k = scale log2(e) q.k,  w_k = 2^(t_k - m),  out = sum w_k v_k / sum w_k       m: a running reference at most 8 below the maximum of t
+//   t_k = scale log2(e) q.k,  w_k = 2^(t_k - m),  out = sum w_k v_k / sum w_k       m: a running reference, 7 to 15 below the maximum of t
 //
-// (8-bit cells: the scales join the scores and weights as in attention_decode.cu: codes are exact in fp16, no rounding is added.)
+// (8-bit cells: the scales join the scores and weights as in attention_decode.cu: codes are exact in fp16, no rounding is added.  Weights up to 2^15 for
+// the reason given there.)
 //
 // An item is up to 256 query rows: two tiles of 128, each new tokens times the query heads of a cache head, so that a cell is
 // fetched once for all heads that share it.  With no more than 128 rows the two tiles hold the same rows and take the key tiles in turn.
@@ -388,10 +389,10 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 float top = fmaxf(t0, t1);
                 if (!C::CODES) top *= scale2;
                 // Both threads of a row keep the same reference: they agree whether some row of their two warps wants another one.
-                if (pair_any(pair_bar, first || top > m + 8.f)) {
+                if (pair_any(pair_bar, first || top - m > 15.f)) {
                     *own = top;
                     pair_sync(pair_bar);
-                    const float up = fmaxf(m, fmaxf(top, *other)), f = m == -INFINITY ? 0.f : ex2(m - up);
+                    const float up = fmaxf(m, fmaxf(top, *other) - 7.f), f = m == -INFINITY ? 0.f : ex2(m - up);
                     m = up;
                     if (!first) {   // (the scores came after the product before, so the sums are complete)
                         l *= f;

@@ -1,10 +1,14 @@
 // Attention of few new tokens: up to 8 or 16 query rows (new tokens times query heads to a cache head) read a cache head together.
 //
-//   t_k = scale log2(e) q.k,  w_k = 2^(t_k - m),  out = sum w_k v_k / sum w_k          m: the running maximum of t
+//   t_k = scale log2(e) q.k,  w_k = 2^(t_k - m),  out = sum w_k v_k / sum w_k          m: 15 below the running maximum of t
 //
 // An 8-bit cell is code * scale.  The products take the codes as they are (exact in fp16), a key's scale joins its score, and a value's
 // scale its weight: t'_k = t_k + log2(scale_v), w'_k = 2^(t'_k - m'), out = sum w'_k code_k / sum w'_k / scale_v, so that the weights
-// that are rounded to fp16 for the second product are at most 1 and no rounding is added.
+// that are rounded to fp16 for the second product are at most 2^15 and no rounding is added.
+//
+// The largest weight is 2^15 and not 1 because fp16 holds less than 11 bits of what is below 2^-14 and nothing of what is below 2^-25.  A value row of zeros has the scale 1 and
+// may so have the largest w' without a part in the result: beside it nothing was left of rows of values around 0.01 (scale 2^-13) whose weights are 2^12 times smaller.
+// (Scores from 2^27 on are 16 apart, and so may m be from their maximum: a weight of 2^16 is infinite, and such a row is computed once more.)
 //
 // Bound by the bytes of the cache: every cell is read once, for all rows, and a cell does 4 rows flops per byte.  So: twelve warps per block and
 // one block per SM, each warp with a ring of its own of 8 KB stages that tensor copies fill (16 to 64 keys with their values),
@@ -398,6 +402,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) top[b][i] = fmaxf(top[b][i], __shfl_xor_sync(0xffffffffu, top[b][i], d));
+                    top[b][i] -= 15.f;   // (rounded once, before it is compared and kept: otherwise the same maximum may seem to grow)
                     grows |= top[b][i] > st.m[b][i];
                 }
             if (__any_sync(0xffffffffu, grows)) {
