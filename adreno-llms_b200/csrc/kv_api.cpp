@@ -68,11 +68,16 @@ static bool rows_overlap(const Rows& a, const Rows& b, int rows) {
 }
 static bool share(const void* p, size_t np, const void* q, size_t nq) { return p && q && (const char*)p < (const char*)q + nq && (const char*)q < (const char*)p + np; }
 static size_t scale_bytes(const KvView& v) { return cache_bytes(v) / ((size_t)v.dim * kv_cell_bytes(v.fmt)) * 2; }
-static bool rows_over_cache(const Rows& r, int rows, const KvView& v) {
-    const size_t n = rows_bytes(r, rows), nc = cache_bytes(v), ns = scale_bytes(v);
-    return share(r.p, n, v.k, nc) || share(r.p, n, v.v, nc) || share(r.p, n, v.k_scale, ns) || share(r.p, n, v.v_scale, ns);
+static bool over_cache(const void* p, size_t n, const KvView& v) {
+    const size_t nc = cache_bytes(v), ns = scale_bytes(v);
+    return share(p, n, v.k, nc) || share(p, n, v.v, nc) || share(p, n, v.k_scale, ns) || share(p, n, v.v_scale, ns);
 }
+static bool rows_over_cache(const Rows& r, int rows, const KvView& v) { return over_cache(r.p, rows_bytes(r, rows), v); }
 // (what a call writes must not be what tells it where to)
+static bool cache_over_batch(const KvView& v, const nn_kv_batch* b) {
+    return over_cache(b->row_start, 4 * ((size_t)b->num_seqs + 1), v) || over_cache(b->kv_len, 4 * (size_t)b->num_seqs, v) ||
+           over_cache(b->page_table, 4 * (size_t)b->num_seqs * b->table_stride, v);
+}
 static bool rows_over_batch(const Rows& r, const nn_kv_batch* b) {
     const size_t n = rows_bytes(r, b->num_rows);
     return share(r.p, n, b->row_start, 4 * ((size_t)b->num_seqs + 1)) || share(r.p, n, b->kv_len, 4 * (size_t)b->num_seqs) ||
@@ -200,12 +205,14 @@ static int kv_write(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf 
             return NN_FAIL(NN_ERR_ARG, "%s: q_out overlaps k, v, the cache or the batch", who);
     }
     if (rows_over_cache(rk, b->num_rows, a.c) || rows_over_cache(rv, b->num_rows, a.c)) return NN_FAIL(NN_ERR_ARG, "%s: k or v lies in the cache", who);
+    if (cache_over_batch(a.c, b)) return NN_FAIL(NN_ERR_ARG, "%s: the cache overlaps the batch's row_start, kv_len or page_table", who);
     if (rotary_dim) {
         if (rotary_dim < 0 || rotary_dim > D || rotary_dim % 16 != 0) return NN_FAIL(NN_ERR_ARG, "%s: rotary_dim=%d: a multiple of 16, at most %d", who, rotary_dim, D);
         if (!cos_f32 || !sin_f32 || !aligned(cos_f32, 16) || !aligned(sin_f32, 16)) return NN_FAIL(NN_ERR_ARG, "%s: cos and sin must be there and 16-byte aligned", who);
         if (table_len <= 0) return NN_FAIL(NN_ERR_ARG, "%s: table_len=%d", who, table_len);
         const size_t n = rows_bytes(ro, b->num_rows), table = (size_t)table_len * (rotary_dim / 2) * 4;
         if (q && (share(ro.p, n, cos_f32, table) || share(ro.p, n, sin_f32, table))) return NN_FAIL(NN_ERR_ARG, "%s: q_out overlaps cos or sin", who);
+        if (over_cache(cos_f32, table, a.c) || over_cache(sin_f32, table, a.c)) return NN_FAIL(NN_ERR_ARG, "%s: the cache overlaps cos or sin", who);
     }
     a.q = rq.p;
     a.q_out = const_cast<uint16_t*>(ro.p);
