@@ -9,17 +9,19 @@
 // fetched once for all heads that share it.  With no more than 128 rows the two tiles hold the same rows and take the key tiles in turn.
 // A block is one of each SM:
 //   * warps 0-7 and 8-15: the softmax of one query tile each, two threads per row, 64 keys each (one thread per row left two warps to a
-//     scheduler, which were idle half of the time on each other's latencies: 3500 clocks for a pair of tiles of 64 dims, 2650 here): scores come
+//     scheduler, which were idle half of the time on each other's latencies: 3500 clocks for a pair of tiles of 64 dims, 2800 here): scores come
 //     from tensor memory and stay in registers, the weights go back there as fp16 in the scores' place (the A operand of the second product).  The
 //     sums of outputs stay in tensor memory and are scaled again only when a row's maximum has grown by more than 2^8.
 //   * warp 16: issues all tcgen05.mma: scores = Q K^T (both K-major), out += weights V (V as it lies in the cache, MN-major).  While one
 //     query tile is in its softmax the other one has the tensor cores.
 //   * warp 17: tensor copies (fp16: straight into the operands; 8-bit: codes into a ring of parts of tiles).
 //   * warps 18 and 19 (cells of 128 dims: 20-23), 8-bit cells only: codes to fp16 operands, and the keys' factors.
-// What bounds it: two tiles of 128 x 128 scores take 2048 clocks of the SM's exponential units and 16 D of its tensor cores.  2048 tokens of
-// 32 heads to 8, to 16384 positions: fp16 of 64 dims 354 us (700 TFLOP/s; the exponentials alone 270), of 128 dims 440 us (1170 TFLOP/s).
-// 8-bit cells (64 dims 437 to 447, 128 dims 595 to 598 us) are bound by what expands them: codes go through shared memory twice, and the factors of
-// 128 keys are read from there by every row.
+// What bounds it: two tiles of 128 x 128 scores take 2048 clocks of the SM's exponential units and 16 D of its tensor cores; they take 2800 (fp16 of 64
+// dims), 3240 (of 128) and with codes 3900 and 4700 to 4800, since a query tile's products wait for its softmax and the softmax for its scores.  2048 tokens of
+// 32 heads to 8, to 16384 positions: fp16 of 64 dims 352 us (730 TFLOP/s; the exponentials alone some 235), of 128 dims 447 us (1150 TFLOP/s).
+// 8-bit cells (64 dims 442 to 447, 128 dims 607 to 610 us) are bound by what expands them: codes go through shared memory twice, and the factors of
+// 128 keys are read from there by every row.  An item costs 7500 clocks besides its keys (128 dims: 15500), of which 2400 (5400) are waits for its last products: the
+// warps that store its result begin the next softmax.
 #include <type_traits>
 
 #include "attention_maps.h"
