@@ -52,7 +52,7 @@ struct nn_context {
     size_t norm_scratch_bytes = 0;
     float* sk_scratch = nullptr;   // partial sums of blocks that share a tile (balanced K-streaming)
     unsigned* sk_flags = nullptr;
-    void* attn_work = nullptr;     // the attention's counters and partial results (made with the first cache)
+    void* attn_work = nullptr;     // the attention's counters and partial results (made with the first cache or the first attention)
     void* flush_buf = nullptr;
     size_t flush_bytes = 0;
     bool use_pdl = true;

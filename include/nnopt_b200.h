@@ -213,7 +213,9 @@ int nn_linear_argmax(nn_context* ctx, int N, int K, nn_buf x, nn_buf W, nn_buf l
  *                     k <= p and, with window > 0, k > p - window or k < sinks (the first tokens stay visible).  Query head h reads
  *                     head h / (q_heads / kv_heads) of the cache.  A row that sees nothing (a position below 0) gives zeros.
  *                     What hidden cells hold, NaN and infinities included, has no influence.  out must not overlap q.
- *                     scale finite and positive. ------------------------------------------------------------------ */
+ *                     scale finite and positive.  Scores, maxima and sums are 32 bits; the softmax's weights are rounded to fp16 for their product with
+ *                     the values (rows that see an infinity or a NaN: not), 11 bits of each, or 2^-32 of the row's largest.
+ *                     One kernel serves all sequences of a call, by max_new: a chunk and single tokens are mostly faster as two calls. ------------------------------------------------------------------ */
 enum { NN_KV_FP16 = 0, NN_KV_INT8 = 1, NN_KV_FP8 = 2 /* e4m3 */ };
 typedef struct nn_kv_batch {
     int num_seqs, num_rows, max_new, max_len, table_stride;
