@@ -115,6 +115,11 @@ def load():
         "nn_rope_kv_write": ([vp, vp, pkb, vp, vp, i, i, i, vp, i64, vp, i64, vp, i64, vp, i64], i),
         "nn_kv_read": ([vp, vp, pkb, vp, i64, vp, i64], i),
         "nn_attention": ([vp, vp, pkb, i, vp, i64, vp, i64, ctypes.c_float, i, i], i),
+        "nn_tree_layout": ([vp, pkb, vp, i, vp, vp], i),
+        "nn_rope_kv_write_at": ([vp, vp, pkb, vp, vp, vp, i, i, i, vp, i64, vp, i64, vp, i64, vp, i64], i),
+        "nn_attention_tree": ([vp, vp, pkb, i, vp, i64, vp, i64, ctypes.c_float, i, vp], i),
+        "nn_kv_move": ([vp, pvp, i, pkb, vp], i), "nn_kv_reorder": ([vp, pvp, i, pkb, i, vp], i),
+        "nn_beam_select": ([vp, i, i, i, vp, i64, vp, vp, i, i, vp, vp, vp, vp], i),
     }
     for name, (args, res) in sig.items():
         if hasattr(L, name):
@@ -129,6 +134,10 @@ def _check(rc):
     if rc != 0:
         raise NNError(rc, load().nn_last_error().decode())
     return rc
+
+
+def _handles(caches):
+    return (ctypes.c_void_p * max(1, len(caches)))(*(c.h for c in caches))
 
 
 class Context:
@@ -275,6 +284,26 @@ class Context:
 
     def attention(self, cache, batch, q_heads, q, q_stride, out, out_stride, scale, window=0, sinks=0):
         _check(self.L.nn_attention(self.h, cache.h, batch, q_heads, q, q_stride, out, out_stride, scale, window, sinks))
+
+    # -- several continuations of a sequence: drafted trees and beams --
+    def tree_layout(self, batch, parent, mask_words, mask, position):
+        _check(self.L.nn_tree_layout(self.h, batch, parent, mask_words, mask, position))
+
+    def rope_kv_write_at(self, cache, batch, position, cos, sin, table_len, rotary_dim, q_heads, q, q_stride, q_out, q_out_stride, k, k_stride, v, v_stride):
+        _check(self.L.nn_rope_kv_write_at(self.h, cache.h, batch, position, cos, sin, table_len, rotary_dim, q_heads, q, q_stride, q_out, q_out_stride,
+                                          k, k_stride, v, v_stride))
+
+    def attention_tree(self, cache, batch, q_heads, q, q_stride, out, out_stride, scale, mask_words, mask):
+        _check(self.L.nn_attention_tree(self.h, cache.h, batch, q_heads, q, q_stride, out, out_stride, scale, mask_words, mask))
+
+    def kv_move(self, caches, batch, source):
+        _check(self.L.nn_kv_move(self.h, _handles(caches), len(caches), batch, source))
+
+    def kv_reorder(self, caches, batch, beams, parent):
+        _check(self.L.nn_kv_reorder(self.h, _handles(caches), len(caches), batch, beams, parent))
+
+    def beam_select(self, groups, beams, vocab, logits, logits_stride, score, done, eos, picks, out_score, out_token, out_parent, out_done):
+        _check(self.L.nn_beam_select(self.h, groups, beams, vocab, logits, logits_stride, score, done, eos, picks, out_score, out_token, out_parent, out_done))
 
     def l2_flush(self):
         _check(self.L.nn_l2_flush(self.h))

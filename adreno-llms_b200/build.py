@@ -9,12 +9,13 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libnnopt_b200.so")
-SOURCES = ["api.cpp", "weights.cpp", "comm.cpp", "comm_kernels.cu", "gemv_stream.cu", "gemv_batch.cu", "stage_image.cu", "decode_plan.cu", "plan.cpp", "gemv_generic.cu", "misc.cu", "gemm_tc.cu", "noalloc.cu", "kv_api.cpp", "kv_cache.cu", "attention.cu", "attention_decode.cu", "attention_chunk.cu"]
+SOURCES = ["api.cpp", "weights.cpp", "comm.cpp", "comm_kernels.cu", "gemv_stream.cu", "gemv_batch.cu", "stage_image.cu", "decode_plan.cu", "plan.cpp", "gemv_generic.cu", "misc.cu", "gemm_tc.cu", "noalloc.cu", "kv_api.cpp", "branch_api.cpp", "kv_cache.cu", "kv_branch.cu", "beam.cu", "attention.cu", "attention_decode.cu", "attention_chunk.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -38,8 +39,7 @@ def build(force=False, verbose=False):
     if not force and not _stale():
         return LIB
     os.makedirs(LIB_DIR, exist_ok=True)
-    objs = []
-    for src in sources():
+    def compiled(src):
         obj = os.path.join(LIB_DIR, os.path.basename(src) + ".o")
         cmd = [_nvcc(), *ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC,-Wall", "-x", "cu", "-c", src, "-o", obj]
         if verbose:
@@ -47,14 +47,16 @@ def build(force=False, verbose=False):
         if not force and os.path.exists(obj) and all(
                 os.path.getmtime(obj) > os.path.getmtime(os.path.join(CSRC, f)) for f in os.listdir(CSRC)
                 if f.endswith((".h", ".cuh")) or os.path.join(CSRC, f) == src):
-            objs.append(obj)
-            continue
+            return obj
         r = subprocess.run(cmd, capture_output=True, text=True)
         if verbose or r.returncode:
             sys.stderr.write(r.stdout + r.stderr)
         if r.returncode:
             raise RuntimeError(f"nvcc failed on {src}")
-        objs.append(obj)
+        return obj
+
+    with ThreadPoolExecutor(os.cpu_count()) as pool:
+        objs = list(pool.map(compiled, sources()))
     cmd = [_nvcc(), *ARCH, "-shared", "-o", LIB, *objs, "-cudart", "static", "-ldl", "-lpthread"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:

@@ -32,6 +32,7 @@ struct KvWriteArgs {
     const uint16_t* v;
     const float* cos;        // [table_len][rotary / 2]
     const float* sin;
+    const int* position;     // [num_rows], of the rotation; null: that of the row's cell
     int table_len, rotary;   // rotary 0: no rotation
     int q_heads;
     int64_t q_stride, qo_stride, k_stride, v_stride;   // values from row to row
@@ -58,6 +59,8 @@ struct AttnArgs {
     int64_t q_stride, o_stride;
     float scale;
     int window, sinks;       // window 0: none
+    const uint32_t* tree;    // masks of the new tokens, [row][tree_words]; null: each sees all up to itself
+    int tree_words;
     int* status;
     unsigned* counters;      // blocks of a shared item that have arrived (0 between launches)
     int4* items;             // shared items, by the block that begins them

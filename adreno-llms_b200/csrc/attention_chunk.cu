@@ -232,7 +232,7 @@ __device__ __forceinline__ bool join_parts(const AttnArgs& a, const Segment& sg,
     return on && !fine;
 }
 
-template <int FMT, int D>
+template <int FMT, int D, bool TREE>
 __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_kernel(const __grid_constant__ AttnMaps maps, const AttnArgs a) {
     using C = Chunk<FMT, D>;
     constexpr int RAWS = C::CODES ? C::RAWS : 1;
@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     w.tile = BN;
     w.window = a.window;
     w.sinks = a.sinks;
+    w.tree_words = TREE ? a.tree_words : 0;
     w.extra = ATTN_CHUNK_EXTRA;
     Steps& steps = reinterpret_cast<Steps*>(smem + C::O_WALK)[warp];
     Segment& sg = steps.sg;
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
             const bool on = r < rows.per * w.group && t <= rows.last(i) && hg < a.group;
             const int row = sg.row0 + t, head = kv_head * a.group + hg, pos = on ? sg.len - sg.n + t : -1, lo = window_begin(pos < 0 ? 0 : pos, w.window);
             // positions of the tile's first and last token
-            const int pmin = sg.len - sg.n + rows.first(i), pmax = sg.len - sg.n + rows.last(i), lo_max = window_begin(pmax < 0 ? 0 : pmax, w.window);
+            const int pmin = TREE ? sg.p0(w) : sg.len - sg.n + rows.first(i), pmax = sg.len - sg.n + rows.last(i), lo_max = window_begin(pmax < 0 ? 0 : pmax, w.window);
             float m = -INFINITY, l = 0.f;
             bool first = true;
             for (int j = rows.turns ? i : 0; j < sg.count; j += rows.turns ? 2 : 1) {
@@ -375,7 +376,9 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                     }
                     if (edge) {
                         const int at = k0 + c * 64 + cb * 32;
-                        uint32_t seen = low_bits(pos + 1 - at) & (~low_bits(lo - at) | low_bits(w.sinks - at));
+                        uint32_t seen;
+                        if (TREE) seen = on ? tree_bits(a.tree + (int64_t)row * a.tree_words, a.tree_words, at, sg.len - sg.n, sg.len) : 0u;
+                        else seen = low_bits(pos + 1 - at) & (~low_bits(lo - at) | low_bits(w.sinks - at));
                         const unsigned there = here >> (4 * c + 2 * cb);
                         seen &= ((there & 1u) ? 0xFFFFu : 0u) | ((there & 2u) ? 0xFFFF0000u : 0u);
 #pragma unroll
@@ -550,13 +553,13 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
                 if (sg.count != sg.total && !(*joined & (sg.first ? 1 : 2))) continue;
                 const ItemRows rows(sg, w);
                 const int kv_head = sg.vhead / parts, x = warp >> 1, rr = (x & 3) * 32 + lane, g = rr % w.group, t = rows.first(x >> 2) + rr / w.group;
-                const int hg = (sg.vhead % parts) * w.group + g, row = sg.row0 + t, head = kv_head * a.group + hg, pos = sg.len - sg.n + t;
+                const int hg = (sg.vhead % parts) * w.group + g, row = sg.row0 + t, head = kv_head * a.group + hg, pos = sg.len - sg.n + (TREE ? 0 : t);
                 const bool on = !(rows.turns && x >= 4) && rr < rows.per * w.group && t <= rows.last(x >> 2) && hg < a.group;
                 const bool marked = on && (*reinterpret_cast<const volatile uint16_t*>(a.out + (int64_t)row * a.o_stride + (int64_t)head * D) & 0x7FFF) > 0x7C00;
                 for (unsigned left = __ballot_sync(0xffffffffu, marked) & (warp & 1 ? 0xAAAAAAAAu : 0x55555555u); left; left &= left - 1) {
                     const int from = __ffs(left) - 1;
                     const int r2 = __shfl_sync(0xffffffffu, row, from), h2 = __shfl_sync(0xffffffffu, head, from), p2 = __shfl_sync(0xffffffffu, pos, from);
-                    if (!attend_row<FMT, D>(a, sg.seq, sg.len, p2, r2, h2) && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
+                    if (!attend_row<FMT, D, TREE>(a, sg.seq, sg.len, p2, r2, h2) && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
                 }
             }
         }
@@ -830,7 +833,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
 
 // Joins the parts of items that blocks share: block (b, y) the rows 32 y .. of the item that block b of the kernel above began and did not finish.
 constexpr int JOIN_THREADS = 256;
-template <int FMT, int D>
+template <int FMT, int D, bool TREE>
 __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const AttnArgs a) {
     pdl_wait_prior_grid();
     const int b0 = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -840,12 +843,13 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Attn
     const int parts = (a.group + 127) / 128;
     w.group = (a.group + parts - 1) / parts;
     w.tokens = 2 * (128 / w.group);
+    w.tree_words = TREE ? a.tree_words : 0;
     const SeqWork q = load_seq(a.s, w, it.x);
     const int t0 = it.z * w.tokens, t1 = min(t0 + w.tokens, q.n) - 1, per = w.tokens / 2, r = blockIdx.y * 32 + lane, i = r >> 7;
     const int t = t0 + i * per + (r & 127) / w.group, hg = (it.y % parts) * w.group + (r & 127) % w.group;
     const bool on = (r & 127) < per * w.group && t <= min(t1, t0 + (i + 1) * per - 1) && hg < a.group;
     if (!__syncthreads_or(on)) return;
-    const int row = q.row0 + t, head = it.y / parts * a.group + hg, pos = q.len - q.n + t;
+    const int row = q.row0 + t, head = it.y / parts * a.group + hg, pos = q.len - q.n + (TREE ? 0 : t);
     const float4* base = reinterpret_cast<const float4*>(a.parts);
     auto part = [&](int b) { return base + (int64_t)(2 * b + (b == b0 ? 1 : 0)) * (ATTN_CHUNK_PART / 16); };
     float m = -INFINITY;
@@ -897,12 +901,12 @@ __global__ void __launch_bounds__(JOIN_THREADS) attention_join_kernel(const Attn
     for (unsigned left = again; left; left &= left - 1, ++k) {
         const int from = __ffs(left) - 1;
         const int r2 = __shfl_sync(0xffffffffu, row, from), h2 = __shfl_sync(0xffffffffu, head, from), p2 = __shfl_sync(0xffffffffu, pos, from);
-        if (k % (JOIN_THREADS / 32) == warp && !attend_row<FMT, D>(a, it.x, q.len, p2, r2, h2) && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
+        if (k % (JOIN_THREADS / 32) == warp && !attend_row<FMT, D, TREE>(a, it.x, q.len, p2, r2, h2) && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
     }
 }
 
-template <int FMT, int D>
-cudaError_t launch(const AttnArgs& a, const AttnMaps& maps, int blocks, cudaStream_t st, bool pdl, int* kernels) {
+template <int FMT, int D, bool TREE>
+cudaError_t launch_one(const AttnArgs& a, const AttnMaps& maps, int blocks, cudaStream_t st, bool pdl, int* kernels) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(Chunk<FMT, D>::THREADS);
@@ -913,18 +917,23 @@ cudaError_t launch(const AttnArgs& a, const AttnMaps& maps, int blocks, cudaStre
     attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, attention_chunk_kernel<FMT, D>, maps, a);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, attention_chunk_kernel<FMT, D, TREE>, maps, a);
     *kernels = a.join_here ? 1 : 2;
     if (e != cudaSuccess || a.join_here) return e;
     cfg.gridDim = dim3((unsigned)blocks, 8);
     cfg.blockDim = dim3(JOIN_THREADS);
     cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, attention_join_kernel<FMT, D>, a);
+    return cudaLaunchKernelEx(&cfg, attention_join_kernel<FMT, D, TREE>, a);
+}
+template <int FMT, int D>
+cudaError_t launch(const AttnArgs& a, const AttnMaps& maps, int blocks, cudaStream_t st, bool pdl, int* kernels) {
+    return a.tree ? launch_one<FMT, D, true>(a, maps, blocks, st, pdl, kernels) : launch_one<FMT, D, false>(a, maps, blocks, st, pdl, kernels);
 }
 
 template <int FMT, int D>
 cudaError_t configure() {
-    return cudaFuncSetAttribute(attention_chunk_kernel<FMT, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Chunk<FMT, D>::SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(attention_chunk_kernel<FMT, D, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, Chunk<FMT, D>::SMEM);
+    return e != cudaSuccess ? e : cudaFuncSetAttribute(attention_chunk_kernel<FMT, D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, Chunk<FMT, D>::SMEM);
 }
 
 }  // namespace

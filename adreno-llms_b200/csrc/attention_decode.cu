@@ -175,7 +175,7 @@ __device__ __forceinline__ Quad add_up(Quad q, int k, int quads, int count, At&&
     return q;
 }
 
-template <int FMT, int D, int NB>
+template <int FMT, int D, int NB, bool TREE>
 __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __grid_constant__ AttnMaps maps, const AttnArgs a) {
     using S = Shape<FMT, D>;
     constexpr bool CODES = FMT != KV_FP16;
@@ -196,6 +196,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
     w.tile = S::KT;
     w.window = a.window;
     w.sinks = a.sinks;
+    w.tree_words = TREE ? a.tree_words : 0;
     w.extra = ATTN_DECODE_EXTRA;
     Walk walk = find_work(a.s, &w, WARPS, a.status);
     if (walk.u >= walk.end) return;
@@ -298,12 +299,12 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
         };
         auto head_of = [&](int r) { return sg.vhead * w.group + r - token_of(r) * w.group; };
         auto pos_of = [&](int r) { return sg.len - sg.n + sg.qt * w.tokens + token_of(r); };
-        int pos[NB][2];   // of this lane's rows of scores
+        int pos[NB][2];   // of this lane's rows of scores (TREE: the rows of the operands, -1: none)
         uint32_t q[NB][S::DG][2];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) pos[b][h] = row_of(8 * b + 2 * c + h) >= 0 ? pos_of(8 * b + 2 * c + h) : -1;
+            for (int h = 0; h < 2; ++h) pos[b][h] = TREE ? row_of(8 * b + 2 * c + h) : row_of(8 * b + 2 * c + h) >= 0 ? pos_of(8 * b + 2 * c + h) : -1;
             const int row = row_of(8 * b + quad);
             const uint32_t* src = reinterpret_cast<const uint32_t*>(a.q + (int64_t)max(row, 0) * a.q_stride + (int64_t)head_of(8 * b + quad) * D);
 #pragma unroll
@@ -340,6 +341,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
                         asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_at<FMT, D>(vb, r, i % (S::ROW / 16))), "r"(0) : "memory");
                 }
                 __syncwarp();
+            }
+            uint32_t tree[NB][2][(S::KT + 31) / 32];   // the stage's keys that this lane's rows see
+            if (TREE && edge) {
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int x = 0; x < (S::KT + 31) / 32; ++x)
+                            tree[b][i][x] = pos[b][i] < 0 ? 0u : tree_bits(a.tree + (int64_t)pos[b][i] * a.tree_words, a.tree_words, k0 + 32 * x, sg.len - sg.n, sg.len);
             }
             // ---- scores: rows are keys quad and quad + 8 of 16, columns the queries ----
             float s[NB][S::KG][4];
@@ -395,7 +406,8 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
                         for (int i = 0; i < 2; ++i) {
                             float& y = s[b][t][2 * h + i];
                             y = CODES ? fmaf(y, fa, fb) : y * fa;
-                            if (edge && !(key_visible(k0 + x, pos[b][i], w.window, w.sinks) && (here >> (x >> box_shift) & 1u))) y = -INFINITY;
+                            if (edge && !((TREE ? tree[b][i][x >> 5] >> (x & 31) & 1u : key_visible(k0 + x, pos[b][i], w.window, w.sinks)) && (here >> (x >> box_shift) & 1u)))
+                                y = -INFINITY;
                             top[b][i] = fmaxf(top[b][i], y);
                         }
                 }
@@ -565,7 +577,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
             for (unsigned left = again; left; left &= left - 1) {
                 const int r = __ffs(left) - 1, row = row_of(r);
                 if (row < 0 || turn++ % WARPS != warp) continue;
-                if (!attend_row<FMT, D>(a, sg.seq, sg.len, pos_of(r), row, head_of(r)) && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
+                if (!attend_row<FMT, D, TREE>(a, sg.seq, sg.len, TREE ? sg.len - sg.n : pos_of(r), row, head_of(r)) && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
             }
         }
         if (!last) __syncthreads();   // (the buffers are free again)
@@ -575,18 +587,16 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
         for (int i = issued < STAGES ? 0 : issued - STAGES; i < issued; ++i) mbar_wait_bounded_warp(bars + (i % STAGES) * 8, (i / STAGES) & 1);
 }
 
-template <int FMT, int D, int NB>
-cudaError_t configure() {
-    return cudaFuncSetAttribute(attention_decode_kernel<FMT, D, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+template <int FMT, int D>
+auto kernel(bool one_tile, bool tree) {
+    return tree ? one_tile ? attention_decode_kernel<FMT, D, 1, true> : attention_decode_kernel<FMT, D, 2, true>
+                : one_tile ? attention_decode_kernel<FMT, D, 1, false> : attention_decode_kernel<FMT, D, 2, false>;
 }
 template <int FMT, int D>
 cudaError_t configure() {
-    const cudaError_t e = configure<FMT, D, 1>();
-    return e != cudaSuccess ? e : configure<FMT, D, 2>();
-}
-template <int FMT, int D>
-auto kernel(bool one_tile) {
-    return one_tile ? attention_decode_kernel<FMT, D, 1> : attention_decode_kernel<FMT, D, 2>;
+    cudaError_t e = cudaSuccess;
+    for (int i = 0; i < 4 && e == cudaSuccess; ++i) e = cudaFuncSetAttribute(kernel<FMT, D>(i & 1, i & 2), cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    return e;
 }
 
 }  // namespace
@@ -603,9 +613,10 @@ int attention_decode_keys(int fmt, int dim) { return PART / (dim * kv_cell_bytes
 
 cudaError_t launch_attention_decode(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl) {
     const bool one = (long long)a.group * max_new <= 8;   // one tile of 8 rows
-    auto k = a.c.fmt == KV_FP16 ? (a.c.dim == 64 ? kernel<KV_FP16, 64>(one) : kernel<KV_FP16, 128>(one))
-             : a.c.fmt == KV_INT8 ? (a.c.dim == 64 ? kernel<KV_INT8, 64>(one) : kernel<KV_INT8, 128>(one))
-                                  : (a.c.dim == 64 ? kernel<KV_FP8, 64>(one) : kernel<KV_FP8, 128>(one));
+    const bool tree = a.tree != nullptr;
+    auto k = a.c.fmt == KV_FP16 ? (a.c.dim == 64 ? kernel<KV_FP16, 64>(one, tree) : kernel<KV_FP16, 128>(one, tree))
+             : a.c.fmt == KV_INT8 ? (a.c.dim == 64 ? kernel<KV_INT8, 64>(one, tree) : kernel<KV_INT8, 128>(one, tree))
+                                  : (a.c.dim == 64 ? kernel<KV_FP8, 64>(one, tree) : kernel<KV_FP8, 128>(one, tree));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(sm_count < ATTN_MAX_BLOCKS ? sm_count : ATTN_MAX_BLOCKS));
     cfg.blockDim = dim3(THREADS);

@@ -31,8 +31,9 @@ struct CellDims {
     }
 };
 
-// Query head `head` of row `row`, position `pos` in sequence `seq` of length `len`; false: a page number was out of range (its keys count as hidden).
-template <int FMT, int D>
+// Query head `head` of row `row`, position `pos` in sequence `seq` of length `len` (TREE: `pos` is that of the sequence's first new token, and the row's mask
+// tells which of them it sees); false: a page number was out of range (its keys count as hidden).
+template <int FMT, int D, bool TREE>
 __device__ bool attend_row(const AttnArgs& a, int seq, int len, int pos, int row, int head) {
     constexpr int N = D / 32, G = 8;
     const int lane = threadIdx.x & 31, kv_head = head / a.group, mask = (1 << a.c.page_shift) - 1;
@@ -43,9 +44,9 @@ __device__ bool attend_row(const AttnArgs& a, int seq, int len, int pos, int row
     qw.load(a.q + row * a.q_stride + (int64_t)head * D, 0, lane);
     qw.floats(q);
     const float scale = a.scale * 1.4426950408889634f;   // exponents are powers of two
-    const int lo = window_begin(pos, a.window), end = min(pos + 1, len);
+    const int lo = TREE ? 0 : window_begin(pos, a.window), end = TREE ? len : min(pos + 1, len);
     for (int key0 = 0; key0 < end && l == l; key0 += G) {   // (once the sum is a NaN the row is)
-        if (key0 + G <= lo && key0 >= a.sinks) key0 = lo / G * G;
+        if (!TREE && key0 + G <= lo && key0 >= a.sinks) key0 = lo / G * G;
         const int page = table[key0 >> a.c.page_shift];
         if (!page_ok(page, a.c.num_pages)) {
             ok = false;
@@ -63,6 +64,7 @@ __device__ bool attend_row(const AttnArgs& a, int seq, int len, int pos, int row
                 vs[i] = a.c.v_scale[at + i];
             }
         }
+        const uint32_t tree = TREE ? tree_bits(a.tree + (int64_t)row * a.tree_words, a.tree_words, key0, pos, len) : 0u;
         float s[G];
 #pragma unroll
         for (int i = 0; i < G; ++i) {
@@ -79,7 +81,7 @@ __device__ bool attend_row(const AttnArgs& a, int seq, int len, int pos, int row
 #pragma unroll
         for (int i = 0; i < G; ++i) {
             const int key = key0 + i;
-            if (key >= end || (key < lo && key >= a.sinks)) continue;
+            if (TREE ? !(tree >> i & 1u) : key >= end || (key < lo && key >= a.sinks)) continue;
             any = true;
             const float t = s[i] * scale, up = fmaxf(m, t), old = m == up ? 1.f : exp2f(m - up);
             const float w = t == -INFINITY ? 0.f : exp2f(t - up);   // (a NaN score makes w, and so the row, NaN)

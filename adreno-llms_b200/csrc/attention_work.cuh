@@ -22,6 +22,7 @@ struct WorkShape {
     int vheads;    // items side by side: cache heads (times the parts of a head's query heads)
     int tile;      // keys of a unit
     int window, sinks;
+    int tree_words;   // of a row's mask; 0: no tree.  With a tree every item sees keys up to the sequence's last one, and there is no window
     unsigned extra;   // units of an item besides its key tiles
     unsigned chunk;   // units of a block, and whether items are filled up to it
     bool pad;
@@ -38,26 +39,28 @@ struct Segment {
     int first, count;       // key tiles [first, first + count) of the item
     int total;              // key tiles of the item
     unsigned unit0;         // number of the item's first key tile
-    // positions of the item's first and last token
-    __device__ __forceinline__ int p0(const WorkShape& w) const { return len - n + qt * w.tokens; }
-    __device__ __forceinline__ int p1(const WorkShape& w) const { return len - n + min((qt + 1) * w.tokens, n) - 1; }
+    // positions of the item's first and last token; of a tree: the last one that all rows see, and that some row may see
+    __device__ __forceinline__ int p0(const WorkShape& w) const { return w.tree_words ? len - n - 1 : len - n + qt * w.tokens; }
+    __device__ __forceinline__ int p1(const WorkShape& w) const { return w.tree_words ? len - 1 : len - n + min((qt + 1) * w.tokens, n) - 1; }
     __device__ __forceinline__ TileRange tiles(const WorkShape& w) const { return visible_tiles(p0(w), p1(w), w.window, w.sinks, w.tile); }
 };
 
 __device__ __forceinline__ SeqWork load_seq(const KvSeqs& s, const WorkShape& w, int i, bool* bad = nullptr, bool* descends = nullptr) {
     const int start = s.row_start[i], end = s.row_start[i + 1];
     const SeqExtent e = seq_extent(start, end, s.kv_len[i], s.num_rows, s.max_len);
-    if (bad) *bad = e.bad;
-    if (descends) *descends = end < start;
     SeqWork q;
     q.row0 = e.row0;
     q.n = e.row1 - e.row0;
+    const bool wide = w.tree_words && q.n > 32 * w.tree_words;   // more tokens than a mask has bits: no work
+    if (wide) q.n = 0;
+    if (bad) *bad = e.bad || wide;
+    if (descends) *descends = end < start;
     q.len = e.len;
     q.tiles_q = q.n <= w.tokens ? (q.n > 0) : (q.n + w.tokens - 1) / w.tokens;   // (a division costs as much as a load from the L2)
     return q;
 }
 __device__ __forceinline__ int item_tiles(const SeqWork& q, const WorkShape& w, int qt) {
-    const int p0 = q.len - q.n + qt * w.tokens, p1 = q.len - q.n + min((qt + 1) * w.tokens, q.n) - 1;
+    const int p0 = w.tree_words ? q.len - q.n - 1 : q.len - q.n + qt * w.tokens, p1 = w.tree_words ? q.len - 1 : q.len - q.n + min((qt + 1) * w.tokens, q.n) - 1;
     return max(1, visible_tiles(p0, p1, w.window, w.sinks, w.tile).tiles());
 }
 // Units of all query tiles of a sequence; by each lane for one of its own.  (Where some lane's sequence has many, the warp goes through them

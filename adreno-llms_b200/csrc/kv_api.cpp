@@ -6,24 +6,10 @@
 #include <string>
 
 #include "../../include/nnopt_b200.h"
-#include "attention.h"
-#include "attention_maps.h"
-#include "internal.h"
 #include "kernels.h"
+#include "kv_api.h"
 
 using namespace nnb;
-
-struct nn_kv_cache {
-    int device;
-    KvView view;
-    AttnMaps maps;
-};
-
-static bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
-static size_t cache_bytes(const KvView& v) {
-    return ((size_t)v.num_pages * v.kv_heads << v.page_shift) * (size_t)v.dim * kv_cell_bytes(v.fmt);
-}
 
 #define CUDA_TRY(call)                                                                        \
     do {                                                                                      \
@@ -47,41 +33,6 @@ static int attention_workspace(nn_context* c, const char* who) {
     }
     c->attn_work = work;
     return NN_OK;
-}
-
-// Rows of `width` values at a distance of `stride`.
-struct Rows {
-    const uint16_t* p;
-    int64_t stride, width;
-};
-static size_t rows_bytes(const Rows& r, int rows) { return ((size_t)(rows - 1) * r.stride + r.width) * 2; }
-
-// Whether two sets of rows share memory.  Of equal stride they may be columns of one buffer (q, k and v of a fused projection).
-static bool rows_overlap(const Rows& a, const Rows& b, int rows) {
-    const char *pa = (const char*)a.p, *pb = (const char*)b.p;
-    if (pa >= pb + rows_bytes(b, rows) || pb >= pa + rows_bytes(a, rows)) return false;
-    if (a.stride != b.stride) return true;
-    const int64_t pitch = a.stride * 2;
-    int64_t d = (int64_t)((intptr_t)pb - (intptr_t)pa) % pitch;
-    if (d < 0) d += pitch;
-    return d < a.width * 2 || d + b.width * 2 > pitch;
-}
-static bool share(const void* p, size_t np, const void* q, size_t nq) { return p && q && (const char*)p < (const char*)q + nq && (const char*)q < (const char*)p + np; }
-static size_t scale_bytes(const KvView& v) { return cache_bytes(v) / ((size_t)v.dim * kv_cell_bytes(v.fmt)) * 2; }
-static bool over_cache(const void* p, size_t n, const KvView& v) {
-    const size_t nc = cache_bytes(v), ns = scale_bytes(v);
-    return share(p, n, v.k, nc) || share(p, n, v.v, nc) || share(p, n, v.k_scale, ns) || share(p, n, v.v_scale, ns);
-}
-static bool rows_over_cache(const Rows& r, int rows, const KvView& v) { return over_cache(r.p, rows_bytes(r, rows), v); }
-// (what a call writes must not be what tells it where to)
-static bool cache_over_batch(const KvView& v, const nn_kv_batch* b) {
-    return over_cache(b->row_start, 4 * ((size_t)b->num_seqs + 1), v) || over_cache(b->kv_len, 4 * (size_t)b->num_seqs, v) ||
-           over_cache(b->page_table, 4 * (size_t)b->num_seqs * b->table_stride, v);
-}
-static bool rows_over_batch(const Rows& r, const nn_kv_batch* b) {
-    const size_t n = rows_bytes(r, b->num_rows);
-    return share(r.p, n, b->row_start, 4 * ((size_t)b->num_seqs + 1)) || share(r.p, n, b->kv_len, 4 * (size_t)b->num_seqs) ||
-           share(r.p, n, b->page_table, 4 * (size_t)b->num_seqs * b->table_stride);
 }
 
 extern "C" int nn_kv_cache_create(nn_context* c, int format, int num_pages, int page_size, int kv_heads, int head_dim, nn_buf k, nn_buf v,
@@ -144,48 +95,9 @@ static int take_rows(const void* p, int64_t stride, int heads, int dim, const ch
     return NN_OK;
 }
 
-// *empty: there is nothing to do.
-static int take_batch(nn_context* c, const nn_kv_cache* h, const nn_kv_batch* b, const char* who, KvSeqs* s, bool* empty) {
-    *empty = false;
-    if (!h || !b) return NN_FAIL(NN_ERR_ARG, "%s: null cache or batch", who);
-    if (b->num_seqs < 0 || b->num_rows < 0) return NN_FAIL(NN_ERR_ARG, "%s: num_seqs=%d num_rows=%d", who, b->num_seqs, b->num_rows);
-    if (b->num_seqs == 0 || b->num_rows == 0) {
-        *empty = true;
-        return NN_OK;
-    }
-    if (b->max_len > 1 << 30) return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: max_len=%d is more than 2^30", who, b->max_len);
-    if (b->max_new <= 0 || b->max_len <= 0 || b->table_stride <= 0)
-        return NN_FAIL(NN_ERR_ARG, "%s: max_new=%d max_len=%d table_stride=%d", who, b->max_new, b->max_len, b->table_stride);
-    if (!b->row_start || !b->kv_len || !b->page_table) return NN_FAIL(NN_ERR_ARG, "%s: null row_start, kv_len or page_table", who);
-    if (!aligned(b->row_start, 4) || !aligned(b->kv_len, 4) || !aligned(b->page_table, 4))
-        return NN_FAIL(NN_ERR_ARG, "%s: row_start, kv_len and page_table must be 4-byte aligned", who);
-    if ((long long)b->table_stride << h->view.page_shift < b->max_len)
-        return NN_FAIL(NN_ERR_ARG, "%s: max_len=%d is more than a page table row of %d pages of %d positions holds", who, b->max_len, b->table_stride, 1 << h->view.page_shift);
-    s->row_start = (const int*)b->row_start;
-    s->kv_len = (const int*)b->kv_len;
-    s->page_table = (const int*)b->page_table;
-    s->num_seqs = b->num_seqs;
-    s->num_rows = b->num_rows;
-    s->table_stride = b->table_stride;
-    s->max_len = b->max_len;
-    return NN_OK;
-}
-
-// Last of the checks (the others need no GPU).  The calling thread may have another device current.
-static int make_current(nn_context* c, const nn_kv_cache* h, const char* who) {
-    if (!c) return NN_FAIL(NN_ERR_ARG, "%s: null context", who);
-    if (h->device != c->device) return NN_FAIL(NN_ERR_ARG, "%s: the cache was made for device %d, the context is of device %d", who, h->device, c->device);
-    int now = -1;
-    if (cudaGetDevice(&now) != cudaSuccess || now != c->device) {
-        const cudaError_t e = cudaSetDevice(c->device);
-        if (e != cudaSuccess) return NN_FAIL(NN_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
-    }
-    return NN_OK;
-}
-
 static const char* kv_name(int fmt) { return fmt == KV_FP16 ? "fp16" : fmt == KV_INT8 ? "int8" : "fp8"; }
 
-static int kv_write(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf cos_f32, nn_buf sin_f32, int table_len, int rotary_dim, int q_heads, nn_buf q,
+static int kv_write(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf position, nn_buf cos_f32, nn_buf sin_f32, int table_len, int rotary_dim, int q_heads, nn_buf q,
                     int64_t q_stride, nn_buf q_out, int64_t q_out_stride, nn_buf k, int64_t k_stride, nn_buf v, int64_t v_stride, const char* who) {
     KvWriteArgs a = {};
     bool empty;
@@ -214,10 +126,17 @@ static int kv_write(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf 
         if (q && (share(ro.p, n, cos_f32, table) || share(ro.p, n, sin_f32, table))) return NN_FAIL(NN_ERR_ARG, "%s: q_out overlaps cos or sin", who);
         if (over_cache(cos_f32, table, a.c) || over_cache(sin_f32, table, a.c)) return NN_FAIL(NN_ERR_ARG, "%s: the cache overlaps cos or sin", who);
     }
+    if (position) {
+        const size_t n = 4 * (size_t)b->num_rows;
+        if (!aligned(position, 4)) return NN_FAIL(NN_ERR_ARG, "%s: position must be 4-byte aligned", who);
+        if (over_cache(position, n, a.c) || (q && share(ro.p, rows_bytes(ro, b->num_rows), position, n)))
+            return NN_FAIL(NN_ERR_ARG, "%s: the cache or q_out overlaps position", who);
+    }
     a.q = rq.p;
     a.q_out = const_cast<uint16_t*>(ro.p);
     a.k = rk.p;
     a.v = rv.p;
+    a.position = (const int*)position;
     a.cos = (const float*)cos_f32;
     a.sin = (const float*)sin_f32;
     a.table_len = table_len;
@@ -243,13 +162,20 @@ static int kv_write(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf 
 }
 
 extern "C" int nn_kv_write(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf k, int64_t k_stride, nn_buf v, int64_t v_stride) {
-    return kv_write(c, h, b, nullptr, nullptr, 0, 0, 0, nullptr, 0, nullptr, 0, k, k_stride, v, v_stride, "nn_kv_write");
+    return kv_write(c, h, b, nullptr, nullptr, nullptr, 0, 0, 0, nullptr, 0, nullptr, 0, k, k_stride, v, v_stride, "nn_kv_write");
 }
 
 extern "C" int nn_rope_kv_write(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf cos_f32, nn_buf sin_f32, int table_len, int rotary_dim, int q_heads,
                                 nn_buf q, int64_t q_stride, nn_buf q_out, int64_t q_out_stride, nn_buf k, int64_t k_stride, nn_buf v, int64_t v_stride) {
     if (rotary_dim == 0) return NN_FAIL(NN_ERR_ARG, "nn_rope_kv_write: rotary_dim is 0 (nn_kv_write does not rotate)");
-    return kv_write(c, h, b, cos_f32, sin_f32, table_len, rotary_dim, q_heads, q, q_stride, q_out, q_out_stride, k, k_stride, v, v_stride, "nn_rope_kv_write");
+    return kv_write(c, h, b, nullptr, cos_f32, sin_f32, table_len, rotary_dim, q_heads, q, q_stride, q_out, q_out_stride, k, k_stride, v, v_stride, "nn_rope_kv_write");
+}
+
+extern "C" int nn_rope_kv_write_at(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf position, nn_buf cos_f32, nn_buf sin_f32, int table_len, int rotary_dim,
+                                   int q_heads, nn_buf q, int64_t q_stride, nn_buf q_out, int64_t q_out_stride, nn_buf k, int64_t k_stride, nn_buf v, int64_t v_stride) {
+    if (rotary_dim == 0) return NN_FAIL(NN_ERR_ARG, "nn_rope_kv_write_at: rotary_dim is 0 (nn_kv_write does not rotate)");
+    if (!position) return NN_FAIL(NN_ERR_ARG, "nn_rope_kv_write_at: position is null (nn_rope_kv_write rotates to the positions of the cells)");
+    return kv_write(c, h, b, position, cos_f32, sin_f32, table_len, rotary_dim, q_heads, q, q_stride, q_out, q_out_stride, k, k_stride, v, v_stride, "nn_rope_kv_write_at");
 }
 
 extern "C" int nn_kv_read(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, nn_buf k_out, int64_t k_stride, nn_buf v_out, int64_t v_stride) {
@@ -279,9 +205,9 @@ extern "C" int nn_kv_read(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, n
     return NN_OK;
 }
 
-extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, int q_heads, nn_buf q, int64_t q_stride, nn_buf out, int64_t out_stride, float scale,
-                            int window, int sinks) {
-    const char* who = "nn_attention";
+// mask null: without a tree.
+static int attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, int q_heads, nn_buf q, int64_t q_stride, nn_buf out, int64_t out_stride, float scale, int window,
+                     int sinks, int mask_words, nn_buf mask, const char* who) {
     AttnArgs a = {};
     bool empty;
     int rc = take_batch(c, h, b, who, &a.s, &empty);
@@ -295,6 +221,12 @@ extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b,
         return NN_FAIL(NN_ERR_ARG, "%s: out overlaps q, the cache or the batch", who);
     if (!(scale > 0.f) || !std::isfinite(scale)) return NN_FAIL(NN_ERR_ARG, "%s: scale=%g: finite and positive", who, (double)scale);
     if (window < 0 || sinks < 0) return NN_FAIL(NN_ERR_ARG, "%s: window=%d sinks=%d", who, window, sinks);
+    if (mask) {
+        const size_t n = 4 * (size_t)b->num_rows * mask_words;
+        if (share(ro.p, rows_bytes(ro, b->num_rows), mask, n)) return NN_FAIL(NN_ERR_ARG, "%s: out overlaps the mask", who);
+    }
+    a.tree = (const uint32_t*)mask;
+    a.tree_words = mask_words;
     a.q = rq.p;
     a.out = const_cast<uint16_t*>(ro.p);
     a.q_heads = q_heads;
@@ -308,7 +240,7 @@ extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b,
         return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: num_seqs=%d num_rows=%d max_len=%d: more than 2^30 tiles of work", who, b->num_seqs, b->num_rows, b->max_len);
     if ((rc = make_current(c, h, who)) || (rc = attention_workspace(c, who))) return rc;
     a.status = c->status_dev;
-    ProfScope prof(c, [&] { return std::string("attention_") + kv_name(a.c.fmt) + "_seqs" + std::to_string(b->num_seqs) + "_rows" + std::to_string(b->num_rows); });
+    ProfScope prof(c, [&] { return std::string(mask ? "attention_tree_" : "attention_") + kv_name(a.c.fmt) + "_seqs" + std::to_string(b->num_seqs) + "_rows" + std::to_string(b->num_rows); });
     a.counters = (unsigned*)c->attn_work;
     a.items = (int4*)((char*)c->attn_work + ATTN_COUNTER_BYTES);
     a.parts = (char*)c->attn_work + ATTN_HEAD_BYTES;
@@ -318,4 +250,19 @@ extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b,
     c->in_flight.wrote(out, rows_bytes(ro, b->num_rows));
     c->launches += kernels;
     return NN_OK;
+}
+
+extern "C" int nn_attention(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, int q_heads, nn_buf q, int64_t q_stride, nn_buf out, int64_t out_stride, float scale,
+                            int window, int sinks) {
+    return attention(c, h, b, q_heads, q, q_stride, out, out_stride, scale, window, sinks, 0, nullptr, "nn_attention");
+}
+
+extern "C" int nn_attention_tree(nn_context* c, nn_kv_cache* h, const nn_kv_batch* b, int q_heads, nn_buf q, int64_t q_stride, nn_buf out, int64_t out_stride, float scale,
+                                 int mask_words, nn_buf mask) {
+    const char* who = "nn_attention_tree";
+    if (!h || !b) return NN_FAIL(NN_ERR_ARG, "%s: null cache or batch", who);
+    const int rc = take_words(b, mask_words, who);
+    if (rc) return rc;
+    if (b->num_seqs > 0 && b->num_rows > 0 && (!mask || !aligned(mask, 4))) return NN_FAIL(NN_ERR_ARG, "%s: the mask must be there and 4-byte aligned", who);
+    return attention(c, h, b, q_heads, q, q_stride, out, out_stride, scale, 0, 0, mask_words, mask, who);
 }

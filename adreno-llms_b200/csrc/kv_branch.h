@@ -1,0 +1,67 @@
+// Launch interface of what moves sequences about in the paged cache: drafted trees, cells that move, beams.
+#pragma once
+#include "attention.h"
+
+namespace nnb {
+
+struct TreeLayoutArgs {
+    KvSeqs s;                // (without a page table)
+    const int* parent;       // [num_rows], among the sequence's new rows; -1: none
+    uint32_t* mask;          // [num_rows][words]
+    int* position;           // [num_rows]
+    int words;
+    int* status;
+};
+cudaError_t launch_tree_layout(const TreeLayoutArgs& a, cudaStream_t st, bool pdl);
+
+// The cell rows of one layer, as bytes.
+struct CellRows {
+    uint8_t* k;
+    uint8_t* v;
+    uint16_t* k_scale;   // null without scales
+    uint16_t* v_scale;
+    int num_pages, kv_heads, row_bytes;
+};
+// Layers of one launch (kernel arguments may have 4 KB everywhere).
+constexpr int MOST_LAYERS = 64;
+struct CellRowsOfLayers {
+    CellRows c[MOST_LAYERS];
+    int n;
+};
+
+struct KvMoveArgs {
+    CellRowsOfLayers caches;
+    KvSeqs s;
+    const int* source;       // [num_rows]: where the row's cells are now
+    int page_shift, most_heads;
+    int* status;
+};
+cudaError_t launch_kv_move(const KvMoveArgs& a, cudaStream_t st, bool pdl);
+
+constexpr int MOST_BEAMS = 32;
+struct KvReorderArgs {
+    CellRowsOfLayers caches;
+    KvSeqs s;                // beam after beam, group after group
+    const int* parent;       // [num_seqs], among the group's beams; -1: itself
+    int beams, page_shift, most_heads, num_pages;   // num_pages: the fewest of these caches
+    bool with_table;         // whether this launch exchanges the page table's entries
+    int* status;
+};
+cudaError_t launch_kv_reorder(const KvReorderArgs& a, cudaStream_t st, bool pdl);
+
+// The best continuations of groups of beams.
+constexpr int MOST_PICKS = 32, MOST_BEAM_ROWS = 8192;
+struct BeamSelectArgs {
+    const uint16_t* logits;  // [groups * beams][stride]
+    int64_t stride;
+    const float* score;      // [groups][beams]
+    const int* done;         // [groups][beams], or null
+    float* out_score;        // [groups][picks]
+    int* out_token;
+    int* out_parent;
+    int* out_done;           // or null
+    int groups, beams, vocab, picks, eos;
+};
+cudaError_t launch_beam_select(const BeamSelectArgs& a, cudaStream_t st, bool pdl);
+
+}  // namespace nnb

@@ -75,7 +75,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
     if (r >= a.s.num_rows) return;
     const RowPlace at = place_of_row(a.s, r);
     if (at.none) return;
-    if (at.bad || (a.rotary && at.pos >= a.table_len)) {
+    const int turn = a.position && !at.bad ? a.position[r] : at.pos;
+    if (at.bad || (a.rotary && (turn < 0 || turn >= a.table_len))) {
         if (lane == 0) a.status[STATUS_BAD_TABLE] = 1;
         return;
     }
@@ -88,8 +89,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
     const bool turns = j < a.rotary / 16;
     float c[8], s[8];
     if (turns) {
-        const float4* ct = reinterpret_cast<const float4*>(a.cos + (int64_t)at.pos * (a.rotary / 2) + 8 * j);
-        const float4* st = reinterpret_cast<const float4*>(a.sin + (int64_t)at.pos * (a.rotary / 2) + 8 * j);
+        const float4* ct = reinterpret_cast<const float4*>(a.cos + (int64_t)turn * (a.rotary / 2) + 8 * j);
+        const float4* st = reinterpret_cast<const float4*>(a.sin + (int64_t)turn * (a.rotary / 2) + 8 * j);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const float4 x = ct[i], y = st[i];

@@ -62,4 +62,18 @@ NNB_HD TileRange visible_tiles(int p0, int p1, int window, int sinks, int tile) 
     return r;
 }
 
+// A drafted tree: the last keys of a sequence, from position `base` on, are its new tokens.  A row sees all keys before them, and of them those of its mask:
+// bit j of its words for key base + j.
+constexpr int TREE_MOST_WORDS = 32;
+NNB_HD uint32_t low_bits32(int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; }
+// Keys at, at + 1, .. at + 31 that the row sees, as bits.  (at - base has no overflow: a sequence has at most 32 * words new tokens.)
+NNB_HD uint32_t tree_bits(const uint32_t* mask, int words, int at, int base, int len) {
+    const int off = at - base, w = off >> 5, s = off & 31;
+    uint32_t seen;
+    if (off <= -32) seen = 0xFFFFFFFFu;
+    else if (off < 0) seen = low_bits32(-off) | mask[0] << -off;
+    else seen = (w < words ? mask[w] >> s : 0u) | (s != 0 && w + 1 < words ? mask[w + 1] << (32 - s) : 0u);
+    return seen & low_bits32(len - at);
+}
+
 }  // namespace nnb

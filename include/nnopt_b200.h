@@ -232,6 +232,50 @@ int nn_kv_read(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, nn
 int nn_attention(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, int q_heads, nn_buf q, int64_t q_stride, nn_buf out, int64_t out_stride, float scale,
                  int window, int sinks);
 
+/* ---- several continuations of a sequence over the same cache: drafted tokens that form a tree, and beams.  They have no counterpart in the
+ *      reference, whose decode loop has one sequence and takes the largest logit.
+ *
+ *   nn_tree_layout    the new rows of each sequence are a drafted tree: parent int32 [num_rows] is a row's parent as an index among its sequence's new
+ *                     rows (below its own; -1: it follows the sequence before the draft).  mask uint32 [num_rows][mask_words] gets bit j for new row j where
+ *                     that is the row itself or an ancestor, position int32 [num_rows] the row's place behind the sequence, kv_len - (new rows) + depth.
+ *                     mask_words 1 to 32, with a bit for each of max_new rows.  Of the batch row_start and kv_len are used.  Once a step: all layers share
+ *                     them.  (A program whose trees are always the same may keep the mask.)
+ *   nn_rope_kv_write_at  nn_rope_kv_write with queries and keys rotated to position[row] (int32 [num_rows], below table_len) instead of the cell's own
+ *                     position: a tree's rows lie one behind the other in the cache, whatever their depth.  A row whose position is out of range is left out.
+ *   nn_attention_tree nn_attention where row r sees all positions before the sequence's new rows, and of these the ones in its mask (bits behind the last new
+ *                     row count for nothing; any bits may be set, those of later rows too).  No window.  A row that sees nothing gives zeros.
+ *                     A sequence with more new rows than a mask has bits is left out and reported.
+ *   nn_kv_move        cells go to earlier positions: row r of the batch has the position that it always has (the last row kv_len - 1) and takes over the
+ *                     keys and values, with their scales, of position source[r] of its sequence (int32 [num_rows]), in all `num_caches` caches (the layers
+ *                     of a model, which share their page numbers and page size), as if all of a sequence's rows were read first.  Sources ascend within a
+ *                     sequence and are not before their rows; kv_len counts what is left.  So an accepted path of a tree becomes the sequence's end
+ *                     (source: the places of its rows), and what follows dropped positions moves up to them.  Rotations stay what they were.  Rows
+ *                     with a bad source or page are left out and reported.  A moved row's page must not be another sequence's too.
+ *   nn_beam_select    of `groups` groups of `beams` beams each the `picks` best continuations: total = score[beam] + log_softmax(logits[beam])[token], from
+ *                     fp16 logits [groups * beams][logits_stride] (0: dense) of `vocab` tokens and fp32 scores [groups][beams], in descending order; of equal
+ *                     ones the lowest beam, then the lowest token first.  out_score fp32, out_token and out_parent (the beam) int32, [groups][picks]; where a
+ *                     group has fewer candidates the rest are -infinity, -1, -1.  Totals are compared in 64 bits and rounded to fp32 for out_score.
+ *                     Logits of -infinity are no candidates, nor are beams whose score is -infinity or a NaN, nor rows with a NaN or +infinity.
+ *                     done (int32 [groups][beams], may be NULL): a beam that is not 0 there has ended: it has one candidate, token eos with its score as it
+ *                     is, and its logits are not read.  out_done (int32 [groups][picks], may be NULL): 1 where the token is eos.  With picks == beams, out_score may be
+ *                     score and out_done may be done.  beams and picks up to 32, groups * beams up to 8192.
+ *   nn_kv_reorder     every beam takes over its parent's sequence: the batch's sequences are the beams, group after group, all of a group of the same kv_len;
+ *                     parent int32 [num_seqs] among the beams of the group (as nn_beam_select gives it with picks == beams; -1: the beam itself).  The page table's entries
+ *                     of full pages are taken over in place (it is written); the page that is not full must be each beam's own, and the parent's cells in it are copied to the
+ *                     beam's, in all `num_caches` caches.  Entries behind it stay each beam's own.  So beams share the pages they
+ *                     have in common, and a beam's own pages are those of its table from the first one that was not full when it began.  row_start, num_rows and
+ *                     max_new are not used.  Groups with a bad length, parent or page, or whose pages that are not full coincide, are left as they are and reported.
+ *                     A prompt is given to all beams by parents of 0. ------------------------------------------------------------------ */
+int nn_tree_layout(nn_context* ctx, const nn_kv_batch* batch, nn_buf parent_i32, int mask_words, nn_buf mask_u32, nn_buf position_i32);
+int nn_rope_kv_write_at(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, nn_buf position_i32, nn_buf cos_f32, nn_buf sin_f32, int table_len, int rotary_dim,
+                        int q_heads, nn_buf q, int64_t q_stride, nn_buf q_out, int64_t q_out_stride, nn_buf k, int64_t k_stride, nn_buf v, int64_t v_stride);
+int nn_attention_tree(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, int q_heads, nn_buf q, int64_t q_stride, nn_buf out, int64_t out_stride, float scale,
+                      int mask_words, nn_buf mask_u32);
+int nn_kv_move(nn_context* ctx, nn_kv_cache* const* caches, int num_caches, const nn_kv_batch* batch, nn_buf source_i32);
+int nn_kv_reorder(nn_context* ctx, nn_kv_cache* const* caches, int num_caches, const nn_kv_batch* batch, int beams, nn_buf parent_i32);
+int nn_beam_select(nn_context* ctx, int groups, int beams, int vocab, nn_buf logits_fp16, int64_t logits_stride, nn_buf score_f32, nn_buf done_i32, int eos, int picks,
+                   nn_buf out_score_f32, nn_buf out_token_i32, nn_buf out_parent_i32, nn_buf out_done_i32);
+
 /* Arg-max for callers that are not allowed to allocate device memory (a real-time thread
  * under a no-allocation rule, a host application that owns the whole device heap through its
  * own pool, a service whose memory budget is frozen after start-up).  It has no counterpart
