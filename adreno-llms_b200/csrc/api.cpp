@@ -16,6 +16,7 @@
 #include "attention.h"
 #include "internal.h"
 #include "kernels.h"
+#include "kv_branch.h"
 #include "plan.h"
 
 using namespace nnb;
@@ -189,6 +190,10 @@ extern "C" int nn_init(int device, nn_context** out) {
         delete c;
         return NN_FAIL(NN_ERR_CUDA, "nn_init: cudaMalloc failed");
     }
+    if (cudaMalloc(&c->beam_work, BEAM_WORK_BYTES) != cudaSuccess || cudaMemset(c->beam_work, 0, BEAM_WORK_BYTES) != cudaSuccess) {
+        delete c;
+        return NN_FAIL(NN_ERR_CUDA, "nn_init: cudaMalloc failed");
+    }
     if ((e = stream_configure()) != cudaSuccess) {
         delete c;
         return NN_FAIL(NN_ERR_CUDA, "nn_init: kernel configuration failed: %s", cudaGetErrorString(e));
@@ -213,6 +218,7 @@ extern "C" int nn_shutdown(nn_context* c) {
     for (auto& kv : c->registry) free_scale_pad(kv.second);
     if (c->flush_buf) cudaFree(c->flush_buf);
     if (c->attn_work) cudaFree(c->attn_work);
+    if (c->beam_work) cudaFree(c->beam_work);
     if (c->argmax_slot) cudaFree(c->argmax_slot);
     if (c->norm_scratch) cudaFree(c->norm_scratch);
     if (c->stage_img) cudaFree(c->stage_img);

@@ -184,9 +184,14 @@ extern "C" int nn_beam_select(nn_context* c, int groups, int beams, int vocab, n
         if (share(outs[i], no, logits, nl) || (!in_place_score && share(outs[i], no, score, ni)) || (!in_place_done && share(outs[i], no, done, ni)))
             return NN_FAIL(NN_ERR_ARG, "%s: an output overlaps logits, score or done", who);
     }
+    BeamSelectArgs a = {};
+    beam_segments((int)rows, vocab, c ? c->sm_count : 1, &a.segs, &a.per_seg);
+    if ((long long)rows * a.segs > BEAM_PARTS)
+        return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: %d rows of %d logits are more than %d segments of 16384", who, (int)rows, vocab, BEAM_PARTS);
     int rc;
     if ((rc = make_current(c, nullptr, who))) return rc;
-    BeamSelectArgs a = {};
+    a.counters = (unsigned*)c->beam_work;
+    a.parts = (char*)c->beam_work + MOST_BEAM_ROWS * sizeof(unsigned);
     a.logits = (const uint16_t*)logits;
     a.stride = stride;
     a.score = (const float*)score;
@@ -201,7 +206,7 @@ extern "C" int nn_beam_select(nn_context* c, int groups, int beams, int vocab, n
     a.picks = picks;
     a.eos = eos;
     ProfScope prof(c, [&] { return std::string("beam_select_groups") + std::to_string(groups) + "x" + std::to_string(beams) + "_n" + std::to_string(vocab); });
-    const cudaError_t e = launch_beam_select(a, c->stream, c->use_pdl);
+    const cudaError_t e = launch_beam_select(a, c->sm_count, c->stream, c->use_pdl);
     if (e != cudaSuccess) return NN_FAIL(NN_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
     for (const void* o : outs) c->in_flight.wrote(o, no);
     c->launches++;

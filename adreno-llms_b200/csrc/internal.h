@@ -53,6 +53,7 @@ struct nn_context {
     float* sk_scratch = nullptr;   // partial sums of blocks that share a tile (balanced K-streaming)
     unsigned* sk_flags = nullptr;
     void* attn_work = nullptr;     // the attention's counters and partial results (made with the first cache or the first attention)
+    void* beam_work = nullptr;     // the beam selection's counters and segments' results
     void* flush_buf = nullptr;
     size_t flush_bytes = 0;
     bool use_pdl = true;

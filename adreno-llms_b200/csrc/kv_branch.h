@@ -61,7 +61,14 @@ struct BeamSelectArgs {
     int* out_parent;
     int* out_done;           // or null
     int groups, beams, vocab, picks, eos;
+    int segs, per_seg;       // segments of a row, vectors of 8 values of a segment (set by the launch)
+    unsigned* counters;      // [MOST_BEAM_ROWS], 0 between launches
+    void* parts;             // [BEAM_PARTS] results of segments
 };
-cudaError_t launch_beam_select(const BeamSelectArgs& a, cudaStream_t st, bool pdl);
+// The workspace, one call at a time: counters, parts.
+constexpr int BEAM_PARTS = 32768;
+constexpr size_t BEAM_PART_BYTES = 8 + 4 * MOST_PICKS, BEAM_WORK_BYTES = MOST_BEAM_ROWS * sizeof(unsigned) + BEAM_PARTS * BEAM_PART_BYTES;
+void beam_segments(int rows, int vocab, int sm_count, int* segs, int* per_seg);
+cudaError_t launch_beam_select(const BeamSelectArgs& a, int sm_count, cudaStream_t st, bool pdl);
 
 }  // namespace nnb
