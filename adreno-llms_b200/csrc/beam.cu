@@ -4,14 +4,14 @@
 //
 // and of an ended beam only (b, eos) with score_b.  The largest totals come first, of equal ones the lowest beam, then the lowest token.
 //
-// Bound by the logits' bytes, each read once.  A row is cut into segments, a block each; a thread has up to CHUNK vectors of 8 values of its segment and
-// keeps their maximum, where it first was, and the sum of exponentials behind it.  The row's best `picks` values lie in those threads' shares whose
-// maxima are the `picks` best ones: every other share has `picks` values before all of its own.  So no value needs a place in a list while the
-// logits stream by, whatever their order; the last block of a group reads the few shares again that matter (picks * CHUNK vectors of a row).
-//
+// Bound by the logits' bytes, each read once.  A row is cut into segments, a block each; a thread has every 256th vector of 8 values of its segment, its share, and
+// keeps their maximum and the sum of exponentials behind it.  The row's best `picks` values lie in those shares whose maxima are the `picks`
+// best ones: every other share has `picks` values before all of its own.  So no value needs a place in a list while the logits stream by, whatever
+// their order.  The row's last block finds those shares, reads them again, a value to a thread, and has the row's candidates; the group's last
+// block joins its rows' lists.
 // Within a row the fp16 values and the tokens decide, exactly.  Across rows the totals do, in 64 bits.  Exponentials are taken of differences to the
 // thread's maximum (exact), in 32 bits: a maximum is exactly 1, the others are 2^-22 off at most, and so is the sum; a row of 151936 values of N(0, 2.5) has a sum that is some
-// 2^-28 off, its errors being different for each value.  Everything depends on differences alone: rows that are shifted against each other
+// 2^-27 off, its errors being different for each value.  Everything depends on differences alone: rows that are shifted against each other
 // give the same logarithms.
 #include <cuda_fp16.h>
 
@@ -22,7 +22,8 @@ namespace nnb {
 namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, BATCH = 4;
-constexpr int CHUNK = 8;                    // vectors of a thread at most
+constexpr int TOPS = MOST_PICKS / 4;        // maxima of a warp that are compared with the other warps'
+constexpr int ROOM = 2048;                  // keys that a block compares with one another
 constexpr unsigned NO_VALUE = 0x03FFu;      // the code of -infinity
 
 __device__ __forceinline__ float ex2(float x) {
@@ -39,45 +40,60 @@ __device__ __forceinline__ float value_of(unsigned code) {
     return __half2float(__ushort_as_half((uint16_t)(code & 0x8000u ? code & 0x7FFFu : ~code)));
 }
 
-// 32 keys of a warp, the largest first
-template <class Key>
-__device__ __forceinline__ Key larger(Key a, Key b) { return a > b ? a : b; }
-template <class Key>
-__device__ __forceinline__ Key smaller(Key a, Key b) { return a > b ? b : a; }
-template <class Key>
-__device__ __forceinline__ Key ordered(Key x) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-        for (int d = size >> 1; d > 0; d >>= 1) {
-            const Key y = __shfl_xor_sync(0xffffffffu, x, d);
-            x = ((lane & d) == 0) == ((lane & size) == 0 || size == 32) ? larger(x, y) : smaller(x, y);
-        }
-    return x;
+// What follows is short code: a block goes through the kernel once, and instructions that no block of its SM has used before come from the L2 (unrolled,
+// with sorting networks: joining the lists of 4 beams took 33 thousand clocks, of which two thousand were work).
+
+// The place of keys[i] among `n` different ones: how many are larger.
+using Key = unsigned long long;
+__device__ __noinline__ int place_among(const Key* keys, int n, Key mine) {
+    int larger = 0;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) larger += keys[i] > mine;
+    return larger;
 }
-// The 32 largest of two such lists
-template <class Key>
-__device__ __forceinline__ Key merged(Key a, Key b) {
-    const int lane = threadIdx.x & 31;
-    a = larger(a, __shfl_sync(0xffffffffu, b, 31 - lane));
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) {
-        const Key y = __shfl_xor_sync(0xffffffffu, a, d);
-        a = (lane & d) == 0 ? larger(a, y) : smaller(a, y);
+
+constexpr double LN2 = 0.693147180559945309417;
+// exp(x), x <= 0: 2^n times the exponential's series of what is left, at most ln 2 / 2 (11 terms: 2^-44)
+__device__ __forceinline__ double exp_of(double x) {
+    if (!(x > -700.)) return x == x ? 0. : x;
+    const double n = rint(x * (1. / LN2)), f = fma(n, -LN2, x);
+    double p = 1. / 3628800.;
+    p = fma(p, f, 1. / 362880.);
+    p = fma(p, f, 1. / 40320.);
+    p = fma(p, f, 1. / 5040.);
+    p = fma(p, f, 1. / 720.);
+    p = fma(p, f, 1. / 120.);
+    p = fma(p, f, 1. / 24.);
+    p = fma(p, f, 1. / 6.);
+    p = fma(p, f, 0.5);
+    p = fma(p, f, 1.);
+    p = fma(p, f, 1.);
+    return p * __longlong_as_double((long long)(n + 1023.) << 52);
+}
+// log(x), x positive and finite: with x = 2^n m and z = (m - 1) / (m + 1), n ln 2 + 2 (z + z^3 / 3 + z^5 / 5 + ..); |z| <= 0.172 (9 terms: 2^-50)
+__device__ __forceinline__ double log_of(double x) {
+    const long long bits = __double_as_longlong(x);
+    int n = (int)(bits >> 52) - 1023;
+    double m = __longlong_as_double((bits & 0xFFFFFFFFFFFFFll) | 1023ll << 52);
+    if (m > 1.4142135623730951) {
+        m *= 0.5;
+        ++n;
     }
-    return a;
-}
-template <class Key, class At>
-__device__ __forceinline__ Key merged8(At&& at) {
-    Key x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = at(i);
-#pragma unroll
-    for (int n = 4; n > 0; n >>= 1)
-#pragma unroll
-        for (int i = 0; i < n; ++i) x[i] = merged(x[i], x[i + n]);
-    return x[0];
+    const double d = m + 1.;
+    double r = (double)__fdividef(1.f, (float)d);   // its reciprocal, by Newton's method
+    r = r * fma(-d, r, 2.);
+    r = r * fma(-d, r, 2.);
+    const double z = (m - 1.) * r, q = z * z;
+    double p = 1. / 17.;
+    p = fma(p, q, 1. / 15.);
+    p = fma(p, q, 1. / 13.);
+    p = fma(p, q, 1. / 11.);
+    p = fma(p, q, 1. / 9.);
+    p = fma(p, q, 1. / 7.);
+    p = fma(p, q, 1. / 5.);
+    p = fma(p, q, 1. / 3.);
+    p = fma(p, q, 1.);
+    return fma((double)n, LN2, 2. * z * p);
 }
 
 // A row of logits as vectors of 8 tokens, wherever the row begins (so that equal rows are added up in the same order and give the same bits).
@@ -87,16 +103,22 @@ struct Row {
     int vocab;
     __device__ __forceinline__ Row(const uint16_t* row, int v) : p(row), vocab(v) {}
     __device__ __forceinline__ int vectors() const { return (vocab + 7) / 8; }
-    __device__ __forceinline__ uint4 load(int i) const {
+    // Of these vectors, whole ones at 16-byte boundaries, the first `plain` are.
+    __device__ __forceinline__ int plain() const { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 ? vocab / 8 : 0; }
+    __device__ __forceinline__ uint4 load_plain(int i) const {
+        uint4 x;
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(p + (int64_t)8 * i));
+        return x;
+    }
+    __device__ __forceinline__ uint4 load(int i) const { return i < plain() ? load_plain(i) : load_any(p, vocab, i); }
+    static __device__ __noinline__ uint4 load_any(const uint16_t* p, int vocab, int i) {
         const int off = (int)(reinterpret_cast<uintptr_t>(p) & 15);   // the same for all of the row's vectors
         const uint16_t* const at = p + (int64_t)8 * i;
-        uint4 x;
-        if (off == 0 && 8 * i + 8 <= vocab) {
-            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "l"(at));
-        } else if (off != 0 && i > 0 && 8 * i + 16 - off / 2 <= vocab) {   // two pieces at 16-byte boundaries; the second is the next thread's first
+        uint32_t w[8];
+        if (off != 0 && i > 0 && 8 * i + 16 - off / 2 <= vocab) {   // two pieces at 16-byte boundaries; the second is the next thread's first
             const uint4* const two = reinterpret_cast<const uint4*>(at - off / 2);
             const uint4 a = __ldg(two), b = __ldg(two + 1);
-            uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
             if (off & 8) {
 #pragma unroll
                 for (int j = 0; j < 6; ++j) w[j] = w[j + 2];
@@ -109,203 +131,339 @@ struct Row {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
             }
-            x = make_uint4(w[0], w[1], w[2], w[3]);
         } else {
-            uint32_t w[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int t = 8 * i + 2 * j;
                 w[j] = (t < vocab ? at[2 * j] : 0xFC00u) | (uint32_t)(t + 1 < vocab ? at[2 * j + 1] : 0xFC00u) << 16;
             }
-            x = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        return x;
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
 };
 __device__ __forceinline__ __half2 as_half2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
-__device__ __forceinline__ float most_of(const uint4& x) {
-    const __half2 m = __hmax2(__hmax2(as_half2(x.x), as_half2(x.y)), __hmax2(as_half2(x.z), as_half2(x.w)));
-    return __half2float(__hmax(__low2half(m), __high2half(m)));
+__device__ __forceinline__ __half2 most_of(const uint4& x) { return __hmax2(__hmax2(as_half2(x.x), as_half2(x.y)), __hmax2(as_half2(x.z), as_half2(x.w))); }
+__device__ __forceinline__ __half most_of(__half2 x) { return __hmax(__low2half(x), __high2half(x)); }
+
+struct Part {   // of a segment
+    unsigned key[THREADS];   // of each thread's share: code of its largest value << 16 | 0xFFFF - the vector of the segment where that is first
+    double sum;              // of exponentials behind the segment's largest value
+    unsigned top, unused;    // that value's code
+};
+struct Candidates {   // of a row, the best first
+    Key total[MOST_PICKS];   // order_of; 0: none
+    int token[MOST_PICKS];
+};
+static_assert(sizeof(Part) == BEAM_PART_BYTES && sizeof(Candidates) == BEAM_ROW_BYTES, "workspace");
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d, x = *reinterpret_cast<const uint64_t*>(&a), y = *reinterpret_cast<const uint64_t*>(&b);
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+    return *reinterpret_cast<const float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d, x = *reinterpret_cast<const uint64_t*>(&a), y = *reinterpret_cast<const uint64_t*>(&b);
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
+    return *reinterpret_cast<const float2*>(&d);
 }
 
-struct Part {   // of a segment: the sum of exponentials behind its largest value
-    double sum;
-    unsigned keys[MOST_PICKS];   // code << 16 | 0xFFFF - vector in the segment: its threads' largest values, in order
-};
-static_assert(sizeof(Part) == BEAM_PART_BYTES, "workspace");
+constexpr float LOG2E = 1.4426950408889634f;
 
-__global__ void __launch_bounds__(THREADS) beam_select_kernel(const BeamSelectArgs a) {
-    __shared__ unsigned lists[WARPS][32];
+// 64-bit numbers in order as whole ones, none of them 0; and back
+__device__ __forceinline__ unsigned long long order_of(double t) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(t == 0 ? 0. : t);
+    return u >> 63 ? ~u : u | 1ull << 63;
+}
+__device__ __forceinline__ double total_of(unsigned long long u) { return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u)); }
+
+// Whether this block is the last of `n` to arrive; what all of them have written before is visible to it then.  (Its first warp has written.)
+__device__ __forceinline__ bool last_of(unsigned* counter, unsigned n, volatile int* flag) {
+    if (threadIdx.x < 32) __syncwarp();
+    if (threadIdx.x == 0) {
+        unsigned before;
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+        if (before == n - 1) *counter = 0u;
+        *flag = before == n - 1;
+    }
+    __syncthreads();
+    return *flag != 0;
+}
+
+__global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelectArgs a) {
+    __shared__ __align__(16) Key found[ROOM];
+    __shared__ Key ranked[MOST_PICKS], best[MOST_PICKS];
+    __shared__ unsigned tops[WARPS][TOPS];
     __shared__ double sums[WARPS];
-    __shared__ double totals[MOST_BEAMS][MOST_PICKS];   // of each beam its best candidates, in order
-    __shared__ int tokens[MOST_BEAMS][MOST_PICKS], flag;
+    __shared__ int flag, count;
+    static_assert(sizeof(Candidates) * MOST_BEAMS <= sizeof(found), "room");
     pdl_launch_dependents();
     pdl_wait_prior_grid();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / a.segs, seg = blockIdx.x - row * a.segs, group = row / a.beams;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / a.segs, seg = blockIdx.x - row * a.segs, group = row / a.beams, picks = a.picks;
     // A beam that has ended, or has no score, is not looked at.
-    auto looked_at = [&](int r) { return !(a.done && a.done[r] != 0) && a.score[r] > -INFINITY; };
+    const float score = a.score[row];
+    const bool looked_at = !(a.done && a.done[row] != 0) && score > -INFINITY;
     Part* const parts = reinterpret_cast<Part*>(a.parts);
-    if (looked_at(row)) {
-        const Row x(a.logits + (int64_t)row * a.stride, a.vocab);
-        const int begin = seg * a.per_seg, end = min(x.vectors(), begin + a.per_seg);
-        float most = -INFINITY, sum = 0.f, rest = 0.f;   // (rest: what rounding has taken from the sum)
+    const Row x(a.logits + (int64_t)row * a.stride, a.vocab);
+    if (looked_at) {
+        const int begin = seg * a.per_seg, end = min(x.vectors(), begin + a.per_seg), plain = min(x.plain(), end);
+        __half most = __ushort_as_half(0xFC00);
+        float sum = 0.f, rest = 0.f;   // (rest: what rounding has taken from the sum)
         int at = 0;
+#pragma unroll 1
         for (int i0 = begin + tid; i0 < end; i0 += THREADS * BATCH) {
             uint4 v[BATCH];
+            if (i0 + (BATCH - 1) * THREADS < plain) {
 #pragma unroll
-            for (int j = 0; j < BATCH; ++j) v[j] = i0 + j * THREADS < end ? x.load(i0 + j * THREADS) : make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
-            float m[BATCH];
+                for (int j = 0; j < BATCH; ++j) v[j] = x.load_plain(i0 + j * THREADS);
+            } else {
+#pragma unroll
+                for (int j = 0; j < BATCH; ++j) v[j] = i0 + j * THREADS < end ? x.load(i0 + j * THREADS) : make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
+            }
+            __half2 m[BATCH];
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) m[j] = most_of(v[j]);
-            const float up = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-            if (up > most) {
-                const float f = ex2((most - up) * 1.4426950408889634f);
+            const __half up = most_of(__hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3])));
+            if (__hgt(up, most)) {
+                const float f = ex2((__half2float(most) - __half2float(up)) * LOG2E);
                 sum *= f;
                 rest *= f;
                 most = up;
-#pragma unroll
-                for (int j = BATCH - 1; j >= 0; --j)
-                    if (m[j] == up) at = i0 + j * THREADS - begin;
+                int j = 0;
+                while (j < BATCH - 1 && !__heq(most_of(j == 0 ? m[0] : j == 1 ? m[1] : m[2]), up)) ++j;
+                at = i0 + j * THREADS - begin;
             }
-            const float ref = most == -INFINITY ? 0.f : most;
-            float s[BATCH];
+            const float ref = __heq(most, __ushort_as_half(0xFC00)) ? 0.f : -__half2float(most);
+            float2 s[BATCH];
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
                 const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-                float e[8];
+                float2 e[4];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const float2 y = __half22float2(as_half2(w[q]));
-                    e[2 * q] = ex2((y.x - ref) * 1.4426950408889634f);
-                    e[2 * q + 1] = ex2((y.y - ref) * 1.4426950408889634f);
+                    const float2 t = mul2(add2(__half22float2(as_half2(w[q])), make_float2(ref, ref)), make_float2(LOG2E, LOG2E));
+                    e[q] = make_float2(ex2(t.x), ex2(t.y));
                 }
-                s[j] = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+                s[j] = add2(add2(e[0], e[1]), add2(e[2], e[3]));
             }
-            const float more = (s[0] + s[1]) + (s[2] + s[3]), whole = __fadd_rn(sum, more), back = __fsub_rn(whole, sum);   // the sum's error (D. Knuth, The Art of Computer Programming 2, 4.2.2)
+            const float2 both = add2(add2(s[0], s[1]), add2(s[2], s[3]));
+            // the sum's rounding is kept (D. Knuth, The Art of Computer Programming 2, 4.2.2)
+            const float more = both.x + both.y, whole = __fadd_rn(sum, more), back = __fsub_rn(whole, sum);
             rest += __fadd_rn(__fsub_rn(sum, __fsub_rn(whole, back)), __fsub_rn(more, back));
             sum = whole;
         }
-        const unsigned code = code_of(__half_as_ushort(__float2half_rn(most)));
-        const unsigned list = ordered(code > NO_VALUE ? code << 16 | (0xFFFFu - at) : 0u);
-        lists[warp][lane] = list;
-        __syncthreads();
-        unsigned top = 0;
-#pragma unroll
-        for (int i = 0; i < WARPS; ++i) top = larger(top, lists[i][0]);
-        double mine = 0;
-        if (sum != 0.f) mine = ((double)sum + (double)rest) * exp((double)most - (double)value_of(top >> 16));
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
-        if (lane == 0) sums[warp] = mine;
         Part& part = parts[blockIdx.x];
+        const unsigned code = code_of(__half_as_ushort(most));
+        part.key[tid] = code > NO_VALUE ? code << 16 | (0xFFFFu - at) : 0u;
+        const unsigned warp_top = __reduce_max_sync(0xffffffffu, code);
+        double whole = sum != 0.f ? ((double)sum + (double)rest) * (double)ex2((__half2float(most) - value_of(warp_top)) * LOG2E) : 0.0;
+#pragma unroll 1
+        for (int d = 16; d > 0; d >>= 1) whole += __shfl_xor_sync(0xffffffffu, whole, d);
+        if (lane == 0) {
+            tops[warp][0] = warp_top;
+            sums[warp] = whole;
+        }
+        __threadfence();
+        __syncthreads();
         if (warp == 0) {
-            const unsigned best = merged8<unsigned>([&](int i) { return lists[i][lane]; });
-            if (lane < a.picks) part.keys[lane] = best;
+            const unsigned mine = lane < WARPS ? tops[lane][0] : 0u, top = __reduce_max_sync(0xffffffffu, mine);
+            double s = lane < WARPS ? sums[lane] : 0.0;
+            if (s != 0) s *= (double)ex2((value_of(mine) - value_of(top)) * LOG2E);
+#pragma unroll 1
+            for (int d = WARPS / 2; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+            if (lane == 0) {
+                part.sum = s;
+                part.top = top;
+            }
+        }
+    }
+    // ---- the row's last block: its candidates ----
+    if (a.segs > 1 && !last_of(a.counters + row, a.segs, &flag)) return;
+    if (a.segs == 1) {
+        __threadfence_block();
+        __syncthreads();
+    }
+    Candidates* const rows = reinterpret_cast<Candidates*>(a.rows);
+    Candidates& out = rows[row];
+    if (looked_at) {
+        const Part* const p = parts + (int64_t)row * a.segs;
+        // The best keys so far are found's first ones; what comes next is put behind them.  By all threads: the `picks` largest of all of them, in order.
+        auto settle = [&]() {
+            __syncthreads();
+            const int n = count;
+#pragma unroll 1
+            for (int i = tid; i < n; i += THREADS) {
+                const Key k = found[i];
+                const int place = place_among(found, n, k);
+                if (place < picks) ranked[place] = k;
+            }
+            __syncthreads();
+            if (tid < min(n, picks)) found[tid] = ranked[tid];
+            if (tid == 0) count = min(n, picks);
+            __syncthreads();
+        };
+        constexpr int AHEAD = 6;   // loads in flight; so many keys of each thread may come before the next look at how many there are
+        static_assert(MOST_PICKS + AHEAD * THREADS <= ROOM, "room");
+        // the segments' largest values and sums; each thread's best key
+        unsigned top = 0, top0 = 0;
+        double y0 = 0.;
+        for (int s = lane; s < a.segs; s += 32) {   // (each warp for itself)
+            const unsigned c = __ldcg(&p[s].top);
+            if (s == lane) {
+                top0 = c;
+                y0 = __ldcg(&p[s].sum);
+            }
+            top = max(top, c);
+        }
+        unsigned mine = 0, k[AHEAD];   // (k: of the segments s0 ..)
+        auto keys_from = [&](int s0) {
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) k[j] = s0 + j < a.segs ? __ldcg(&p[s0 + j].key[tid]) : 0u;
+        };
+        const int last = (a.segs - 1) / AHEAD * AHEAD;
+#pragma unroll 1
+        for (int s0 = last; s0 >= 0; s0 -= AHEAD) {
+            keys_from(s0);
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) mine = max(mine, k[j] >> 16);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        const double most = value_of(top);
+        // Twice `picks` of these, a quarter of that many the largest ones of each warp: no share whose code is below the `picks`-th of them can be among the best.
+        const int each = (picks + 3) / 4;
+        unsigned left = mine > NO_VALUE ? mine << 8 | tid : 0u;
+#pragma unroll 1
+        for (int i = 0; i < each; ++i) {
+            const unsigned m = __reduce_max_sync(0xffffffffu, left);
+            if (left == m) left = 0;
+            if (lane == i) tops[warp][i] = m;
+        }
+        if (tid == 0) count = flag = 0;
+        __syncthreads();
+        if (tid < WARPS * TOPS && tid % TOPS < each) {
+            const unsigned my = tops[tid / TOPS][tid % TOPS];
+            int larger = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+                for (int j = 0; j < each; ++j) larger += tops[w][j] > my;
+            if (larger == picks - 1) flag = (int)(my >> 8);   // (one thread's; none where fewer have values)
         }
         __syncthreads();
-        if (tid == 0) {
-            double s = 0;
-#pragma unroll
-            for (int i = 0; i < WARPS; ++i) s += sums[i];
-            part.sum = s;
-        }
-    }
-    // ---- the group's last block has the parts of all of its rows ----
-    __threadfence();
-    __syncthreads();
-    if (tid == 0) {
-        const bool last = atomicAdd(a.counters + group, 1u) == (unsigned)(a.beams * a.segs - 1);
-        if (last) a.counters[group] = 0u;
-        flag = last;
-    }
-    __syncthreads();
-    if (!flag) return;
-    __threadfence();
-    for (int b = warp; b < a.beams; b += WARPS) {
-        const int r = group * a.beams + b;
-        double total = -INFINITY;
-        int token = -1;
-        if (looked_at(r)) {
-            const Row x(a.logits + (int64_t)r * a.stride, a.vocab);
-            const Part* const p = parts + (int64_t)r * a.segs;
-            // the shares with the best values, and the row's largest one
-            using Key = unsigned long long;
-            Key best = 0;
-            for (int s0 = 0; s0 < a.segs; s0 += 8) {
-                const Key more = merged8<Key>([&](int i) {
-                    const int s = s0 + i;
-                    const unsigned k = s < a.segs && lane < a.picks ? __ldcg(&p[s].keys[lane]) : 0u;
-                    return k ? (Key)(k >> 16) << 32 | (0xFFFFFFFFu - (unsigned)(s * a.per_seg + (0xFFFF - (int)(k & 0xFFFFu)))) : (Key)0;
-                });
-                best = s0 ? merged(best, more) : more;
-            }
-            const float most = value_of((unsigned)(__shfl_sync(0xffffffffu, best, 0) >> 32));
-            double sum = 0;
-            for (int s = lane; s < a.segs; s += 32) {
-                const unsigned k = __ldcg(&p[s].keys[0]);
-                const double y = __ldcg(&p[s].sum);
-                if (y != 0) sum += k ? y * exp((double)value_of(k >> 16) - (double)most) : y;
-            }
-#pragma unroll
-            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            if (sum > 0 && sum < INFINITY && most < INFINITY) {
-                // their values that are not below the least of these maxima, one after the other into a list
-                const int shares = __popc(__ballot_sync(0xffffffffu, lane < a.picks && best != 0)), steps = (a.per_seg + THREADS - 1) / THREADS;
-                const unsigned last = (unsigned)(__shfl_sync(0xffffffffu, best, shares - 1) >> 32), least = shares == a.picks ? last : 0u;   // (fewer shares: all of their values)
-                Key list = 0;
-                for (int i0 = 0; i0 < shares * steps; i0 += 32) {
-                    const int i = i0 + lane, from = i / steps;
-                    const int home = (int)(0xFFFFFFFFu - (unsigned)__shfl_sync(0xffffffffu, best, from & 31)), s = home / a.per_seg;
-                    const int vec = s * a.per_seg + (home - s * a.per_seg) % THREADS + (i - from * steps) * THREADS;
-                    const bool there = i < shares * steps && vec < min(x.vectors(), (s + 1) * a.per_seg);
-                    const uint4 v = there ? x.load(vec) : make_uint4(0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u, 0xFC00FC00u);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        Key least = (Key)(unsigned)flag << 32;
 #pragma unroll 1
-                    for (int e = 0; e < 8; ++e) {
-                        const uint32_t two = e < 4 ? e < 2 ? w[0] : w[1] : e < 6 ? w[2] : w[3];
-                        const unsigned code = code_of((uint16_t)(e & 1 ? two >> 16 : two));
-                        const Key key = (Key)code << 32 | (0xFFFFFFFFu - (unsigned)(8 * vec + e));
-                        for (unsigned left = __ballot_sync(0xffffffffu, code >= least && code > NO_VALUE); left; left &= left - 1) {
-                            const Key k = __shfl_sync(0xffffffffu, key, __ffs(left) - 1), before = __shfl_up_sync(0xffffffffu, list, 1);
-                            const int place = __popc(__ballot_sync(0xffffffffu, list > k));
-                            if (lane >= place) list = lane == place ? k : before;
-                        }
-                    }
-                }
-                if (list != 0 && lane < a.picks) {
-                    token = (int)(0xFFFFFFFFu - (unsigned)list);
-                    total = (double)a.score[r] + (((double)value_of((unsigned)(list >> 32)) - (double)most) - log(sum));
-                }
+        for (int s0 = 0; s0 < a.segs; s0 += AHEAD) {
+            if (s0) keys_from(s0);
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const Key key = (Key)(k[j] >> 16) << 32 | (0xFFFFFFFFu - (unsigned)((s0 + j) * a.per_seg + (int)(0xFFFFu - (k[j] & 0xFFFFu))));
+                if (k[j] != 0 && key >= least) found[atomicAdd(&count, 1)] = key;
             }
-        } else if (lane == 0 && a.score[r] > -INFINITY) {   // it has ended
-            total = a.score[r];
-            token = a.eos;
+            if (s0 + AHEAD >= a.segs) break;
+            __syncthreads();
+            if (count > ROOM - AHEAD * THREADS) {   // (equal values)
+                settle();
+                least = found[picks - 1];
+            }
+            __syncthreads();
         }
-        if (lane < a.picks) {
-            totals[b][lane] = total;
-            tokens[b][lane] = token;
+        settle();
+        // The shares' values that are not below the least of the maxima (of fewer shares than picks: all), a value to a thread; and the row's sum.
+        const int shares = count, steps = (a.per_seg + THREADS - 1) / THREADS, values = steps * 8;
+        if (tid < shares) best[tid] = found[tid];
+        least = shares == picks ? found[picks - 1] >> 32 << 32 : (Key)(NO_VALUE + 1) << 32;
+        __syncthreads();
+        if (tid == 0) count = 0;
+        __syncthreads();
+        // (a share to a warp)
+#pragma unroll 1
+        for (int s0 = 0; s0 < shares; s0 += WARPS) {
+            const int first = s0 + warp < shares ? (int)(0xFFFFFFFFu - (unsigned)best[s0 + warp]) : -1, s = first / a.per_seg;
+            const int token0 = 8 * (s * a.per_seg + (first - s * a.per_seg) % THREADS), end = min(a.vocab, 8 * (s + 1) * a.per_seg);
+#pragma unroll 1
+            for (int in0 = lane; in0 - lane < values; in0 += 32 * AHEAD) {
+                int token[AHEAD];
+                uint16_t h[AHEAD];
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const int in = in0 + 32 * j;
+                    token[j] = token0 + in / 8 * (8 * THREADS) + in % 8;
+                    h[j] = first >= 0 && in < values && token[j] < end ? x.p[token[j]] : (uint16_t)0xFC00;
+                }
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) {
+                    const unsigned c = code_of(h[j]);
+                    const Key key = (Key)c << 32 | (0xFFFFFFFFu - (unsigned)token[j]);
+                    if (c > NO_VALUE && key >= least) found[atomicAdd(&count, 1)] = key;
+                }
+                if (s0 + WARPS >= shares && in0 - lane + 32 * AHEAD >= values) break;
+                __syncthreads();
+                if (count > ROOM - AHEAD * THREADS) {   // (equal values)
+                    settle();
+                    least = found[picks - 1];
+                }
+                __syncthreads();
+            }
         }
+        if (warp == WARPS - 1) {
+            double sum = y0 != 0 ? top0 > NO_VALUE ? y0 * exp_of((double)value_of(top0) - most) : y0 : 0.;
+#pragma unroll 1
+            for (int i = lane + 32; i < a.segs; i += 32) {
+                const unsigned c = __ldcg(&p[i].top);
+                const double y = __ldcg(&p[i].sum);
+                if (y != 0) sum += c > NO_VALUE ? y * exp_of((double)value_of(c) - most) : y;
+            }
+#pragma unroll 1
+            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            // (a NaN or an infinity among the values: no candidates)
+            sum = sum > 0 && sum < INFINITY && most < INFINITY ? log_of(sum) : -1.;
+            if (lane == 0) sums[0] = sum;
+        }
+        settle();
+        if (tid < picks) {
+            const double norm = sums[0];
+            const bool there = tid < count && norm >= 0;
+            const Key k = there ? found[tid] : 0;
+            out.total[tid] = there ? order_of((double)score + (((double)value_of((unsigned)(k >> 32)) - most) - norm)) : 0ull;
+            out.token[tid] = (int)(0xFFFFFFFFu - (unsigned)k);
+        }
+    } else if (tid < picks) {   // one candidate of a beam that has ended, none without a score
+        out.total[tid] = tid == 0 && score > -INFINITY ? order_of(score) : 0ull;
+        out.token[tid] = a.eos;
+    }
+    // ---- the group's last block: the beams' lists joined, a beam to a lane ----
+    __syncthreads();   // (picks fit into a warp: the first one has written)
+    if (a.beams > 1 && !last_of(a.counters + MOST_BEAM_ROWS + group, a.beams, &flag)) return;
+    Candidates* const all = reinterpret_cast<Candidates*>(found);
+    {
+        const uint4* const from = reinterpret_cast<const uint4*>(rows + (int64_t)group * a.beams);
+        for (int i = tid; i < a.beams * (int)(sizeof(Candidates) / 16); i += THREADS) reinterpret_cast<uint4*>(all)[i] = __ldcg(from + i);
     }
     __syncthreads();   // (scores and flags have been read: they may be the outputs)
     if (warp != 0) return;
-    // ---- the beams' lists joined: a beam to a lane ----
-    int next = 0;   // candidates of this lane's beam that have been taken
-    for (int p = 0; p < a.picks; ++p) {
-        const bool there = lane < a.beams && next < a.picks && tokens[lane][next] >= 0;
-        double most = there ? totals[lane][next] : -INFINITY;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, d));
-        const unsigned hit = __ballot_sync(0xffffffffu, there && totals[lane][next] == most);
-        const int b = __ffs(hit) - 1;
-        const int64_t o = (int64_t)group * a.picks + p;
-        if (lane == (hit ? b : 0)) {
-            const int token = hit ? tokens[lane][next] : -1;
-            a.out_score[o] = hit ? (float)most : -INFINITY;
-            a.out_token[o] = token;
-            a.out_parent[o] = b;
-            if (a.out_done) a.out_done[o] = hit && token == a.eos;
-            if (hit) ++next;
+    auto candidate = [&](int j) { return lane < a.beams && j < picks ? all[lane].total[j] : 0ull; };
+    int taken = 0, parent = -1, place = 0;
+    Key head = candidate(0), next = candidate(1);
+#pragma unroll 1
+    for (int p = 0; p < picks; ++p) {
+        const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(head >> 32));
+        const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(head >> 32) == high ? (unsigned)head : 0u);
+        if ((high | low) == 0) break;
+        const int b = __ffs(__ballot_sync(0xffffffffu, head == ((Key)high << 32 | low))) - 1;
+        const int j = __shfl_sync(0xffffffffu, taken, b);
+        if (lane == b) {
+            head = next;
+            next = candidate(++taken + 1);
         }
+        if (lane == p) {
+            parent = b;
+            place = j;
+        }
+    }
+    if (lane < picks) {
+        const int64_t o = (int64_t)group * picks + lane;
+        const int token = parent < 0 ? -1 : all[parent].token[place];
+        a.out_score[o] = parent < 0 ? -INFINITY : (float)total_of(all[parent].total[place]);
+        a.out_token[o] = token;
+        a.out_parent[o] = parent;
+        if (a.out_done) a.out_done[o] = token >= 0 && token == a.eos;
     }
 }
 
@@ -326,13 +484,11 @@ cudaError_t launch_beam_select(const BeamSelectArgs& given, int sm_count, cudaSt
     return cudaLaunchKernelEx(&cfg, beam_select_kernel, a);
 }
 
-// Segments of a row: as many as its vectors need at CHUNK to a thread, more where the rows alone would leave SMs idle, but none with less than a vector for
-// each thread.
+// Segments of a row, in whole rounds of loads: of so many that there are some 16 blocks for each SM, and of no more vectors than have numbers of 16 bits.
 void beam_segments(int rows, int vocab, int sm_count, int* segs, int* per_seg) {
-    const int vectors = (vocab + 7) / 8, least = (vectors + THREADS * CHUNK - 1) / (THREADS * CHUNK), most = (vectors + THREADS - 1) / THREADS;
-    int n = sm_count / rows;
-    n = n < least ? least : n > most ? most : n;
-    *per_seg = (vectors + n - 1) / n;
+    const int vectors = (vocab + 7) / 8, round = THREADS * BATCH, rounds = (vectors + round - 1) / round;
+    const long long n = ((long long)rounds * rows + 16 * sm_count - 1) / (16 * sm_count);
+    *per_seg = (int)(n < 64 ? n : 64) * round;
     *segs = (vectors + *per_seg - 1) / *per_seg;
 }
 

@@ -167,6 +167,7 @@ extern "C" int nn_beam_select(nn_context* c, int groups, int beams, int vocab, n
     if (groups < 0 || vocab < 1) return NN_FAIL(NN_ERR_ARG, "%s: groups=%d vocab=%d", who, groups, vocab);
     if (beams < 1 || beams > MOST_BEAMS || picks < 1 || picks > MOST_PICKS)
         return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: beams=%d picks=%d: 1 to %d and 1 to %d", who, beams, picks, MOST_BEAMS, MOST_PICKS);
+    if (vocab > MOST_VOCAB) return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: vocab=%d is more than %d", who, vocab, MOST_VOCAB);
     if ((long long)groups * beams > MOST_BEAM_ROWS) return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: %d groups of %d beams are more than %d rows", who, groups, beams, MOST_BEAM_ROWS);
     if (groups == 0) return make_current(c, nullptr, who);
     if (!logits || !score || !out_score || !out_token || !out_parent) return NN_FAIL(NN_ERR_ARG, "%s: null logits, score, out_score, out_token or out_parent", who);
@@ -187,11 +188,12 @@ extern "C" int nn_beam_select(nn_context* c, int groups, int beams, int vocab, n
     BeamSelectArgs a = {};
     beam_segments((int)rows, vocab, c ? c->sm_count : 1, &a.segs, &a.per_seg);
     if ((long long)rows * a.segs > BEAM_PARTS)
-        return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: %d rows of %d logits are more than %d segments of 16384", who, (int)rows, vocab, BEAM_PARTS);
+        return NN_FAIL(NN_ERR_UNSUPPORTED, "%s: %d rows of %d logits are more than %d segments of 524288", who, (int)rows, vocab, BEAM_PARTS);
     int rc;
     if ((rc = make_current(c, nullptr, who))) return rc;
     a.counters = (unsigned*)c->beam_work;
-    a.parts = (char*)c->beam_work + MOST_BEAM_ROWS * sizeof(unsigned);
+    a.rows = (char*)c->beam_work + BEAM_COUNTER_BYTES;
+    a.parts = (char*)a.rows + MOST_BEAM_ROWS * BEAM_ROW_BYTES;
     a.logits = (const uint16_t*)logits;
     a.stride = stride;
     a.score = (const float*)score;

@@ -50,7 +50,7 @@ struct KvReorderArgs {
 cudaError_t launch_kv_reorder(const KvReorderArgs& a, cudaStream_t st, bool pdl);
 
 // The best continuations of groups of beams.
-constexpr int MOST_PICKS = 32, MOST_BEAM_ROWS = 8192;
+constexpr int MOST_PICKS = 32, MOST_BEAM_ROWS = 8192, MOST_VOCAB = 1 << 26;
 struct BeamSelectArgs {
     const uint16_t* logits;  // [groups * beams][stride]
     int64_t stride;
@@ -62,12 +62,14 @@ struct BeamSelectArgs {
     int* out_done;           // or null
     int groups, beams, vocab, picks, eos;
     int segs, per_seg;       // segments of a row, vectors of 8 values of a segment (set by the launch)
-    unsigned* counters;      // [MOST_BEAM_ROWS], 0 between launches
+    unsigned* counters;      // [2 * MOST_BEAM_ROWS], 0 between launches: of rows, of groups
+    void* rows;              // [MOST_BEAM_ROWS] candidates of rows
     void* parts;             // [BEAM_PARTS] results of segments
 };
-// The workspace, one call at a time: counters, parts.
-constexpr int BEAM_PARTS = 32768;
-constexpr size_t BEAM_PART_BYTES = 8 + 4 * MOST_PICKS, BEAM_WORK_BYTES = MOST_BEAM_ROWS * sizeof(unsigned) + BEAM_PARTS * BEAM_PART_BYTES;
+// The workspace, one call at a time: counters, rows, parts.
+constexpr int BEAM_PARTS = 8192;
+constexpr size_t BEAM_PART_BYTES = 4 * 256 + 16, BEAM_ROW_BYTES = 12 * MOST_PICKS, BEAM_COUNTER_BYTES = 2 * MOST_BEAM_ROWS * sizeof(unsigned),
+                 BEAM_WORK_BYTES = BEAM_COUNTER_BYTES + MOST_BEAM_ROWS * BEAM_ROW_BYTES + BEAM_PARTS * BEAM_PART_BYTES;
 void beam_segments(int rows, int vocab, int sm_count, int* segs, int* per_seg);
 cudaError_t launch_beam_select(const BeamSelectArgs& a, int sm_count, cudaStream_t st, bool pdl);
 

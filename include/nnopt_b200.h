@@ -258,7 +258,8 @@ int nn_attention(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, 
  *                     Logits of -infinity are no candidates, nor are beams whose score is -infinity or a NaN, nor rows with a NaN or +infinity.
  *                     done (int32 [groups][beams], may be NULL): a beam that is not 0 there has ended: it has one candidate, token eos with its score as it
  *                     is, and its logits are not read.  out_done (int32 [groups][picks], may be NULL): 1 where the token is eos.  With picks == beams, out_score may be
- *                     score and out_done may be done.  beams and picks up to 32, groups * beams up to 8192.
+ *                     score and out_done may be done.  beams and picks up to 32, vocab up to 2^26, groups * beams up to 8192
+ *                     and up to 8192 segments of 524288 logits in all.
  *   nn_kv_reorder     every beam takes over its parent's sequence: the batch's sequences are the beams, group after group, all of a group of the same kv_len;
  *                     parent int32 [num_seqs] among the beams of the group (as nn_beam_select gives it with picks == beams; -1: the beam itself).  The page table's entries
  *                     of full pages are taken over in place (it is written); the page that is not full must be each beam's own, and the parent's cells in it are copied to the
