@@ -194,7 +194,7 @@ extern "C" int nn_init(int device, nn_context** out) {
         delete c;
         return NN_FAIL(NN_ERR_CUDA, "nn_init: cudaMalloc failed");
     }
-    if ((e = stream_configure()) != cudaSuccess) {
+    if ((e = stream_configure()) != cudaSuccess || (e = branch_configure()) != cudaSuccess) {
         delete c;
         return NN_FAIL(NN_ERR_CUDA, "nn_init: kernel configuration failed: %s", cudaGetErrorString(e));
     }

@@ -45,8 +45,23 @@ cudaError_t attention_configure() {
 //   20     e4m3 of 128     18.1 / 19.8     42.2 / 34.9      167 / 132
 //   64     fp16 of 64      12.2 / 14.0     30.3 / 22.4      133 / 67
 //   64     int8 of 64      14.9 / 16.7     34.6 / 27.8      159 / 92
+//
+// Trees go by what the first kernel has to read: its items (of 16 rows, all of them to the sequence's end) and their keys.  That one / this one, us:
+//   items   rows   cells           400         2000         8000        32000 positions
+//   4         64   fp16 of 64    8.6 / 13.8   9.0 / 14.2  10.9 / 17.7  14.8 / 36.6
+//   16       105   int8 of 64    8.4 / 15.5  11.1 / 16.7  16.6 / 22.2  36.8 / 33.0
+//   16       105   fp16 of 128   9.5 / 18.9  12.6 / 19.8  21.4 / 24.0  59.4 / 39.5
+//   28        96   e4m3 of 128  10.7 / 17.8  16.0 / 20.2  39.6 / 27.7   134 / 46.9
+//   32        64   fp16 of 64    9.6 / 13.9  12.7 / 15.1  22.2 / 19.5  72.8 / 31.8
+//   64        64   int8 of 64   16.8 / 15.6  19.4 / 17.2  29.7 / 24.6  88.6 / 56.4
 static bool few_rows(const AttnArgs& a, int max_new) {
     const long long rows = (long long)a.group * max_new;
+    if (a.tree && rows > 16) {
+        if (a.group > 16) return false;
+        const int tokens = 16 / a.group;
+        const double items = (double)a.s.num_seqs * a.c.kv_heads * ((max_new + tokens - 1) / tokens);
+        return items <= 32 && items * a.s.max_len <= 1 << 17;
+    }
     if (a.group > 16 || rows > 64) return false;
     if (rows <= 16) return true;
     if (a.c.dim != 64) return false;

@@ -37,6 +37,7 @@ struct KvMoveArgs {
     int* status;
 };
 cudaError_t launch_kv_move(const KvMoveArgs& a, cudaStream_t st, bool pdl);
+cudaError_t branch_configure();   // once for each device
 
 constexpr int MOST_BEAMS = 32;
 struct KvReorderArgs {
