@@ -23,7 +23,7 @@ namespace {
 
 constexpr int THREADS = 256, WARPS = THREADS / 32, BATCH = 4;
 constexpr int TOPS = MOST_PICKS / 4;        // maxima of a warp that are compared with the other warps'
-constexpr int ROOM = 2048;                  // keys that a block compares with one another
+constexpr int ROOM = 3136;                  // keys that a block compares with one another
 constexpr unsigned NO_VALUE = 0x03FFu;      // the code of -infinity
 
 __device__ __forceinline__ float ex2(float x) {
@@ -175,9 +175,9 @@ __device__ __forceinline__ unsigned long long order_of(double t) {
 }
 __device__ __forceinline__ double total_of(unsigned long long u) { return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u)); }
 
-// Whether this block is the last of `n` to arrive; what all of them have written before is visible to it then.  (Its first warp has written.)
+// Whether this block is the last of `n` to arrive; what all of their threads have written before is visible to it then.
 __device__ __forceinline__ bool last_of(unsigned* counter, unsigned n, volatile int* flag) {
-    if (threadIdx.x < 32) __syncwarp();
+    __syncthreads();
     if (threadIdx.x == 0) {
         unsigned before;
         asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
@@ -190,10 +190,11 @@ __device__ __forceinline__ bool last_of(unsigned* counter, unsigned n, volatile 
 
 __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelectArgs a) {
     __shared__ __align__(16) Key found[ROOM];
-    __shared__ Key ranked[MOST_PICKS], best[MOST_PICKS];
-    __shared__ unsigned tops[WARPS][TOPS];
+    __shared__ Key best[MOST_PICKS];
+    __shared__ Key best_of[WARPS * TOPS];
+    __shared__ unsigned tops[WARPS];
     __shared__ double sums[WARPS];
-    __shared__ int flag, count;
+    __shared__ int flag, count, homes[MOST_PICKS];
     static_assert(sizeof(Candidates) * MOST_BEAMS <= sizeof(found), "room");
     pdl_launch_dependents();
     pdl_wait_prior_grid();
@@ -258,13 +259,12 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
 #pragma unroll 1
         for (int d = 16; d > 0; d >>= 1) whole += __shfl_xor_sync(0xffffffffu, whole, d);
         if (lane == 0) {
-            tops[warp][0] = warp_top;
+            tops[warp] = warp_top;
             sums[warp] = whole;
         }
-        __threadfence();
         __syncthreads();
         if (warp == 0) {
-            const unsigned mine = lane < WARPS ? tops[lane][0] : 0u, top = __reduce_max_sync(0xffffffffu, mine);
+            const unsigned mine = lane < WARPS ? tops[lane] : 0u, top = __reduce_max_sync(0xffffffffu, mine);
             double s = lane < WARPS ? sums[lane] : 0.0;
             if (s != 0) s *= (double)ex2((value_of(mine) - value_of(top)) * LOG2E);
 #pragma unroll 1
@@ -276,16 +276,13 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
         }
     }
     // ---- the row's last block: its candidates ----
-    if (a.segs > 1 && !last_of(a.counters + row, a.segs, &flag)) return;
-    if (a.segs == 1) {
-        __threadfence_block();
-        __syncthreads();
-    }
+    if (a.segs == 1) __syncthreads();
+    else if (!last_of(a.counters + row, a.segs, &flag)) return;
     Candidates* const rows = reinterpret_cast<Candidates*>(a.rows);
     Candidates& out = rows[row];
     if (looked_at) {
         const Part* const p = parts + (int64_t)row * a.segs;
-        // The best keys so far are found's first ones; what comes next is put behind them.  By all threads: the `picks` largest of all of them, in order.
+        // By all threads: the `picks` largest keys of those found, in order, and how many there are.
         auto settle = [&]() {
             __syncthreads();
             const int n = count;
@@ -293,38 +290,35 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
             for (int i = tid; i < n; i += THREADS) {
                 const Key k = found[i];
                 const int place = place_among(found, n, k);
-                if (place < picks) ranked[place] = k;
+                if (place < picks) best[place] = k;
             }
             __syncthreads();
-            if (tid < min(n, picks)) found[tid] = ranked[tid];
-            if (tid == 0) count = min(n, picks);
+            return min(n, picks);
+        };
+        // The same where another look might find no room: they are the first ones that are found then.
+        auto make_room = [&]() {
+            const int n = settle();
+            if (tid < n) found[tid] = best[tid];
+            if (tid == 0) count = n;
             __syncthreads();
         };
         constexpr int AHEAD = 6;   // loads in flight; so many keys of each thread may come before the next look at how many there are
-        static_assert(MOST_PICKS + AHEAD * THREADS <= ROOM, "room");
-        // the segments' largest values and sums; each thread's best key
-        unsigned top = 0, top0 = 0;
-        double y0 = 0.;
-        for (int s = lane; s < a.segs; s += 32) {   // (each warp for itself)
-            const unsigned c = __ldcg(&p[s].top);
-            if (s == lane) {
-                top0 = c;
-                y0 = __ldcg(&p[s].sum);
-            }
-            top = max(top, c);
-        }
+        static_assert(MOST_PICKS + 2 * AHEAD * THREADS <= ROOM, "room");
+        // each thread's best key; the segments' largest values and sums
         unsigned mine = 0, k[AHEAD];   // (k: of the segments s0 ..)
         auto keys_from = [&](int s0) {
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) k[j] = s0 + j < a.segs ? __ldcg(&p[s0 + j].key[tid]) : 0u;
         };
-        const int last = (a.segs - 1) / AHEAD * AHEAD;
-#pragma unroll 1
-        for (int s0 = last; s0 >= 0; s0 -= AHEAD) {
-            keys_from(s0);
+        keys_from(0);
+        unsigned top = lane < a.segs ? __ldcg(&p[lane].top) : 0u;
+        const unsigned top0 = top;
+        const double y0 = lane < a.segs ? __ldcg(&p[lane].sum) : 0.;
+        for (int s = lane + 32; s < a.segs; s += 32) top = max(top, __ldcg(&p[s].top));   // (each warp for itself)
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) mine = max(mine, k[j] >> 16);
-        }
+        for (int j = 0; j < AHEAD; ++j) mine = max(mine, k[j] >> 16);
+#pragma unroll 4
+        for (int s = AHEAD; s < a.segs; ++s) mine = max(mine, __ldcg(&p[s].key[tid]) >> 16);
         top = __reduce_max_sync(0xffffffffu, top);
         const double most = value_of(top);
         // Twice `picks` of these, a quarter of that many the largest ones of each warp: no share whose code is below the `picks`-th of them can be among the best.
@@ -334,18 +328,11 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
         for (int i = 0; i < each; ++i) {
             const unsigned m = __reduce_max_sync(0xffffffffu, left);
             if (left == m) left = 0;
-            if (lane == i) tops[warp][i] = m;
+            if (lane == i) best_of[warp * each + i] = m;
         }
         if (tid == 0) count = flag = 0;
         __syncthreads();
-        if (tid < WARPS * TOPS && tid % TOPS < each) {
-            const unsigned my = tops[tid / TOPS][tid % TOPS];
-            int larger = 0;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w)
-                for (int j = 0; j < each; ++j) larger += tops[w][j] > my;
-            if (larger == picks - 1) flag = (int)(my >> 8);   // (one thread's; none where fewer have values)
-        }
+        if (tid < WARPS * each && place_among(best_of, WARPS * each, best_of[tid]) == picks - 1) flag = (int)(best_of[tid] >> 8);   // (one thread's; none where fewer have values)
         __syncthreads();
         Key least = (Key)(unsigned)flag << 32;
 #pragma unroll 1
@@ -359,72 +346,82 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
             if (s0 + AHEAD >= a.segs) break;
             __syncthreads();
             if (count > ROOM - AHEAD * THREADS) {   // (equal values)
-                settle();
-                least = found[picks - 1];
+                make_room();
+                least = best[picks - 1];
             }
             __syncthreads();
         }
-        settle();
         // The shares' values that are not below the least of the maxima (of fewer shares than picks: all), a value to a thread; and the row's sum.
-        const int shares = count, steps = (a.per_seg + THREADS - 1) / THREADS, values = steps * 8;
-        if (tid < shares) best[tid] = found[tid];
-        least = shares == picks ? found[picks - 1] >> 32 << 32 : (Key)(NO_VALUE + 1) << 32;
+        const int shares = settle(), steps = (a.per_seg + THREADS - 1) / THREADS, values = steps * 8;
+        least = shares == picks ? best[picks - 1] >> 32 << 32 : (Key)(NO_VALUE + 1) << 32;
+        if (tid == 0) {
+            count = 0;
+            sums[0] = -1.;   // (without shares there are no candidates)
+        }
+        if (tid < shares) homes[tid] = (int)(0xFFFFFFFFu - (unsigned)best[tid]);
         __syncthreads();
-        if (tid == 0) count = 0;
-        __syncthreads();
-        // (a share to a warp)
+        // (two shares to a warp at a time)
+        int home[2], stop[2] = {0, 0};
 #pragma unroll 1
-        for (int s0 = 0; s0 < shares; s0 += WARPS) {
-            const int first = s0 + warp < shares ? (int)(0xFFFFFFFFu - (unsigned)best[s0 + warp]) : -1, s = first / a.per_seg;
-            const int token0 = 8 * (s * a.per_seg + (first - s * a.per_seg) % THREADS), end = min(a.vocab, 8 * (s + 1) * a.per_seg);
+        for (int s0 = 0; s0 < shares; s0 += 2 * WARPS) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int share = s0 + q * WARPS + warp;
+                home[q] = -1;
+                if (share < shares) {
+                    const int first = homes[share], s = first / a.per_seg;
+                    home[q] = 8 * (s * a.per_seg + (first - s * a.per_seg) % THREADS);
+                    stop[q] = min(a.vocab, 8 * (s + 1) * a.per_seg);
+                }
+            }
 #pragma unroll 1
             for (int in0 = lane; in0 - lane < values; in0 += 32 * AHEAD) {
-                int token[AHEAD];
-                uint16_t h[AHEAD];
+                uint16_t h[2][AHEAD];
+                auto token_of = [&](int q, int j) { return home[q] + (in0 + 32 * j) / 8 * (8 * THREADS) + (in0 + 32 * j) % 8; };
 #pragma unroll
-                for (int j = 0; j < AHEAD; ++j) {
-                    const int in = in0 + 32 * j;
-                    token[j] = token0 + in / 8 * (8 * THREADS) + in % 8;
-                    h[j] = first >= 0 && in < values && token[j] < end ? x.p[token[j]] : (uint16_t)0xFC00;
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int j = 0; j < AHEAD; ++j) h[q][j] = home[q] >= 0 && in0 + 32 * j < values && token_of(q, j) < stop[q] ? x.p[token_of(q, j)] : (uint16_t)0xFC00;
+                if (warp == WARPS - 1 && s0 == 0 && in0 == lane) {   // meanwhile the last warp has the row's sum
+                    double sum = y0 != 0 ? top0 > NO_VALUE ? y0 * exp_of((double)value_of(top0) - most) : y0 : 0.;
+#pragma unroll 1
+                    for (int i = lane + 32; i < a.segs; i += 32) {
+                        const unsigned c = __ldcg(&p[i].top);
+                        const double y = __ldcg(&p[i].sum);
+                        if (y != 0) sum += c > NO_VALUE ? y * exp_of((double)value_of(c) - most) : y;
+                    }
+#pragma unroll 1
+                    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+                    // (a NaN or an infinity among the values: no candidates)
+                    sum = sum > 0 && sum < INFINITY && most < INFINITY ? log_of(sum) : -1.;
+                    if (lane == 0) sums[0] = sum;
                 }
 #pragma unroll
-                for (int j = 0; j < AHEAD; ++j) {
-                    const unsigned c = code_of(h[j]);
-                    const Key key = (Key)c << 32 | (0xFFFFFFFFu - (unsigned)token[j]);
-                    if (c > NO_VALUE && key >= least) found[atomicAdd(&count, 1)] = key;
-                }
-                if (s0 + WARPS >= shares && in0 - lane + 32 * AHEAD >= values) break;
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int j = 0; j < AHEAD; ++j) {
+                        const unsigned c = code_of(h[q][j]);
+                        const Key key = (Key)c << 32 | (0xFFFFFFFFu - (unsigned)token_of(q, j));
+                        if (c > NO_VALUE && key >= least) found[atomicAdd(&count, 1)] = key;
+                    }
+                if (s0 + 2 * WARPS >= shares && in0 - lane + 32 * AHEAD >= values) break;
                 __syncthreads();
-                if (count > ROOM - AHEAD * THREADS) {   // (equal values)
-                    settle();
-                    least = found[picks - 1];
+                if (count > ROOM - 2 * AHEAD * THREADS) {   // (equal values)
+                    make_room();
+                    least = best[picks - 1];
                 }
                 __syncthreads();
             }
         }
-        if (warp == WARPS - 1) {
-            double sum = y0 != 0 ? top0 > NO_VALUE ? y0 * exp_of((double)value_of(top0) - most) : y0 : 0.;
-#pragma unroll 1
-            for (int i = lane + 32; i < a.segs; i += 32) {
-                const unsigned c = __ldcg(&p[i].top);
-                const double y = __ldcg(&p[i].sum);
-                if (y != 0) sum += c > NO_VALUE ? y * exp_of((double)value_of(c) - most) : y;
-            }
-#pragma unroll 1
-            for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            // (a NaN or an infinity among the values: no candidates)
-            sum = sum > 0 && sum < INFINITY && most < INFINITY ? log_of(sum) : -1.;
-            if (lane == 0) sums[0] = sum;
-        }
-        settle();
-        if (tid < picks) {
+        const int n = settle();
+        if (tid < MOST_PICKS) {
             const double norm = sums[0];
-            const bool there = tid < count && norm >= 0;
-            const Key k = there ? found[tid] : 0;
+            const bool there = tid < n && norm >= 0;
+            const Key k = there ? best[tid] : 0;
             out.total[tid] = there ? order_of((double)score + (((double)value_of((unsigned)(k >> 32)) - most) - norm)) : 0ull;
             out.token[tid] = (int)(0xFFFFFFFFu - (unsigned)k);
         }
-    } else if (tid < picks) {   // one candidate of a beam that has ended, none without a score
+    } else if (tid < MOST_PICKS) {   // one candidate of a beam that has ended, none without a score
         out.total[tid] = tid == 0 && score > -INFINITY ? order_of(score) : 0ull;
         out.token[tid] = a.eos;
     }
@@ -437,33 +434,46 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
         for (int i = tid; i < a.beams * (int)(sizeof(Candidates) / 16); i += THREADS) reinterpret_cast<uint4*>(all)[i] = __ldcg(from + i);
     }
     __syncthreads();   // (scores and flags have been read: they may be the outputs)
-    if (warp != 0) return;
-    auto candidate = [&](int j) { return lane < a.beams && j < picks ? all[lane].total[j] : 0ull; };
-    int taken = 0, parent = -1, place = 0;
-    Key head = candidate(0), next = candidate(1);
+    // A candidate's place: its own beam's before it, and of each other beam those that come before it.
+    int there = 0;
 #pragma unroll 1
-    for (int p = 0; p < picks; ++p) {
-        const unsigned high = __reduce_max_sync(0xffffffffu, (unsigned)(head >> 32));
-        const unsigned low = __reduce_max_sync(0xffffffffu, (unsigned)(head >> 32) == high ? (unsigned)head : 0u);
-        if ((high | low) == 0) break;
-        const int b = __ffs(__ballot_sync(0xffffffffu, head == ((Key)high << 32 | low))) - 1;
-        const int j = __shfl_sync(0xffffffffu, taken, b);
-        if (lane == b) {
-            head = next;
-            next = candidate(++taken + 1);
+    for (int i = tid; i < a.beams * picks; i += THREADS) {
+        const int b = i / picks, j = i - b * picks;
+        const Key mine = all[b].total[j];
+        if (mine == 0) continue;
+        ++there;
+        int place = j;
+#pragma unroll 2
+        for (int c = 0; c < a.beams; ++c) {
+            const Key* const list = all[c].total;
+            int before = 0;
+#pragma unroll
+            for (int step = MOST_PICKS / 2; step > 0; step >>= 1) {
+                const Key k = list[before + step - 1];
+                if (k > mine || (k == mine && c < b)) before += step;
+            }
+            const Key k = list[before];
+            before += k > mine || (k == mine && c < b);
+            place += c == b ? 0 : before;
         }
-        if (lane == p) {
-            parent = b;
-            place = j;
+        if (place < picks) {
+            const int64_t o = (int64_t)group * picks + place;
+            const int token = all[b].token[j];
+            a.out_score[o] = (float)total_of(mine);
+            a.out_token[o] = token;
+            a.out_parent[o] = b;
+            if (a.out_done) a.out_done[o] = token == a.eos;
         }
     }
-    if (lane < picks) {
-        const int64_t o = (int64_t)group * picks + lane;
-        const int token = parent < 0 ? -1 : all[parent].token[place];
-        a.out_score[o] = parent < 0 ? -INFINITY : (float)total_of(all[parent].total[place]);
-        a.out_token[o] = token;
-        a.out_parent[o] = parent;
-        if (a.out_done) a.out_done[o] = token >= 0 && token == a.eos;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    if (there) atomicAdd(&count, there);
+    __syncthreads();
+    if (tid >= count && tid < picks) {   // no more candidates
+        const int64_t o = (int64_t)group * picks + tid;
+        a.out_score[o] = -INFINITY;
+        a.out_token[o] = a.out_parent[o] = -1;
+        if (a.out_done) a.out_done[o] = 0;
     }
 }
 
