@@ -34,6 +34,22 @@ cudaError_t attention_configure() {
     return e != cudaSuccess ? e : attention_chunk_configure();
 }
 
+// Trees whose cells the kernel for few rows can read again and again: in items of 8 rows (its form of 16 rows needs more registers than it has), all of them to
+// the sequence's end.  That kernel with 8 rows / with 16 / the kernel for many rows, us, by the items of 16 rows that there would be:
+//   items   rows   cells               400                2000                8000           32000 positions
+//   4         64   fp16 of 64     8.2 / 10.3 / 13.8   9.0 / 11.1 / 14.2  10.9 / 14.1 / 17.7   14.8 /    / 36.6
+//   16       105   int8 of 64     8.4 / 10.6 / 15.5  11.0 / 13.4 / 16.7  16.6 / 18.2 / 22.2   36.8 /    / 33.0
+//   16       105   fp16 of 128    9.5 / 14.7 / 18.9  12.6 / 18.4 / 19.8  21.4 / 27.1 / 24.0   59.4 /    / 39.5
+//   28        96   e4m3 of 128   10.7 / 18.2 / 17.8  15.9 / 21.1 / 20.2  39.7 / 33.3 / 27.7    134 /    / 46.9
+//   32        64   fp16 of 64     9.5 / 10.6 / 13.9  12.8 / 12.7 / 15.1  22.1 / 17.9 / 19.5   72.8 /    / 31.8
+//   64        64   int8 of 64    16.8 / 11.3 / 15.6  19.3 / 17.5 / 17.2  29.8 / 30.4 / 24.6   88.6 /    / 56.4
+bool small_tree(const AttnArgs& a, int max_new) {
+    if (!a.tree || a.group > 8) return false;
+    const int tokens = 16 / a.group;
+    const double items = (double)a.s.num_seqs * a.c.kv_heads * ((max_new + tokens - 1) / tokens);
+    return items <= 32 && items * a.s.max_len <= 1 << 17;
+}
+
 // Few rows to a cache head go to the kernel that reads the cache once for every 16 of them, more to the one that reads it once for 256 but starts
 // slower and, with codes, expands them first.  That one / this one, us, 4 cache heads:
 //   rows   cells            1 x 2048        8 x 4096        32 x 8192 positions
@@ -45,23 +61,9 @@ cudaError_t attention_configure() {
 //   20     e4m3 of 128     18.1 / 19.8     42.2 / 34.9      167 / 132
 //   64     fp16 of 64      12.2 / 14.0     30.3 / 22.4      133 / 67
 //   64     int8 of 64      14.9 / 16.7     34.6 / 27.8      159 / 92
-//
-// Trees go by what the first kernel has to read: its items (of 16 rows, all of them to the sequence's end) and their keys.  That one / this one, us:
-//   items   rows   cells           400         2000         8000        32000 positions
-//   4         64   fp16 of 64    8.6 / 13.8   9.0 / 14.2  10.9 / 17.7  14.8 / 36.6
-//   16       105   int8 of 64    8.4 / 15.5  11.1 / 16.7  16.6 / 22.2  36.8 / 33.0
-//   16       105   fp16 of 128   9.5 / 18.9  12.6 / 19.8  21.4 / 24.0  59.4 / 39.5
-//   28        96   e4m3 of 128  10.7 / 17.8  16.0 / 20.2  39.6 / 27.7   134 / 46.9
-//   32        64   fp16 of 64    9.6 / 13.9  12.7 / 15.1  22.2 / 19.5  72.8 / 31.8
-//   64        64   int8 of 64   16.8 / 15.6  19.4 / 17.2  29.7 / 24.6  88.6 / 56.4
 static bool few_rows(const AttnArgs& a, int max_new) {
     const long long rows = (long long)a.group * max_new;
-    if (a.tree && rows > 16) {
-        if (a.group > 16) return false;
-        const int tokens = 16 / a.group;
-        const double items = (double)a.s.num_seqs * a.c.kv_heads * ((max_new + tokens - 1) / tokens);
-        return items <= 32 && items * a.s.max_len <= 1 << 17;
-    }
+    if (a.tree && rows > 16) return small_tree(a, max_new);
     if (a.group > 16 || rows > 64) return false;
     if (rows <= 16) return true;
     if (a.c.dim != 64) return false;

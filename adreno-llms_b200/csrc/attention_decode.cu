@@ -612,7 +612,7 @@ cudaError_t attention_decode_configure() {
 int attention_decode_keys(int fmt, int dim) { return PART / (dim * kv_cell_bytes(fmt)); }
 
 cudaError_t launch_attention_decode(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl) {
-    const bool one = (long long)a.group * max_new <= 8;   // one tile of 8 rows
+    const bool one = (long long)a.group * max_new <= 8 || small_tree(a, max_new);   // one tile of 8 rows
     const bool tree = a.tree != nullptr;
     auto k = a.c.fmt == KV_FP16 ? (a.c.dim == 64 ? kernel<KV_FP16, 64>(one, tree) : kernel<KV_FP16, 128>(one, tree))
              : a.c.fmt == KV_INT8 ? (a.c.dim == 64 ? kernel<KV_INT8, 64>(one, tree) : kernel<KV_INT8, 128>(one, tree))

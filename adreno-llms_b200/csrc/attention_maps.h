@@ -15,6 +15,7 @@ struct AttnMaps {
 };
 bool encode_attention_maps(const KvView& c, AttnMaps* maps);
 
+bool small_tree(const AttnArgs& a, int max_new);
 int attention_decode_keys(int fmt, int dim);   // keys of a stage: what a copy takes, if a page is that long
 cudaError_t attention_decode_configure();
 cudaError_t launch_attention_decode(const AttnArgs& a, const AttnMaps& maps, int max_new, int sm_count, cudaStream_t st, bool pdl);
