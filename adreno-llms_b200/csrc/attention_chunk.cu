@@ -286,6 +286,7 @@ __global__ void __launch_bounds__(Chunk<FMT, D>::THREADS, 1) attention_chunk_ker
     w.sinks = a.sinks;
     w.tree_words = TREE ? a.tree_words : 0;
     w.extra = ATTN_CHUNK_EXTRA;
+    w.second = TREE ? 2 * ATTN_CHUNK_EXTRA : 0;   // (other calls keep the order of sums that they have had)
     Steps& steps = reinterpret_cast<Steps*>(smem + C::O_WALK)[warp];
     Segment& sg = steps.sg;
     {

@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(THREADS, 1) attention_decode_kernel(const __gr
     w.sinks = a.sinks;
     w.tree_words = TREE ? a.tree_words : 0;
     w.extra = ATTN_DECODE_EXTRA;
+    w.second = 0;
     Walk walk = find_work(a.s, &w, WARPS, a.status);
     if (walk.u >= walk.end) return;
 

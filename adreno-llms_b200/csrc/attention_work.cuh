@@ -24,6 +24,7 @@ struct WorkShape {
     int window, sinks;
     int tree_words;   // of a row's mask; 0: no tree.  With a tree every item sees keys up to the sequence's last one, and there is no window
     unsigned extra;   // units of an item besides its key tiles
+    unsigned second;  // what a second segment costs a block, in units; 0: not looked at
     unsigned chunk;   // units of a block, and whether items are filled up to it
     bool pad;
     __device__ __forceinline__ unsigned units(unsigned tiles) const { return pad ? (tiles + chunk - 1) / chunk * chunk : tiles + extra; }
@@ -165,6 +166,9 @@ __device__ __forceinline__ Walk find_work(const KvSeqs& s, WorkShape* w, unsigne
     total *= w->vheads;
     items *= w->vheads;
     w->pad = 2 * items <= gridDim.x;
+    // Where items are long, filling them up costs more than a second segment (a tree of 64 tokens over 17000 to 33000 positions of each of 8 sequences, 32 heads to 8
+    // of 128 dims: fp16 278 us filled up, 203 not; e4m3 427 and 264; over 4400 to 8200 positions 86 and 69).
+    if (w->second && w->pad) w->pad = (total + gridDim.x - items - 1) / (gridDim.x - items) <= (total + items * extra) / gridDim.x + w->second;
     const unsigned blocks = w->pad ? gridDim.x - items : gridDim.x;   // (filled up, items take up to one more block each)
     if (!w->pad) {
         w->extra = extra;
