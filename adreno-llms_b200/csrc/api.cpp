@@ -248,9 +248,9 @@ extern "C" int nn_sync(nn_context* c) {
         cudaMemsetAsync(c->sk_flags, 0, SK_MAX_BLOCKS * sizeof(unsigned), c->stream);
         if (c->attn_work) cudaMemsetAsync(c->attn_work, 0, ATTN_COUNTER_BYTES, c->stream);
         return NN_FAIL(NN_ERR_TIMEOUT, "a device-side bounded wait ran out (status %d); results of the last calls are invalid%s", s,
-                       bad_table ? " (and a page number, length or position of a key/value batch was out of range)" : "");
+                       bad_table ? " (and a page number, length, position or parent of a key/value batch was out of range)" : "");
     }
-    if (bad_table) return NN_FAIL(NN_ERR_ARG, "a page number, length or position of a key/value batch was out of range; the rows and keys it concerned were left out");
+    if (bad_table) return NN_FAIL(NN_ERR_ARG, "a page number, length, position or parent of a key/value batch was out of range; the rows and keys it concerned were left out");
     return NN_OK;
 }
 

@@ -60,7 +60,7 @@ const char* nn_version(void);
 int nn_init(int device_ordinal, nn_context** out_ctx);
 int nn_shutdown(nn_context* ctx); /* frees registry entries and library-owned buffers */
 void* nn_stream(nn_context* ctx); /* the cudaStream_t every call is ordered on */
-int nn_sync(nn_context* ctx);     /* host wait; also reports a recorded device-side timeout, or a bad page or length of a key/value batch */
+int nn_sync(nn_context* ctx);     /* host wait; also reports a recorded device-side timeout, or a bad page, length or parent of a key/value batch */
 int nn_device_info(nn_context* ctx, int* sm_count, size_t* l2_bytes, size_t* hbm_bytes);
 
 /* ---- buffers: clCreateBuffer / clEnqueueWriteBuffer / clEnqueueReadBuffer /
@@ -238,6 +238,7 @@ int nn_attention(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, 
  *   nn_tree_layout    the new rows of each sequence are a drafted tree: parent int32 [num_rows] is a row's parent as an index among its sequence's new
  *                     rows (below its own; -1: it follows the sequence before the draft).  mask uint32 [num_rows][mask_words] gets bit j for new row j where
  *                     that is the row itself or an ancestor, position int32 [num_rows] the row's place behind the sequence, kv_len - (new rows) + depth.
+ *                     A parent out of range counts as -1 and is reported; sequences with more new rows than positions or than a mask has bits are left out.
  *                     mask_words 1 to 32, with a bit for each of max_new rows.  Of the batch row_start and kv_len are used.  Once a step: all layers share
  *                     them.  (A program whose trees are always the same may keep the mask.)
  *   nn_rope_kv_write_at  nn_rope_kv_write with queries and keys rotated to position[row] (int32 [num_rows], below table_len) instead of the cell's own
@@ -254,7 +255,9 @@ int nn_attention(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, 
  *   nn_beam_select    of `groups` groups of `beams` beams each the `picks` best continuations: total = score[beam] + log_softmax(logits[beam])[token], from
  *                     fp16 logits [groups * beams][logits_stride] (0: dense) of `vocab` tokens and fp32 scores [groups][beams], in descending order; of equal
  *                     ones the lowest beam, then the lowest token first.  out_score fp32, out_token and out_parent (the beam) int32, [groups][picks]; where a
- *                     group has fewer candidates the rest are -infinity, -1, -1.  Totals are compared in 64 bits and rounded to fp32 for out_score.
+ *                     group has fewer candidates the rest are -infinity, -1, -1.  Totals are compared in 64 bits and rounded to fp32 for out_score; the exponentials
+ *                     behind them have 32 bits, so that totals of different beams which are nearer than 2^-20 may come in either order (rows that are equal, or shifted
+ *                     against each other by a constant, give the same logarithms).
  *                     Logits of -infinity are no candidates, nor are beams whose score is -infinity or a NaN, nor rows with a NaN or +infinity.
  *                     done (int32 [groups][beams], may be NULL): a beam that is not 0 there has ended: it has one candidate, token eos with its score as it
  *                     is, and its logits are not read.  out_done (int32 [groups][picks], may be NULL): 1 where the token is eos.  With picks == beams, out_score may be

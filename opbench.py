@@ -1,5 +1,7 @@
 """Time one operator on one GPU:  python opbench.py --fmt q4 --n 28672 --k 8192 --m 1
                                 python opbench.py --op attention --cache int8 --seqs 16 --new 1 --len 4096 --heads 16 --kv-heads 8 --dim 64
+                                python opbench.py --op attention_tree --cache fp8 --seqs 8 --new 64 --len 8192 --heads 32 --kv-heads 8 --dim 128
+                                python opbench.py --op beam_select --seqs 64 --beams 8 --picks 16 --vocab 151936
 
 Prints one JSON line: microseconds per launch (CUDA events around `reps` back-to-back launches
 that rotate through enough weight copies to exceed L2), algorithmic GB/s and TFLOP/s.  Weights are
@@ -55,11 +57,25 @@ def cache_op(pkg, ctx, args, l2, rng):
     seen = [min(p + 1, args.window) + min(args.sinks, max(0, p + 1 - args.window)) if args.window else p + 1 for p in range(ln - n, ln)]
     keys = min(ln, args.window + n - 1 + args.sinks) if args.window else ln
     cell_row = D * eb + (2 if scaled else 0)
+    # drafted trees of two branches to a token; rows that move up over as many others; beams of which the odd ones take over their neighbours' sequences
+    tree = [(1 << j) | (1 << j // 2) | 1 for j in range(n)] if args.op == "attention_tree" else []
+    words = -(-n // 32)
+    mask = up(np.tile(np.array([[m >> 32 * w & 0xFFFFFFFF for w in range(words)] for m in tree], np.uint32).reshape(-1), S)) if tree else None
+    source = up(np.tile(np.arange(ln - n, ln, dtype=np.int32), S))
+    parent = up((np.arange(S, dtype=np.int32) % args.beams) & ~1)
+    if args.op == "kv_move":
+        b.kv_len = up(np.full(S, max(n, ln - n), np.int32))
 
     def run(i):
         c = caches[i % copies]
         if args.op == "attention":
             ctx.attention(c, b, hq, q, 0, out, 0, D ** -0.5, args.window, args.sinks)
+        elif args.op == "attention_tree":
+            ctx.attention_tree(c, b, hq, q, 0, out, 0, D ** -0.5, words, mask)
+        elif args.op == "kv_move":
+            ctx.kv_move([c], b, source)
+        elif args.op == "kv_reorder":
+            ctx.kv_reorder([c], b, args.beams, parent)
         elif args.op == "kv_write":
             ctx.rope_kv_write(c, b, cos, sin, ln, D, hq, q, 0, out, 0, rows[0], 0, rows[1], 0)
         else:
@@ -77,13 +93,42 @@ def cache_op(pkg, ctx, args, l2, rng):
     us = ctx.elapsed_ms(e0, e1) * 1e3 / args.reps
     ctx.sync()
     moved = {"attention": S * 2 * hk * keys * cell_row + 4 * S * n * hq * D, "kv_write": S * n * (2 * hk * (cell_row + 2 * D) + 4 * hq * D + 4 * D),
-             "kv_read": S * n * 2 * hk * (cell_row + 2 * D)}[args.op]
-    flops = 4.0 * S * hq * D * sum(seen) if args.op == "attention" else 0.0
+             "kv_read": S * n * 2 * hk * (cell_row + 2 * D), "attention_tree": S * 2 * hk * ln * cell_row + 4 * S * n * hq * D,
+             "kv_move": S * n * 4 * hk * cell_row, "kv_reorder": (S // 2) * (8 * (ln // P) + (ln % P) * 4 * hk * cell_row)}[args.op]
+    flops = 4.0 * S * hq * D * sum(seen) if args.op == "attention" else 4.0 * S * hq * D * n * (ln - n + 1) if args.op == "attention_tree" else 0.0
     print(json.dumps({"op": args.op, "cache": args.cache, "seqs": S, "new": n, "len": ln, "heads": hq, "kv_heads": hk, "dim": D, "page": P, "window": args.window,
                       "sinks": args.sinks, "us_per_call": round(us, 3), "algorithmic_bytes": moved, "gbps": round(moved / (us * 1e-6) / 1e9, 1),
                       "tflops": round(flops / (us * 1e-6) / 1e12, 2), "kernels_per_call": (ctx.launch_count() - l0) / args.reps, "caches": copies}), flush=True)
     for c in caches:
         c.close()
+    ctx.close()
+    return 0
+
+
+def beam_op(ctx, args, l2, rng):
+    """The selection of each group's best continuations, rotating through enough logits to exceed the L2."""
+    G, B, V, n = args.seqs, args.beams, args.vocab, args.picks
+    nbytes = 2 * G * B * V
+    copies = args.copies if args.copies > 0 else int(max(1, min(64, -(-2 * l2 // nbytes) + 1)))
+    logits = [ctx.upload((rng.standard_normal((G * B, V)) * 2.5).astype(np.float16)) for _ in range(copies)]
+    score = ctx.upload(-np.cumsum(rng.random((G, B)), axis=1).astype(np.float32))
+    outs = [ctx.alloc(4 * G * n) for _ in range(3)]
+
+    def run(i):
+        ctx.beam_select(G, B, V, logits[i % copies], 0, score, None, -1, n, *outs, None)
+
+    for i in range(args.warmup):
+        run(i)
+    e0, e1 = ctx.event(), ctx.event()
+    ctx.sync()
+    ctx.record(e0)
+    for i in range(args.reps):
+        run(i)
+    ctx.record(e1)
+    us = ctx.elapsed_ms(e0, e1) * 1e3 / args.reps
+    ctx.sync()
+    print(json.dumps({"op": args.op, "groups": G, "beams": B, "vocab": V, "picks": n, "us_per_call": round(us, 3), "algorithmic_bytes": nbytes,
+                      "gbps": round(nbytes / (us * 1e-6) / 1e9, 1), "copies": copies}), flush=True)
     ctx.close()
     return 0
 
@@ -94,9 +139,12 @@ def main():
     ap.add_argument("--n", type=int, default=151936)
     ap.add_argument("--k", type=int, default=896)
     ap.add_argument("--m", type=int, default=1)
-    ap.add_argument("--op", default="linear", choices=["linear", "add", "swiglu", "kv_write", "kv_read", "attention"])
+    ap.add_argument("--op", default="linear", choices=["linear", "add", "swiglu", "kv_write", "kv_read", "attention", "attention_tree", "kv_move", "kv_reorder", "beam_select"])
     ap.add_argument("--cache", default="fp16", choices=["fp16", "int8", "fp8"], help="cells of the key/value cache")
-    ap.add_argument("--seqs", type=int, default=1)
+    ap.add_argument("--seqs", type=int, default=1, help="sequences (kv_reorder: all beams of all groups; beam_select: groups)")
+    ap.add_argument("--beams", type=int, default=4)
+    ap.add_argument("--picks", type=int, default=4)
+    ap.add_argument("--vocab", type=int, default=49152)
     ap.add_argument("--new", type=int, default=1, help="new tokens of each sequence")
     ap.add_argument("--len", type=int, default=4096, help="positions of each sequence, the new tokens included")
     ap.add_argument("--heads", type=int, default=16)
@@ -115,7 +163,9 @@ def main():
     ctx = pkg.Context(args.device)
     _, l2, _ = ctx.device_info()
     rng = np.random.default_rng(1)
-    if args.op in ("kv_write", "kv_read", "attention"):
+    if args.op == "beam_select":
+        return beam_op(ctx, args, l2, rng)
+    if args.op in ("kv_write", "kv_read", "attention", "attention_tree", "kv_move", "kv_reorder"):
         return cache_op(pkg, ctx, args, l2, rng)
     fmt, N, K, M = args.fmt, args.n, args.k, args.m
     blk = min(N, 2048)   # timing does not depend on the values: quantise a block of rows and repeat it
