@@ -43,13 +43,29 @@ __device__ __forceinline__ float value_of(unsigned code) {
 // What follows is short code: a block goes through the kernel once, and instructions that no block of its SM has used before come from the L2 (unrolled,
 // with sorting networks: joining the lists of 4 beams took 33 thousand clocks, of which two thousand were work).
 
-// The place of keys[i] among `n` different ones: how many are larger.
+// The places among `n` different keys of all of them, by the whole block: take(place, key).  Few keys have several threads each, next to one another, which go through a
+// part of the list.
 using Key = unsigned long long;
-__device__ __noinline__ int place_among(const Key* keys, int n, Key mine) {
-    int larger = 0;
+template <class Take>
+__device__ __forceinline__ void places_of(const Key* keys, int n, Take&& take) {
+    const int shift = n <= THREADS / 8 ? 3 : n <= THREADS / 4 ? 2 : n <= THREADS / 2 ? 1 : 0, parts = 1 << shift, part = threadIdx.x & (parts - 1);
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += THREADS >> shift) {
+        const int i = i0 + (threadIdx.x >> shift);
+        const Key mine = i < n ? keys[i] : ~0ull;
+        int larger = 0, also = 0;
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) larger += keys[i] > mine;
-    return larger;
+        for (int p = part; p < n / 2; p += parts) {
+            const ulonglong2 two = reinterpret_cast<const ulonglong2*>(keys)[p];
+            larger += two.x > mine;
+            also += two.y > mine;
+        }
+        if ((n & 1) && part == 0) larger += keys[n - 1] > mine;
+        larger += also;
+#pragma unroll 1
+        for (int d = 1; d < parts; d <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, d);
+        if (i < n && part == 0) take(larger, mine);
+    }
 }
 
 constexpr double LN2 = 0.693147180559945309417;
@@ -151,7 +167,7 @@ struct Part {   // of a segment
     unsigned top, unused;    // that value's code
 };
 struct Candidates {   // of a row, the best first
-    Key total[MOST_PICKS];   // order_of; 0: none
+    Key total[MOST_PICKS];   // order_of, the last five bits replaced by 31 - beam: of equal totals the lowest beam is first; 0: none
     int token[MOST_PICKS];
 };
 static_assert(sizeof(Part) == BEAM_PART_BYTES && sizeof(Candidates) == BEAM_ROW_BYTES, "workspace");
@@ -191,7 +207,7 @@ __device__ __forceinline__ bool last_of(unsigned* counter, unsigned n, volatile 
 __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelectArgs a) {
     __shared__ __align__(16) Key found[ROOM];
     __shared__ Key best[MOST_PICKS];
-    __shared__ Key best_of[WARPS * TOPS];
+    __shared__ __align__(16) Key best_of[WARPS * TOPS];
     __shared__ unsigned tops[WARPS];
     __shared__ double sums[WARPS];
     __shared__ int flag, count, homes[MOST_PICKS];
@@ -280,18 +296,16 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
     else if (!last_of(a.counters + row, a.segs, &flag)) return;
     Candidates* const rows = reinterpret_cast<Candidates*>(a.rows);
     Candidates& out = rows[row];
+    const Key last_bits = 31 - (row - group * a.beams);
     if (looked_at) {
         const Part* const p = parts + (int64_t)row * a.segs;
         // By all threads: the `picks` largest keys of those found, in order, and how many there are.
         auto settle = [&]() {
             __syncthreads();
             const int n = count;
-#pragma unroll 1
-            for (int i = tid; i < n; i += THREADS) {
-                const Key k = found[i];
-                const int place = place_among(found, n, k);
+            places_of(found, n, [&](int place, Key k) {
                 if (place < picks) best[place] = k;
-            }
+            });
             __syncthreads();
             return min(n, picks);
         };
@@ -301,6 +315,15 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
             if (tid < n) found[tid] = best[tid];
             if (tid == 0) count = n;
             __syncthreads();
+        };
+        // A key to the found ones, by whole warps: one place after the other (with an atomic operation of each lane, 157 values of a small vocabulary took 8000 clocks).
+        auto add = [&](bool take, Key key) {
+            const unsigned who = __ballot_sync(0xffffffffu, take);
+            if (who == 0) return;
+            int to = 0;
+            if (lane == 0) to = atomicAdd(&count, __popc(who));
+            to = __shfl_sync(0xffffffffu, to, 0) + __popc(who & ((1u << lane) - 1u));
+            if (take) found[to] = key;
         };
         constexpr int AHEAD = 6;   // loads in flight; so many keys of each thread may come before the next look at how many there are
         static_assert(MOST_PICKS + 2 * AHEAD * THREADS <= ROOM, "room");
@@ -332,7 +355,10 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
         }
         if (tid == 0) count = flag = 0;
         __syncthreads();
-        if (tid < WARPS * each && place_among(best_of, WARPS * each, best_of[tid]) == picks - 1) flag = (int)(best_of[tid] >> 8);   // (one thread's; none where fewer have values)
+        // (those of threads without values are 0, and so may be the picks-th: no bar)
+        places_of(best_of, WARPS * each, [&](int place, Key k) {
+            if (place == picks - 1 && k != 0) flag = (int)(k >> 8);
+        });
         __syncthreads();
         Key least = (Key)(unsigned)flag << 32;
 #pragma unroll 1
@@ -341,7 +367,7 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
                 const Key key = (Key)(k[j] >> 16) << 32 | (0xFFFFFFFFu - (unsigned)((s0 + j) * a.per_seg + (int)(0xFFFFu - (k[j] & 0xFFFFu))));
-                if (k[j] != 0 && key >= least) found[atomicAdd(&count, 1)] = key;
+                add(k[j] != 0 && key >= least, key);
             }
             if (s0 + AHEAD >= a.segs) break;
             __syncthreads();
@@ -381,8 +407,11 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
 #pragma unroll
-                    for (int j = 0; j < AHEAD; ++j) h[q][j] = home[q] >= 0 && in0 + 32 * j < values && token_of(q, j) < stop[q] ? x.p[token_of(q, j)] : (uint16_t)0xFC00;
-                if (warp == WARPS - 1 && s0 == 0 && in0 == lane) {   // meanwhile the last warp has the row's sum
+                    for (int j = 0; j < AHEAD; ++j) {
+                        h[q][j] = 0xFC00;
+                        if (home[q] >= 0 && in0 + 32 * j < values && token_of(q, j) < stop[q]) h[q][j] = x.p[token_of(q, j)];
+                    }
+                if (warp == WARPS - 1 && s0 + 2 * WARPS >= shares && in0 == lane) {   // meanwhile the last warp has the row's sum
                     double sum = y0 != 0 ? top0 > NO_VALUE ? y0 * exp_of((double)value_of(top0) - most) : y0 : 0.;
 #pragma unroll 1
                     for (int i = lane + 32; i < a.segs; i += 32) {
@@ -400,9 +429,10 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
                 for (int q = 0; q < 2; ++q)
 #pragma unroll
                     for (int j = 0; j < AHEAD; ++j) {
+                        if (home[q] < 0 || in0 - lane + 32 * j >= values) break;   // (of the whole warp)
                         const unsigned c = code_of(h[q][j]);
                         const Key key = (Key)c << 32 | (0xFFFFFFFFu - (unsigned)token_of(q, j));
-                        if (c > NO_VALUE && key >= least) found[atomicAdd(&count, 1)] = key;
+                        add(c > NO_VALUE && key >= least, key);
                     }
                 if (s0 + 2 * WARPS >= shares && in0 - lane + 32 * AHEAD >= values) break;
                 __syncthreads();
@@ -418,11 +448,11 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
             const double norm = sums[0];
             const bool there = tid < n && norm >= 0;
             const Key k = there ? best[tid] : 0;
-            out.total[tid] = there ? order_of((double)score + (((double)value_of((unsigned)(k >> 32)) - most) - norm)) : 0ull;
+            out.total[tid] = there ? (order_of((double)score + (((double)value_of((unsigned)(k >> 32)) - most) - norm)) & ~31ull) | last_bits : 0ull;
             out.token[tid] = (int)(0xFFFFFFFFu - (unsigned)k);
         }
     } else if (tid < MOST_PICKS) {   // one candidate of a beam that has ended, none without a score
-        out.total[tid] = tid == 0 && score > -INFINITY ? order_of(score) : 0ull;
+        out.total[tid] = tid == 0 && score > -INFINITY ? (order_of(score) & ~31ull) | last_bits : 0ull;
         out.token[tid] = a.eos;
     }
     // ---- the group's last block: the beams' lists joined, a beam to a lane ----
@@ -436,6 +466,7 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
     __syncthreads();   // (scores and flags have been read: they may be the outputs)
     // A candidate's place: its own beam's before it, and of each other beam those that come before it.
     int there = 0;
+    const int half = picks > 1 ? 1 << (31 - __clz(picks - 1)) : 0;   // (a list has up to 2 * half candidates)
 #pragma unroll 1
     for (int i = tid; i < a.beams * picks; i += THREADS) {
         const int b = i / picks, j = i - b * picks;
@@ -448,12 +479,9 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
             const Key* const list = all[c].total;
             int before = 0;
 #pragma unroll
-            for (int step = MOST_PICKS / 2; step > 0; step >>= 1) {
-                const Key k = list[before + step - 1];
-                if (k > mine || (k == mine && c < b)) before += step;
-            }
-            const Key k = list[before];
-            before += k > mine || (k == mine && c < b);
+            for (int step = MOST_PICKS / 2; step > 0; step >>= 1)
+                if (step <= half && list[before + step - 1] > mine) before += step;
+            before += list[before] > mine;
             place += c == b ? 0 : before;
         }
         if (place < picks) {
