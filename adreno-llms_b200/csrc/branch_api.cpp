@@ -38,8 +38,8 @@ extern "C" int nn_tree_layout(nn_context* c, const nn_kv_batch* b, nn_buf parent
     return NN_OK;
 }
 
-// The caches of several layers that share their page numbers.  Of a context, or all without one.
-static int take_caches(nn_kv_cache* const* caches, int n, const char* who) {
+// The caches of several layers that share their page numbers; *num_pages: the fewest of any, so that a page is good in all of them or in none.
+static int take_caches(nn_kv_cache* const* caches, int n, const char* who, int* num_pages) {
     if (n < 0 || (n > 0 && !caches)) return NN_FAIL(NN_ERR_ARG, "%s: num_caches=%d caches=%p", who, n, (const void*)caches);
     struct Range {
         const char *lo, *hi;
@@ -50,9 +50,11 @@ static int take_caches(nn_kv_cache* const* caches, int n, const char* who) {
     } catch (...) {
         return NN_FAIL(NN_ERR_ARG, "%s: out of host memory", who);
     }
+    *num_pages = INT_MAX;
     for (int i = 0; i < n; ++i) {
         if (!caches[i]) return NN_FAIL(NN_ERR_ARG, "%s: cache %d is null", who, i);
         const KvView& v = caches[i]->view;
+        *num_pages = std::min(*num_pages, v.num_pages);
         if (v.page_shift != caches[0]->view.page_shift)
             return NN_FAIL(NN_ERR_ARG, "%s: cache %d has pages of %d positions, the first one of %d", who, i, 1 << v.page_shift, 1 << caches[0]->view.page_shift);
         if (caches[i]->device != caches[0]->device) return NN_FAIL(NN_ERR_ARG, "%s: cache %d is of another device than the first one", who, i);
@@ -69,17 +71,15 @@ static int take_caches(nn_kv_cache* const* caches, int n, const char* who) {
     return NN_OK;
 }
 static CellRows cell_rows(const KvView& v) {
-    return CellRows{(uint8_t*)v.k, (uint8_t*)v.v, v.k_scale, v.v_scale, v.num_pages, v.kv_heads, v.dim * kv_cell_bytes(v.fmt)};
+    return CellRows{(uint8_t*)v.k, (uint8_t*)v.v, v.k_scale, v.v_scale, v.kv_heads, v.dim * kv_cell_bytes(v.fmt)};
 }
-// MOST_LAYERS caches from `first` on, and the most heads and fewest pages of them.
-static void layers_from(nn_kv_cache* const* caches, int num, int first, CellRowsOfLayers* to, int* most_heads, int* num_pages) {
+// MOST_LAYERS caches from `first` on, and the most heads of them.
+static void layers_from(nn_kv_cache* const* caches, int num, int first, CellRowsOfLayers* to, int* most_heads) {
     to->n = std::min(num - first, MOST_LAYERS);
     *most_heads = 1;
-    *num_pages = INT_MAX;
     for (int i = 0; i < to->n; ++i) {
         to->c[i] = cell_rows(caches[first + i]->view);
         *most_heads = std::max(*most_heads, to->c[i].kv_heads);
-        *num_pages = std::min(*num_pages, to->c[i].num_pages);
     }
 }
 static void wrote_caches(nn_context* c, nn_kv_cache* const* caches, int n) {
@@ -97,7 +97,7 @@ extern "C" int nn_kv_move(nn_context* c, nn_kv_cache* const* caches, int num_cac
     const char* who = "nn_kv_move";
     KvMoveArgs a = {};
     bool empty;
-    int rc = take_caches(caches, num_caches, who), unused;
+    int rc = take_caches(caches, num_caches, who, &a.num_pages);
     if (rc) return rc;
     if (!b) return NN_FAIL(NN_ERR_ARG, "%s: null batch", who);
     if (num_caches == 0) return make_current(c, nullptr, who);
@@ -113,7 +113,7 @@ extern "C" int nn_kv_move(nn_context* c, nn_kv_cache* const* caches, int num_cac
     a.status = c->status_dev;
     ProfScope prof(c, [&] { return std::string("kv_move_layers") + std::to_string(num_caches) + "_rows" + std::to_string(b->num_rows); });
     for (int first = 0; first < num_caches; first += MOST_LAYERS) {
-        layers_from(caches, num_caches, first, &a.caches, &a.most_heads, &unused);
+        layers_from(caches, num_caches, first, &a.caches, &a.most_heads);
         const cudaError_t e = launch_kv_move(a, c->stream, c->use_pdl);
         if (e != cudaSuccess) return NN_FAIL(NN_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));
         c->launches++;
@@ -126,7 +126,7 @@ extern "C" int nn_kv_reorder(nn_context* c, nn_kv_cache* const* caches, int num_
     const char* who = "nn_kv_reorder";
     KvReorderArgs a = {};
     bool empty;
-    int rc = take_caches(caches, num_caches, who);
+    int rc = take_caches(caches, num_caches, who, &a.num_pages);
     if (rc) return rc;
     if (!b) return NN_FAIL(NN_ERR_ARG, "%s: null batch", who);
     if (num_caches == 0) return NN_FAIL(NN_ERR_ARG, "%s: no caches", who);
@@ -149,7 +149,7 @@ extern "C" int nn_kv_reorder(nn_context* c, nn_kv_cache* const* caches, int num_
     a.status = c->status_dev;
     ProfScope prof(c, [&] { return std::string("kv_reorder_layers") + std::to_string(num_caches) + "_seqs" + std::to_string(b->num_seqs); });
     for (int first = 0; first < num_caches; first += MOST_LAYERS) {
-        layers_from(caches, num_caches, first, &a.caches, &a.most_heads, &a.num_pages);
+        layers_from(caches, num_caches, first, &a.caches, &a.most_heads);
         a.with_table = first == 0;
         const cudaError_t e = launch_kv_reorder(a, c->stream, c->use_pdl);
         if (e != cudaSuccess) return NN_FAIL(NN_ERR_CUDA, "%s: launch failed: %s", who, cudaGetErrorString(e));

@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(MOVE_THREADS) kv_move_kernel(const __grid_cons
                         page = table[src >> shift];
                         to_page = table[dst >> shift];
                     }
-                    if (page_ok(page, c.num_pages) && page_ok(to_page, c.num_pages)) {
+                    if (page_ok(page, a.num_pages) && page_ok(to_page, a.num_pages)) {
                         from = (int)cell_row(page, head, src & slots, c.kv_heads, shift);
                         to = (int)cell_row(to_page, head, dst & slots, c.kv_heads, shift);
                         if (scales) list.scale[tid] = scales[from];

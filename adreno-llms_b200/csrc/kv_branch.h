@@ -20,7 +20,7 @@ struct CellRows {
     uint8_t* v;
     uint16_t* k_scale;   // null without scales
     uint16_t* v_scale;
-    int num_pages, kv_heads, row_bytes;
+    int kv_heads, row_bytes;
 };
 // Layers of one launch (kernel arguments may have 4 KB everywhere).
 constexpr int MOST_LAYERS = 64;
@@ -33,7 +33,7 @@ struct KvMoveArgs {
     CellRowsOfLayers caches;
     KvSeqs s;
     const int* source;       // [num_rows]: where the row's cells are now
-    int page_shift, most_heads;
+    int page_shift, most_heads, num_pages;   // num_pages: the fewest of all layers
     int* status;
 };
 cudaError_t launch_kv_move(const KvMoveArgs& a, cudaStream_t st, bool pdl);
@@ -44,7 +44,7 @@ struct KvReorderArgs {
     CellRowsOfLayers caches;
     KvSeqs s;                // beam after beam, group after group
     const int* parent;       // [num_seqs], among the group's beams; -1: itself
-    int beams, page_shift, most_heads, num_pages;   // num_pages: the fewest of these caches
+    int beams, page_shift, most_heads, num_pages;   // num_pages: the fewest of all layers
     bool with_table;         // whether this launch exchanges the page table's entries
     int* status;
 };

@@ -251,7 +251,7 @@ int nn_attention(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, 
  *                     of a model, which share their page numbers and page size), as if all of a sequence's rows were read first.  Sources ascend within a
  *                     sequence and are not before their rows; kv_len counts what is left.  So an accepted path of a tree becomes the sequence's end
  *                     (source: the places of its rows), and what follows dropped positions moves up to them.  Rotations stay what they were.  Rows
- *                     with a bad source or page are left out and reported.  A moved row's page must not be another sequence's too.
+ *                     with a bad source or page (a page that one of the caches does not have) are left out and reported.  A moved row's page must not be another sequence's too.
  *   nn_beam_select    of `groups` groups of `beams` beams each the `picks` best continuations: total = score[beam] + log_softmax(logits[beam])[token], from
  *                     fp16 logits [groups * beams][logits_stride] (0: dense) of `vocab` tokens and fp32 scores [groups][beams], in descending order; of equal
  *                     ones the lowest beam, then the lowest token first.  out_score fp32, out_token and out_parent (the beam) int32, [groups][picks]; where a

@@ -44,7 +44,7 @@ cudaError_t launch_kv_read(const KvReadArgs&, cudaStream_t, bool) { return launc
 cudaError_t launch_attention(const AttnArgs& a, const AttnMaps&, int, int, cudaStream_t, bool, int* n) { return *n = 1, a.tree && a.tree_words == 2 && !a.window ? launched() : cudaErrorUnknown; }
 cudaError_t launch_tree_layout(const TreeLayoutArgs&, cudaStream_t, bool) { return launched(); }
 static void count(const CellRowsOfLayers& c, int most_heads) { layers += c.n; heads = most_heads; }
-cudaError_t launch_kv_move(const KvMoveArgs& a, cudaStream_t, bool) { return count(a.caches, a.most_heads), launched(); }
+cudaError_t launch_kv_move(const KvMoveArgs& a, cudaStream_t, bool) { return count(a.caches, a.most_heads), pages = a.num_pages, launched(); }
 cudaError_t launch_kv_reorder(const KvReorderArgs& a, cudaStream_t, bool) { return count(a.caches, a.most_heads), tables += a.with_table, pages = a.num_pages, launched(); }
 cudaError_t launch_beam_select(const BeamSelectArgs& a, int sms, cudaStream_t, bool) { return a.counters && a.rows && a.parts && sms == 148 ? launched() : cudaErrorUnknown; }
 void beam_segments(int, int, int, int* segs, int* per) { *segs = 3, *per = 1024; }
@@ -95,6 +95,11 @@ int main() {
     launches = layers = 0;
     CHECK(nn_kv_reorder(&zero, many, 130, &batch, 2, at(23)) == NN_OK && launches == 3 && layers == 130 && tables == 1 && pages == 4);   // (6 and 4)
     CHECK(nn_kv_reorder(&zero, many, 64, &batch, 2, at(23)) == NN_OK && launches == 4 && pages == 4 && heads == 5);
+    // a page is in all layers or in none, whichever launch they are in (the last of these alone has 6)
+    pages = 0;
+    CHECK(nn_kv_move(&zero, many + 1, 65, &batch, at(23)) == NN_OK && pages == 4);
+    pages = 0;
+    CHECK(nn_kv_reorder(&zero, many + 1, 65, &batch, 2, at(23)) == NN_OK && pages == 4);
     // the segments have room
     CHECK(nn_beam_select(&zero, 2731, 1, 100, at(40), 0, at(41), nullptr, -1, 4, at(42), at(43), at(44), nullptr) == NN_ERR_UNSUPPORTED && strstr(error, "segments"));
     CHECK(nn_beam_select(&zero, 2730, 1, 100, at(40), 0, at(41), nullptr, -1, 4, at(42), at(43), at(44), nullptr) == NN_OK);
