@@ -179,3 +179,30 @@ def test_rows_beyond_32_bits(nnb, ctx):
     check(got, logits, vocab, score, None, -1, 4, "far rows")
     for b in (buf, sb, *outs):
         ctx.free(b)
+
+
+@pytest.mark.parametrize("vocab,beams", [(200003, 1), (400000, 2), (1000000, 1), (30000, 24)])
+def test_equal_values_in_many_places(nnb, ctx, vocab, beams):
+    """More equal values than a block compares at once, among the shares' largest ones and within shares: the first tokens of them."""
+    rng = np.random.default_rng(101)
+    flat = np.full(vocab, 0.25, np.float16)
+    few = (rng.integers(0, 2, vocab) * 3).astype(np.float16)
+    edge = np.where(np.arange(vocab) % 9000 < 20, 4.0, rng.integers(-2, 4, vocab)).astype(np.float16)      # twenty in a row, in every segment
+    rows = np.stack([flat, few, edge])
+    logits = np.ascontiguousarray(np.repeat(rows[:, None], beams, 1))
+    score = np.repeat([[-0.5], [-1.0], [-1.5]], beams, 1).astype(np.float32)
+    for picks in (8, 31, 32):
+        got = run(nnb, ctx, logits, vocab, score, None, -1, picks)
+        check(got, logits, vocab, score, None, -1, picks, f"equal values of {vocab}")
+
+
+def test_scores_that_are_not_finite(nnb, ctx):
+    """An infinite score is none, of a beam that goes on and of one that has ended."""
+    logits, score = draw(2, 4, 700, 102)
+    done = np.array([[0, 0, 1, 1], [1, 0, 0, 0]], np.int32)
+    score[0, 1] = score[0, 2] = score[1, 0] = np.inf
+    score[1, 2] = -np.inf
+    got = run(nnb, ctx, logits, 700, score, done, 9, 6)
+    none = np.where(np.isfinite(score), score, -np.inf).astype(np.float32)
+    check(got, logits, 700, none, np.where(np.isfinite(score), done, 0), 9, 6, "scores that are not finite")
+    assert not np.isin(got[2][0], (1, 2)).any() and not np.isin(got[2][1], (0, 2)).any()

@@ -212,3 +212,28 @@ def test_bad_groups_are_left_as_they_are(nnb, ctx, what):
     layers.close()
     for x in (tb, kb, pb):
         ctx.free(x)
+
+
+def test_pages_that_one_layer_does_not_have(nnb, ctx):
+    """Layers with more pages than others: what the smallest does not have is bad in all of them."""
+    page = 16
+    large, small = (Layers(nnb, ctx, [(fmt, 2, 64)], n, page, 83) for fmt, n in (("fp16", 8), ("int8", 4)))
+    both = large.handles + small.handles
+    # a sequence in both, one with a page that only the first has
+    table = np.array([[0, 1], [2, 5]], np.int32)
+    up = [ctx.upload(np.ascontiguousarray(a, np.int32)) for a in ([0, 1, 2], [10, 10], table, [20, 20], [30, 30], [1, 0])]
+    ctx.kv_move(both, nnb.KVBatch(2, 2, 1, 32, 2, *up[:3]), up[3])
+    with pytest.raises(nnb.NNError):
+        ctx.sync()
+    for layers in (large, small):
+        layers.move([((0, 9), (1, 4))])
+        layers.check()
+    ctx.kv_reorder(both, nnb.KVBatch(2, 0, 0, 32, 2, None, up[4], up[2]), 2, up[5])     # (the beams change places)
+    with pytest.raises(nnb.NNError):
+        ctx.sync()
+    for layers in (large, small):
+        layers.check()
+        layers.close()
+    assert np.array_equal(ctx.download(up[2], table.shape, np.int32), table)
+    for x in up:
+        ctx.free(x)
