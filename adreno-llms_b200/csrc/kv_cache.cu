@@ -68,11 +68,27 @@ constexpr int WARPS = 4;
 template <int FMT, int D, bool SPREAD>
 __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs a) {
     constexpr int LANES = D / 16, HEADS = 32 / LANES * (SPREAD ? WARPS : 1);   // threads of a head's row; heads at a time
-    constexpr int AHEAD = SPREAD ? 1 : 3;                                      // loads of so many heads in flight
+    constexpr int AHEAD = SPREAD ? 1 : FMT == KV_FP16 ? 4 : 3;                 // loads of so many heads in flight
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = SPREAD ? blockIdx.x : blockIdx.x * WARPS + warp;
     if (r >= a.s.num_rows) return;
+    const int j = lane % LANES, nq = a.q ? a.q_heads : 0, heads = nq + 2 * a.c.kv_heads, first = (SPREAD ? threadIdx.x : lane) / LANES;
+    int pa, pb;
+    piece_pair(j, a.rotary, pa, pb);
+    auto load = [&](int h, uint4 (&in)[2]) {
+        in[0] = in[1] = make_uint4(0, 0, 0, 0);
+        if (h < heads) {
+            const uint16_t* src = h < nq ? a.q + r * a.q_stride + (int64_t)h * D
+                                         : h < nq + a.c.kv_heads ? a.k + r * a.k_stride + (int64_t)(h - nq) * D : a.v + r * a.v_stride + (int64_t)(h - nq - a.c.kv_heads) * D;
+            in[0] = reinterpret_cast<const uint4*>(src)[pa];
+            in[1] = reinterpret_cast<const uint4*>(src)[pb];
+        }
+    };
+    // Spread: the row's first heads are on their way while its place is looked up, and later ones while those before them are worked on (414 rows of 48 heads of 128 dims, e4m3:
+    // 5.0 us without, 4.7 with; 7118 rows by a warp each 35 without, 50 with).
+    uint4 in[AHEAD][2];
+    if (SPREAD) load(first, in[0]);
     const RowPlace at = place_of_row(a.s, r);
     if (at.none) return;
     const int turn = a.position && !at.bad ? a.position[r] : at.pos;
@@ -83,9 +99,6 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
     const int page = a.s.page_table[(int64_t)at.seq * a.s.table_stride + (at.pos >> a.c.page_shift)], slot = at.pos & ((1 << a.c.page_shift) - 1);
     const bool cell = page_ok(page, a.c.num_pages);
     if (!cell && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
-    const int j = lane % LANES;
-    int pa, pb;
-    piece_pair(j, a.rotary, pa, pb);
     const bool turns = j < a.rotary / 16;
     float c[8], s[8];
     if (turns) {
@@ -98,58 +111,52 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
             s[4 * i] = y.x, s[4 * i + 1] = y.y, s[4 * i + 2] = y.z, s[4 * i + 3] = y.w;
         }
     }
-    const int nq = a.q ? a.q_heads : 0, heads = nq + 2 * a.c.kv_heads, first = (SPREAD ? threadIdx.x : lane) / LANES;
     for (int h0 = 0; h0 < heads; h0 += HEADS * AHEAD) {   // (whole warps stay together for the shuffles)
-        uint4 in[AHEAD][2];
+        if (!SPREAD) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int h = h0 + u * HEADS + first;
-            in[u][0] = in[u][1] = make_uint4(0, 0, 0, 0);
-            if (h < heads) {
-                const uint16_t* src = h < nq ? a.q + r * a.q_stride + (int64_t)h * D
-                                             : h < nq + a.c.kv_heads ? a.k + r * a.k_stride + (int64_t)(h - nq) * D : a.v + r * a.v_stride + (int64_t)(h - nq - a.c.kv_heads) * D;
-                in[u][0] = reinterpret_cast<const uint4*>(src)[pa];
-                in[u][1] = reinterpret_cast<const uint4*>(src)[pb];
-            }
+            for (int u = 0; u < AHEAD; ++u) load(h0 + u * HEADS + first, in[u]);
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int h = h0 + u * HEADS + first;
             const bool on = h < heads, is_q = h < nq, is_k = !is_q && h < nq + a.c.kv_heads;
+            uint4 px = in[u][0], py = in[u][1];
+            if (SPREAD) load(h + HEADS, in[u]);
             float x[8], y[8];
-            unpack8(in[u][0], x);
-            unpack8(in[u][1], y);
+            unpack8(px, x);
+            unpack8(py, y);
             if (turns && (is_q || is_k)) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float t1 = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i]));
-                    const float t2 = __fadd_rn(__fmul_rn(y[i], c[i]), __fmul_rn(x[i], s[i]));
-                    x[i] = __half2float(__float2half_rn(t1));
-                    y[i] = __half2float(__float2half_rn(t2));
+                    const float t1 = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i])), t2 = __fadd_rn(__fmul_rn(y[i], c[i]), __fmul_rn(x[i], s[i]));
+                    x[i] = t1;
+                    y[i] = t2;
                 }
+            }
+            if (FMT == KV_FP16 || is_q || is_k) {
+                px = pack8(x);
+                py = pack8(y);
             }
             if (is_q) {   // (h < nq <= heads)
                 uint4* dst = reinterpret_cast<uint4*>(a.q_out + r * a.qo_stride + (int64_t)h * D);
-                dst[pa] = pack8(x);
-                dst[pb] = pack8(y);
+                dst[pa] = px;
+                dst[pb] = py;
             }
             const bool store = on && !is_q && cell;
             const int64_t row = store ? cell_row(page, is_k ? h - nq : h - nq - a.c.kv_heads, slot, a.c.kv_heads, a.c.page_shift) : 0;
             if (FMT == KV_FP16) {
                 if (store) {
                     uint4* dst = reinterpret_cast<uint4*>((uint16_t*)(is_k ? a.c.k : a.c.v) + row * D);
-                    dst[pa] = pack8(x);
-                    dst[pb] = pack8(y);
+                    dst[pa] = px;
+                    dst[pb] = py;
                 }
             } else if (__any_sync(0xffffffffu, store)) {
-                float most = 0.f;
-                bool nan = false;
+                const uint32_t w[8] = {px.x, px.y, px.z, px.w, py.x, py.y, py.z, py.w};
+                __half2 top = __habs2(*reinterpret_cast<const __half2*>(&w[0]));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    most = fmaxf(most, fmaxf(fabsf(x[i]), fabsf(y[i])));
-                    nan |= x[i] != x[i] || y[i] != y[i];
-                }
-                if (nan) most = INFINITY;
+                for (int i = 1; i < 8; ++i) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const __half2*>(&w[i])));
+                float most = __half2float(__hmax_nan(__low2half(top), __high2half(top)));
+                if (most != most) most = INFINITY;
 #pragma unroll
                 for (int o = LANES / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 if (store) {
@@ -157,6 +164,10 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
                     const float f = half_float(sc), inverse = __frcp_rn(f);
                     const bool whole = sc != 0x7FFF;
                     uint2* dst = reinterpret_cast<uint2*>((uint8_t*)(is_k ? a.c.k : a.c.v) + row * D);
+                    if (is_k) {   // (as they were rounded)
+                        unpack8(px, x);
+                        unpack8(py, y);
+                    }
                     dst[pa] = whole ? encode8<FMT>(x, f, inverse) : make_uint2(0, 0);
                     dst[pb] = whole ? encode8<FMT>(y, f, inverse) : make_uint2(0, 0);
                     if (j == 0) (is_k ? a.c.k_scale : a.c.v_scale)[row] = sc;
@@ -240,7 +251,8 @@ cudaError_t launch(void (*kernel)(const Args), const Args& a, int grid, cudaStre
 }
 
 // A row in four warps is ready sooner, a row in one has more loads in flight and fewer blocks to start.  Four warps / one, us, in a recorded chain of calls:
-// writes of 32 + 2 x 8 heads of 128 dims, fp16: 1 row 2.5 / 4.3, 1200 rows 5.1 / 7.9, 2400 rows 8.4 / 8.1, 8192 rows 35.4 / 34.0; of 9 + 2 x 3 heads of 64:
+// writes of 32 + 2 x 8 heads of 128 dims, fp16: 1 row 2.5 / 4.3, 1200 rows 5.1 / 7.9, 3079 rows 16.0 / 17.0, 5607 rows 25.0 / 24.3; e4m3: 3079 rows 18.0 / 20.6, 5607 rows
+// 29.6 / 26.6; of 9 + 2 x 3 heads of 64:
 // 1 row 1.9 / 2.1, 256 rows 2.4 / 2.3, 2400 rows 4.8 / 3.3.  Reads of 3 heads of 64 dims, int8: 1200 rows 2.5 / 2.8, 2400 rows
 // 4.1 / 2.8; of 8 heads of 128 dims: 1 row 1.8 / 2.9, 2400 rows 4.6 / 7.1, 65536 rows of 16 heads, e4m3,
 // 135 / 143; but of 8 heads of 64, e4m3, 70 / 50, of 4 heads of 128, fp16, 71 / 43.
@@ -249,7 +261,7 @@ constexpr int FEW_ROWS = 592;   // (four blocks for each SM)
 template <int FMT, int D>
 cudaError_t write_rows(const KvWriteArgs& a, cudaStream_t st, bool pdl) {
     const bool wide = ((a.q ? a.q_heads : 0) + 2 * a.c.kv_heads) * (D / 16) >= 2 * WARPS * 32;   // a row is work for four warps more than once
-    if (a.s.num_rows <= (wide ? 4 * FEW_ROWS : FEW_ROWS)) return launch(kv_write_kernel<FMT, D, true>, a, a.s.num_rows, st, pdl);
+    if (a.s.num_rows <= (wide ? 8 * FEW_ROWS : FEW_ROWS)) return launch(kv_write_kernel<FMT, D, true>, a, a.s.num_rows, st, pdl);
     return launch(kv_write_kernel<FMT, D, false>, a, (a.s.num_rows - 1) / WARPS + 1, st, pdl);
 }
 template <int FMT, int D>
