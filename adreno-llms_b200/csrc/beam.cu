@@ -8,13 +8,13 @@
 // keeps their maximum and the sum of exponentials behind it.  The row's best `picks` values lie in those shares whose maxima are the `picks`
 // best ones: every other share has `picks` values before all of its own.  So no value needs a place in a list while the logits stream by, whatever
 // their order.  The row's last block finds those shares, reads them again, a value to a thread, and has the row's candidates; the group's last
-// block joins its rows' lists.
+// block joins its rows' lists.  Where there are few blocks each does so for its segment, and the group's last one joins the segments' lists (DIRECT).
 // Within a row the fp16 values and the tokens decide, exactly.  Across rows the totals do, in 64 bits.  Exponentials are taken of differences to the
 // thread's maximum (exact), in 32 bits: a maximum is exactly 1, the others are 2^-22 off at most, and so is the sum; a row of 151936 values of N(0, 2.5) has a sum that is some
 // 2^-27 off, its errors being different for each value.  Everything depends on differences alone: rows that are shifted against each other
 // give the same logarithms.
 // 64 groups of 8 beams of 151936 fp16 logits, 16 picks: 44 us (3.5 TB/s; the bytes alone 24).  The exponential unit has 36 thousand clocks of it, the logits altogether 52 (27 us),
-// the last rows' steps behind them 8 us.  One group of 4 beams of 49152: 9.5 us, all of it such steps.
+// the last rows' steps behind them 8 us.  One group of 4 beams of 49152: 8.1 us, all of it such steps.
 #include <cuda_fp16.h>
 
 #include "kv_branch.h"
@@ -26,6 +26,7 @@ namespace {
 constexpr int THREADS = 256, WARPS = THREADS / 32, BATCH = 4;
 constexpr int TOPS = MOST_PICKS / 4;        // maxima of a warp that are compared with the other warps'
 constexpr int ROOM = 3136;                  // keys that a block compares with one another
+constexpr int DIRECT_MOST = 1024, DIRECT_LISTS = 128;   // candidates and segments of a group that its last block joins without the rows' lists
 constexpr unsigned NO_VALUE = 0x03FFu;      // the code of -infinity
 
 __device__ __forceinline__ float ex2(float x) {
@@ -172,7 +173,12 @@ struct Candidates {   // of a row, the best first
     Key total[MOST_PICKS];   // order_of, the last five bits replaced by 31 - beam: of equal totals the lowest beam is first; 0: none
     int token[MOST_PICKS];
 };
-static_assert(sizeof(Part) == BEAM_PART_BYTES && sizeof(Candidates) == BEAM_ROW_BYTES, "workspace");
+struct Best {   // of a segment, the best first
+    Key key[MOST_PICKS];   // value's code << 32 | 0xFFFFFFFF - token; 0: none
+    double sum;            // as in Part
+    unsigned top, unused[29];
+};
+static_assert(sizeof(Part) == BEAM_PART_BYTES && sizeof(Candidates) == BEAM_ROW_BYTES && sizeof(Best) == BEAM_ROW_BYTES, "workspace");
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     uint64_t d, x = *reinterpret_cast<const uint64_t*>(&a), y = *reinterpret_cast<const uint64_t*>(&b);
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(x), "l"(y));
@@ -206,23 +212,161 @@ __device__ __forceinline__ bool last_of(unsigned* counter, unsigned n, volatile 
     return *flag != 0;
 }
 
+// The group's picks from its segments' candidates: rows' sums, totals, and of those that may be among the picks the place of each.
+struct JoinRoom {
+    ulonglong2 left[DIRECT_MOST];   // total as in Candidates, and key as in Best
+    Key some[DIRECT_LISTS];
+    double norm[MOST_BEAMS], most[MOST_BEAMS];
+    unsigned bar;                   // of totals' upper halves
+    int count, there;
+};
+__device__ __forceinline__ void join_segments(const BeamSelectArgs& a, int group, JoinRoom& room) {
+    const int tid = threadIdx.x, lane = tid & 31, picks = a.picks, per_beam = a.segs * picks, num = a.beams * a.segs, n = num * picks;
+    const Best* const lists = reinterpret_cast<const Best*>(a.rows) + (int64_t)group * num;
+    constexpr int EACH = DIRECT_MOST / THREADS;
+    Key key[EACH], total[EACH];
+    float score[EACH];
+    bool ended[EACH];
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+        key[u] = total[u] = 0;
+        score[u] = 0.f;
+        ended[u] = false;
+        const int i = tid + u * THREADS;
+        if (i < n) {
+            const int l = i / picks, b = i / per_beam;
+            key[u] = __ldcg(&lists[l].key[i - l * picks]);   // (of rows that are not looked at: left from another call)
+            score[u] = a.score[group * a.beams + b];
+            ended[u] = a.done && a.done[group * a.beams + b] != 0;
+        }
+    }
+#pragma unroll 1
+    for (int b = tid >> 5; b < a.beams; b += WARPS) {   // a row to a warp
+        const Best* const p = lists + b * a.segs;
+        const unsigned top0 = lane < a.segs ? __ldcg(&p[lane].top) : 0u;
+        const double y0 = lane < a.segs ? __ldcg(&p[lane].sum) : 0.;
+        unsigned top = top0;
+        for (int s = lane + 32; s < a.segs; s += 32) top = max(top, __ldcg(&p[s].top));
+        top = __reduce_max_sync(0xffffffffu, top);
+        const double most = value_of(top);
+        double sum = y0 != 0 ? top0 > NO_VALUE ? y0 * exp_of((double)value_of(top0) - most) : y0 : 0.;
+        for (int s = lane + 32; s < a.segs; s += 32) {
+            const unsigned c = __ldcg(&p[s].top);
+            const double y = __ldcg(&p[s].sum);
+            if (y != 0) sum += c > NO_VALUE ? y * exp_of((double)value_of(c) - most) : y;
+        }
+#pragma unroll 1
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane == 0) {
+            room.norm[b] = sum > 0 && sum < INFINITY && most < INFINITY ? log_of(sum) : -1.;   // (-1: a NaN or an infinity among the values, no candidates)
+            room.most[b] = most;
+        }
+    }
+    const bool few = n <= THREADS / 4;   // (all are compared with all)
+    if (tid == 0) {
+        room.bar = few ? 0u : ~0u;
+        room.count = room.there = 0;
+    }
+    __syncthreads();
+    // Where `each`-th totals of that many lists are not below a total, it is not below the last pick's.
+    const int each = (picks + num - 1) / num, enough = (picks + each - 1) / each;
+    int there = 0;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+        const int i = tid + u * THREADS;
+        if (i < n) {
+            const int l = i / picks, b = i / per_beam;
+            if (ended[u]) key[u] = i == b * per_beam ? 0xFFFFFFFFu - (unsigned)a.eos : 0u;
+            if (key[u] != 0 && fabsf(score[u]) < INFINITY && (ended[u] || room.norm[b] >= 0)) {
+                const double t = ended[u] ? (double)score[u] : (double)score[u] + (((double)value_of((unsigned)(key[u] >> 32)) - room.most[b]) - room.norm[b]);
+                total[u] = (order_of(t) & ~31ull) | (unsigned)(31 - b);
+                ++there;
+            }
+            if (i - l * picks == each - 1) room.some[l] = total[u];
+        }
+    }
+    there = __reduce_add_sync(0xffffffffu, there);
+    if (lane == 0 && there) atomicAdd(&room.there, there);
+    if (!few) {
+        __syncthreads();
+        places_of(room.some, num, [&](int place, Key k) {
+            if (place < enough) atomicMin(&room.bar, (unsigned)(k >> 32));   // (0: fewer lists have so many)
+        });
+    }
+    __syncthreads();   // (scores and flags have been read: they may be the outputs)
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+        if (u * THREADS >= n) break;
+        const bool stays = total[u] != 0 && (unsigned)(total[u] >> 32) >= room.bar;
+        const unsigned who = __ballot_sync(0xffffffffu, stays);
+        int to = 0;
+        if (lane == 0 && who) to = atomicAdd(&room.count, __popc(who));
+        to = __shfl_sync(0xffffffffu, to, 0) + __popc(who & ((1u << lane) - 1u));
+        if (stays) room.left[to] = make_ulonglong2(total[u], key[u]);
+    }
+    __syncthreads();
+    const int left = room.count, shift = left <= THREADS / 8 ? 3 : left <= THREADS / 4 ? 2 : left <= THREADS / 2 ? 1 : 0, threads = 1 << shift, part = tid & (threads - 1);
+#pragma unroll 1
+    for (int i0 = 0; i0 < left; i0 += THREADS >> shift) {
+        const int i = i0 + (tid >> shift);
+        const ulonglong2 mine = room.left[i < left ? i : 0];
+        int place = 0;
+#pragma unroll 2
+        for (int j = part; j < left; j += threads) {
+            const ulonglong2 other = room.left[j];
+            place += other.x > mine.x || (other.x == mine.x && other.y > mine.y);
+        }
+#pragma unroll 1
+        for (int d = 1; d < threads; d <<= 1) place += __shfl_xor_sync(0xffffffffu, place, d);
+        if (i < left && part == 0 && place < picks) {
+            const int64_t o = (int64_t)group * picks + place;
+            const int token = (int)(0xFFFFFFFFu - (unsigned)mine.y);
+            a.out_score[o] = (float)total_of(mine.x);
+            a.out_token[o] = token;
+            a.out_parent[o] = 31 - (int)(mine.x & 31);
+            if (a.out_done) a.out_done[o] = token == a.eos;
+        }
+    }
+    if (tid >= room.there && tid < picks) {   // no more candidates
+        const int64_t o = (int64_t)group * picks + tid;
+        a.out_score[o] = -INFINITY;
+        a.out_token[o] = a.out_parent[o] = -1;
+        if (a.out_done) a.out_done[o] = 0;
+    }
+}
+
 // (six blocks to an SM, for loads in flight: with five and more registers 44.5 us where it is 42.8)
-__global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelectArgs a) {
+template <bool DIRECT>
+__global__ void __launch_bounds__(THREADS, DIRECT ? 4 : 6) beam_select_kernel(const BeamSelectArgs a) {
     __shared__ __align__(16) Key found[ROOM];
     __shared__ Key best[MOST_PICKS];
     __shared__ __align__(16) Key best_of[WARPS * TOPS];
     __shared__ unsigned tops[WARPS];
     __shared__ double sums[WARPS];
     __shared__ int flag, count, homes[MOST_PICKS];
-    static_assert(sizeof(Candidates) * MOST_BEAMS <= sizeof(found), "room");
+    static_assert(sizeof(Candidates) * MOST_BEAMS <= sizeof(found) && sizeof(JoinRoom) <= sizeof(found), "room");
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, row = blockIdx.x / a.segs, seg = blockIdx.x - row * a.segs, group = row / a.beams, picks = a.picks;
     // A beam that has ended, or has no score, is not looked at.
     const float score = a.score[row];
     const bool scored = fabsf(score) < INFINITY, looked_at = scored && !(a.done && a.done[row] != 0);
+    constexpr bool direct = DIRECT;
+    unsigned own = 0;          // (direct) this thread's share as in Part::key
     Part* const parts = reinterpret_cast<Part*>(a.parts);
+    Best& list = reinterpret_cast<Best*>(a.rows)[blockIdx.x];   // (direct)
     const Row x(a.logits + (int64_t)row * a.stride, a.vocab);
+    auto segment_sum = [&](double& sum, unsigned& top) {   // of the warps' ones, by a warp
+        const unsigned mine = lane < WARPS ? tops[lane] : 0u, most = __reduce_max_sync(0xffffffffu, mine);
+        double s = lane < WARPS ? sums[lane] : 0.0;
+        if (s != 0) s *= (double)ex2((value_of(mine) - value_of(most)) * LOG2E);
+#pragma unroll 1
+        for (int d = WARPS / 2; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if (lane == 0) {
+            sum = s;
+            top = most;
+        }
+    };
     if (looked_at) {
         const int begin = seg * a.per_seg, end = min(x.vectors(), begin + a.per_seg), plain = min(x.plain(), end);
         __half most = __ushort_as_half(0xFC00);
@@ -272,7 +416,8 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
         }
         Part& part = parts[blockIdx.x];
         const unsigned code = code_of(__half_as_ushort(most));
-        part.key[tid] = code > NO_VALUE ? code << 16 | (0xFFFFu - at) : 0u;
+        own = code > NO_VALUE ? code << 16 | (0xFFFFu - at) : 0u;
+        if (!direct) part.key[tid] = own;
         const unsigned warp_top = __reduce_max_sync(0xffffffffu, code);
         double whole = sum != 0.f ? ((double)sum + (double)rest) * (double)ex2((__half2float(most) - value_of(warp_top)) * LOG2E) : 0.0;
 #pragma unroll 1
@@ -282,25 +427,18 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
             sums[warp] = whole;
         }
         __syncthreads();
-        if (warp == 0) {
-            const unsigned mine = lane < WARPS ? tops[lane] : 0u, top = __reduce_max_sync(0xffffffffu, mine);
-            double s = lane < WARPS ? sums[lane] : 0.0;
-            if (s != 0) s *= (double)ex2((value_of(mine) - value_of(top)) * LOG2E);
-#pragma unroll 1
-            for (int d = WARPS / 2; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            if (lane == 0) {
-                part.sum = s;
-                part.top = top;
-            }
-        }
+        if (!direct && warp == 0) segment_sum(part.sum, part.top);
     }
     // ---- the row's last block: its candidates ----
-    if (a.segs == 1) __syncthreads();
-    else if (!last_of(a.counters + row, a.segs, &flag)) return;
+    if (!direct) {
+        if (a.segs == 1) __syncthreads();
+        else if (!last_of(a.counters + row, a.segs, &flag)) return;
+    }
     Candidates* const rows = reinterpret_cast<Candidates*>(a.rows);
     Candidates& out = rows[row];
     const Key last_bits = 31 - (row - group * a.beams);
     if (looked_at) {
+        const int seg0 = direct ? seg : 0, segs = direct ? 1 : a.segs;   // (direct: a segment as the row is)
         const Part* const p = parts + (int64_t)row * a.segs;
         // By all threads: the `picks` largest keys of those found, in order, and how many there are.
         auto settle = [&]() {
@@ -334,17 +472,18 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
         unsigned mine = 0, k[AHEAD];   // (k: of the segments s0 ..)
         auto keys_from = [&](int s0) {
 #pragma unroll
-            for (int j = 0; j < AHEAD; ++j) k[j] = s0 + j < a.segs ? __ldcg(&p[s0 + j].key[tid]) : 0u;
+            for (int j = 0; j < AHEAD; ++j) k[j] = !direct && s0 + j < segs ? __ldcg(&p[s0 + j].key[tid]) : 0u;
         };
         keys_from(0);
-        unsigned top = lane < a.segs ? __ldcg(&p[lane].top) : 0u;
+        if (direct) k[0] = own;
+        unsigned top = !direct && lane < segs ? __ldcg(&p[lane].top) : 0u;
         const unsigned top0 = top;
-        const double y0 = lane < a.segs ? __ldcg(&p[lane].sum) : 0.;
-        for (int s = lane + 32; s < a.segs; s += 32) top = max(top, __ldcg(&p[s].top));   // (each warp for itself)
+        const double y0 = !direct && lane < segs ? __ldcg(&p[lane].sum) : 0.;
+        for (int s = lane + 32; s < segs; s += 32) top = max(top, __ldcg(&p[s].top));   // (each warp for itself)
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) mine = max(mine, k[j] >> 16);
 #pragma unroll 4
-        for (int s = AHEAD; s < a.segs; ++s) mine = max(mine, __ldcg(&p[s].key[tid]) >> 16);
+        for (int s = AHEAD; s < segs; ++s) mine = max(mine, __ldcg(&p[s].key[tid]) >> 16);
         top = __reduce_max_sync(0xffffffffu, top);
         const double most = value_of(top);
         // Twice `picks` of these, a quarter of that many the largest ones of each warp: no share whose code is below the `picks`-th of them can be among the best.
@@ -365,14 +504,14 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
         __syncthreads();
         Key least = (Key)(unsigned)flag << 32;
 #pragma unroll 1
-        for (int s0 = 0; s0 < a.segs; s0 += AHEAD) {
+        for (int s0 = 0; s0 < segs; s0 += AHEAD) {
             if (s0) keys_from(s0);
 #pragma unroll
             for (int j = 0; j < AHEAD; ++j) {
-                const Key key = (Key)(k[j] >> 16) << 32 | (0xFFFFFFFFu - (unsigned)((s0 + j) * a.per_seg + (int)(0xFFFFu - (k[j] & 0xFFFFu))));
+                const Key key = (Key)(k[j] >> 16) << 32 | (0xFFFFFFFFu - (unsigned)((seg0 + s0 + j) * a.per_seg + (int)(0xFFFFu - (k[j] & 0xFFFFu))));
                 add(k[j] != 0 && key >= least, key);
             }
-            if (s0 + AHEAD >= a.segs) break;
+            if (s0 + AHEAD >= segs) break;
             __syncthreads();
             if (count > ROOM - AHEAD * THREADS) {   // (equal values)
                 make_room();
@@ -385,8 +524,9 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
         least = shares == picks ? best[picks - 1] >> 32 << 32 : (Key)(NO_VALUE + 1) << 32;
         if (tid == 0) {
             count = 0;
-            sums[0] = -1.;   // (without shares there are no candidates)
+            if (!direct) sums[0] = -1.;   // (without shares there are no candidates)
         }
+        if (direct && shares == 0 && warp == 0) segment_sum(list.sum, list.top);
         if (tid < shares) homes[tid] = (int)(0xFFFFFFFFu - (unsigned)best[tid]);
         __syncthreads();
         // (two shares to a warp at a time)
@@ -414,10 +554,12 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
                         h[q][j] = 0xFC00;
                         if (home[q] >= 0 && in0 + 32 * j < values && token_of(q, j) < stop[q]) h[q][j] = x.p[token_of(q, j)];
                     }
-                if (warp == WARPS - 1 && s0 + 2 * WARPS >= shares && in0 == lane) {   // meanwhile the last warp has the row's sum
+                if (direct) {
+                    if (warp == WARPS - 1 && s0 == 0 && in0 == lane) segment_sum(list.sum, list.top);
+                } else if (warp == WARPS - 1 && s0 + 2 * WARPS >= shares && in0 == lane) {   // meanwhile the last warp has the row's sum
                     double sum = y0 != 0 ? top0 > NO_VALUE ? y0 * exp_of((double)value_of(top0) - most) : y0 : 0.;
 #pragma unroll 1
-                    for (int i = lane + 32; i < a.segs; i += 32) {
+                    for (int i = lane + 32; i < segs; i += 32) {
                         const unsigned c = __ldcg(&p[i].top);
                         const double y = __ldcg(&p[i].sum);
                         if (y != 0) sum += c > NO_VALUE ? y * exp_of((double)value_of(c) - most) : y;
@@ -447,20 +589,27 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
             }
         }
         const int n = settle();
-        if (tid < MOST_PICKS) {
+        if (direct) {
+            if (tid < picks) list.key[tid] = tid < n ? best[tid] : 0ull;
+        } else if (tid < MOST_PICKS) {
             const double norm = sums[0];
             const bool there = tid < n && norm >= 0;
             const Key k = there ? best[tid] : 0;
             out.total[tid] = there ? (order_of((double)score + (((double)value_of((unsigned)(k >> 32)) - most) - norm)) & ~31ull) | last_bits : 0ull;
             out.token[tid] = (int)(0xFFFFFFFFu - (unsigned)k);
         }
-    } else if (tid < MOST_PICKS) {   // one candidate of a beam that has ended, none without a score
+    } else if (!direct && tid < MOST_PICKS) {   // one candidate of a beam that has ended, none without a score
         out.total[tid] = tid == 0 && scored ? (order_of(score) & ~31ull) | last_bits : 0ull;
         out.token[tid] = a.eos;
     }
     // ---- the group's last block: the beams' lists joined, a beam to a lane ----
     __syncthreads();   // (picks fit into a warp: the first one has written)
-    if (a.beams > 1 && !last_of(a.counters + MOST_BEAM_ROWS + group, a.beams, &flag)) return;
+    const int blocks = direct ? a.beams * a.segs : a.beams;   // to come
+    if (blocks > 1 && !last_of(a.counters + MOST_BEAM_ROWS + group, blocks, &flag)) return;
+    if (direct) {
+        join_segments(a, group, *reinterpret_cast<JoinRoom*>(found));
+        return;
+    }
     Candidates* const all = reinterpret_cast<Candidates*>(found);
     {
         const uint4* const from = reinterpret_cast<const uint4*>(rows + (int64_t)group * a.beams);
@@ -513,6 +662,11 @@ __global__ void __launch_bounds__(THREADS, 6) beam_select_kernel(const BeamSelec
 cudaError_t launch_beam_select(const BeamSelectArgs& given, int sm_count, cudaStream_t st, bool pdl) {
     BeamSelectArgs a = given;
     beam_segments(a.groups * a.beams, a.vocab, sm_count, &a.segs, &a.per_seg);
+    // Few blocks look for their segments' candidates themselves, which saves the rows' counters and a trip to the parts; of many, in several rounds, most have
+    // nothing to do with that.  So / by rows, us: 1 x 4 beams of 49152, 4 picks 8.1 / 9.2; of 151936 9.1 / 12.6; 8 x 5 of 65535, 5 picks 13.3 / 15.7; 64 x 4 of 8192, 8 picks
+    // 11.3 / 13.1; 100 x 4 of 1000, 4 picks 9.7 / 12.0.  Without segments there is less to save and rows' lists are joined sooner where they are long: 11 x 14 of 157, 28 picks 18.6 / 16.7.
+    const int lists = a.beams * a.segs, candidates = lists * a.picks;
+    const bool direct = a.groups * lists <= 4 * sm_count && lists <= DIRECT_LISTS && candidates <= (a.segs > 1 ? DIRECT_MOST : DIRECT_MOST / 8);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.groups * a.beams * a.segs));
     cfg.blockDim = dim3(THREADS);
@@ -522,7 +676,7 @@ cudaError_t launch_beam_select(const BeamSelectArgs& given, int sm_count, cudaSt
     attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, beam_select_kernel, a);
+    return cudaLaunchKernelEx(&cfg, direct ? beam_select_kernel<true> : beam_select_kernel<false>, a);
 }
 
 // Segments of a row, in whole rounds of loads: of so many that there are some 16 blocks for each SM, and of no more vectors than have numbers of 16 bits.

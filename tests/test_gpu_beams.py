@@ -206,3 +206,20 @@ def test_scores_that_are_not_finite(nnb, ctx):
     none = np.where(np.isfinite(score), score, -np.inf).astype(np.float32)
     check(got, logits, 700, none, np.where(np.isfinite(score), done, 0), 9, 6, "scores that are not finite")
     assert not np.isin(got[2][0], (1, 2)).any() and not np.isin(got[2][1], (0, 2)).any()
+
+
+@pytest.mark.parametrize("groups,beams,vocab,picks", [(1, 16, 49152, 10), (1, 16, 49152, 11), (1, 21, 49152, 8), (1, 22, 49152, 8), (98, 1, 49152, 7), (99, 1, 49152, 7), (4, 16, 1000, 8), (4, 17, 1000, 8),
+                                                   (1, 2, 500000, 2), (37, 4, 32000, 1)])
+def test_few_and_many_segments(nnb, ctx, groups, beams, vocab, picks):
+    """Calls on both sides of what decides whether rows' or segments' candidates are joined: some beams ended, without a score or with a NaN, results in place; the next call
+    finds lists of another one's."""
+    for seed in (111, 112):
+        logits, score = draw(groups, beams, vocab, seed)
+        rng = np.random.default_rng(seed)
+        done = (rng.random((groups, beams)) < 0.2).astype(np.int32)
+        score[rng.random((groups, beams)) < 0.1] = -np.inf
+        bad = rng.random((groups, beams)) < 0.1
+        logits[bad, rng.integers(0, vocab)] = np.nan
+        for in_place in (False, True)[:1 + (picks == beams)]:
+            got = run(nnb, ctx, logits, vocab, score, done, vocab // 2, picks, in_place)
+            check(got, logits, vocab, score, done, vocab // 2, picks, f"{groups}x{beams} of {vocab}, {picks} picks")
