@@ -89,9 +89,10 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
     // 5.0 us without, 4.7 with; 7118 rows by a warp each 35 without, 50 with).
     uint4 in[AHEAD][2];
     if (SPREAD) load(first, in[0]);
-    const RowPlace at = place_of_row(a.s, r);
+    const int given = a.position ? a.position[r] : 0;
+    const RowPlace at = place_of_row_soon(a.s, r);
     if (at.none) return;
-    const int turn = a.position && !at.bad ? a.position[r] : at.pos;
+    const int turn = a.position && !at.bad ? given : at.pos;
     if (at.bad || (a.rotary && (turn < 0 || turn >= a.table_len))) {
         if (lane == 0) a.status[STATUS_BAD_TABLE] = 1;
         return;

@@ -3,6 +3,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <climits>
+
 #include "attention.h"
 #include "ptx.cuh"
 
@@ -70,6 +72,40 @@ __device__ __forceinline__ RowPlace place_of_row(const KvSeqs& s, int r) {
     const SeqExtent e = seq_extent(s.row_start[p.seq], s.row_start[p.seq + 1], s.kv_len[p.seq], s.num_rows, s.max_len);
     p.pos = e.len - (e.row1 - r);
     p.bad = e.bad || p.pos < 0 || r < e.row0 || r >= e.row1;
+    return p;
+}
+// The same with one trip to memory for each 64 sequences: a lane has the numbers of one in either half of them.  (For writes: 64 rows of 48 heads of 128 dims, e4m3, 3.4 us by
+// the one above, 3.1 by this; reads of 65536 rows 217 and 222.)
+__device__ __forceinline__ RowPlace place_of_row_soon(const KvSeqs& s, int r) {
+    const int lane = threadIdx.x & 31;
+    RowPlace p;
+    p.seq = p.pos = 0;
+    p.none = true;
+    p.bad = false;
+    for (int i0 = 0; i0 < s.num_seqs; i0 += 64) {
+        int start[2], end[2], len[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const int i = i0 + 32 * g + lane, j = min(i, s.num_seqs - 1);
+            start[g] = s.row_start[j];
+            end[g] = s.row_start[j + 1];
+            len[g] = s.kv_len[j];
+            if (i >= s.num_seqs) end[g] = INT_MAX;
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            const unsigned before = __ballot_sync(0xffffffffu, end[g] <= r);   // sequences that end at or before it (they ascend)
+            if (before == 0xffffffffu) continue;
+            const int from = __popc(before), first = __shfl_sync(0xffffffffu, start[g], from), last = __shfl_sync(0xffffffffu, end[g], from), kv_len = __shfl_sync(0xffffffffu, len[g], from);
+            p.seq = i0 + 32 * g + from;
+            p.none = p.seq >= s.num_seqs || (p.seq == 0 && r < first);
+            if (p.none) return p;
+            const SeqExtent e = seq_extent(first, last, kv_len, s.num_rows, s.max_len);
+            p.pos = e.len - (e.row1 - r);
+            p.bad = e.bad || p.pos < 0 || r < e.row0 || r >= e.row1;
+            return p;
+        }
+    }
     return p;
 }
 
