@@ -190,7 +190,8 @@ extern "C" int nn_init(int device, nn_context** out) {
         delete c;
         return NN_FAIL(NN_ERR_CUDA, "nn_init: cudaMalloc failed");
     }
-    if (cudaMalloc(&c->beam_work, BEAM_WORK_BYTES) != cudaSuccess || cudaMemset(c->beam_work, 0, BEAM_WORK_BYTES) != cudaSuccess) {
+    if (cudaMalloc(&c->beam_work, BEAM_WORK_BYTES) != cudaSuccess || cudaMemset(c->beam_work, 0, BEAM_WORK_BYTES) != cudaSuccess ||
+        cudaStreamSynchronize(cudaStreamLegacy) != cudaSuccess) {   // (the context's stream does not wait for the memory that is set above)
         delete c;
         return NN_FAIL(NN_ERR_CUDA, "nn_init: cudaMalloc failed");
     }
