@@ -199,7 +199,8 @@ __device__ __forceinline__ unsigned long long order_of(double t) {
 }
 __device__ __forceinline__ double total_of(unsigned long long u) { return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u)); }
 
-// Whether this block is the last of `n` to arrive; what all of their threads have written before is visible to it then.
+// Whether this block is the last of `n` to arrive; what all of their threads have written before is visible to it then.  There is no barrier behind the reads of
+// the flag: between two of these calls nobody else writes it, and the next one begins with a barrier.
 __device__ __forceinline__ bool last_of(unsigned* counter, unsigned n, volatile int* flag) {
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -344,6 +345,7 @@ __global__ void __launch_bounds__(THREADS, DIRECT ? 4 : 6) beam_select_kernel(co
     __shared__ unsigned tops[WARPS];
     __shared__ double sums[WARPS];
     __shared__ int flag, count, homes[MOST_PICKS];
+    __shared__ unsigned bar;   // (a word of its own: a warp may still be reading what last_of has left in its flag)
     static_assert(sizeof(Candidates) * MOST_BEAMS <= sizeof(found) && sizeof(JoinRoom) <= sizeof(found), "room");
     pdl_launch_dependents();
     pdl_wait_prior_grid();
@@ -495,14 +497,14 @@ __global__ void __launch_bounds__(THREADS, DIRECT ? 4 : 6) beam_select_kernel(co
             if (left == m) left = 0;
             if (lane == i) best_of[warp * each + i] = m;
         }
-        if (tid == 0) count = flag = 0;
+        if (tid == 0) count = 0, bar = 0u;
         __syncthreads();
         // (those of threads without values are 0, and so may be the picks-th: no bar)
         places_of(best_of, WARPS * each, [&](int place, Key k) {
-            if (place == picks - 1 && k != 0) flag = (int)(k >> 8);
+            if (place == picks - 1 && k != 0) bar = (unsigned)(k >> 8);
         });
         __syncthreads();
-        Key least = (Key)(unsigned)flag << 32;
+        Key least = (Key)bar << 32;
 #pragma unroll 1
         for (int s0 = 0; s0 < segs; s0 += AHEAD) {
             if (s0) keys_from(s0);
