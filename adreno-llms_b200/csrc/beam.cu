@@ -9,12 +9,14 @@
 // best ones: every other share has `picks` values before all of its own.  So no value needs a place in a list while the logits stream by, whatever
 // their order.  The row's last block finds those shares, reads them again, a value to a thread, and has the row's candidates; the group's last
 // block joins its rows' lists.  Where there are few blocks each does so for its segment, and the group's last one joins the segments' lists (DIRECT).
-// Within a row the fp16 values and the tokens decide, exactly.  Across rows the totals do, in 64 bits.  Exponentials are taken of differences to the
-// thread's maximum (exact), in 32 bits: a maximum is exactly 1, the others are 2^-22 off at most, and so is the sum; a row of 151936 values of N(0, 2.5) has a sum that is some
-// 2^-27 off, its errors being different for each value.  Everything depends on differences alone: rows that are shifted against each other
-// give the same logarithms.
-// 64 groups of 8 beams of 151936 fp16 logits, 16 picks: 44 us (3.5 TB/s; the bytes alone 24).  The exponential unit has 36 thousand clocks of it, the logits altogether 52 (27 us),
-// the last rows' steps behind them 8 us.  One group of 4 beams of 49152: 8.1 us, all of it such steps.
+// Within a row the fp16 values and the tokens decide, exactly.  Across rows the totals do, in 64 bits.  Exponentials are taken of differences to the largest value that their warp has seen, in 32 bits.
+// A maximum is exactly 1; a value d below it is off by what rounding takes from d and from its product with log2 e (half a step each), by that constant (d 2^-26) and by
+// ex2 (2^-22, measured: 0.61 of that), equal values by the same.  From there on sums are scaled in 64 bits (a maximum that rises, warps, segments): in 32 bits and for each thread, 64 rising maxima
+// of a thread put the logarithm 2 2^-20 off.  So a warp's 65536 values, one peak and the others equal, 6 to 8 below it, are the worst: 1.5 2^-20, with five steps of adding up, whatever the row's length, and
+// totals that are 2^-18 apart come in order.  (Measured of such rows: 0.9 2^-20 between two; of 151936 values of N(0, 2.5), whose errors are different ones, some 2^-27 each.)  For that the
+// serving batch below takes 3 % longer.  Everything depends on differences alone: rows that are shifted against each other give the same logarithms.
+// 64 groups of 8 beams of 151936 fp16 logits, 16 picks: 46 us (3.4 TB/s; the bytes alone 24).  The exponential unit has 36 thousand clocks of it, the logits altogether some 54 (28 us),
+// the last rows' steps behind them 8 us.  One group of 4 beams of 49152: 8.5 us, all of it such steps.
 #include <cuda_fp16.h>
 
 #include "kv_branch.h"
@@ -32,6 +34,12 @@ constexpr unsigned NO_VALUE = 0x03FFu;      // the code of -infinity
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// the largest number of a warp (NaN: of the others)
+__device__ __forceinline__ float warp_max(float x) {
+    float y;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
     return y;
 }
 // fp16 numbers in order as whole ones, both zeros the same
@@ -72,7 +80,7 @@ __device__ __forceinline__ void places_of(const Key* keys, int n, Take&& take) {
 }
 
 constexpr double LN2 = 0.693147180559945309417;
-// exp(x), x <= 0: 2^n times the exponential's series of what is left, at most ln 2 / 2 (11 terms: 2^-44)
+// exp(x), x <= 0: 2^n times the exponential's series of what is left, at most ln 2 / 2 (11 terms: 2^-41)
 __device__ __forceinline__ double exp_of(double x) {
     if (!(x > -700.)) return x == x ? 0. : x;
     const double n = rint(x * (1. / LN2)), f = fma(n, -LN2, x);
@@ -336,7 +344,7 @@ __device__ __forceinline__ void join_segments(const BeamSelectArgs& a, int group
     }
 }
 
-// (six blocks to an SM, for loads in flight: with five and more registers 44.5 us where it is 42.8)
+// (six blocks to an SM, for loads in flight: with five and more registers 47.4 us where it is 45.8)
 template <bool DIRECT>
 __global__ void __launch_bounds__(THREADS, DIRECT ? 4 : 6) beam_select_kernel(const BeamSelectArgs a) {
     __shared__ __align__(16) Key found[ROOM];
@@ -361,7 +369,7 @@ __global__ void __launch_bounds__(THREADS, DIRECT ? 4 : 6) beam_select_kernel(co
     auto segment_sum = [&](double& sum, unsigned& top) {   // of the warps' ones, by a warp
         const unsigned mine = lane < WARPS ? tops[lane] : 0u, most = __reduce_max_sync(0xffffffffu, mine);
         double s = lane < WARPS ? sums[lane] : 0.0;
-        if (s != 0) s *= (double)ex2((value_of(mine) - value_of(most)) * LOG2E);
+        if (s != 0) s *= exp_of((double)value_of(mine) - (double)value_of(most));
 #pragma unroll 1
         for (int d = WARPS / 2; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
         if (lane == 0) {
@@ -372,10 +380,11 @@ __global__ void __launch_bounds__(THREADS, DIRECT ? 4 : 6) beam_select_kernel(co
     if (looked_at) {
         const int begin = seg * a.per_seg, end = min(x.vectors(), begin + a.per_seg), plain = min(x.plain(), end);
         __half most = __ushort_as_half(0xFC00);
+        float peak = -INFINITY;        // the warp's largest value: sums are of exponentials of differences to that
         float sum = 0.f, rest = 0.f;   // (rest: what rounding has taken from the sum)
         int at = 0;
 #pragma unroll 1
-        for (int i0 = begin + tid; i0 < end; i0 += THREADS * BATCH) {
+        for (int i0 = begin + tid; i0 - lane < end; i0 += THREADS * BATCH) {   // (whole warps stay together)
             uint4 v[BATCH];
             if (i0 + (BATCH - 1) * THREADS < plain) {
 #pragma unroll
@@ -388,16 +397,22 @@ __global__ void __launch_bounds__(THREADS, DIRECT ? 4 : 6) beam_select_kernel(co
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) m[j] = most_of(v[j]);
             const __half up = most_of(__hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3])));
+            const float higher = warp_max(__half2float(up));
+            if (higher > peak) {   // (of the whole warp)
+                if (peak > -INFINITY) {
+                    const double all = ((double)sum + (double)rest) * exp_of((double)peak - (double)higher);
+                    sum = (float)all;
+                    rest = (float)(all - (double)sum);
+                }
+                peak = higher;
+            }
             if (__hgt(up, most)) {
-                const float f = ex2((__half2float(most) - __half2float(up)) * LOG2E);
-                sum *= f;
-                rest *= f;
                 most = up;
                 int j = 0;
                 while (j < BATCH - 1 && !__heq(most_of(j == 0 ? m[0] : j == 1 ? m[1] : m[2]), up)) ++j;
                 at = i0 + j * THREADS - begin;
             }
-            const float ref = __heq(most, __ushort_as_half(0xFC00)) ? 0.f : -__half2float(most);
+            const float ref = peak == -INFINITY ? 0.f : -peak;
             float2 s[BATCH];
 #pragma unroll
             for (int j = 0; j < BATCH; ++j) {
@@ -420,12 +435,11 @@ __global__ void __launch_bounds__(THREADS, DIRECT ? 4 : 6) beam_select_kernel(co
         const unsigned code = code_of(__half_as_ushort(most));
         own = code > NO_VALUE ? code << 16 | (0xFFFFu - at) : 0u;
         if (!direct) part.key[tid] = own;
-        const unsigned warp_top = __reduce_max_sync(0xffffffffu, code);
-        double whole = sum != 0.f ? ((double)sum + (double)rest) * (double)ex2((__half2float(most) - value_of(warp_top)) * LOG2E) : 0.0;
+        double whole = (double)sum + (double)rest;
 #pragma unroll 1
         for (int d = 16; d > 0; d >>= 1) whole += __shfl_xor_sync(0xffffffffu, whole, d);
         if (lane == 0) {
-            tops[warp] = warp_top;
+            tops[warp] = code_of(__half_as_ushort(__float2half_rn(peak)));
             sums[warp] = whole;
         }
         __syncthreads();
@@ -665,8 +679,8 @@ cudaError_t launch_beam_select(const BeamSelectArgs& given, int sm_count, cudaSt
     BeamSelectArgs a = given;
     beam_segments(a.groups * a.beams, a.vocab, sm_count, &a.segs, &a.per_seg);
     // Few blocks look for their segments' candidates themselves, which saves the rows' counters and a trip to the parts; of many, in several rounds, most have
-    // nothing to do with that.  So / by rows, us: 1 x 4 beams of 49152, 4 picks 8.1 / 9.2; of 151936 9.1 / 12.6; 8 x 5 of 65535, 5 picks 13.3 / 15.7; 64 x 4 of 8192, 8 picks
-    // 11.3 / 13.1; 100 x 4 of 1000, 4 picks 9.7 / 12.0.  Without segments there is less to save and rows' lists are joined sooner where they are long: 11 x 14 of 157, 28 picks 18.6 / 16.7.
+    // nothing to do with that.  So / by rows, us: 1 x 4 beams of 49152, 4 picks 8.5 / 9.6; of 151936 11.4 / 13.5; 8 x 5 of 65535, 5 picks 13.8 / 16.9; 64 x 4 of 8192, 8 picks
+    // 11.9 / 14.9; 100 x 4 of 1000, 4 picks 10.1 / 13.0.  Without segments there is less to save and rows' lists are joined sooner where they are long: 11 x 14 of 157, 28 picks 37 / 25.
     const int lists = a.beams * a.segs, candidates = lists * a.picks;
     const bool direct = a.groups * lists <= 4 * sm_count && lists <= DIRECT_LISTS && candidates <= (a.segs > 1 ? DIRECT_MOST : DIRECT_MOST / 8);
     cudaLaunchConfig_t cfg = {};
@@ -682,7 +696,7 @@ cudaError_t launch_beam_select(const BeamSelectArgs& given, int sm_count, cudaSt
 }
 
 // Segments of a row, in whole rounds of loads: of so many that there are some 16 blocks for each SM, and of no more vectors than have numbers of 16 bits.
-// (64 groups of 8 beams of 151936 logits with some 6 / 10 / 16 / 24 / 40 blocks for each SM: 49.2 / 47.1 / 42.8 / 46.0 / 49.6 us; fewer leave SMs without work at the end, more have more
+// (64 groups of 8 beams of 151936 logits with some 6 / 10 / 16 / 24 / 40 blocks for each SM: 51.9 / 48.5 / 45.7 / 48.6 / 51.6 us; fewer leave SMs without work at the end, more have more
 // parts to read and counters to wait for)
 void beam_segments(int rows, int vocab, int sm_count, int* segs, int* per_seg) {
     const int vectors = (vocab + 7) / 8, round = THREADS * BATCH, rounds = (vectors + round - 1) / round;

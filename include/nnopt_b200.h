@@ -256,7 +256,7 @@ int nn_attention(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, 
  *                     fp16 logits [groups * beams][logits_stride] (0: dense) of `vocab` tokens and fp32 scores [groups][beams], in descending order (of a beam's own its larger
  *                     logits); of equal ones the lowest beam, then the lowest token first.  out_score fp32, out_token and out_parent (the beam) int32, [groups][picks]; where a
  *                     group has fewer candidates the rest are -infinity, -1, -1.  Totals are compared in 64 bits and rounded to fp32 for out_score; the exponentials
- *                     behind them have 32 bits, so that totals of different beams which are nearer than 2^-20 may come in either order (rows that are equal, or shifted
+ *                     behind them have 32 bits, so that totals of different beams which are nearer than 2^-18 may come in either order (rows that are equal, or shifted
  *                     against each other by a constant, give the same logarithms).
  *                     Logits of -infinity are no candidates, nor are beams whose score is not finite, nor rows with a NaN or +infinity.
  *                     done (int32 [groups][beams], may be NULL): a beam that is not 0 there has ended: it has one candidate, token eos with its score as it
