@@ -85,10 +85,9 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
             in[1] = reinterpret_cast<const uint4*>(src)[pb];
         }
     };
-    // Spread: the row's first heads are on their way while its place is looked up, and later ones while those before them are worked on (414 rows of 48 heads of 128 dims, e4m3:
-    // 5.0 us without, 4.7 with; 7118 rows by a warp each 35 without, 50 with).
+    // Spread: the row's first heads are on their way while its page is looked up (not before its place is known: rows of no sequence are not read), and later ones while those before
+    // them are worked on (7118 rows by a warp each: 35 without, 50 with).
     uint4 in[AHEAD][2];
-    if (SPREAD) load(first, in[0]);
     const int given = a.position ? a.position[r] : 0;
     const RowPlace at = place_of_row_soon(a.s, r);
     if (at.none) return;
@@ -97,6 +96,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
         if (lane == 0) a.status[STATUS_BAD_TABLE] = 1;
         return;
     }
+    if (SPREAD) load(first, in[0]);
     const int page = a.s.page_table[(int64_t)at.seq * a.s.table_stride + (at.pos >> a.c.page_shift)], slot = at.pos & ((1 << a.c.page_shift) - 1);
     const bool cell = page_ok(page, a.c.num_pages);
     if (!cell && lane == 0) a.status[STATUS_BAD_TABLE] = 1;

@@ -242,7 +242,8 @@ int nn_attention(nn_context* ctx, nn_kv_cache* cache, const nn_kv_batch* batch, 
  *                     mask_words 1 to 32, with a bit for each of max_new rows.  Of the batch row_start and kv_len are used.  Once a step: all layers share
  *                     them.  (A program whose trees are always the same may keep the mask.)
  *   nn_rope_kv_write_at  nn_rope_kv_write with queries and keys rotated to position[row] (int32 [num_rows], below table_len) instead of the cell's own
- *                     position: a tree's rows lie one behind the other in the cache, whatever their depth.  A row whose position is out of range is left out.
+ *                     position: a tree's rows lie one behind the other in the cache, whatever their depth.  A row whose position is out of range is left out (entries of
+ *                     rows of no sequence count for nothing).
  *   nn_attention_tree nn_attention where row r sees all positions before the sequence's new rows, and of these the ones in its mask (bits behind the last new
  *                     row count for nothing; any bits may be set, those of later rows too).  No window.  A row that sees nothing gives zeros.
  *                     A sequence with more new rows than a mask has bits is left out and reported.
