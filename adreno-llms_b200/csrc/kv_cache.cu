@@ -68,7 +68,7 @@ constexpr int WARPS = 4;
 template <int FMT, int D, bool SPREAD>
 __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs a) {
     constexpr int LANES = D / 16, HEADS = 32 / LANES * (SPREAD ? WARPS : 1);   // threads of a head's row; heads at a time
-    constexpr int AHEAD = SPREAD ? 1 : FMT == KV_FP16 && D == 128 ? 4 : 3;      // loads of so many heads in flight
+    constexpr int AHEAD = SPREAD ? 1 : FMT == KV_FP16 ? 4 : 3;                // loads of so many heads in flight
     pdl_launch_dependents();
     pdl_wait_prior_grid();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = SPREAD ? blockIdx.x : blockIdx.x * WARPS + warp;
@@ -85,8 +85,6 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
             in[1] = reinterpret_cast<const uint4*>(src)[pb];
         }
     };
-    // Spread: the row's first heads are on their way while its page is looked up (not before its place is known: rows of no sequence are not read), and later ones while those before
-    // them are worked on (7118 rows by a warp each: 35 without, 50 with).
     uint4 in[AHEAD][2];
     const int given = a.position ? a.position[r] : 0;
     const RowPlace at = place_of_row_soon(a.s, r);
@@ -96,7 +94,7 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
         if (lane == 0) a.status[STATUS_BAD_TABLE] = 1;
         return;
     }
-    if (SPREAD) load(first, in[0]);
+    if (SPREAD) load(first, in[0]);   // (on its way while the page is looked up; rows of no sequence are not read)
     const int page = a.s.page_table[(int64_t)at.seq * a.s.table_stride + (at.pos >> a.c.page_shift)], slot = at.pos & ((1 << a.c.page_shift) - 1);
     const bool cell = page_ok(page, a.c.num_pages);
     if (!cell && lane == 0) a.status[STATUS_BAD_TABLE] = 1;
@@ -113,29 +111,24 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
         }
     }
     for (int h0 = 0; h0 < heads; h0 += HEADS * AHEAD) {   // (whole warps stay together for the shuffles)
-        if (!SPREAD) {
 #pragma unroll
-            for (int u = 0; u < AHEAD; ++u) load(h0 + u * HEADS + first, in[u]);
-        }
+        for (int u = 0; u < AHEAD; ++u)
+            if (!SPREAD || h0 > 0) load(h0 + u * HEADS + first, in[u]);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             const int h = h0 + u * HEADS + first;
             const bool on = h < heads, is_q = h < nq, is_k = !is_q && h < nq + a.c.kv_heads;
             uint4 px = in[u][0], py = in[u][1];
-            if (SPREAD) load(h + HEADS, in[u]);
             float x[8], y[8];
-            unpack8(px, x);
-            unpack8(py, y);
             if (turns && (is_q || is_k)) {
+                unpack8(px, x);
+                unpack8(py, y);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float t1 = __fsub_rn(__fmul_rn(x[i], c[i]), __fmul_rn(y[i], s[i])), t2 = __fadd_rn(__fmul_rn(y[i], c[i]), __fmul_rn(x[i], s[i]));
                     x[i] = t1;
                     y[i] = t2;
                 }
-            }
-            // (fp16: by lanes without a cell too where that was faster: 2048 rows of 18 heads of 64 dims 3.68 us so, 3.56 otherwise; 3079 rows of 48 heads of 128 17.0 and 18.2)
-            if (FMT == KV_FP16 ? D == 128 || is_q || (on && cell) : is_q || is_k) {
                 px = pack8(x);
                 py = pack8(y);
             }
@@ -166,10 +159,8 @@ __global__ void __launch_bounds__(WARPS * 32) kv_write_kernel(const KvWriteArgs 
                     const float f = half_float(sc), inverse = __frcp_rn(f);
                     const bool whole = sc != 0x7FFF;
                     uint2* dst = reinterpret_cast<uint2*>((uint8_t*)(is_k ? a.c.k : a.c.v) + row * D);
-                    if (is_k) {   // (as they were rounded)
-                        unpack8(px, x);
-                        unpack8(py, y);
-                    }
+                    unpack8(px, x);   // (as they were rounded)
+                    unpack8(py, y);
                     dst[pa] = whole ? encode8<FMT>(x, f, inverse) : make_uint2(0, 0);
                     dst[pb] = whole ? encode8<FMT>(y, f, inverse) : make_uint2(0, 0);
                     if (j == 0) (is_k ? a.c.k_scale : a.c.v_scale)[row] = sc;
@@ -253,9 +244,11 @@ cudaError_t launch(void (*kernel)(const Args), const Args& a, int grid, cudaStre
 }
 
 // A row in four warps is ready sooner, a row in one has more loads in flight and fewer blocks to start.  Four warps / one, us, in a recorded chain of calls:
-// writes of 32 + 2 x 8 heads of 128 dims, fp16: 1 row 2.5 / 4.3, 1200 rows 5.1 / 7.9, 3079 rows 16.0 / 17.0, 5607 rows 25.0 / 24.3; e4m3: 3079 rows 18.0 / 20.6, 5607 rows
-// 29.6 / 26.6; of 9 + 2 x 3 heads of 64:
-// 1 row 1.9 / 2.1, 256 rows 2.4 / 2.3, 2400 rows 4.8 / 3.3.  Reads of 3 heads of 64 dims, int8: 1200 rows 2.5 / 2.8, 2400 rows
+// writes of 32 + 2 x 8 heads of 128 dims, fp16: 1 row 2.5 / 4.0, 1200 rows 5.7 / 7.5, 2368 rows 11.6 / 11.4, 2960 rows 14.3 / 14.0, 3079 rows 14.7 / 16.9, 4736 rows 20.8 / 20.8, 7118 rows 29.7 / 30.1;
+// e4m3: 2368 rows 12.4 / 12.8, 2960 rows 15.5 / 14.1, 3079 rows 15.9 / 18.8, 4736 rows 22.5 / 23.3, 5607 rows 26.2 / 25.4; of 48 + 2 x 8 heads of 64, e4m3: 2368 rows 9.0 / 9.0, 2960 rows
+// 11.2 / 10.3, 3079 rows 11.6 / 13.4, 4736 rows 16.5 / 16.7, 5607 rows 18.8 / 18.4: rows by a warp each are worth it where they just fit on the SMs at once (five blocks of four to an SM) and where they are very many.
+// Of 9 + 2 x 3 heads of 64: 1 row 1.9 / 2.1, 256 rows 2.4 / 2.3, 2400 rows 4.8 / 3.3.  (Registers count: four warps to a row with later heads' loads on their way while earlier ones are worked on
+// need 72 instead of 64, an SM holds seven blocks instead of eight, and 1200 to 2700 rows took 4 to 12 % longer.)  Reads of 3 heads of 64 dims, int8: 1200 rows 2.5 / 2.8, 2400 rows
 // 4.1 / 2.8; of 8 heads of 128 dims: 1 row 1.8 / 2.9, 2400 rows 4.6 / 7.1, 65536 rows of 16 heads, e4m3,
 // 135 / 143; but of 8 heads of 64, e4m3, 70 / 50, of 4 heads of 128, fp16, 71 / 43.
 constexpr int FEW_ROWS = 592;   // (four blocks for each SM)
@@ -263,7 +256,8 @@ constexpr int FEW_ROWS = 592;   // (four blocks for each SM)
 template <int FMT, int D>
 cudaError_t write_rows(const KvWriteArgs& a, cudaStream_t st, bool pdl) {
     const bool wide = ((a.q ? a.q_heads : 0) + 2 * a.c.kv_heads) * (D / 16) >= 2 * WARPS * 32;   // a row is work for four warps more than once
-    if (a.s.num_rows <= (wide ? 8 * FEW_ROWS : FEW_ROWS)) return launch(kv_write_kernel<FMT, D, true>, a, a.s.num_rows, st, pdl);
+    const int rows = a.s.num_rows;
+    if (wide ? rows <= 4 * FEW_ROWS || (rows > 5 * FEW_ROWS && rows <= 8 * FEW_ROWS) : rows <= FEW_ROWS) return launch(kv_write_kernel<FMT, D, true>, a, a.s.num_rows, st, pdl);
     return launch(kv_write_kernel<FMT, D, false>, a, (a.s.num_rows - 1) / WARPS + 1, st, pdl);
 }
 template <int FMT, int D>
