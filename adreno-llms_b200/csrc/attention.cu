@@ -35,7 +35,8 @@ cudaError_t attention_configure() {
 }
 
 // Trees whose cells the kernel for few rows can read again and again: in items of 8 rows (its form of 16 rows needs more registers than it has), all of them to
-// the sequence's end.  That kernel with 8 rows / with 16 / the kernel for many rows, us, by the items of 16 rows that there would be:
+// the sequence's end.  How long sequences are the host does not know: it goes by max_len, the bound that a call (or a recording, for all of its replays) declares, so that 26 tokens of 9 heads to 3 over
+// 700 positions take 9.6 us up to a bound of 7281 positions and 15.6 behind it.  That kernel with 8 rows / with 16 / the kernel for many rows, us, by the items of 16 rows that there would be:
 //   items   rows   cells               400                2000                8000           32000 positions
 //   4         64   fp16 of 64     8.2 / 10.3 / 13.8   9.0 / 11.1 / 14.2  10.9 / 14.1 / 17.7   14.8 /    / 36.6
 //   16       105   int8 of 64     8.4 / 10.6 / 15.5  11.0 / 13.4 / 16.7  16.6 / 18.2 / 22.2   36.8 /    / 33.0

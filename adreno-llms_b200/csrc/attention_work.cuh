@@ -167,7 +167,7 @@ __device__ __forceinline__ Walk find_work(const KvSeqs& s, WorkShape* w, unsigne
     items *= w->vheads;
     w->pad = 2 * items <= gridDim.x;
     // Where items are long, filling them up costs more than a second segment (a tree of 64 tokens over 17000 to 33000 positions of each of 8 sequences, 32 heads to 8
-    // of 128 dims: fp16 278 us filled up, 203 not; e4m3 427 and 264; over 4400 to 8200 positions 86 and 69).
+    // of 128 dims: fp16 297 us filled up, 221 not; e4m3 453 and 278; over 4400 to 8200 positions 93 and 74, e4m3 139 and 99).
     if (w->second && w->pad) w->pad = (total + gridDim.x - items - 1) / (gridDim.x - items) <= (total + items * extra) / gridDim.x + w->second;
     const unsigned blocks = w->pad ? gridDim.x - items : gridDim.x;   // (filled up, items take up to one more block each)
     if (!w->pad) {

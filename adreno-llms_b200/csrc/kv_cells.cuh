@@ -74,8 +74,8 @@ __device__ __forceinline__ RowPlace place_of_row(const KvSeqs& s, int r) {
     p.bad = e.bad || p.pos < 0 || r < e.row0 || r >= e.row1;
     return p;
 }
-// The same with one trip to memory for each 64 sequences: a lane has the numbers of one in either half of them.  (For writes: 64 rows of 48 heads of 128 dims, e4m3, 3.4 us by
-// the one above, 3.1 by this; reads of 65536 rows 217 and 222.)
+// The same with one trip to memory for each 64 sequences: a lane has the numbers of one in either half of them.  (For writes: 64 rows of 48 heads of 128 dims, e4m3, 3.2 us by
+// the one above, 3.0 by this; reads of 65536 rows 217 and 222.)
 __device__ __forceinline__ RowPlace place_of_row_soon(const KvSeqs& s, int r) {
     const int lane = threadIdx.x & 31;
     RowPlace p;
