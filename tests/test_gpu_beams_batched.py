@@ -29,3 +29,28 @@ def test_the_same_call_again_and_again(nnb, ctx, groups, beams, vocab, picks):
         assert all(np.array_equal(a, b) for a, b in zip(got, first)), turn
     for b in (lb, sb, *outs):
         ctx.free(b)
+
+
+@pytest.mark.parametrize("groups,beams,vocab,picks", [(1, 8, 5000, 5), (2, 8, 60001, 9), (60, 8, 60001, 9)])
+def test_rows_without_numbers(nnb, ctx, groups, beams, vocab, picks):
+    """Rows of nothing but NaN, of NaN where one warp, one round or one segment reads, of infinities, and of no logit until the last token."""
+    logits, score = draw(1, beams, vocab, 122)
+    x = logits[0]
+    x[0] = np.nan
+    x[1] = -np.float16(np.nan)
+    x[2, 256:512] = np.nan
+    x[3, vocab // 2:] = np.nan
+    x[4] = np.inf
+    x[5] = -np.inf
+    x[5, -1] = 3
+    x[6, :vocab - 3] = -np.inf
+    lb, sb = ctx.upload(np.repeat(logits, groups, 0)), ctx.upload(np.repeat(score, groups, 0))
+    outs = [ctx.alloc(4 * groups * picks) for _ in range(3)]
+    ctx.beam_select(groups, beams, vocab, lb, 0, sb, None, -1, picks, *outs, None)
+    ctx.sync()
+    got = [ctx.download(o, (groups, picks), t) for o, t in zip(outs, (np.float32, np.int32, np.int32))]
+    for g in range(groups):
+        check([a[g:g + 1] for a in got] + [None], logits, vocab, score, None, -1, picks, "without numbers")
+    assert set(got[2][0][got[2][0] >= 0]) <= {5, 6, 7}
+    for b in (lb, sb, *outs):
+        ctx.free(b)
